@@ -51,8 +51,16 @@ typedef enum rq_dtype { RQ_F32 = 0, RQ_F16 = 1 } rq_dtype;
  *                   rusty-loader/src/lib.rs:155-218): unsigned codes u,
  *                   f32 scale and bias per `group` consecutive elements of the
  *                   flattened row-major index i = n*k_in + k:
- *                   W[i] = f32(u[i]) * scales[i/group] + biases[i/group]. */
-typedef enum rq_qformat { RQ_Q_ROWWISE_I8 = 0, RQ_Q_AFFINE_U8 = 1 } rq_qformat;
+ *                   W[i] = f32(u[i]) * scales[i/group] + biases[i/group].
+ *  RQ_Q_AFFINE_U4 : the same with 4-bit codes (MLX's 4-bit affine layout; the
+ *                   reference reads 8-bit checkpoints only): element i is the
+ *                   low nibble of byte i/2 for even i, the high nibble for odd
+ *                   i; k_in is even and a multiple of group, so a row is
+ *                   k_in/2 bytes and k_in/group groups.  Served by
+ *                   rq_qweight_dequantize, rq_qmatmul, rq_qmatmul_lora (_ex),
+ *                   rq_mlp_swiglu (_noalloc); the others refuse it with
+ *                   RQ_ERR_UNSUPPORTED (their size queries return 0). */
+typedef enum rq_qformat { RQ_Q_ROWWISE_I8 = 0, RQ_Q_AFFINE_U8 = 1, RQ_Q_AFFINE_U4 = 2 } rq_qformat;
 
 /* A quantized Linear weight in [out, in] ("W[n_out, k_in]", K contiguous)
  * orientation: Y = X . deq(W)^T, the semantics of the reference's `matmul_bt`
@@ -60,14 +68,14 @@ typedef enum rq_qformat { RQ_Q_ROWWISE_I8 = 0, RQ_Q_AFFINE_U8 = 1 } rq_qformat;
  * is {FP32, FP16}, lib.rs:57-76); quantized weights travel as raw buffer
  * triplets (lib.rs:4939-4946).  This struct is that triplet plus its shape. */
 typedef struct rq_qweight {
-    const void *codes;    /* device, n_out*k_in bytes, row-major           */
+    const void *codes;    /* device, n_out*k_in bytes (U4: half), row-major */
     const float *scales;  /* device, ROWWISE: [n_out]; AFFINE: [n_groups]  */
     const float *biases;  /* device, AFFINE: [n_groups] or NULL (= 0)      */
     int64_t n_out;
     int64_t k_in;
     int32_t format;       /* rq_qformat                                    */
     int32_t group;        /* AFFINE: elements per group (64 in reference)  */
-    const float *prep;    /* AFFINE, optional: the table rq_qweight_prepare
+    const float *prep;    /* AFFINE_U8, optional: the table rq_qweight_prepare
                            * built from these scales and biases, or NULL   */
 } rq_qweight;
 
@@ -324,6 +332,69 @@ size_t rq_qmatmul_dx_mfma_workspace(int64_t m, int64_t n_out);
 int rq_qmatmul_dx_mfma(rq_ctx *ctx, const rq_qweight *w, const void *table, const void *dy, rq_dtype dy_dtype,
                        void *dx, rq_dtype dx_dtype, int64_t m, void *workspace, size_t workspace_bytes,
                        rq_stream stream);
+
+/* ---- attention ------------------------------------------------------------
+ * GQA attention as entry points of their own (the reference's
+ * flash_attention_v2.wgsl:74 under Attention::forward,
+ * rusty-graph/src/lib.rs:191-283, for one sequence): several prompts at once,
+ * and drafted tokens over a KV cache.
+ *   out[t, h] = sum_j p_j v[j, g] / sum_j p_j,  p_j = exp(scale q[t, h].k[j, g]),
+ * g = h / (n_heads / n_kv_heads), over the keys j that the entry point lets
+ * token t see; a token that sees none gets zeros.  What a token does not see
+ * does not reach its result, infinities and NaN included.  fp16 tensors go
+ * through the fp16 matrix cores (scores, sums and accumulators f32, p rounded
+ * to fp16), f32 ones through the f32 matrix cores; out is rounded once.
+ * Pointers are 16-byte aligned, row strides multiples of 16 bytes
+ * (RQ_ERR_UNSUPPORTED otherwise); out overlaps no input. */
+typedef struct rq_attn {
+    int32_t n_heads;
+    int32_t n_kv_heads;  /* divides n_heads                                    */
+    int32_t head_dim;    /* 64 or 128                                          */
+    int32_t dtype;       /* rq_dtype of q, k, v and out                        */
+    float scale;         /* of q.k; 0 selects 1 / sqrt(head_dim)               */
+    int32_t reserved;    /* 0                                                  */
+    /* elements between the rows of consecutive tokens; 0: the rows are packed
+     * (n_heads * head_dim for q and out, n_kv_heads * head_dim for k and v).
+     * The heads of a row lie side by side. */
+    int64_t q_row, k_row, v_row, out_row;
+} rq_attn;
+
+/* Causal attention over packed prompts: sequence s is tokens
+ * starts[s] .. starts[s+1]-1 of q, k and v, and each token sees itself and
+ * the tokens before it in its sequence.  starts: device int32[n_seqs + 1],
+ * ascending within 0..tokens (values outside are clamped); sequences may be
+ * empty.  Rows of out that belong to no sequence are left as they were. */
+int rq_attn_packed(rq_ctx *ctx, const rq_attn *attn, const void *q, const void *k, const void *v,
+                   const int32_t *starts, int32_t n_seqs, int64_t tokens, void *out, rq_stream stream);
+
+/* A KV cache: position p of sequence s and KV head g at
+ * k + s * seq_stride + g * head_stride + p * pos_stride (elements; all three 0:
+ * [n_seqs][n_kv_heads][capacity][head_dim]), v alike. */
+typedef struct rq_kv_cache {
+    const void *k, *v;
+    int64_t seq_stride, head_stride, pos_stride;
+    int32_t n_seqs;
+    int32_t capacity;  /* positions per sequence */
+} rq_kv_cache;
+
+/* Attention of drafted tokens (a tree per sequence) over the cache.  Sequence
+ * s has lengths[s] cached positions (device int32[n_seqs], clamped to
+ * 0..capacity) and the drafted tokens i = 0, 1, ... whose queries are rows
+ * starts[s] + i of q (starts as in rq_attn_packed, at most max_nodes tokens
+ * per sequence, 1..64: rows past that are left as they were) and whose keys
+ * and values are already cached at positions lengths[s] + i.  Token i sees
+ * every cached position below lengths[s] and the drafted tokens j whose bit j
+ * of mask[starts[s] + i] is set (device uint64[tokens]; bits past the
+ * sequence's tokens or the capacity name nothing).  mask NULL: each token sees
+ * itself and the drafted tokens before it (a chain; one token per sequence is
+ * a plain decode step).  Of attn, k_row and v_row are not used.  workspace:
+ * rq_attn_tree_workspace(...) bytes, 16-byte aligned, one per call in flight
+ * (a captured call keeps its own). */
+size_t rq_attn_tree_workspace(const rq_attn *attn, int32_t n_seqs, int64_t tokens, int32_t max_nodes,
+                              int32_t capacity);
+int rq_attn_tree(rq_ctx *ctx, const rq_attn *attn, const rq_kv_cache *cache, const void *q, const int32_t *starts,
+                 const int32_t *lengths, const uint64_t *mask, int64_t tokens, int32_t max_nodes, void *out,
+                 void *workspace, size_t workspace_bytes, rq_stream stream);
 
 /* ---- int8-weight Llama greedy decode ------------------------------------
  * LlamaModel::forward (rusty-graph/src/lib.rs:420-436) over LlamaBlock

@@ -27,6 +27,7 @@ RQ_F32 = 0
 RQ_F16 = 1
 RQ_Q_ROWWISE_I8 = 0
 RQ_Q_AFFINE_U8 = 1
+RQ_Q_AFFINE_U4 = 2
 RQ_AFFINE_FMA = 1
 RQ_LORA_TREE = 1
 
@@ -41,6 +42,33 @@ class rq_qweight(ctypes.Structure):
         ("format", c_int32),
         ("group", c_int32),
         ("prep", c_void_p),
+    ]
+
+
+class rq_attn(ctypes.Structure):
+    _fields_ = [
+        ("n_heads", c_int32),
+        ("n_kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("dtype", c_int32),
+        ("scale", ctypes.c_float),
+        ("reserved", c_int32),
+        ("q_row", c_int64),
+        ("k_row", c_int64),
+        ("v_row", c_int64),
+        ("out_row", c_int64),
+    ]
+
+
+class rq_kv_cache(ctypes.Structure):
+    _fields_ = [
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("seq_stride", c_int64),
+        ("head_stride", c_int64),
+        ("pos_stride", c_int64),
+        ("n_seqs", c_int32),
+        ("capacity", c_int32),
     ]
 
 
@@ -120,6 +148,10 @@ _SIGNATURES = {
     "rq_qweight_dx_table": [_P, POINTER(rq_qweight), _P, c_size_t, _P],
     "rq_qmatmul_dx_mfma_workspace": [c_int64, c_int64],
     "rq_qmatmul_dx_mfma": [_P, POINTER(rq_qweight), _P, _P, c_int, _P, c_int, c_int64, _P, c_size_t, _P],
+    "rq_attn_packed": [_P, POINTER(rq_attn), _P, _P, _P, _P, c_int32, c_int64, _P, _P],
+    "rq_attn_tree_workspace": [POINTER(rq_attn), c_int32, c_int64, c_int32, c_int32],
+    "rq_attn_tree": [_P, POINTER(rq_attn), POINTER(rq_kv_cache), _P, _P, _P, _P, c_int64, c_int32, _P, _P, c_size_t,
+                     _P],
     "rq_llama_create": [_P, POINTER(rq_llama_config), POINTER(rq_llama_weights), POINTER(c_void_p)],
     "rq_llama_destroy": [_P],
     "rq_llama_prefill": [_P, POINTER(c_int32), c_int32, _P],
@@ -138,7 +170,8 @@ _SIGNATURES = {
 }
 _RESTYPES = {"rq_status_string": c_char_p, "rq_last_error": c_char_p, "rq_qmatmul_lora_workspace": c_size_t,
              "rq_qmatmul_lora_ex_workspace": c_size_t, "rq_qweight_prep_bytes": c_size_t,
-             "rq_qweight_dx_table_bytes": c_size_t, "rq_qmatmul_dx_mfma_workspace": c_size_t}
+             "rq_qweight_dx_table_bytes": c_size_t, "rq_qmatmul_dx_mfma_workspace": c_size_t,
+             "rq_attn_tree_workspace": c_size_t}
 
 
 class RqError(RuntimeError):

@@ -42,15 +42,20 @@ bool mul_ok(int64_t a, int64_t b, int64_t *out) {
 
 using namespace rq;
 
-int rq::check_qweight(const rq_qweight *w) {
+int rq::check_qweight(const rq_qweight *w, bool u4) {
     if (!w) return fail(RQ_ERR_INVALID_ARGUMENT, "null weight");
-    if (w->format != RQ_Q_ROWWISE_I8 && w->format != RQ_Q_AFFINE_U8)
+    if (w->format != RQ_Q_ROWWISE_I8 && w->format != RQ_Q_AFFINE_U8 && w->format != RQ_Q_AFFINE_U4)
         return fail(RQ_ERR_INVALID_ARGUMENT, "unknown weight format %d", w->format);
+    if (w->format == RQ_Q_AFFINE_U4 && !u4)
+        return fail(RQ_ERR_UNSUPPORTED, "4-bit weights are not served by this entry point");
     if (w->n_out < 0 || w->k_in < 0) return fail(RQ_ERR_SHAPE, "negative weight shape");
     int64_t n;
     if (!mul_ok(w->n_out, w->k_in, &n)) return fail(RQ_ERR_SHAPE, "weight shape overflows");
-    if (w->format == RQ_Q_AFFINE_U8 && w->group <= 0)
+    if (w->format != RQ_Q_ROWWISE_I8 && w->group <= 0)
         return fail(RQ_ERR_INVALID_ARGUMENT, "affine weight needs group > 0");
+    if (w->format == RQ_Q_AFFINE_U4 && (w->k_in % 2 != 0 || w->k_in % w->group != 0))
+        return fail(RQ_ERR_SHAPE, "4-bit weight: k_in %lld must be even and a multiple of group %d", (long long)w->k_in,
+                    w->group);
     if (n > 0 && !w->codes) return fail(RQ_ERR_INVALID_ARGUMENT, "null codes");
     if (w->n_out > 0 && !w->scales) return fail(RQ_ERR_INVALID_ARGUMENT, "null scales");
     if (w->prep && (w->format != RQ_Q_AFFINE_U8 || !aligned(w->prep, 16)))
@@ -407,11 +412,12 @@ int rq_affine_dequantize(rq_ctx *ctx, const uint32_t *weight, size_t n_weight_wo
 
 int rq_qweight_dequantize(rq_ctx *ctx, const rq_qweight *w, float *out, rq_stream stream) {
     RQ_ENTER(ctx);
-    int st = check_qweight(w);
+    int st = check_qweight(w, true);
     if (st != RQ_OK) return st;
     const size_t n = (size_t)w->n_out * (size_t)w->k_in;
     if (n == 0) return RQ_OK;
     if (!out) return fail(RQ_ERR_INVALID_ARGUMENT, "null output");
+    if (w->format == RQ_Q_AFFINE_U4) return launch_dequantize4(*w, out, pick(ctx, stream));
     if (w->format == RQ_Q_ROWWISE_I8)
         return launch_rowwise_dequantize((const int8_t *)w->codes, w->scales, out, w->n_out, w->k_in,
                                          pick(ctx, stream));
@@ -485,6 +491,7 @@ rq::GemmWorkspace rq::gemm_workspace(const rq_ctx *ctx, hipStream_t s) {
 // tuned paths do not serve.
 int rq::qmatmul_dispatch(rq_ctx *ctx, const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dtype yt,
                          int64_t m, const GemmWorkspace &ws, hipStream_t s) {
+    if (w.format == RQ_Q_AFFINE_U4) return launch_linear4(w, x, xt, y, yt, m, s);
     if (w.k_in > 0) {
         // 1-2 tokens: the VALU dot2 GEMV; 3-16: the MFMA GEMV (measured faster
         // from 3 tokens on, e.g. 4096x4096 m = 4: 7.2 -> 6.3 us); the VALU
@@ -508,7 +515,8 @@ int rq::qmatmul_dispatch(rq_ctx *ctx, const rq_qweight &w, const void *x, rq_dty
 int rq::swiglu_check(const rq_qweight *gate, const rq_qweight *up, const rq_qweight *down, rq_dtype x_dtype,
                      rq_dtype y_dtype, int64_t m) {
     int st;
-    if ((st = check_qweight(gate)) != RQ_OK || (st = check_qweight(up)) != RQ_OK || (st = check_qweight(down)) != RQ_OK)
+    if ((st = check_qweight(gate, true)) != RQ_OK || (st = check_qweight(up, true)) != RQ_OK ||
+        (st = check_qweight(down, true)) != RQ_OK)
         return st;
     if ((x_dtype != RQ_F16 && x_dtype != RQ_F32) || (y_dtype != RQ_F16 && y_dtype != RQ_F32))
         return fail(RQ_ERR_INVALID_ARGUMENT, "dtype must be RQ_F16 or RQ_F32");
@@ -533,6 +541,16 @@ int rq::swiglu_run(rq_ctx *ctx, const rq_qweight &gate, const rq_qweight &up, co
     // no intermediate features: h is empty and the down projection's
     // reduction too (y = 0)
     if (I == 0) return qmatmul_dispatch(ctx, down, h, RQ_F16, y, y_dtype, m, ws, s);
+    if (gate.format == RQ_Q_AFFINE_U4 || up.format == RQ_Q_AFFINE_U4) {
+        // 4-bit gate or up: two products into the two halves of the workspace,
+        // then h = silu(g) * u in place over the first half
+        _Float16 *g = static_cast<_Float16 *>(h), *u = g + m * I;
+        int st = qmatmul_dispatch(ctx, gate, x, x_dtype, g, RQ_F16, m, ws, s);
+        if (st == RQ_OK) st = qmatmul_dispatch(ctx, up, x, x_dtype, u, RQ_F16, m, ws, s);
+        if (st == RQ_OK) st = launch_silu_mul(g, u, g, m * I, s);
+        if (st != RQ_OK) return st;
+        return qmatmul_dispatch(ctx, down, h, RQ_F16, y, y_dtype, m, ws, s);
+    }
     int st = RQ_ERR_UNSUPPORTED;
     if (m <= 2) st = launch_swiglu_decode(gate, up, x, x_dtype, h, (int)m, s);
     if (st == RQ_ERR_UNSUPPORTED && m <= 16) st = launch_swiglu_mfma(gate, up, x, x_dtype, h, (int)m, s);
@@ -561,7 +579,7 @@ extern "C" {
 int rq_qmatmul(rq_ctx *ctx, const rq_qweight *w, const void *x, rq_dtype x_dtype, void *y, rq_dtype y_dtype,
                int64_t m, rq_stream stream) {
     RQ_ENTER(ctx);
-    int st = check_qweight(w);
+    int st = check_qweight(w, true);
     if (st != RQ_OK) return st;
     if ((x_dtype != RQ_F16 && x_dtype != RQ_F32) || (y_dtype != RQ_F16 && y_dtype != RQ_F32))
         return fail(RQ_ERR_INVALID_ARGUMENT, "dtype must be RQ_F16 or RQ_F32");

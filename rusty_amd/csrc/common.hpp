@@ -45,8 +45,9 @@ int enter(rq_ctx *ctx);
 inline hipStream_t pick(rq_ctx *ctx, rq_stream s) { return s ? static_cast<hipStream_t>(s) : ctx->stream; }
 // a*b without overflow; false if it does not fit in int64 (or is negative).
 bool mul_ok(int64_t a, int64_t b, int64_t *out);
-// Validates an rq_qweight descriptor (format, shape, null pointers).
-int check_qweight(const rq_qweight *w);
+// Validates an rq_qweight descriptor (format, shape, null pointers); u4: the
+// caller serves 4-bit codes too (else they are RQ_ERR_UNSUPPORTED).
+int check_qweight(const rq_qweight *w, bool u4 = false);
 
 #define RQ_ENTER(ctx)                       \
     do {                                    \
@@ -164,6 +165,9 @@ int launch_swiglu_mfma(const rq_qweight &gate, const rq_qweight &up, const void 
                        hipStream_t s);
 int launch_swiglu_generic(const rq_qweight &gate, const rq_qweight &up, const void *x, rq_dtype xt, void *h,
                           int64_t m, hipStream_t s);
+// 4-bit affine weights (RQ_Q_AFFINE_U4): W to f32, and Y = X . W^T for any m.
+int launch_dequantize4(const rq_qweight &w, float *out, hipStream_t s);
+int launch_linear4(const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dtype yt, int64_t m, hipStream_t s);
 int launch_silu_mul(const void *g, const void *u, void *h, int64_t n, hipStream_t s);
 // dX[m, k_in] = dY[m, n_out] . deq(W), W dequantized while staged (f32 fma, ascending n_out).
 int launch_qmatmul_dx(const rq_qweight &w, const void *dy, rq_dtype dyt, void *dx, rq_dtype dxt, int64_t m,

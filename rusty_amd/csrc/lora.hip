@@ -275,7 +275,7 @@ int lora_run(rq_ctx *ctx, const rq_qweight *w, const void *x, rq_dtype x_dtype, 
              const float *lora_b, int64_t rank, void *y, rq_dtype y_dtype, int64_t m, unsigned flags, void *workspace,
              size_t workspace_bytes, rq_stream stream) {
     RQ_ENTER(ctx);
-    int st = check_qweight(w);
+    int st = check_qweight(w, true);
     if (st != RQ_OK) return st;
     if ((x_dtype != RQ_F16 && x_dtype != RQ_F32) || (y_dtype != RQ_F16 && y_dtype != RQ_F32))
         return fail(RQ_ERR_INVALID_ARGUMENT, "dtype must be RQ_F16 or RQ_F32");

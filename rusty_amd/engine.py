@@ -44,6 +44,8 @@ class DType(enum.Enum):
     I8 = np.int8
     U8 = np.uint8
     U32 = np.uint32
+    I32 = np.int32
+    U64 = np.uint64
 
     @property
     def np(self):
@@ -221,6 +223,41 @@ class QuantizedTensor:
         if prepare:
             qt.prepare(ctx)
         return qt
+
+    @classmethod
+    def affine4(cls, ctx: WgpuContext, u: np.ndarray, scales: np.ndarray, biases: np.ndarray | None,
+                group: int = 64) -> "QuantizedTensor":
+        """4-bit affine codes ``u[n_out, k_in]`` (values 0..15, one per array
+        element here; two per byte on the device), f32 scale and bias per
+        ``group`` elements of a row: RQ_Q_AFFINE_U4."""
+        u = np.asarray(u)
+        n, k = u.shape
+        if k % 2 or group <= 0 or k % group:
+            raise ValueError(f"k_in {k} must be even and a multiple of group {group}")
+        if u.size and (u.min() < 0 or u.max() > 15):
+            raise ValueError("4-bit codes are 0..15")
+        u = u.astype(np.uint8)
+        packed = UnifiedTensor.new(ctx, u[:, 0::2] | (u[:, 1::2] << 4), dtype=DType.U8)
+        dev = lambda a: UnifiedTensor.new(  # noqa: E731
+            ctx, np.ascontiguousarray(a, dtype=np.float32).reshape(n, -1), dtype=DType.FP32)
+        return cls.from_affine4(packed, dev(scales), None if biases is None else dev(biases), group)
+
+    @classmethod
+    def from_affine4(cls, codes: UnifiedTensor, scales: UnifiedTensor, biases: UnifiedTensor | None,
+                     group: int = 64) -> "QuantizedTensor":
+        """The same from device tensors: packed codes U8 [n_out, k_in / 2] (the
+        even element in the low nibble), scales and biases f32 with
+        k_in / group values per row."""
+        n, k = codes.shape[0], 2 * codes.shape[1]
+        if codes.dtype is not DType.U8 or scales.dtype is not DType.FP32 \
+                or (biases is not None and biases.dtype is not DType.FP32):
+            raise ValueError("4-bit weight: codes must be U8, scales and biases FP32")
+        if group <= 0 or k % group:
+            raise ValueError(f"k_in {k} must be a multiple of group {group}")
+        need = n * (k // group)
+        if scales.numel != need or (biases is not None and biases.numel != need):
+            raise ValueError(f"{n}x{k} weight with group {group} needs {need} scales/biases")
+        return cls(codes, scales, biases, n, k, _lib.RQ_Q_AFFINE_U4, group)
 
     def prepare(self, ctx: WgpuContext, stream=None) -> None:
         """Builds the prefill GEMM's scale table of an affine weight
@@ -415,3 +452,65 @@ class ComputeEngine:
         call("rq_mlp_swiglu", ctx.handle, ctypes.byref(dg), ctypes.byref(du), ctypes.byref(dd), x.ptr,
              _XDT[x.dtype], h.ptr, out.ptr, _XDT[out.dtype], m, _stream(stream))
         return h
+
+    # ---- attention ----------------------------------------------------------
+    def attn_packed(self, ctx: WgpuContext, q: UnifiedTensor, k: UnifiedTensor, v: UnifiedTensor,
+                    starts: UnifiedTensor, out: UnifiedTensor, scale: float | None = None, q_row: int | None = None,
+                    k_row: int | None = None, v_row: int | None = None, out_row: int | None = None,
+                    stream=None) -> None:
+        """Causal GQA attention over packed prompts (rq_attn_packed): q and out
+        [tokens, n_heads, head_dim], k and v [tokens, n_kv_heads, head_dim],
+        ``starts`` I32 [n_seqs + 1] on the device.  ``*_row``: elements between
+        the rows of consecutive tokens where they are not packed (q, k and v in
+        the rows of one fused q/k/v product)."""
+        if len(q.shape) != 3 or len(k.shape) != 3 or k.shape != v.shape or out.shape != q.shape \
+                or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+            raise ValueError(f"q {q.shape} / k {k.shape} / v {v.shape} / out {out.shape}: expected [tokens, heads, dim]")
+        a = _attn(q, k, v, out, k.shape[1], scale)
+        a.q_row, a.k_row, a.v_row, a.out_row = q_row or 0, k_row or 0, v_row or 0, out_row or 0
+        if starts.dtype is not DType.I32 or starts.numel < 1:
+            raise ValueError("starts must be I32 [n_seqs + 1]")
+        call("rq_attn_packed", ctx.handle, ctypes.byref(a), q.ptr, k.ptr, v.ptr, starts.ptr, starts.numel - 1,
+             q.shape[0], out.ptr, _stream(stream))
+
+    def attn_tree(self, ctx: WgpuContext, q: UnifiedTensor, k: UnifiedTensor, v: UnifiedTensor,
+                  starts: UnifiedTensor, lengths: UnifiedTensor, mask: UnifiedTensor | None, out: UnifiedTensor,
+                  max_nodes: int, scale: float | None = None, workspace: UnifiedTensor | None = None,
+                  q_row: int | None = None, out_row: int | None = None, strides: Sequence[int] | None = None,
+                  stream=None) -> None:
+        """Attention of drafted tokens over a KV cache (rq_attn_tree): q and out
+        [tokens, n_heads, head_dim], the cache k and v [n_seqs, n_kv_heads,
+        capacity, head_dim] (``strides``: elements between sequences, heads and
+        positions where it is laid out otherwise), ``starts`` I32 [n_seqs + 1],
+        ``lengths`` I32 [n_seqs], ``mask`` U64 [tokens] or None (chains)."""
+        if len(q.shape) != 3 or len(k.shape) != 4 or k.shape != v.shape or out.shape != q.shape \
+                or k.shape[3] != q.shape[2]:
+            raise ValueError(f"q {q.shape} / out {out.shape}: expected [tokens, heads, dim]; k {k.shape} / v {v.shape}: "
+                             "expected [n_seqs, kv heads, capacity, dim]")
+        n_seqs, n_kv, capacity, _ = k.shape
+        if starts.dtype is not DType.I32 or starts.numel != n_seqs + 1 or lengths.dtype is not DType.I32 \
+                or lengths.numel != n_seqs or (mask is not None and (mask.dtype is not DType.U64
+                                                                    or mask.numel != q.shape[0])):
+            raise ValueError("starts I32 [n_seqs + 1], lengths I32 [n_seqs] and mask U64 [tokens] do not match")
+        a = _attn(q, k, v, out, n_kv, scale)
+        a.q_row, a.out_row = q_row or 0, out_row or 0
+        ss, sh, sp = strides or (0, 0, 0)
+        c = _lib.rq_kv_cache(k.ptr, v.ptr, ss, sh, sp, n_seqs, capacity)
+        if workspace is None:
+            workspace = self.attn_tree_workspace(ctx, q, k, max_nodes)
+        call("rq_attn_tree", ctx.handle, ctypes.byref(a), ctypes.byref(c), q.ptr, starts.ptr, lengths.ptr,
+             mask.ptr if mask is not None else None, q.shape[0], max_nodes, out.ptr, workspace.ptr, workspace.nbytes,
+             _stream(stream))
+
+    def attn_tree_workspace(self, ctx: WgpuContext, q: UnifiedTensor, k: UnifiedTensor,
+                            max_nodes: int) -> UnifiedTensor:
+        """A workspace for ``attn_tree`` calls of these shapes (one per call in flight)."""
+        a = _attn(q, k, k, q, k.shape[1], None)
+        need = int(_lib.lib().rq_attn_tree_workspace(ctypes.byref(a), k.shape[0], q.shape[0], max_nodes, k.shape[2]))
+        return UnifiedTensor.empty(ctx, [max(need, 1)], DType.U8)
+
+
+def _attn(q, k, v, out, n_kv, scale):
+    if q.dtype not in _XDT or k.dtype is not q.dtype or v.dtype is not q.dtype or out.dtype is not q.dtype:
+        raise ValueError("q, k, v and out must all be FP16 or all FP32")
+    return _lib.rq_attn(q.shape[1], n_kv, q.shape[2], _XDT[q.dtype], 0.0 if scale is None else scale, 0, 0, 0, 0, 0)
