@@ -3,111 +3,572 @@
 //
 //   out[t, h] = sum_j p_j v[j] / sum_j p_j,  p_j = 2^(c q.k_j - m),  c = scale log2 e
 //
-// over the keys j token t sees, with the running maximum m of c q.k and the
-// running sum kept in f32 and earlier sums rescaled when m rises.
+// over the keys j token t sees, in one pass over the keys: m is a running
+// maximum of c q.k, and earlier sums are rescaled when it rises.
+//
+// A block works on the rows of one key/value head of one sequence, a row being
+// a (token, query head) pair, token-major: the n_heads / n_kv_heads query heads of
+// a token share the keys, so one pass over K and V serves them all, short
+// sequences and single tokens fill the matrix instructions' 32 columns, and every
+// row of a block ends near the same key.  K and V pass through LDS in tiles of KT
+// keys (DMA, a ring of NS tiles, one barrier per tile).  Of the block's waves, WR take
+// different 32 rows and KG different 32 keys of each tile (KG partial softmaxes per
+// row, joined through LDS at the end).
+//
+// Matrix instructions: S^T = K . Q^T (A: 32 keys from LDS, B: the wave's 32
+// rows of Q, held in registers), so a row's scores lie in one lane column --
+// lane l holds keys 8 (r / 4) + 4 (l / 32) + r % 4, r < 16, of row l % 32 --
+// and the maximum is in-lane plus one exchange with lane l ^ 32.  Then O^T = V^T . P^T
+// takes P as it stands as the B operand, V^T in the key order that gives: for
+// fp16 by transposing LDS reads, for f32 one key per half-wave and instruction.
+// LDS rows are swizzled by 16-byte chunks so that these reads cover the banks.
 #include <math.h>
 
+#include <algorithm>
+
 #include "common.hpp"
+#include "lds_dma.hpp"
 
 namespace rq {
 namespace {
 
 constexpr int kMaxNodes = 64;
+constexpr int64_t kMaxRow = (int64_t)1 << 21;  // elements of a row stride: a tile's offsets stay below 2^31 bytes
 
-// What both kernels read; strides in elements.
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// What the kernels read; strides in elements.
 struct AttnArgs {
     const void *q, *k, *v;
     void *out;
     const int *starts, *lengths;
     const uint64_t *mask;
-    int64_t q_row, k_row, v_row, out_row;  // packed: rows of consecutive tokens
-    int64_t seq_stride, head_stride, pos_stride;  // tree: the cache
+    int64_t q_row, out_row;
+    int64_t seq_stride, head_stride;  // tree: the cache
+    int k_row, v_row;                 // between a head's consecutive keys
     int n_heads, n_kv, n_seqs, capacity, max_nodes;
     int tokens;
-    float scale;  // times log2 e
+    int splits;   // tree: the most pieces a sequence's keys are cut into
+    float *part;  // splits > 1: sums [tokens][n_heads][splits][dim], then (m, l) [tokens][n_heads][splits]
+    float c;      // |scale| log2 e
+    int neg;      // scale < 0: q enters negated
 };
 
 __device__ __forceinline__ int seq_start(const AttnArgs &a, int s) { return min(max(a.starts[s], 0), a.tokens); }
 
-// The sequence that holds token t, or -1: the last s with starts[s] <= t, if t
-// lies before its end.
-__device__ __forceinline__ int seq_of(const AttnArgs &a, int t) {
-    int lo = 0, hi = a.n_seqs;  // starts[lo] <= t (if any), starts[hi] > t or hi = n_seqs
-    if (seq_start(a, 0) > t) return -1;
+// The largest s < n_seqs with key(s) <= x (0 if there is none); key ascending.
+template <typename F>
+__device__ __forceinline__ int last_at_most(int n_seqs, int64_t x, F key) {
+    int lo = 0, hi = n_seqs;
     while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (seq_start(a, mid) <= t) lo = mid;
+        const int mid = (int)(((unsigned)lo + (unsigned)hi) / 2);
+        if (key(mid) <= x) lo = mid;
         else hi = mid;
     }
-    return t < seq_start(a, lo + 1) ? lo : -1;
+    return lo;
 }
 
-// One wave per (token, head): lane l holds dims l, l + 64, ...
-template <typename T, int HD, bool TREE>
-__global__ __launch_bounds__(64) void k_attn_rows(AttnArgs a) {
-    constexpr int E = HD / 64;
-    const int t = blockIdx.x / a.n_heads, h = blockIdx.x % a.n_heads, lane = threadIdx.x;
-    const int s = seq_of(a, t);
-    if (s < 0) return;
-    const int g = h / (a.n_heads / a.n_kv), s0 = seq_start(a, s), i = t - s0;
-    const T *q = static_cast<const T *>(a.q) + (int64_t)t * a.q_row + (int64_t)h * HD;
-    const T *kb, *vb;
-    int64_t ks, vs;
-    int before, nodes;  // keys 0..before-1, then before + j for the bits j < nodes of see
-    uint64_t see;
-    if (TREE) {
-        nodes = min(seq_start(a, s + 1) - s0, a.max_nodes);
-        if (i >= nodes) return;
+// Of n drafted positions, those that token t, the i-th of its sequence, sees, as bits.
+__device__ __forceinline__ uint64_t tree_sees(const AttnArgs &a, int t, int i, int n) {
+    const uint64_t all = n > 0 ? ~0ull >> (64 - n) : 0;
+    return (a.mask ? a.mask[t] : ~0ull >> (63 - i)) & all;
+}
+
+// One sequence of a tree call: its tokens, and the keys cached before and with them.
+struct TreeSeq {
+    int s0, nodes;      // first token, tokens served
+    int before, keys;   // cached positions before them; all positions there are
+    __device__ __forceinline__ TreeSeq(const AttnArgs &a, int s) {
+        s0 = seq_start(a, s);
+        nodes = min(max(seq_start(a, s + 1) - s0, 0), a.max_nodes);
         before = min(max(a.lengths[s], 0), a.capacity);
-        nodes = min(nodes, a.capacity - before);
-        see = a.mask ? a.mask[t] : (~0ull >> (63 - i));
-        kb = static_cast<const T *>(a.k) + s * a.seq_stride + g * a.head_stride;
-        vb = static_cast<const T *>(a.v) + s * a.seq_stride + g * a.head_stride;
-        ks = vs = a.pos_stride;
+        keys = before + min(nodes, a.capacity - before);
+    }
+    // tiles of kt keys per piece, for at most `splits` pieces
+    __device__ __forceinline__ int per_piece(int kt, int splits) const {
+        const int tiles = (keys + kt - 1) / kt;
+        return max(1, (tiles + splits - 1) / splits);
+    }
+};
+
+template <typename T, int HD, int WR, int KG, bool TREE>
+struct Shape {
+    static constexpr int NW = WR * KG;
+    static constexpr int ROW = HD * (int)sizeof(T), CH = ROW / 16;
+    static constexpr int KT = KG == 1 ? 64 : 32 * KG;  // keys per tile
+    static constexpr int TPW = KT / 32 / KG;           // 32-key pieces of it per wave
+    static constexpr int TILE = KT * ROW;              // bytes of one operand's tile
+    static constexpr int NS = 6 * TILE <= 49152 ? 3 : 2;
+};
+
+template <typename T, int HD, int WR, int KG, bool TREE>
+__global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
+    using SH = Shape<T, HD, WR, KG, TREE>;
+    constexpr bool F16 = sizeof(T) == 2;
+    constexpr int NW = SH::NW, ROW = SH::ROW, CH = SH::CH, KT = SH::KT, TPW = SH::TPW, TILE = SH::TILE, NS = SH::NS;
+    constexpr int BR = 32 * WR, DT = HD / 32;
+    constexpr int KS = F16 ? HD / 16 : HD / 8;  // 16-byte pieces of a row per lane (both halves: 32 bytes)
+    constexpr int RPU = 1024 / ROW;             // rows per DMA unit (1 KiB)
+    constexpr int UW = TILE / 1024 / NW;        // units per wave and operand
+    static_assert(UW >= 1 && TILE % (1024 * NW) == 0, "every wave moves whole units");
+    constexpr int RING = NS * 2 * TILE;
+    static_assert(KG == 1 || (KG - 1) * WR * DT * 16 * 256 <= RING, "the partial sums reuse the ring");
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[RING];
+    __shared__ float joined[KG > 1 ? KG : 1][2][KG > 1 ? 32 * WR : 1];
+
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = wv % WR, kg = wv / WR;
+    const int col = lane & 31, hf = lane >> 5;
+    const int grp = a.n_heads / a.n_kv, g = blockIdx.x % a.n_kv;
+
+    // the block's sequence, rows and keys
+    int s0, nq, r0, nkeys, first = 0, ntiles, pieces = 1, piece = 0, before = 0;
+    const char *kb, *vb;  // key 0 of this head
+    if constexpr (TREE) {
+        const int rbs = (a.max_nodes * grp + BR - 1) / BR;
+        int b = blockIdx.x / a.n_kv;
+        const int rb = b % rbs;
+        b /= rbs;
+        const int s = b % a.n_seqs;
+        piece = b / a.n_seqs;
+        const TreeSeq q(a, s);
+        s0 = q.s0;
+        nq = q.nodes;
+        r0 = rb * BR;
+        before = __builtin_amdgcn_readfirstlane(q.before);
+        nkeys = q.keys;
+        const int per = q.per_piece(KT, a.splits), tiles = (nkeys + KT - 1) / KT;
+        pieces = max(1, (tiles + per - 1) / per);
+        if (r0 >= nq * grp || piece >= pieces) return;
+        first = __builtin_amdgcn_readfirstlane(piece * per);
+        ntiles = min(per, tiles - piece * per);
+        const int64_t at = s * a.seq_stride + g * a.head_stride;
+        kb = static_cast<const char *>(a.k) + at * (int64_t)sizeof(T);
+        vb = static_cast<const char *>(a.v) + at * (int64_t)sizeof(T);
     } else {
-        before = i + 1;
-        nodes = 0;
-        see = 0;
-        kb = static_cast<const T *>(a.k) + (int64_t)s0 * a.k_row + (int64_t)g * HD;
-        vb = static_cast<const T *>(a.v) + (int64_t)s0 * a.v_row + (int64_t)g * HD;
-        ks = a.k_row;
-        vs = a.v_row;
+        // Row tiles of the sequences, one after another: sequence s has the
+        // indexes from starts[s] grp / BR + s on, at least as many as it needs.
+        // The last first: a long prompt's heaviest tiles start early.
+        const int64_t t = gridDim.x / a.n_kv - 1 - blockIdx.x / a.n_kv;
+        auto tile0 = [&](int s) { return (int64_t)seq_start(a, s) * grp / BR + s; };
+        const int s = last_at_most(a.n_seqs, t, tile0);
+        s0 = seq_start(a, s);
+        nq = max(seq_start(a, s + 1) - s0, 0);
+        const int64_t row = (t - tile0(s)) * BR;
+        if (row < 0 || row >= (int64_t)nq * grp) return;
+        // rows are counted from the tile's first token on
+        const int skip = (int)(row / grp);
+        r0 = (int)(row - (int64_t)skip * grp);
+        s0 += skip;
+        before = skip;  // tokens of the sequence before token 0 of these
+        nq -= skip;
+        nkeys = before + min(nq, (r0 + BR - 1) / grp + 1);
+        ntiles = (nkeys + KT - 1) / KT;
+        const int64_t seq = (int64_t)(s0 - skip);
+        kb = static_cast<const char *>(a.k) + (seq * a.k_row + g * HD) * (int64_t)sizeof(T);
+        vb = static_cast<const char *>(a.v) + (seq * a.v_row + g * HD) * (int64_t)sizeof(T);
     }
-    float qv[E], o[E], m = -INFINITY, l = 0.0f;
-    for (int e = 0; e < E; ++e) {
-        qv[e] = (float)q[lane + 64 * e];
-        o[e] = 0.0f;
+    s0 = __builtin_amdgcn_readfirstlane(s0);
+    nkeys = __builtin_amdgcn_readfirstlane(nkeys);
+    ntiles = __builtin_amdgcn_readfirstlane(ntiles);
+
+    // this lane's row
+    const int r = r0 + 32 * wr + col, qi = r / grp, head = g * grp + (r - qi * grp);
+    const bool live = qi < nq;
+    const uint64_t see = TREE && live ? tree_sees(a, s0 + qi, qi, nkeys - before) : 0;
+    // of the wave's rows: the last key any of them sees, and the first that some do not
+    const int w_lo = __builtin_amdgcn_readfirstlane((r0 + 32 * wr) / grp);
+    const int w_hi = __builtin_amdgcn_readfirstlane(min((r0 + 32 * wr + 31) / grp, nq - 1));
+    const bool idle = w_lo >= nq;  // no row at all
+    const int key_end = idle ? 0 : TREE ? nkeys : before + w_hi + 1;
+    const int masked_from = idle ? 0 : TREE ? before : before + w_lo + 1;
+    // bit j: whether this lane's row sees key key0 + j
+    auto visible = [&](int key0) -> uint64_t {
+        if constexpr (TREE) {
+            const int d = before - key0;  // keys of these that are cached positions
+            if (d >= 64) return ~0ull;
+            if (d >= 0) return (see << d) | ((1ull << d) - 1);
+            return d > -64 ? see >> -d : 0;
+        } else {
+            const int n = before + qi + 1 - key0;
+            return n >= 64 ? ~0ull : n > 0 ? (1ull << n) - 1 : 0;
+        }
+    };
+
+    uint4 qf[KS];
+    {
+        const char *qp = static_cast<const char *>(a.q) + ((int64_t)(s0 + qi) * a.q_row + head * HD) * (int64_t)sizeof(T);
+        const uint32_t flip = a.neg ? (F16 ? 0x80008000u : 0x80000000u) : 0u;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (live) v = *reinterpret_cast<const uint4 *>(qp + 32 * s + 16 * hf);
+            qf[s] = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
+        }
     }
-    for (int j = 0; j < before + nodes; ++j) {
-        if (j >= before && !(see >> (j - before) & 1)) continue;
-        float sc = 0.0f;
-        for (int e = 0; e < E; ++e) sc = __builtin_fmaf(qv[e], (float)kb[j * ks + lane + 64 * e], sc);
-        for (int w = 32; w > 0; w >>= 1) sc += __shfl_xor(sc, w, 64);
-        sc *= a.scale;
-        const float mn = fmaxf(m, sc), base = mn == -INFINITY ? 0.0f : mn;
-        const float al = exp2f(m - base), p = exp2f(sc - base);
-        m = mn;
-        l = l * al + p;
-        for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(p, (float)vb[j * vs + lane + 64 * e], o[e] * al);
+
+    // LDS chunk c of row r holds global chunk c ^ f(r)
+    auto fk = [](int r) { return F16 && HD == 64 ? (r >> 1) & 7 : r & 15; };
+    auto fv = [](int r) { return F16 ? (HD == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2) : ((r >> 2) & 1) << 3; };
+    const uint32_t kst = (uint32_t)a.k_row * (uint32_t)sizeof(T), vst = (uint32_t)a.v_row * (uint32_t)sizeof(T);
+    uint32_t koff[UW], voff[UW];
+#pragma unroll
+    for (int u = 0; u < UW; ++u) {
+        const int row = (wv * UW + u) * RPU + lane / CH, c = lane % CH;
+        koff[u] = (uint32_t)row * kst + (uint32_t)((c ^ fk(row)) * 16);
+        voff[u] = (uint32_t)row * vst + (uint32_t)((c ^ fv(row)) * 16);
     }
-    const bool none = TREE && before == 0 && (nodes == 0 || !(see & (~0ull >> (64 - nodes))));
-    T *out = static_cast<T *>(a.out) + (int64_t)t * a.out_row + (int64_t)h * HD;
-    for (int e = 0; e < E; ++e) out[lane + 64 * e] = (T)(none ? 0.0f : o[e] / l);
+    const uint32_t lds0 = lds_addr(&lds[0]);
+    // tile kt of this block into its ring place; keys past the end read as zero
+    auto dma = [&](int kt) {
+        const int key0 = (first + kt) * KT;
+        const int rows = kt < ntiles ? min(KT, nkeys - key0) : 0;
+        const auto rk = make_rsrc_s(kb + (int64_t)key0 * kst, rows > 0 ? (uint32_t)(rows - 1) * kst + ROW : 0u);
+        const auto rv = make_rsrc_s(vb + (int64_t)key0 * vst, rows > 0 ? (uint32_t)(rows - 1) * vst + ROW : 0u);
+        const uint32_t base = lds0 + (uint32_t)(kt % NS) * (2 * TILE) + (uint32_t)(wv * UW) * 1024u;
+#pragma unroll
+        for (int u = 0; u < UW; ++u) {
+            dma16(rk, base + (uint32_t)u * 1024u, koff[u]);
+            dma16(rv, base + (uint32_t)TILE + (uint32_t)u * 1024u, voff[u]);
+        }
+    };
+#pragma unroll
+    for (int kt = 0; kt < NS - 1; ++kt) dma(kt);
+
+    float mc = -__builtin_inff(), l = 0.0f;  // running maximum (scaled), this lane's share of the sum
+    floatx16 o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
+
+    // byte offsets of this lane's reads within its 32-key pieces
+    const int kp = 32 * kg * TPW;  // the wave's first key of a tile
+    uint32_t ka[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) ka[s] = (uint32_t)((kp + col) * ROW + (((2 * s + hf) ^ fk(col)) * 16));
+    uint32_t va[DT][2];
+    if constexpr (F16) {
+        // 16 lanes take a block of 4 keys x 16 dims; each gets one dim's 4 keys
+        const int i16 = lane & 15;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = 4 * hf + i16 / 4 + 8 * e, ch = 4 * d + 2 * ((lane >> 4) & 1) + (i16 & 3) / 2;
+                va[d][e] = (uint32_t)((kp + row) * ROW + ((ch ^ fv(row)) * 16) + (i16 & 1) * 8);
+            }
+    } else {
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+            va[d][0] = va[d][1] = (uint32_t)((kp + 4 * hf) * ROW + (((8 * d + col / 4) ^ (hf << 3)) * 16) + (col & 3) * 4);
+    }
+    typedef short short4v __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) short4v lds_short4;
+    typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
+    typedef __attribute__((address_space(3))) const float lds_float;
+    typedef __attribute__((address_space(3))) const _Float16 lds_half;
+
+    // the wave's pieces of the tile at LDS address tb, its first key key0
+    auto keys = [&](auto masked_c, uint32_t tb, int key0) {
+        constexpr bool MASKED = decltype(masked_c)::value;
+        floatx16 sc[TPW];
+#pragma unroll
+        for (int i = 0; i < TPW; ++i) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[i][e] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const u32x4 kf = *(lds_u32x4 *)(uintptr_t)(tb + ka[s] + (uint32_t)(i * 32 * ROW));
+                if constexpr (F16) {
+                    sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, kf),
+                                                                   __builtin_bit_cast(half8, qf[s]), sc[i], 0, 0, 0);
+                } else {
+                    // (whole vectors: a bit_cast of one element would read element 0)
+                    const floatx4 kv = __builtin_bit_cast(floatx4, kf), qv = __builtin_bit_cast(floatx4, qf[s]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        sc[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(kv[e], qv[e], sc[i], 0, 0, 0);
+                }
+            }
+        }
+        const uint64_t sees = MASKED ? visible(key0) : 0;
+        if constexpr (MASKED) {
+            const uint64_t mine = sees >> (4 * hf);
+#pragma unroll
+            for (int i = 0; i < TPW; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    sc[i][e] = mine >> (32 * i + 8 * (e >> 2) + (e & 3)) & 1 ? sc[i][e] : -__builtin_inff();
+        }
+        float mt = sc[0][0];
+#pragma unroll
+        for (int i = 0; i < TPW; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mt = fmaxf(mt, sc[i][e]);
+        mt = fmaxf(mt, __shfl_xor(mt, 32)) * a.c;
+        // The maximum may lag by 6 (weights up to 2^6): a row's sums are then
+        // rescaled a few times in all, not in most tiles.
+        const bool rose = mt > mc + 6.0f;
+        if (__builtin_amdgcn_ballot_w64(rose)) {
+            const float alpha = rose ? __builtin_amdgcn_exp2f(mc - mt) : 1.0f;
+            mc = rose ? mt : mc;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
+        }
+        const float off = mc == -__builtin_inff() ? 0.0f : -mc;  // no key yet: every weight is 2^-inf
+#pragma unroll
+        for (int i = 0; i < TPW; ++i) {
+            float t[4];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i][e], a.c, off));
+                sc[i][e] = p;
+                t[e & 3] = e < 4 ? p : t[e & 3] + p;
+            }
+            l += (t[0] + t[1]) + (t[2] + t[3]);
+        }
+        const uint32_t vt = tb + TILE;
+        if constexpr (MASKED) {
+            // A value that is not finite must not meet the zero weight of a
+            // row that does not see its key: such a piece is summed by element.
+            float z = 0.0f;
+#pragma unroll
+            for (int u = 0; u < TPW * 32 * ROW / 1024; ++u) {
+                const u32x4 x = *(lds_u32x4 *)(uintptr_t)(vt + (uint32_t)(kp * ROW + u * 1024 + lane * 16));
+                const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (F16) {
+                        const h2_t h = __builtin_bit_cast(h2_t, xw[e]) * (h2_t){(_Float16)0.0f, (_Float16)0.0f};
+                        z += (float)(h.x + h.y);
+                    } else {
+                        z = __builtin_fmaf(__builtin_bit_cast(float, xw[e]), 0.0f, z);
+                    }
+                }
+            }
+            if (__builtin_amdgcn_ballot_w64(z != z)) {
+                for (int kk = 0; kk < 32 * TPW; ++kk) {
+                    float p = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < TPW; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            p = kk / 32 == i && 4 * (kk % 32 / 8) + kk % 4 == e ? sc[i][e] : p;
+                    p = __shfl(p, col + 32 * (kk / 4 % 2));
+                    if constexpr (F16) p = (float)(_Float16)p;
+                    const bool seen = sees >> kk & 1;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int dim = 32 * d + 8 * (e >> 2) + 4 * hf + (e & 3), row = kp + kk;
+                            const uint32_t at = vt + (uint32_t)(row * ROW) +
+                                                (uint32_t)(((dim * (int)sizeof(T) / 16) ^ fv(row)) * 16) +
+                                                (uint32_t)(dim * (int)sizeof(T) % 16);
+                            float x;
+                            if constexpr (F16) x = (float)*(lds_half *)(uintptr_t)at;
+                            else x = *(lds_float *)(uintptr_t)at;
+                            o[d][e] = seen ? __builtin_fmaf(p, x, o[d][e]) : o[d][e];
+                        }
+                }
+                return;
+            }
+        }
+        if constexpr (F16) {
+            half8 pf[TPW][2];
+#pragma unroll
+            for (int i = 0; i < TPW; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) pf[i][e >> 3][e & 7] = (_Float16)sc[i][e];
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                lds_short4 *pa = (lds_short4 *)(uintptr_t)(vt + va[d][0]), *pb = (lds_short4 *)(uintptr_t)(vt + va[d][1]);
+#pragma unroll
+                for (int i = 0; i < TPW; ++i)
+#pragma unroll
+                    for (int s2 = 0; s2 < 2; ++s2) {
+                        const uint2 ua = __builtin_bit_cast(
+                            uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(pa + (2 * i + s2) * 16 * ROW / 8));
+                        const uint2 ub = __builtin_bit_cast(
+                            uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(pb + (2 * i + s2) * 16 * ROW / 8));
+                        const half8 vf = __builtin_bit_cast(half8, make_uint4(ua.x, ua.y, ub.x, ub.y));
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[i][s2], o[d], 0, 0, 0);
+                    }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < TPW; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+                        const float x = *(lds_float *)(uintptr_t)(vt + va[d][0] +
+                                                                  (uint32_t)((32 * i + 8 * (e >> 2) + (e & 3)) * ROW));
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, sc[i][e], o[d], 0, 0, 0);
+                    }
+        }
+    };
+    for (int kt = 0; kt < ntiles; ++kt) {
+        // tile kt has landed, and every wave is done with the one whose place the next takes
+        wait_vmcnt<(NS - 2) * 2 * UW>();
+        __syncthreads();
+        dma(kt + NS - 1);
+        const int key0 = (first + kt) * KT + kp;
+        const uint32_t tb = lds0 + (uint32_t)(kt % NS) * (2 * TILE);
+        if (key0 + 32 * TPW <= masked_from) keys(std::false_type{}, tb, key0);
+        else if (key0 < key_end) keys(std::true_type{}, tb, key0);
+    }
+    wait_vmcnt<0>();  // no DMA in flight past this point
+
+    l += __shfl_xor(l, 32);
+    if constexpr (KG > 1) {
+        // the key groups' sums through the ring
+        float *co = reinterpret_cast<float *>(lds);
+        __syncthreads();  // every wave is done with it
+        if (kg > 0) {
+            if (hf == 0) {
+                joined[kg][0][32 * wr + col] = mc;
+                joined[kg][1][32 * wr + col] = l;
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) co[((((kg - 1) * WR + wr) * DT + d) * 16 + e) * 64 + lane] = o[d][e];
+        }
+        __syncthreads();
+        if (kg > 0) return;
+        float top = mc;
+#pragma unroll
+        for (int w = 1; w < KG; ++w) top = fmaxf(top, joined[w][0][32 * wr + col]);
+        const float base = top == -__builtin_inff() ? 0.0f : top;
+        const float w0 = __builtin_amdgcn_exp2f(mc - base);
+        l *= w0;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] *= w0;
+#pragma unroll
+        for (int w = 1; w < KG; ++w) {
+            const float ww = __builtin_amdgcn_exp2f(joined[w][0][32 * wr + col] - base);
+            l = __builtin_fmaf(ww, joined[w][1][32 * wr + col], l);
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    o[d][e] = __builtin_fmaf(ww, co[((((w - 1) * WR + wr) * DT + d) * 16 + e) * 64 + lane], o[d][e]);
+        }
+        mc = top;
+    }
+    if (!live) return;
+    if (TREE && pieces > 1) {
+        const int64_t slot = ((int64_t)(s0 + qi) * a.n_heads + head) * a.splits + piece;
+        float *po = a.part + slot * HD;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e4 = 0; e4 < 4; ++e4)
+                *reinterpret_cast<float4 *>(po + 32 * d + 8 * e4 + 4 * hf) =
+                    make_float4(o[d][4 * e4], o[d][4 * e4 + 1], o[d][4 * e4 + 2], o[d][4 * e4 + 3]);
+        if (hf == 0)
+            reinterpret_cast<float2 *>(a.part + (int64_t)a.tokens * a.n_heads * a.splits * HD)[slot] = make_float2(mc, l);
+        return;
+    }
+    const bool none = TREE && before == 0 && see == 0;
+    const float inv = none ? 0.0f : 1.0f / l;
+    T *op = static_cast<T *>(a.out) + (int64_t)(s0 + qi) * a.out_row + head * HD;
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {
+            vec4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (T)(none ? 0.0f : o[d][4 * e4 + e] * inv);
+            *reinterpret_cast<vec4 *>(op + 32 * d + 8 * e4 + 4 * hf) = v;
+        }
 }
 
-int launch_rows(const AttnArgs &a, bool tree, int hd, int dtype, hipStream_t s) {
-    const int64_t blocks = (int64_t)a.tokens * a.n_heads;
-    if (!grid_ok(blocks, 64)) return fail(RQ_ERR_SHAPE, "tokens * n_heads too large");
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64), 0, s, a); };
-    if (dtype == RQ_F16) {
-        if (hd == 64) tree ? go(k_attn_rows<_Float16, 64, true>) : go(k_attn_rows<_Float16, 64, false>);
-        else tree ? go(k_attn_rows<_Float16, 128, true>) : go(k_attn_rows<_Float16, 128, false>);
-    } else {
-        if (hd == 64) tree ? go(k_attn_rows<float, 64, true>) : go(k_attn_rows<float, 64, false>);
-        else tree ? go(k_attn_rows<float, 128, true>) : go(k_attn_rows<float, 128, false>);
+// Joins the pieces of rows whose keys were cut: one wave per (token, head).
+template <typename T, int HD, int KT>
+__global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= (int64_t)a.tokens * a.n_heads) return;
+    const int t = (int)(row / a.n_heads), head = (int)(row - (int64_t)t * a.n_heads), lane = threadIdx.x & 63;
+    const int s = last_at_most(a.n_seqs, t, [&](int i) { return (int64_t)seq_start(a, i); });
+    const TreeSeq q(a, s);
+    const int i = t - q.s0;
+    if (i < 0 || i >= q.nodes) return;
+    const int per = q.per_piece(KT, a.splits), tiles = (q.keys + KT - 1) / KT;
+    const int pieces = (tiles + per - 1) / per;
+    if (pieces <= 1) return;  // written by the block that had them all
+    const float *po = a.part + row * a.splits * HD;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.part + (int64_t)a.tokens * a.n_heads * a.splits * HD) + row * a.splits;
+    float top = -__builtin_inff();
+    for (int p = 0; p < pieces; ++p) top = fmaxf(top, ml[p].x);
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    constexpr int E = HD / 64;
+    float l = 0.0f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.0f;
+    for (int p = 0; p < pieces; ++p) {
+        const float w = __builtin_amdgcn_exp2f(ml[p].x - base);
+        l = __builtin_fmaf(w, ml[p].y, l);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(w, po[p * HD + E * lane + e], o[e]);
     }
+    const bool none = q.before == 0 && tree_sees(a, t, i, q.keys) == 0;
+    T *op = static_cast<T *>(a.out) + (int64_t)t * a.out_row + head * HD + E * lane;
+#pragma unroll
+    for (int e = 0; e < E; ++e) op[e] = (T)(none ? 0.0f : o[e] / l);
+}
+
+// Launches k_attn<T, HD, WR, KG, TREE> with BR = 32 WR rows per block.
+template <typename T, int HD, int WR, int KG, bool TREE>
+int launch(const AttnArgs &a, hipStream_t s) {
+    using SH = Shape<T, HD, WR, KG, TREE>;
+    const int64_t grp = a.n_heads / a.n_kv, br = 32 * WR;
+    const int64_t tiles = TREE ? cdiv(a.max_nodes * grp, br) * a.n_seqs * a.splits : (int64_t)a.tokens * grp / br + a.n_seqs;
+    if (!grid_ok(tiles * a.n_kv, 64 * SH::NW)) return fail(RQ_ERR_SHAPE, "too many rows for one call");
+    hipLaunchKernelGGL((k_attn<T, HD, WR, KG, TREE>), dim3((unsigned)(tiles * a.n_kv)), dim3(64 * SH::NW), 0, s, a);
     RQ_LAUNCH_CHECK();
+    if (TREE && a.splits > 1) {
+        const int64_t blocks = cdiv((int64_t)a.tokens * a.n_heads, 4);
+        if (!grid_ok(blocks, 256)) return fail(RQ_ERR_SHAPE, "too many rows for one call");
+        hipLaunchKernelGGL((k_attn_join<T, HD, SH::KT>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+        RQ_LAUNCH_CHECK();
+    }
     return RQ_OK;
+}
+
+template <typename T, int HD>
+int launch_packed(const AttnArgs &a, hipStream_t s) {
+    return launch<T, HD, 4, 1, false>(a, s);
+}
+
+// Rows of a tree block (32 or 64 or 128 by the rows a sequence may have) and
+// the pieces its keys may be cut into: enough blocks for two per CU.
+int tree_rows(int64_t rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
+int tree_splits(int64_t n_seqs, int64_t n_kv, int64_t rows, int64_t capacity, bool f16) {
+    const int wr = tree_rows(rows);
+    const int64_t blocks = n_seqs * n_kv * cdiv(rows, 32 * wr), kt = wr == 1 && f16 ? 128 : 64;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(blocks, 1), cdiv(capacity, kt), 64}));
+}
+
+template <typename T, int HD>
+int launch_tree(const AttnArgs &a, hipStream_t s) {
+    const int wr = tree_rows((int64_t)a.max_nodes * (a.n_heads / a.n_kv));
+    if (wr == 4) return launch<T, HD, 4, 1, true>(a, s);
+    if (wr == 2) return launch<T, HD, 2, 2, true>(a, s);
+    if constexpr (sizeof(T) == 2) return launch<T, HD, 1, 4, true>(a, s);
+    else return launch<T, HD, 1, 2, true>(a, s);
 }
 
 // The checks both entry points share; fills the strides of a.
@@ -122,20 +583,25 @@ int check_attn(const rq_attn *at, int64_t tokens, AttnArgs &a) {
     if (!isfinite(at->scale)) return fail(RQ_ERR_INVALID_ARGUMENT, "scale must be finite");
     if (tokens < 0 || tokens > 0x7fffffff) return fail(RQ_ERR_SHAPE, "tokens outside 0..2^31-1");
     const int64_t qw = (int64_t)at->n_heads * at->head_dim, kw = (int64_t)at->n_kv_heads * at->head_dim;
-    const int64_t unit = at->dtype == RQ_F16 ? 8 : 4, most = (int64_t)1 << 40;
-    a.q_row = at->q_row ? at->q_row : qw;
-    a.k_row = at->k_row ? at->k_row : kw;
-    a.v_row = at->v_row ? at->v_row : kw;
-    a.out_row = at->out_row ? at->out_row : qw;
-    if (a.q_row < qw || a.out_row < qw || a.k_row < kw || a.v_row < kw || a.q_row > most || a.out_row > most ||
-        a.k_row > most || a.v_row > most)
-        return fail(RQ_ERR_SHAPE, "row stride shorter than a row or out of range");
-    if (a.q_row % unit || a.out_row % unit || a.k_row % unit || a.v_row % unit)
+    const int64_t unit = at->dtype == RQ_F16 ? 8 : 4;
+    const int64_t qr = at->q_row ? at->q_row : qw, kr = at->k_row ? at->k_row : kw, vr = at->v_row ? at->v_row : kw,
+                  orow = at->out_row ? at->out_row : qw;
+    if (qr < qw || orow < qw || kr < kw || vr < kw || qr > kMaxRow || orow > kMaxRow || kr > kMaxRow || vr > kMaxRow)
+        return fail(RQ_ERR_SHAPE, "row strides must hold a row and be at most 2^21 elements");
+    if (qr % unit || orow % unit || kr % unit || vr % unit)
         return fail(RQ_ERR_UNSUPPORTED, "row strides must be multiples of 16 bytes");
+    a.q_row = qr;
+    a.out_row = orow;
+    a.k_row = (int)kr;
+    a.v_row = (int)vr;
     a.n_heads = at->n_heads;
     a.n_kv = at->n_kv_heads;
     a.tokens = (int)tokens;
-    a.scale = (at->scale != 0.0f ? at->scale : 1.0f / sqrtf((float)at->head_dim)) * 1.4426950408889634f;
+    const float scale = at->scale != 0.0f ? at->scale : 1.0f / sqrtf((float)at->head_dim);
+    a.neg = scale < 0.0f;
+    // (not below the normal numbers: a hidden key's -inf times c stays -inf)
+    a.c = (float)std::min(std::max(fabs((double)scale) * 1.4426950408889634, 1.2e-38), 3.4e38);
+    a.splits = 1;
     return RQ_OK;
 }
 
@@ -173,19 +639,19 @@ int check_tree(const rq_attn *attn, const rq_kv_cache *cache, const void *q, con
     const int64_t hd = attn->head_dim, unit = attn->dtype == RQ_F16 ? 8 : 4, most = (int64_t)1 << 40;
     a.seq_stride = cache->seq_stride;
     a.head_stride = cache->head_stride;
-    a.pos_stride = cache->pos_stride;
-    if (a.seq_stride == 0 && a.head_stride == 0 && a.pos_stride == 0) {
-        a.pos_stride = hd;
+    int64_t pos = cache->pos_stride;
+    if (a.seq_stride == 0 && a.head_stride == 0 && pos == 0) {
+        pos = hd;
         a.head_stride = hd * cache->capacity;
         a.seq_stride = a.head_stride * a.n_kv;
     }
     // (a stride that is never taken, of one head or one sequence, may be 0)
-    if (a.head_stride < 0 || a.seq_stride < 0 || a.pos_stride > ((int64_t)1 << 24) || a.head_stride > most ||
+    if (a.head_stride < 0 || a.seq_stride < 0 || pos > kMaxRow || pos < 0 || a.head_stride > most ||
         a.seq_stride > most ||
-        (cache->capacity > 0 && (a.pos_stride < hd || (a.n_kv > 1 && a.head_stride < hd) ||
+        (cache->capacity > 0 && (pos < hd || (a.n_kv > 1 && a.head_stride < hd) ||
                                  (cache->n_seqs > 1 && a.seq_stride < hd))))
         return fail(RQ_ERR_SHAPE, "cache strides shorter than a row or out of range");
-    if (a.pos_stride % unit || a.head_stride % unit || a.seq_stride % unit)
+    if (pos % unit || a.head_stride % unit || a.seq_stride % unit)
         return fail(RQ_ERR_UNSUPPORTED, "cache strides must be multiples of 16 bytes");
     if (cache->n_seqs == 0 || tokens == 0) return RQ_OK;
     if (!q || !out || !starts || !lengths || (cache->capacity > 0 && (!cache->k || !cache->v)))
@@ -197,6 +663,10 @@ int check_tree(const rq_attn *attn, const rq_kv_cache *cache, const void *q, con
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(RQ_ERR_INVALID_ARGUMENT, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
     if (need > 0 && !aligned(workspace, 16)) return fail(RQ_ERR_UNSUPPORTED, "workspace must be 16-byte aligned");
+    a.k_row = a.v_row = (int)pos;
+    a.splits = tree_splits(cache->n_seqs, a.n_kv, (int64_t)max_nodes * (a.n_heads / a.n_kv), cache->capacity,
+                           attn->dtype == RQ_F16);
+    a.part = static_cast<float *>(workspace);
     a.q = q;
     a.k = cache->k;
     a.v = cache->v;
@@ -225,12 +695,22 @@ int rq_attn_packed(rq_ctx *ctx, const rq_attn *attn, const void *q, const void *
     bool run;
     const int st = check_packed(attn, q, k, v, starts, n_seqs, tokens, out, a, run);
     if (st != RQ_OK || !run) return st;
-    return launch_rows(a, false, attn->head_dim, attn->dtype, pick(ctx, stream));
+    hipStream_t s = pick(ctx, stream);
+    if (attn->dtype == RQ_F16)
+        return attn->head_dim == 64 ? launch_packed<_Float16, 64>(a, s) : launch_packed<_Float16, 128>(a, s);
+    return attn->head_dim == 64 ? launch_packed<float, 64>(a, s) : launch_packed<float, 128>(a, s);
 }
 
 size_t rq_attn_tree_workspace(const rq_attn *attn, int32_t n_seqs, int64_t tokens, int32_t max_nodes,
                               int32_t capacity) {
-    return 0;
+    AttnArgs a{};
+    if (n_seqs < 1 || tokens < 1 || max_nodes < 1 || max_nodes > kMaxNodes || capacity < 0 ||
+        check_attn(attn, tokens, a) != RQ_OK)
+        return 0;
+    const int splits = tree_splits(n_seqs, a.n_kv, (int64_t)max_nodes * (a.n_heads / a.n_kv), capacity,
+                                   attn->dtype == RQ_F16);
+    const size_t rows = (size_t)tokens * (size_t)a.n_heads * (size_t)splits;
+    return splits > 1 ? (rows * ((size_t)attn->head_dim * 4 + 8) + 15) / 16 * 16 : 0;
 }
 
 int rq_attn_tree(rq_ctx *ctx, const rq_attn *attn, const rq_kv_cache *cache, const void *q, const int32_t *starts,
@@ -242,7 +722,10 @@ int rq_attn_tree(rq_ctx *ctx, const rq_attn *attn, const rq_kv_cache *cache, con
     const int st = check_tree(attn, cache, q, starts, lengths, mask, tokens, max_nodes, out, workspace,
                               workspace_bytes, a, run);
     if (st != RQ_OK || !run) return st;
-    return launch_rows(a, true, attn->head_dim, attn->dtype, pick(ctx, stream));
+    hipStream_t s = pick(ctx, stream);
+    if (attn->dtype == RQ_F16)
+        return attn->head_dim == 64 ? launch_tree<_Float16, 64>(a, s) : launch_tree<_Float16, 128>(a, s);
+    return attn->head_dim == 64 ? launch_tree<float, 64>(a, s) : launch_tree<float, 128>(a, s);
 }
 
 // For the tests, no part of the C ABI: the argument checks alone (cache NULL:
