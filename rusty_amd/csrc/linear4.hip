@@ -2,7 +2,21 @@
 //   Y[m, n] = sum_k X[m, k] W[n, k],  W[n, k] = u[n, k] s[n, k/G] + b[n, k/G],
 // u in 0..15, two codes a byte (the even k in the low nibble), an f32 scale and
 // bias per G consecutive k of a row.
+//
+// Bound by the weight's bytes: n k / 2 of codes and 8 n k / G of scales and
+// biases, each read once.  Codes enter the products exactly, as fp16 16 + u: a
+// nibble at mantissa bits 6..9 under the exponent of 16.0 (one shift and one
+// v_and_or per two codes, the pairs k and k + 4 of each 8).  Per group, with
+// t = sum (16 + u) x and xs = sum x in f32,
+//   sum (u s + b) x = s t + (b - 16 s) xs,
+// so a weight is never rounded, and the offset costs f32 rounding of terms at
+// most (16 + 15) / 15 times the largest ones.
+//  * m <= 2: k_linear4_dot, v_dot2_f32_f16 with the activation rows in registers;
+//  * m <= 16: k_linear4_mfma, the rows on the matrix cores;
+//  * more: 16 rows at a time, or (many rows) the codes widened to bytes once
+//    and the 8-bit GEMM (launch_linear4).
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 
@@ -10,6 +24,418 @@ namespace rq {
 namespace {
 
 constexpr int TH = 256;
+constexpr uint32_t kOOB = 0x80000000u;  // any offset past a buffer resource reads zero
+
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float f2_t __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void *p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, bytes, 0x00020000);
+}
+// aux bit 1 = non-temporal (streamed once), 0 = default caching
+template <int AUX>
+__device__ __forceinline__ u32x4 bload(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, AUX));
+}
+__device__ __forceinline__ float bload1(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
+}
+__device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2_t, a), __builtin_bit_cast(h2_t, b), c, false);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ float readlane(float v, int l) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+}
+// Sum over the 64 lanes, uniform across the wave.
+__device__ __forceinline__ float wave_total(float v) {
+    v += dpp<0xB1>(v);   // quad_perm [1,0,3,2]
+    v += dpp<0x4E>(v);   // quad_perm [2,3,0,1]
+    v += dpp<0x141>(v);  // row_half_mirror
+    v += dpp<0x140>(v);  // row_mirror: each 16-lane row holds its sum
+    return (readlane(v, 0) + readlane(v, 16)) + (readlane(v, 32) + readlane(v, 48));
+}
+// 8 codes (a dword) -> fp16 16 + u of codes (0, 4), (1, 5), (2, 6), (3, 7).
+__device__ __forceinline__ u32x4 expand8(uint32_t w) {
+    const uint32_t m = 0x03C003C0u, e = 0x4C004C00u;
+    return u32x4{((w << 6) & m) | e, ((w << 2) & m) | e, ((w >> 2) & m) | e, ((w >> 6) & m) | e};
+}
+// 8 consecutive halves in that order: (0, 4), (1, 5), (2, 6), (3, 7).
+__device__ __forceinline__ u32x4 pair_up(u32x4 x) {
+    return u32x4{__builtin_amdgcn_perm(x.z, x.x, 0x05040100u), __builtin_amdgcn_perm(x.z, x.x, 0x07060302u),
+                 __builtin_amdgcn_perm(x.w, x.y, 0x05040100u), __builtin_amdgcn_perm(x.w, x.y, 0x07060302u)};
+}
+
+// 8 f32 values (a, b) times 2^-sh -> hi = fp16(v), lo = fp16(v - hi), as they
+// stand: hi + lo is v to about 2^-22 relative while |v| stays inside fp16's range.
+template <bool SC>
+__device__ __forceinline__ void split8(floatx4 a, floatx4 b, int sh, u32x4 &hi, u32x4 &lo) {
+    const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        f2_t v = {f[2 * e], f[2 * e + 1]};
+        if constexpr (SC) v = f2_t{__builtin_amdgcn_ldexpf(v.x, -sh), __builtin_amdgcn_ldexpf(v.y, -sh)};
+        const h2_t h = __builtin_convertvector(v, h2_t);
+        const h2_t l = __builtin_convertvector((f2_t{v.x - (float)h.x, v.y - (float)h.y}), h2_t);
+        hi[e] = __builtin_bit_cast(uint32_t, h);
+        lo[e] = __builtin_bit_cast(uint32_t, l);
+    }
+}
+
+// m <= M = 1 or 2 rows.  A block owns R * RP weight rows; thread tt of a row
+// group (TPR threads) owns the 16-byte chunks (32 codes, one group) tt, tt +
+// TPR, ... of each of its R rows, so a wave reads 1 KiB of a row at a time, all
+// R * CPT chunks in flight before the first is used.  Rows past N and chunks past K
+// are offsets past the resource and read as zero.  The threads' partial sums
+// meet in LDS; a wave then finishes whole (row, token) sums.
+// XF: f32 rows; each chunk of a row is scaled by the power of two that puts its
+// largest magnitude in [2^14, 2^15) and carried as two fp16 terms.
+template <int M, int CPT, int TPR, int R, bool XF>
+__global__ __launch_bounds__(TH) void k_linear4_dot(const uint8_t *__restrict__ W, const float *__restrict__ scales,
+                                                    const float *__restrict__ biases, const void *__restrict__ X,
+                                                    void *__restrict__ Y, int y_f16, int m_act, int N, int K, int group) {
+    constexpr int RP = TH / TPR, ROWS = R * RP, TASKS = ROWS * M;
+    __shared__ float part[TASKS][TPR];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, rp = t / TPR, tt = t % TPR;
+    const int C = K / 32, gk = K / group, row0 = blockIdx.x * ROWS, rows_here = min(ROWS, N - row0);
+
+    const auto rx = make_rsrc(X, (uint32_t)m_act * (uint32_t)K * (XF ? 4u : 2u));
+    u32x4 xr[CPT][M][XF ? 8 : 4];
+#pragma unroll
+    for (int j = 0; j < CPT; ++j)
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            const int c = tt + TPR * j;
+            const uint32_t off = c < C ? ((uint32_t)m * K + (uint32_t)c * 32) * (XF ? 4u : 2u) : kOOB;
+#pragma unroll
+            for (int i = 0; i < (XF ? 8 : 4); ++i) xr[j][m][i] = bload<0>(rx, off + 16 * i);
+        }
+    float sg[R][CPT], bg[R][CPT];
+    int cg[CPT];
+#pragma unroll
+    for (int j = 0; j < CPT; ++j) cg[j] = (int)((unsigned)(tt + TPR * j) * 32u / (unsigned)group);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < CPT; ++j) {
+            // (a chunk or row that is not there takes group 0's: it meets zeros, or is not stored)
+            const bool ok = tt + TPR * j < C && r * RP + rp < rows_here;
+            const size_t g = ok ? (size_t)(row0 + r * RP + rp) * gk + cg[j] : 0;
+            sg[r][j] = scales[g];
+            bg[r][j] = biases ? biases[g] : 0.0f;
+        }
+    const auto rw = make_rsrc(W + (size_t)row0 * (K / 2), (uint32_t)rows_here * (uint32_t)(K / 2));
+    u32x4 w[R][CPT];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < CPT; ++j) {
+            const int c = tt + TPR * j;
+            w[r][j] = bload<2>(rw, c < C ? (uint32_t)(r * RP + rp) * (uint32_t)(K / 2) + (uint32_t)c * 16u : kOOB);
+        }
+
+    // the activations in the codes' pair order (XF: two terms and 2^e), and their sums
+    u32x4 xh[CPT][M][4], xl[XF ? CPT : 1][XF ? M : 1][4];
+    float pe[XF ? CPT : 1][XF ? M : 1], xs[CPT][M];
+#pragma unroll
+    for (int j = 0; j < CPT; ++j)
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            if constexpr (XF) {
+                float amax = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const floatx4 f = __builtin_bit_cast(floatx4, xr[j][m][i]);
+                    amax = fmaxf(fmaxf(fmaxf(amax, fabsf(f.x)), fmaxf(fabsf(f.y), fabsf(f.z))), fabsf(f.w));
+                }
+                // amax = f 2^E, f in [0.5, 1); an infinite or NaN one gives E = 0 and stays what it is
+                const int ex = max(__builtin_amdgcn_frexp_expf(amax) - 15, -126);
+                pe[j][m] = __builtin_amdgcn_ldexpf(1.0f, ex);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    u32x4 hi, lo;
+                    split8<true>(__builtin_bit_cast(floatx4, xr[j][m][2 * i]),
+                                 __builtin_bit_cast(floatx4, xr[j][m][2 * i + 1]), ex, hi, lo);
+                    xh[j][m][i] = pair_up(hi);
+                    xl[j][m][i] = pair_up(lo);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) xh[j][m][i] = pair_up(xr[j][m][i]);
+            }
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s = dot2(xh[j][m][i][e], 0x3C003C00u, s);
+                    if constexpr (XF) s = dot2(xl[j][m][i][e], 0x3C003C00u, s);
+                }
+            xs[j][m] = XF ? s * pe[j][m] : s;
+        }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        float p[M];
+#pragma unroll
+        for (int m = 0; m < M; ++m) p[m] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < CPT; ++j) {
+            float d[M];
+#pragma unroll
+            for (int m = 0; m < M; ++m) d[m] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const u32x4 u = expand8(w[r][j][i]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int m = 0; m < M; ++m) {
+                        d[m] = dot2(u[e], xh[j][m][i][e], d[m]);
+                        if constexpr (XF) d[m] = dot2(u[e], xl[j][m][i][e], d[m]);
+                    }
+            }
+            const float c = __builtin_fmaf(-16.0f, sg[r][j], bg[r][j]);
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                p[m] = __builtin_fmaf(sg[r][j], XF ? d[m] * pe[j][m] : d[m], p[m]);
+                p[m] = __builtin_fmaf(c, xs[j][m], p[m]);
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < M; ++m) part[(r * RP + rp) * M + m][tt] = p[m];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < (TASKS + 3) / 4; ++i) {
+        const int task = wave + 4 * i;
+        if (task >= TASKS) break;
+        float v = 0.0f;
+#pragma unroll
+        for (int j = 0; j < TPR / 64; ++j) v += part[task][lane + 64 * j];
+        const float y = wave_total(v);
+        const int row = task / M, m = task % M;
+        if (lane == 0 && row < rows_here && m < m_act) {
+            const size_t o = (size_t)m * N + row0 + row;
+            if (y_f16) static_cast<_Float16 *>(Y)[o] = (_Float16)y;
+            else static_cast<float *>(Y)[o] = y;
+        }
+    }
+}
+
+// m <= 16 rows on v_mfma_f32_16x16x32_f16: A = 16 rows of X x 32 k, B = 32 k x
+// 16 weight rows, so lane l has weight row l % 16 and, of the result, rows 4 (l /
+// 16) + r, r < 4, of X.  Per group of GS steps of 32 k: t = X . (16 + U) and (B all ones)
+// xs = the rows' sums, then acc += s t + (b - 16 s) xs with the lane's own s and b.
+// A block of NW waves has RT tiles of 16 weight rows; wave w takes the batches of 256 k
+// w, w + NW, ... (from a per-block rotation: every block reads all of X, and the
+// blocks of one XCD should not ask for the same lines at once), and each
+// activation fragment it loads serves all RT tiles.  Codes are loaded 8 rows x 128
+// bytes per instruction and turned to operand order through the wave's own LDS
+// (chunk c of row r at c ^ (r % 8)); no barrier.  The next batch's loads are in flight while
+// one is multiplied.  The waves' sums meet in LDS.
+// XF: f32 rows as two fp16 terms; a batch whose sums are not finite (values past
+// fp16's range) is multiplied again, each row scaled by a power of two.
+template <int RT, int NW, int GS, bool XF>
+__global__ __launch_bounds__(NW * 64) void k_linear4_mfma(const uint8_t *__restrict__ W,
+                                                          const float *__restrict__ scales,
+                                                          const float *__restrict__ biases,
+                                                          const void *__restrict__ X, void *__restrict__ Y, int y_f16,
+                                                          int m_act, int N, int K, int group) {
+    constexpr int NG = 8 / GS;  // groups of a batch
+    __shared__ floatx4 red[NW][RT][64];
+    __shared__ __attribute__((aligned(16))) uint8_t wt[NW][RT][16 * 128];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int fr = lane & 15, q = lane >> 4, n0 = blockIdx.x * 16 * RT;
+    const int nb = (K + 255) / 256, gk = K / group;
+    const int rot = (int)((blockIdx.x >> 3) * 5u + (blockIdx.x & 7u)) % nb;
+    __amdgpu_buffer_rsrc_t rw[RT], rs[RT], rb[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const int n = n0 + 16 * i, rows = max(0, min(16, N - n));
+        const size_t r0 = rows ? n : 0;
+        rw[i] = make_rsrc(W + r0 * (K / 2), (uint32_t)rows * (uint32_t)(K / 2));
+        rs[i] = make_rsrc(scales + r0 * gk, (uint32_t)rows * (uint32_t)gk * 4u);
+        rb[i] = biases ? make_rsrc(biases + r0 * gk, (uint32_t)rows * (uint32_t)gk * 4u) : make_rsrc(scales, 0);
+    }
+    const auto rx = make_rsrc(X, (uint32_t)m_act * (uint32_t)K * (XF ? 4u : 2u));
+    const uint32_t xrow = (uint32_t)fr * (uint32_t)K + 8u * (uint32_t)q;
+
+    struct Batch {
+        u32x4 w[RT][2], x[XF ? 16 : 8];
+        float s[RT][NG], b[RT][NG];
+    };
+    auto load = [&](Batch &b, int bi) {
+        int bb = bi + rot;
+        bb -= bb >= nb ? nb : 0;
+        const uint32_t k0 = (uint32_t)bb * 256u;
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                // row 8 h + lane / 8, chunk lane % 8 (past K: the next row's codes, which meet zeros)
+                const uint32_t off = (uint32_t)(8 * h + lane / 8) * (uint32_t)(K / 2) + k0 / 2 + 16u * (lane & 7);
+                b.w[i][h] = bload<2>(rw[i], off);
+            }
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const uint32_t k = k0 + 32u * GS * g;
+                const uint32_t off = k < (uint32_t)K ? ((uint32_t)fr * (uint32_t)gk + k / (uint32_t)group) * 4u : kOOB;
+                b.s[i][g] = bload1(rs[i], off);
+                b.b[i][g] = bload1(rb[i], off);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t k = k0 + 32u * j;
+            const bool ok = k < (uint32_t)K;
+            if constexpr (XF) {
+                b.x[2 * j] = bload<0>(rx, ok ? (xrow + k) * 4u : kOOB);
+                b.x[2 * j + 1] = bload<0>(rx, ok ? (xrow + k) * 4u + 16u : kOOB);
+            } else {
+                b.x[j] = bload<0>(rx, ok ? (xrow + k) * 2u : kOOB);
+            }
+        }
+    };
+    floatx4 acc[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    const half8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
+    auto mma = [&](const Batch &b) {
+        uint32_t u[RT][8];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            uint8_t *wl = wt[wave][i];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = 8 * h + lane / 8;
+                *reinterpret_cast<u32x4 *>(wl + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = b.w[i][h];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                u[i][j] = *reinterpret_cast<const uint32_t *>(wl + fr * 128 + ((j ^ (fr & 7)) << 4) + 4 * q);
+        }
+        // sh: power of two of this lane's row of X (scaled)
+        auto run = [&](auto scaled, int sh) {
+            constexpr bool SC = decltype(scaled)::value;
+            int back[4];  // those of the rows 4 q + r that acc holds
+#pragma unroll
+            for (int r = 0; r < 4; ++r) back[r] = SC ? __shfl(sh, 4 * q + r) : 0;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                floatx4 tg[RT], xg = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < RT; ++i) tg[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int e = 0; e < GS; ++e) {
+                    const int j = g * GS + e;
+                    u32x4 hi, lo = {0, 0, 0, 0};
+                    if constexpr (XF)
+                        split8<SC>(__builtin_bit_cast(floatx4, b.x[2 * j]), __builtin_bit_cast(floatx4, b.x[2 * j + 1]),
+                                   sh, hi, lo);
+                    else
+                        hi = b.x[j];
+                    const half8 xh = __builtin_bit_cast(half8, pair_up(hi)), xl = __builtin_bit_cast(half8, pair_up(lo));
+                    xg = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, ones, xg, 0, 0, 0);
+                    if constexpr (XF) xg = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl, ones, xg, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < RT; ++i) {
+                        const half8 wv = __builtin_bit_cast(half8, expand8(u[i][j]));
+                        tg[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, wv, tg[i], 0, 0, 0);
+                        if constexpr (XF) tg[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl, wv, tg[i], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < RT; ++i) {
+                    const float s = b.s[i][g], c = __builtin_fmaf(-16.0f, s, b.b[i][g]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float tv = SC ? __builtin_amdgcn_ldexpf(tg[i][r], back[r]) : tg[i][r];
+                        const float xv = SC ? __builtin_amdgcn_ldexpf(xg[r], back[r]) : xg[r];
+                        acc[i][r] = __builtin_fmaf(c, xv, __builtin_fmaf(s, tv, acc[i][r]));
+                    }
+                }
+            }
+        };
+        if constexpr (XF) {
+            floatx4 old[RT];
+#pragma unroll
+            for (int i = 0; i < RT; ++i) old[i] = acc[i];
+            run(std::false_type{}, 0);
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) bad = bad || !__builtin_isfinite(acc[i][r]);
+            if (__builtin_amdgcn_ballot_w64(bad) != 0) {
+                float amax = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const floatx4 f = __builtin_bit_cast(floatx4, b.x[i]);
+                    amax = fmaxf(fmaxf(fmaxf(amax, fabsf(f.x)), fmaxf(fabsf(f.y), fabsf(f.z))), fabsf(f.w));
+                }
+                amax = fmaxf(amax, __shfl_xor(amax, 16));  // the four lanes of a row
+                amax = fmaxf(amax, __shfl_xor(amax, 32));
+                const int sh = __builtin_amdgcn_frexp_expf(amax) - 15;
+#pragma unroll
+                for (int i = 0; i < RT; ++i) acc[i] = old[i];
+                run(std::true_type{}, sh);
+            }
+        } else {
+            run(std::false_type{}, 0);
+        }
+    };
+    // two batches alternate; the tail is peeled so that every load sits beside
+    // the products of the batch before it
+    const int mb = (nb - wave + NW - 1) / NW;  // this wave's batches (uniform)
+    if (mb > 0) {
+        Batch A, B;
+        load(A, wave);
+        int b = 0;
+        for (; b + 2 < mb; b += 2) {
+            load(B, wave + (b + 1) * NW);
+            __builtin_amdgcn_sched_barrier(0);
+            mma(A);
+            load(A, wave + (b + 2) * NW);
+            __builtin_amdgcn_sched_barrier(0);
+            mma(B);
+        }
+        if (b + 1 < mb) {
+            load(B, wave + (b + 1) * NW);
+            __builtin_amdgcn_sched_barrier(0);
+            mma(A);
+            mma(B);
+        } else {
+            mma(A);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i) red[wave][i][lane] = acc[i];
+    __syncthreads();
+    // tile i is finished by wave i: lane l has weight row l % 16, rows 4 q + r of X
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        if (wave != i % NW) continue;
+        floatx4 v = red[0][i][lane];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) v += red[w][i][lane];
+        const int n = n0 + 16 * i + fr;
+        if (n >= N) continue;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int m = 4 * q + r;
+            if (m >= m_act) break;
+            const size_t o = (size_t)m * N + n;
+            if (y_f16) static_cast<_Float16 *>(Y)[o] = (_Float16)v[r];
+            else static_cast<float *>(Y)[o] = v[r];
+        }
+    }
+}
 
 __global__ __launch_bounds__(TH) void k_dequantize4(const uint8_t *__restrict__ codes, const float *__restrict__ scales,
                                                     const float *__restrict__ biases, float *__restrict__ out,
@@ -63,6 +489,56 @@ __global__ __launch_bounds__(TH) void k_linear4_generic(const uint8_t *__restric
     }
 }
 
+using DotFn = void (*)(const uint8_t *, const float *, const float *, const void *, void *, int, int, int, int, int);
+
+// The m <= 2 kernel of a shape and the weight rows of its blocks.
+template <int M, bool XF, int CPT, int TPR>
+DotFn dot_rows(int *rows) {
+    constexpr int R = 4;
+    *rows = R * (TH / TPR);
+    return k_linear4_dot<M, CPT, TPR, R, XF>;
+}
+template <int M, bool XF>
+DotFn dot_kernel(int64_t K, int *rows) {
+    const int64_t C = K / 32;
+    if (C <= 64) return dot_rows<M, XF, 1, 64>(rows);
+    if (C <= 128) return dot_rows<M, XF, 1, 128>(rows);
+    if (C <= 256) return dot_rows<M, XF, 1, 256>(rows);
+    if (C <= 512) return dot_rows<M, XF, 2, 256>(rows);
+    return nullptr;
+}
+
+// m <= 2; RQ_ERR_UNSUPPORTED outside what the kernel serves.
+int launch_dot(const rq_qweight &w, const void *x, bool xf, void *y, bool yh, int m, hipStream_t s) {
+    int rows = 0;
+    const DotFn fn = m == 1 ? (xf ? dot_kernel<1, true>(w.k_in, &rows) : dot_kernel<1, false>(w.k_in, &rows))
+                            : (xf ? dot_kernel<2, true>(w.k_in, &rows) : dot_kernel<2, false>(w.k_in, &rows));
+    if (!fn) return RQ_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL(fn, dim3((unsigned)cdiv(w.n_out, rows)), dim3(TH), 0, s, (const uint8_t *)w.codes, w.scales,
+                       w.biases, x, y, yh ? 1 : 0, m, (int)w.n_out, (int)w.k_in, w.group);
+    RQ_LAUNCH_CHECK();
+    return RQ_OK;
+}
+
+// m <= 16
+int launch_mfma(const rq_qweight &w, const void *x, bool xf, void *y, bool yh, int m, hipStream_t s) {
+    auto go = [&](auto rt, auto nw, auto gs, auto xfc) {
+        constexpr int RT = decltype(rt)::value, NW = decltype(nw)::value;
+        hipLaunchKernelGGL((k_linear4_mfma<RT, NW, decltype(gs)::value, decltype(xfc)::value>),
+                           dim3((unsigned)cdiv(w.n_out, 16 * RT)), dim3(NW * 64), 0, s, (const uint8_t *)w.codes,
+                           w.scales, w.biases, x, y, yh ? 1 : 0, m, (int)w.n_out, (int)w.k_in, w.group);
+    };
+    auto by_group = [&](auto rt, auto nw, auto xfc) {
+        if (w.group % 128 == 0) go(rt, nw, std::integral_constant<int, 4>{}, xfc);
+        else if (w.group % 64 == 0) go(rt, nw, std::integral_constant<int, 2>{}, xfc);
+        else go(rt, nw, std::integral_constant<int, 1>{}, xfc);
+    };
+    if (xf) by_group(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{}, std::true_type{});
+    else by_group(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{}, std::false_type{});
+    RQ_LAUNCH_CHECK();
+    return RQ_OK;
+}
+
 }  // namespace
 
 int launch_dequantize4(const rq_qweight &w, float *out, hipStream_t s) {
@@ -76,9 +552,25 @@ int launch_dequantize4(const rq_qweight &w, float *out, hipStream_t s) {
 }
 
 int launch_linear4(const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dtype yt, int64_t m, hipStream_t s) {
-    if (!grid_ok(w.n_out, TH)) return fail(RQ_ERR_SHAPE, "n_out too large for the generic kernel");
-    hipLaunchKernelGGL(k_linear4_generic, dim3((unsigned)w.n_out), dim3(TH), 0, s, (const uint8_t *)w.codes, w.scales,
-                       w.biases, (int64_t)w.group, x, xt == RQ_F16 ? 1 : 0, y, yt == RQ_F16 ? 1 : 0, m, w.n_out, w.k_in);
+    const int64_t N = w.n_out, K = w.k_in;
+    const bool xf = xt == RQ_F32, yh = yt == RQ_F16;
+    // Chunks of 32 codes in one group each, 16-byte loads, 32-bit offsets into 16 rows of X and of W
+    const bool fast = K > 0 && w.group % 32 == 0 && K <= (1 << 24) && grid_ok(N, 64) && aligned(w.codes, 16) && aligned(x, 16);
+    if (fast) {
+        const size_t xr = (size_t)K * (xf ? 4 : 2), yr = (size_t)N * (yh ? 2 : 4);
+        for (int64_t m0 = 0; m0 < m; m0 += 16) {
+            const int mc = (int)std::min<int64_t>(16, m - m0);
+            const char *xp = static_cast<const char *>(x) + m0 * xr;
+            char *yp = static_cast<char *>(y) + m0 * yr;
+            int st = mc <= 2 ? launch_dot(w, xp, xf, yp, yh, mc, s) : RQ_ERR_UNSUPPORTED;
+            if (st == RQ_ERR_UNSUPPORTED) st = launch_mfma(w, xp, xf, yp, yh, mc, s);
+            if (st != RQ_OK) return st;
+        }
+        return RQ_OK;
+    }
+    if (!grid_ok(N, TH)) return fail(RQ_ERR_SHAPE, "n_out too large for the generic kernel");
+    hipLaunchKernelGGL(k_linear4_generic, dim3((unsigned)N), dim3(TH), 0, s, (const uint8_t *)w.codes, w.scales,
+                       w.biases, (int64_t)w.group, x, xf ? 0 : 1, y, yh ? 1 : 0, m, N, K);
     RQ_LAUNCH_CHECK();
     return RQ_OK;
 }
