@@ -72,14 +72,14 @@ __device__ __forceinline__ u32x4 pair_up(u32x4 x) {
                  __builtin_amdgcn_perm(x.w, x.y, 0x05040100u), __builtin_amdgcn_perm(x.w, x.y, 0x07060302u)};
 }
 
-// 8 f32 values (a, b) times 2^-sh -> hi = fp16(v), lo = fp16(v - hi), as they
-// stand: hi + lo is v to about 2^-22 relative while |v| stays inside fp16's range.
+// 8 f32 values (a, b) times 2^-sh -> hi = fp16(v), lo = fp16(v - hi) in the
+// codes' pair order: hi + lo is v to about 2^-22 relative while |v| stays inside
+// fp16's range.
 template <bool SC>
 __device__ __forceinline__ void split8(floatx4 a, floatx4 b, int sh, u32x4 &hi, u32x4 &lo) {
-    const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        f2_t v = {f[2 * e], f[2 * e + 1]};
+        f2_t v = {a[e], b[e]};
         if constexpr (SC) v = f2_t{__builtin_amdgcn_ldexpf(v.x, -sh), __builtin_amdgcn_ldexpf(v.y, -sh)};
         const h2_t h = __builtin_convertvector(v, h2_t);
         const h2_t l = __builtin_convertvector((f2_t{v.x - (float)h.x, v.y - (float)h.y}), h2_t);
@@ -158,13 +158,9 @@ __global__ __launch_bounds__(TH) void k_linear4_dot(const uint8_t *__restrict__ 
                 const int ex = max(__builtin_amdgcn_frexp_expf(amax) - 15, -126);
                 pe[j][m] = __builtin_amdgcn_ldexpf(1.0f, ex);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    u32x4 hi, lo;
+                for (int i = 0; i < 4; ++i)
                     split8<true>(__builtin_bit_cast(floatx4, xr[j][m][2 * i]),
-                                 __builtin_bit_cast(floatx4, xr[j][m][2 * i + 1]), ex, hi, lo);
-                    xh[j][m][i] = pair_up(hi);
-                    xl[j][m][i] = pair_up(lo);
-                }
+                                 __builtin_bit_cast(floatx4, xr[j][m][2 * i + 1]), ex, xh[j][m][i], xl[j][m][i]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) xh[j][m][i] = pair_up(xr[j][m][i]);
@@ -239,185 +235,211 @@ __global__ __launch_bounds__(TH) void k_linear4_dot(const uint8_t *__restrict__ 
 // bytes per instruction and turned to operand order through the wave's own LDS
 // (chunk c of row r at c ^ (r % 8)); no barrier.  The next batch's loads are in flight while
 // one is multiplied.  The waves' sums meet in LDS.
+// Scales and biases go through LDS too, whole rows of them first (they lie one
+// after another), as (s, b - 16 s): read by each lane in place they touch 16 cache
+// lines per load, which bounded the kernel (8 x 4096 x 4096 in groups of 64 8.9 us, of 32
+// XXX).  Rows longer than kSegGroups groups take several rounds.
 // XF: f32 rows as two fp16 terms; a batch whose sums are not finite (values past
 // fp16's range) is multiplied again, each row scaled by a power of two.
+constexpr int kSegGroups = 512;
+
 template <int RT, int NW, int GS, bool XF>
 __global__ __launch_bounds__(NW * 64) void k_linear4_mfma(const uint8_t *__restrict__ W,
                                                           const float *__restrict__ scales,
                                                           const float *__restrict__ biases,
                                                           const void *__restrict__ X, void *__restrict__ Y, int y_f16,
                                                           int m_act, int N, int K, int group) {
-    constexpr int NG = 8 / GS;  // groups of a batch
+    constexpr int NG = 8 / GS, NT = NW * 64;  // groups of a batch, threads
     __shared__ floatx4 red[NW][RT][64];
     __shared__ __attribute__((aligned(16))) uint8_t wt[NW][RT][16 * 128];
+    extern __shared__ float2 sc[];  // [16 RT][pitch]
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int fr = lane & 15, q = lane >> 4, n0 = blockIdx.x * 16 * RT;
-    const int nb = (K + 255) / 256, gk = K / group;
-    const int rot = (int)((blockIdx.x >> 3) * 5u + (blockIdx.x & 7u)) % nb;
-    __amdgpu_buffer_rsrc_t rw[RT], rs[RT], rb[RT];
+    const int gk = K / group, pitch = min(gk, kSegGroups) | 1;
+    __amdgpu_buffer_rsrc_t rw[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
         const int n = n0 + 16 * i, rows = max(0, min(16, N - n));
-        const size_t r0 = rows ? n : 0;
-        rw[i] = make_rsrc(W + r0 * (K / 2), (uint32_t)rows * (uint32_t)(K / 2));
-        rs[i] = make_rsrc(scales + r0 * gk, (uint32_t)rows * (uint32_t)gk * 4u);
-        rb[i] = biases ? make_rsrc(biases + r0 * gk, (uint32_t)rows * (uint32_t)gk * 4u) : make_rsrc(scales, 0);
+        rw[i] = make_rsrc(W + (rows ? (size_t)n : 0) * (K / 2), (uint32_t)rows * (uint32_t)(K / 2));
     }
     const auto rx = make_rsrc(X, (uint32_t)m_act * (uint32_t)K * (XF ? 4u : 2u));
     const uint32_t xrow = (uint32_t)fr * (uint32_t)K + 8u * (uint32_t)q;
 
     struct Batch {
         u32x4 w[RT][2], x[XF ? 16 : 8];
-        float s[RT][NG], b[RT][NG];
-    };
-    auto load = [&](Batch &b, int bi) {
-        int bb = bi + rot;
-        bb -= bb >= nb ? nb : 0;
-        const uint32_t k0 = (uint32_t)bb * 256u;
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                // row 8 h + lane / 8, chunk lane % 8 (past K: the next row's codes, which meet zeros)
-                const uint32_t off = (uint32_t)(8 * h + lane / 8) * (uint32_t)(K / 2) + k0 / 2 + 16u * (lane & 7);
-                b.w[i][h] = bload<2>(rw[i], off);
-            }
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const uint32_t k = k0 + 32u * GS * g;
-                const uint32_t off = k < (uint32_t)K ? ((uint32_t)fr * (uint32_t)gk + k / (uint32_t)group) * 4u : kOOB;
-                b.s[i][g] = bload1(rs[i], off);
-                b.b[i][g] = bload1(rb[i], off);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t k = k0 + 32u * j;
-            const bool ok = k < (uint32_t)K;
-            if constexpr (XF) {
-                b.x[2 * j] = bload<0>(rx, ok ? (xrow + k) * 4u : kOOB);
-                b.x[2 * j + 1] = bload<0>(rx, ok ? (xrow + k) * 4u + 16u : kOOB);
-            } else {
-                b.x[j] = bload<0>(rx, ok ? (xrow + k) * 2u : kOOB);
-            }
-        }
+        int g;  // the batch's first group, from the segment's
     };
     floatx4 acc[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     const half8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
-    auto mma = [&](const Batch &b) {
-        uint32_t u[RT][8];
+    for (int g0 = 0; g0 < gk; g0 += kSegGroups) {
+        const int sg = min(kSegGroups, gk - g0), kbeg = g0 * group, klen = sg * group;
+        const int nb = (klen + 255) / 256;
+        const int rot = (int)((blockIdx.x >> 3) * 5u + (blockIdx.x & 7u)) % nb;
+        if (g0) __syncthreads();  // every wave is done with the last segment's scales
+        // scales of 4 elements per thread at a time (row and group by division once per element)
+        const int rows = min(16 * RT, N - n0), total = rows * sg;
+        for (int i0 = t; i0 < total; i0 += 4 * NT) {
+            float s[4], b[4];
+            int at[4];
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            uint8_t *wl = wt[wave][i];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int r = 8 * h + lane / 8;
-                *reinterpret_cast<u32x4 *>(wl + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = b.w[i][h];
+            for (int e = 0; e < 4; ++e) {
+                const int i = min(i0 + e * NT, total - 1), row = i / sg, g = i - row * sg;
+                const size_t src = (size_t)(n0 + row) * gk + g0 + g;
+                s[e] = scales[src];
+                b[e] = biases ? biases[src] : 0.0f;
+                at[e] = row * pitch + g;
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                u[i][j] = *reinterpret_cast<const uint32_t *>(wl + fr * 128 + ((j ^ (fr & 7)) << 4) + 4 * q);
+            for (int e = 0; e < 4; ++e) sc[at[e]] = make_float2(s[e], __builtin_fmaf(-16.0f, s[e], b[e]));
         }
-        // sh: power of two of this lane's row of X (scaled)
-        auto run = [&](auto scaled, int sh) {
-            constexpr bool SC = decltype(scaled)::value;
-            int back[4];  // those of the rows 4 q + r that acc holds
-#pragma unroll
-            for (int r = 0; r < 4; ++r) back[r] = SC ? __shfl(sh, 4 * q + r) : 0;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                floatx4 tg[RT], xg = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int i = 0; i < RT; ++i) tg[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int e = 0; e < GS; ++e) {
-                    const int j = g * GS + e;
-                    u32x4 hi, lo = {0, 0, 0, 0};
-                    if constexpr (XF)
-                        split8<SC>(__builtin_bit_cast(floatx4, b.x[2 * j]), __builtin_bit_cast(floatx4, b.x[2 * j + 1]),
-                                   sh, hi, lo);
-                    else
-                        hi = b.x[j];
-                    const half8 xh = __builtin_bit_cast(half8, pair_up(hi)), xl = __builtin_bit_cast(half8, pair_up(lo));
-                    xg = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, ones, xg, 0, 0, 0);
-                    if constexpr (XF) xg = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl, ones, xg, 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < RT; ++i) {
-                        const half8 wv = __builtin_bit_cast(half8, expand8(u[i][j]));
-                        tg[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, wv, tg[i], 0, 0, 0);
-                        if constexpr (XF) tg[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl, wv, tg[i], 0, 0, 0);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < RT; ++i) {
-                    const float s = b.s[i][g], c = __builtin_fmaf(-16.0f, s, b.b[i][g]);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float tv = SC ? __builtin_amdgcn_ldexpf(tg[i][r], back[r]) : tg[i][r];
-                        const float xv = SC ? __builtin_amdgcn_ldexpf(xg[r], back[r]) : xg[r];
-                        acc[i][r] = __builtin_fmaf(c, xv, __builtin_fmaf(s, tv, acc[i][r]));
-                    }
-                }
-            }
-        };
-        if constexpr (XF) {
-            floatx4 old[RT];
-#pragma unroll
-            for (int i = 0; i < RT; ++i) old[i] = acc[i];
-            run(std::false_type{}, 0);
-            bool bad = false;
+        auto load = [&](Batch &b, int bi) {
+            int bb = bi + rot;
+            bb -= bb >= nb ? nb : 0;
+            const uint32_t k0 = (uint32_t)kbeg + (uint32_t)bb * 256u;
+            b.g = bb * 256 / group;
 #pragma unroll
             for (int i = 0; i < RT; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) bad = bad || !__builtin_isfinite(acc[i][r]);
-            if (__builtin_amdgcn_ballot_w64(bad) != 0) {
-                float amax = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const floatx4 f = __builtin_bit_cast(floatx4, b.x[i]);
-                    amax = fmaxf(fmaxf(fmaxf(amax, fabsf(f.x)), fmaxf(fabsf(f.y), fabsf(f.z))), fabsf(f.w));
+                for (int h = 0; h < 2; ++h) {
+                    // row 8 h + lane / 8, chunk lane % 8 (past K: the next row's codes, which meet zeros)
+                    const uint32_t off = (uint32_t)(8 * h + lane / 8) * (uint32_t)(K / 2) + k0 / 2 + 16u * (lane & 7);
+                    b.w[i][h] = bload<2>(rw[i], off);
                 }
-                amax = fmaxf(amax, __shfl_xor(amax, 16));  // the four lanes of a row
-                amax = fmaxf(amax, __shfl_xor(amax, 32));
-                const int sh = __builtin_amdgcn_frexp_expf(amax) - 15;
 #pragma unroll
-                for (int i = 0; i < RT; ++i) acc[i] = old[i];
-                run(std::true_type{}, sh);
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t k = k0 + 32u * j;
+                const bool ok = k < (uint32_t)(kbeg + klen);
+                if constexpr (XF) {
+                    b.x[2 * j] = bload<0>(rx, ok ? (xrow + k) * 4u : kOOB);
+                    b.x[2 * j + 1] = bload<0>(rx, ok ? (xrow + k) * 4u + 16u : kOOB);
+                } else {
+                    b.x[j] = bload<0>(rx, ok ? (xrow + k) * 2u : kOOB);
+                }
             }
-        } else {
-            run(std::false_type{}, 0);
-        }
-    };
-    // two batches alternate; the tail is peeled so that every load sits beside
-    // the products of the batch before it
-    const int mb = (nb - wave + NW - 1) / NW;  // this wave's batches (uniform)
-    if (mb > 0) {
+        };
+        auto mma = [&](const Batch &b) {
+            uint32_t u[RT][8];
+            float2 sv[RT][NG];
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                uint8_t *wl = wt[wave][i];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int r = 8 * h + lane / 8;
+                    *reinterpret_cast<u32x4 *>(wl + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = b.w[i][h];
+                }
+                // (groups past the row's end, and rows past the weight, meet zeros or are
+                // not stored: any place inside sc does)
+                const int r = min(16 * i + fr, rows - 1);
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const int gi = b.g + g * GS * 32 / group;
+                    sv[i][g] = sc[r * pitch + min(gi, sg - 1)];
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    u[i][j] = *reinterpret_cast<const uint32_t *>(wl + fr * 128 + ((j ^ (fr & 7)) << 4) + 4 * q);
+            }
+            // sh: power of two of this lane's row of X (scaled)
+            auto run = [&](auto scaled, int sh) {
+                constexpr bool SC = decltype(scaled)::value;
+                int back[4];  // those of the rows 4 q + r that acc holds
+#pragma unroll
+                for (int r = 0; r < 4; ++r) back[r] = SC ? __shfl(sh, 4 * q + r) : 0;
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    floatx4 tg[RT], xg = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int i = 0; i < RT; ++i) tg[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int e = 0; e < GS; ++e) {
+                        const int j = g * GS + e;
+                        u32x4 hi, lo = {0, 0, 0, 0};
+                        if constexpr (XF)
+                            split8<SC>(__builtin_bit_cast(floatx4, b.x[2 * j]),
+                                       __builtin_bit_cast(floatx4, b.x[2 * j + 1]), sh, hi, lo);
+                        else
+                            hi = pair_up(b.x[j]);
+                        const half8 xh = __builtin_bit_cast(half8, hi), xl = __builtin_bit_cast(half8, lo);
+                        xg = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, ones, xg, 0, 0, 0);
+                        if constexpr (XF) xg = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl, ones, xg, 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < RT; ++i) {
+                            const half8 wv = __builtin_bit_cast(half8, expand8(u[i][j]));
+                            tg[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, wv, tg[i], 0, 0, 0);
+                            if constexpr (XF) tg[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl, wv, tg[i], 0, 0, 0);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < RT; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float tv = SC ? __builtin_amdgcn_ldexpf(tg[i][r], back[r]) : tg[i][r];
+                            const float xv = SC ? __builtin_amdgcn_ldexpf(xg[r], back[r]) : xg[r];
+                            acc[i][r] = __builtin_fmaf(sv[i][g].y, xv, __builtin_fmaf(sv[i][g].x, tv, acc[i][r]));
+                        }
+                }
+            };
+            if constexpr (XF) {
+                floatx4 old[RT];
+#pragma unroll
+                for (int i = 0; i < RT; ++i) old[i] = acc[i];
+                run(std::false_type{}, 0);
+                bool bad = false;
+#pragma unroll
+                for (int i = 0; i < RT; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) bad = bad || !__builtin_isfinite(acc[i][r]);
+                if (__builtin_amdgcn_ballot_w64(bad) != 0) {
+                    float amax = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const floatx4 f = __builtin_bit_cast(floatx4, b.x[i]);
+                        amax = fmaxf(fmaxf(fmaxf(amax, fabsf(f.x)), fmaxf(fabsf(f.y), fabsf(f.z))), fabsf(f.w));
+                    }
+                    amax = fmaxf(amax, __shfl_xor(amax, 16));  // the four lanes of a row
+                    amax = fmaxf(amax, __shfl_xor(amax, 32));
+                    const int sh = __builtin_amdgcn_frexp_expf(amax) - 15;
+#pragma unroll
+                    for (int i = 0; i < RT; ++i) acc[i] = old[i];
+                    run(std::true_type{}, sh);
+                }
+            } else {
+                run(std::false_type{}, 0);
+            }
+        };
+        // two batches alternate; the tail is peeled so that every load sits beside
+        // the products of the batch before it
+        const int mb = (nb - wave + NW - 1) / NW;  // this wave's batches (uniform)
         Batch A, B;
-        load(A, wave);
-        int b = 0;
-        for (; b + 2 < mb; b += 2) {
-            load(B, wave + (b + 1) * NW);
-            __builtin_amdgcn_sched_barrier(0);
-            mma(A);
-            load(A, wave + (b + 2) * NW);
-            __builtin_amdgcn_sched_barrier(0);
-            mma(B);
-        }
-        if (b + 1 < mb) {
-            load(B, wave + (b + 1) * NW);
-            __builtin_amdgcn_sched_barrier(0);
-            mma(A);
-            mma(B);
-        } else {
-            mma(A);
+        if (mb > 0) load(A, wave);
+        __syncthreads();  // the scales are there
+        if (mb > 0) {
+            int b = 0;
+            for (; b + 2 < mb; b += 2) {
+                load(B, wave + (b + 1) * NW);
+                __builtin_amdgcn_sched_barrier(0);
+                mma(A);
+                load(A, wave + (b + 2) * NW);
+                __builtin_amdgcn_sched_barrier(0);
+                mma(B);
+            }
+            if (b + 1 < mb) {
+                load(B, wave + (b + 1) * NW);
+                __builtin_amdgcn_sched_barrier(0);
+                mma(A);
+                mma(B);
+            } else {
+                mma(A);
+            }
         }
     }
 #pragma unroll
     for (int i = 0; i < RT; ++i) red[wave][i][lane] = acc[i];
     __syncthreads();
-    // tile i is finished by wave i: lane l has weight row l % 16, rows 4 q + r of X
+    // tile i is finished by wave i % NW: lane l has weight row l % 16, rows 4 q + r of X
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
         if (wave != i % NW) continue;
@@ -436,6 +458,9 @@ __global__ __launch_bounds__(NW * 64) void k_linear4_mfma(const uint8_t *__restr
         }
     }
 }
+
+// Bytes of the kernel's scales in LDS.
+size_t scale_lds(int rt, int64_t gk) { return (size_t)16 * rt * (size_t)(std::min<int64_t>(gk, kSegGroups) | 1) * 8; }
 
 __global__ __launch_bounds__(TH) void k_dequantize4(const uint8_t *__restrict__ codes, const float *__restrict__ scales,
                                                     const float *__restrict__ biases, float *__restrict__ out,
@@ -525,8 +550,9 @@ int launch_mfma(const rq_qweight &w, const void *x, bool xf, void *y, bool yh, i
     auto go = [&](auto rt, auto nw, auto gs, auto xfc) {
         constexpr int RT = decltype(rt)::value, NW = decltype(nw)::value;
         hipLaunchKernelGGL((k_linear4_mfma<RT, NW, decltype(gs)::value, decltype(xfc)::value>),
-                           dim3((unsigned)cdiv(w.n_out, 16 * RT)), dim3(NW * 64), 0, s, (const uint8_t *)w.codes,
-                           w.scales, w.biases, x, y, yh ? 1 : 0, m, (int)w.n_out, (int)w.k_in, w.group);
+                           dim3((unsigned)cdiv(w.n_out, 16 * RT)), dim3(NW * 64), (unsigned)scale_lds(RT, w.k_in / w.group), s,
+                           (const uint8_t *)w.codes, w.scales, w.biases, x, y, yh ? 1 : 0, m, (int)w.n_out,
+                           (int)w.k_in, w.group);
     };
     auto by_group = [&](auto rt, auto nw, auto xfc) {
         if (w.group % 128 == 0) go(rt, nw, std::integral_constant<int, 4>{}, xfc);
