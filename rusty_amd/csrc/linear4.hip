@@ -237,8 +237,8 @@ __global__ __launch_bounds__(TH) void k_linear4_dot(const uint8_t *__restrict__ 
 // one is multiplied.  The waves' sums meet in LDS.
 // Scales and biases go through LDS too, whole rows of them first (they lie one
 // after another), as (s, b - 16 s): read by each lane in place they touch 16 cache
-// lines per load, which bounded the kernel (8 x 4096 x 4096 in groups of 64 8.9 us, of 32
-// XXX).  Rows longer than kSegGroups groups take several rounds.
+// lines per load, which bounded the kernel (8 rows, 11008x4096 in groups of 64 21.2 us,
+// 12.6 this way; 4096x11008 in groups of 32 32.3, 16.9).  Rows longer than kSegGroups groups take several rounds.
 // XF: f32 rows as two fp16 terms; a batch whose sums are not finite (values past
 // fp16's range) is multiplied again, each row scaled by a power of two.
 constexpr int kSegGroups = 512;
@@ -559,8 +559,23 @@ int launch_mfma(const rq_qweight &w, const void *x, bool xf, void *y, bool yh, i
         else if (w.group % 64 == 0) go(rt, nw, std::integral_constant<int, 2>{}, xfc);
         else go(rt, nw, std::integral_constant<int, 1>{}, xfc);
     };
-    if (xf) by_group(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{}, std::true_type{});
-    else by_group(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{}, std::false_type{});
+    // Waves and row tiles per block, measured (us, 8 rows, 1 tile of 4 waves / 1 of 8 / 2 of 4; f32 rows
+    // in brackets): 4096x4096 6.9 / 6.5 / 9.4 [10.0 / 10.4 / 13.2], 2048x2048 4.9 / 5.2 / 5.8, 4096x11008
+    // in groups of 32 16.9 / 13.5 / 26.6 [24.9 / 21.4 / 35.4], 11008x4096 12.6 / 16.0 / 13.0 (16 rows
+    // 15.9 / 19.2 / 15.4) [21.2 / 28.2 / 25.0], 32000x2048 18.1 / 28.5 / 14.8 [30.9 / 50.2 / 28.6].
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    using I4 = std::integral_constant<int, 4>;
+    using I8 = std::integral_constant<int, 8>;
+    const int64_t tiles = cdiv(w.n_out, 16);
+    const bool two = tiles >= 1024 || (!xf && m > 8 && tiles > 512), wide = tiles <= 256 && w.k_in > (xf ? 4096 : 2048);
+    auto by_shape = [&](auto xfc) {
+        if (two) by_group(I2{}, I4{}, xfc);
+        else if (wide) by_group(I1{}, I8{}, xfc);
+        else by_group(I1{}, I4{}, xfc);
+    };
+    if (xf) by_shape(std::true_type{});
+    else by_shape(std::false_type{});
     RQ_LAUNCH_CHECK();
     return RQ_OK;
 }
