@@ -52,6 +52,7 @@ struct AttnArgs {
     int k_row, v_row;                 // between a head's consecutive keys
     int n_heads, n_kv, n_seqs, capacity, max_nodes;
     int tokens;
+    int wide;     // packed: row tiles per key/value head that the device takes at once
     int splits;   // tree: the most pieces a sequence's keys are cut into
     float *part;  // splits > 1: sums [tokens][n_heads][splits][dim], then (m, l) [tokens][n_heads][splits]
     float c;      // |scale| log2 e
@@ -60,16 +61,25 @@ struct AttnArgs {
 
 __device__ __forceinline__ int seq_start(const AttnArgs &a, int s) { return min(max(a.starts[s], 0), a.tokens); }
 
-// The largest s < n_seqs with key(s) <= x (0 if there is none); key ascending.
+// The largest s < n_seqs with at(s, starts[s]) <= x (0 if there is none; at
+// ascending), and its bounds; x uniform across the wave.  The 64 lanes probe at
+// once: one memory round trip up to 63 sequences, one more per factor of 64.
 template <typename F>
-__device__ __forceinline__ int last_at_most(int n_seqs, int64_t x, F key) {
-    int lo = 0, hi = n_seqs;
-    while (hi - lo > 1) {
-        const int mid = (int)(((unsigned)lo + (unsigned)hi) / 2);
-        if (key(mid) <= x) lo = mid;
-        else hi = mid;
+__device__ __forceinline__ int find_seq(const AttnArgs &a, int64_t x, int *begin, int *end, F at) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = a.n_seqs;  // the answer is in lo .. lo + n - 1
+    while (n > 63) {
+        const int step = (n + 63) / 64, i = lo + (lane + 1) * step;
+        const bool in = (lane + 1) * step < n;
+        const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(in && at(i, seq_start(a, in ? i : 0)) <= x));
+        lo += c * step;
+        n = min(step, n - c * step);
     }
-    return lo;
+    const int v = seq_start(a, lo + min(lane, n));
+    const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane > 0 && lane < n && at(lo + lane, v) <= x));
+    *begin = __builtin_amdgcn_readlane(v, c);
+    *end = __builtin_amdgcn_readlane(v, c + 1);
+    return lo + c;
 }
 
 // Of n drafted positions, those that token t, the i-th of its sequence, sees, as bits.
@@ -82,9 +92,9 @@ __device__ __forceinline__ uint64_t tree_sees(const AttnArgs &a, int t, int i, i
 struct TreeSeq {
     int s0, nodes;      // first token, tokens served
     int before, keys;   // cached positions before them; all positions there are
-    __device__ __forceinline__ TreeSeq(const AttnArgs &a, int s) {
-        s0 = seq_start(a, s);
-        nodes = min(max(seq_start(a, s + 1) - s0, 0), a.max_nodes);
+    __device__ __forceinline__ TreeSeq(const AttnArgs &a, int s) : TreeSeq(a, s, seq_start(a, s), seq_start(a, s + 1)) {}
+    __device__ __forceinline__ TreeSeq(const AttnArgs &a, int s, int begin, int end) : s0(begin) {
+        nodes = min(max(end - begin, 0), a.max_nodes);
         before = min(max(a.lengths[s], 0), a.capacity);
         keys = before + min(nodes, a.capacity - before);
     }
@@ -152,13 +162,17 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
     } else {
         // Row tiles of the sequences, one after another: sequence s has the
         // indexes from starts[s] grp / BR + s on, at least as many as it needs.
-        // The last first: a long prompt's heaviest tiles start early.
-        const int64_t t = gridDim.x / a.n_kv - 1 - blockIdx.x / a.n_kv;
-        auto tile0 = [&](int s) { return (int64_t)seq_start(a, s) * grp / BR + s; };
-        const int s = last_at_most(a.n_seqs, t, tile0);
-        s0 = seq_start(a, s);
-        nq = max(seq_start(a, s + 1) - s0, 0);
-        const int64_t row = (t - tile0(s)) * BR;
+        // The last first, a long prompt's heaviest; every other run of as many as
+        // the device takes at once the other way round, so that a CU which got
+        // a heavy block gets a light one next.
+        const int total = gridDim.x / a.n_kv, rank = blockIdx.x / a.n_kv, run = rank / a.wide;
+        const int flip = run & 1 ? run * a.wide + min((run + 1) * a.wide, total) - 1 - rank : rank;
+        const int64_t t = total - 1 - flip;
+        auto tile0 = [&](int s, int begin) { return (int64_t)begin * grp / BR + s; };
+        int end;
+        const int s = find_seq(a, t, &s0, &end, tile0);
+        nq = max(end - s0, 0);
+        const int64_t row = (t - tile0(s, s0)) * BR;
         if (row < 0 || row >= (int64_t)nq * grp) return;
         // rows are counted from the tile's first token on
         const int skip = (int)(row / grp);
@@ -279,8 +293,8 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
         floatx16 sc[TPW];
 #pragma unroll
         for (int i = 0; i < TPW; ++i) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) sc[i][e] = 0.0f;
+            const floatx16 zero = {};
+            sc[i] = zero;
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 const u32x4 kf = *(lds_u32x4 *)(uintptr_t)(tb + ka[s] + (uint32_t)(i * 32 * ROW));
@@ -502,8 +516,9 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= (int64_t)a.tokens * a.n_heads) return;
     const int t = (int)(row / a.n_heads), head = (int)(row - (int64_t)t * a.n_heads), lane = threadIdx.x & 63;
-    const int s = last_at_most(a.n_seqs, t, [&](int i) { return (int64_t)seq_start(a, i); });
-    const TreeSeq q(a, s);
+    int begin, end;
+    const int s = find_seq(a, t, &begin, &end, [](int, int at) { return (int64_t)at; });
+    const TreeSeq q(a, s, begin, end);
     const int i = t - q.s0;
     if (i < 0 || i >= q.nodes) return;
     const int per = q.per_piece(KT, a.splits), tiles = (q.keys + KT - 1) / KT;
@@ -548,18 +563,24 @@ int launch(const AttnArgs &a, hipStream_t s) {
     return RQ_OK;
 }
 
+// Rows per block.  Fewer where blocks of 128 would leave CUs without work, and
+// for f32, whose blocks take longest (us, 128 rows / 64 / 32: one prompt of 300 tokens,
+// 32/4 heads of 64, 9.2 / 8.2 / 7.8; three of 417, 1000 and 83 in f32 121 / 70 / 92; one of 2048 39.4 /
+// 38.4 / 53.4, of 8192 with 32/8 heads of 128 659 / 790 / 1642).
 template <typename T, int HD>
-int launch_packed(const AttnArgs &a, hipStream_t s) {
+int launch_packed(const AttnArgs &a, int cus, hipStream_t s) {
+    const int64_t blocks = cdiv((int64_t)a.tokens * a.n_heads, 128);
+    if (sizeof(T) == 4 || blocks < cus) return launch<T, HD, 2, 2, false>(a, s);
     return launch<T, HD, 4, 1, false>(a, s);
 }
 
-// Rows of a tree block (32 or 64 or 128 by the rows a sequence may have) and
-// the pieces its keys may be cut into: enough blocks for two per CU.
+// Rows of a tree block (32, 64 or 128 by the rows a sequence may have) and the
+// pieces its keys may be cut into: one block per CU and layer of rows, pieces of
+// four tiles or more (fp16; joining them costs a launch and a pass over their sums).
 int tree_rows(int64_t rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
 int tree_splits(int64_t n_seqs, int64_t n_kv, int64_t rows, int64_t capacity, bool f16) {
-    const int wr = tree_rows(rows);
-    const int64_t blocks = n_seqs * n_kv * cdiv(rows, 32 * wr), kt = wr == 1 && f16 ? 128 : 64;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(blocks, 1), cdiv(capacity, kt), 64}));
+    const int64_t kt = tree_rows(rows) == 1 && f16 ? 128 : 64, heads = std::max<int64_t>(n_seqs * n_kv, 1);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({256 / heads, cdiv(capacity, kt * (f16 ? 4 : 1)), 64}));
 }
 
 template <typename T, int HD>
@@ -696,9 +717,11 @@ int rq_attn_packed(rq_ctx *ctx, const rq_attn *attn, const void *q, const void *
     const int st = check_packed(attn, q, k, v, starts, n_seqs, tokens, out, a, run);
     if (st != RQ_OK || !run) return st;
     hipStream_t s = pick(ctx, stream);
+    const int cus = ctx->num_cus;
+    a.wide = std::max(1, cus / a.n_kv);
     if (attn->dtype == RQ_F16)
-        return attn->head_dim == 64 ? launch_packed<_Float16, 64>(a, s) : launch_packed<_Float16, 128>(a, s);
-    return attn->head_dim == 64 ? launch_packed<float, 64>(a, s) : launch_packed<float, 128>(a, s);
+        return attn->head_dim == 64 ? launch_packed<_Float16, 64>(a, cus, s) : launch_packed<_Float16, 128>(a, cus, s);
+    return attn->head_dim == 64 ? launch_packed<float, 64>(a, cus, s) : launch_packed<float, 128>(a, cus, s);
 }
 
 size_t rq_attn_tree_workspace(const rq_attn *attn, int32_t n_seqs, int64_t tokens, int32_t max_nodes,
