@@ -25,6 +25,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 #include "lds_dma.hpp"
@@ -287,12 +288,13 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
     typedef __attribute__((address_space(3))) const float lds_float;
     typedef __attribute__((address_space(3))) const _Float16 lds_half;
 
-    // the wave's pieces of the tile at LDS address tb, its first key key0
-    auto keys = [&](auto masked_c, uint32_t tb, int key0) {
+    // the first N of the wave's pieces of the tile at LDS address tb, its first key key0
+    auto keys = [&](auto masked_c, auto n_c, uint32_t tb, int key0) {
         constexpr bool MASKED = decltype(masked_c)::value;
-        floatx16 sc[TPW];
+        constexpr int N = decltype(n_c)::value;
+        floatx16 sc[N];
 #pragma unroll
-        for (int i = 0; i < TPW; ++i) {
+        for (int i = 0; i < N; ++i) {
             const floatx16 zero = {};
             sc[i] = zero;
 #pragma unroll
@@ -313,15 +315,18 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
         const uint64_t sees = MASKED ? visible(key0) : 0;
         if constexpr (MASKED) {
             const uint64_t mine = sees >> (4 * hf);
+            const int upto = before + qi + 1 - key0 - 4 * hf;
 #pragma unroll
-            for (int i = 0; i < TPW; ++i)
+            for (int i = 0; i < N; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    sc[i][e] = mine >> (32 * i + 8 * (e >> 2) + (e & 3)) & 1 ? sc[i][e] : -__builtin_inff();
+                for (int e = 0; e < 16; ++e) {
+                    const int j = 32 * i + 8 * (e >> 2) + (e & 3);
+                    sc[i][e] = (TREE ? mine >> j & 1 : j < upto) ? sc[i][e] : -__builtin_inff();
+                }
         }
         float mt = sc[0][0];
 #pragma unroll
-        for (int i = 0; i < TPW; ++i)
+        for (int i = 0; i < N; ++i)
 #pragma unroll
             for (int e = 0; e < 16; ++e) mt = fmaxf(mt, sc[i][e]);
         mt = fmaxf(mt, __shfl_xor(mt, 32)) * a.c;
@@ -339,7 +344,7 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
         }
         const float off = mc == -__builtin_inff() ? 0.0f : -mc;  // no key yet: every weight is 2^-inf
 #pragma unroll
-        for (int i = 0; i < TPW; ++i) {
+        for (int i = 0; i < N; ++i) {
             float t[4];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -354,25 +359,25 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
             // A value that is not finite must not meet the zero weight of a
             // row that does not see its key: such a piece is summed by element.
             float z = 0.0f;
+            h2_t z2 = {(_Float16)0.0f, (_Float16)0.0f};
 #pragma unroll
-            for (int u = 0; u < TPW * 32 * ROW / 1024; ++u) {
+            for (int u = 0; u < N * 32 * ROW / 1024; ++u) {
                 const u32x4 x = *(lds_u32x4 *)(uintptr_t)(vt + (uint32_t)(kp * ROW + u * 1024 + lane * 16));
                 const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if constexpr (F16) {
-                        const h2_t h = __builtin_bit_cast(h2_t, xw[e]) * (h2_t){(_Float16)0.0f, (_Float16)0.0f};
-                        z += (float)(h.x + h.y);
-                    } else {
+                    if constexpr (F16)
+                        z2 = __builtin_elementwise_fma(__builtin_bit_cast(h2_t, xw[e]), (h2_t){(_Float16)0.0f, (_Float16)0.0f}, z2);
+                    else
                         z = __builtin_fmaf(__builtin_bit_cast(float, xw[e]), 0.0f, z);
-                    }
                 }
             }
+            if constexpr (F16) z = (float)z2.x + (float)z2.y;
             if (__builtin_amdgcn_ballot_w64(z != z)) {
-                for (int kk = 0; kk < 32 * TPW; ++kk) {
+                for (int kk = 0; kk < 32 * N; ++kk) {
                     float p = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < TPW; ++i)
+                    for (int i = 0; i < N; ++i)
 #pragma unroll
                         for (int e = 0; e < 16; ++e)
                             p = kk / 32 == i && 4 * (kk % 32 / 8) + kk % 4 == e ? sc[i][e] : p;
@@ -397,16 +402,16 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
             }
         }
         if constexpr (F16) {
-            half8 pf[TPW][2];
+            half8 pf[N][2];
 #pragma unroll
-            for (int i = 0; i < TPW; ++i)
+            for (int i = 0; i < N; ++i)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) pf[i][e >> 3][e & 7] = (_Float16)sc[i][e];
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 lds_short4 *pa = (lds_short4 *)(uintptr_t)(vt + va[d][0]), *pb = (lds_short4 *)(uintptr_t)(vt + va[d][1]);
 #pragma unroll
-                for (int i = 0; i < TPW; ++i)
+                for (int i = 0; i < N; ++i)
 #pragma unroll
                     for (int s2 = 0; s2 < 2; ++s2) {
                         const uint2 ua = __builtin_bit_cast(
@@ -419,7 +424,7 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < TPW; ++i)
+            for (int i = 0; i < N; ++i)
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
 #pragma unroll
@@ -437,8 +442,10 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
         dma(kt + NS - 1);
         const int key0 = (first + kt) * KT + kp;
         const uint32_t tb = lds0 + (uint32_t)(kt % NS) * (2 * TILE);
-        if (key0 + 32 * TPW <= masked_from) keys(std::false_type{}, tb, key0);
-        else if (key0 < key_end) keys(std::true_type{}, tb, key0);
+        using All = std::integral_constant<int, TPW>;
+        if (key0 + 32 * TPW <= masked_from) keys(std::false_type{}, All{}, tb, key0);
+        else if (key0 + 32 * (TPW - 1) < key_end) keys(std::true_type{}, All{}, tb, key0);
+        else if (key0 < key_end) keys(std::true_type{}, std::integral_constant<int, 1>{}, tb, key0);
     }
     wait_vmcnt<0>();  // no DMA in flight past this point
 
