@@ -435,16 +435,26 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
                     }
             }
         } else {
+            // V's values of 8 keys at a time, all read before the first is used: one by
+            // one, each instruction waited for its own
 #pragma unroll
             for (int i = 0; i < N; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
+                for (int e8 = 0; e8 < 16; e8 += 8) {
+                    float x[8][DT];
 #pragma unroll
-                    for (int d = 0; d < DT; ++d) {
-                        const float x = *(lds_float *)(uintptr_t)(vt + va[d][0] +
-                                                                  (uint32_t)((32 * i + 8 * (e >> 2) + (e & 3)) * ROW));
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, sc[i][e], o[d], 0, 0, 0);
-                    }
+                    for (int e = 0; e < 8; ++e)
+#pragma unroll
+                        for (int d = 0; d < DT; ++d)
+                            x[e][d] = *(lds_float *)(uintptr_t)(vt + va[d][0] +
+                                                                (uint32_t)((32 * i + 8 * ((e8 + e) >> 2) + (e & 3)) * ROW));
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+#pragma unroll
+                        for (int d = 0; d < DT; ++d)
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e][d], sc[i][e8 + e], o[d], 0, 0, 0);
+                }
         }
     };
     for (int kt = 0; kt < ntiles; ++kt) {
