@@ -582,23 +582,41 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
     if (pieces <= 1) return;  // written by the block that had them all
     const float *po = a.part + row * a.splits * HD;
     const float2 *ml = reinterpret_cast<const float2 *>(a.part + (int64_t)a.tokens * a.n_heads * a.splits * HD) + row * a.splits;
-    float top = -__builtin_inff();
-    for (int p = 0; p < pieces; ++p) top = fmaxf(top, ml[p].x);
+    // lane p has piece p's weight (at most 64 pieces); G pieces are added at once, 16 bytes a lane
+    constexpr int L = HD / 4, G = 64 / L;
+    const float2 mine = lane < pieces ? ml[lane] : make_float2(-__builtin_inff(), 0.0f);
+    float top = mine.x;
+#pragma unroll
+    for (int w = 32; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor(top, w));
     const float base = top == -__builtin_inff() ? 0.0f : top;
-    constexpr int E = HD / 64;
-    float l = 0.0f, o[E];
+    const float wt = __builtin_amdgcn_exp2f(mine.x - base);
+    float l = wt * mine.y, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.0f;
-    for (int p = 0; p < pieces; ++p) {
-        const float w = __builtin_amdgcn_exp2f(ml[p].x - base);
-        l = __builtin_fmaf(w, ml[p].y, l);
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(w, po[p * HD + E * lane + e], o[e]);
+    for (int w = 32; w > 0; w >>= 1) l += __shfl_xor(l, w);
+    const int gi = lane / L, at = 4 * (lane % L);
+#pragma unroll 4
+    for (int p = gi; p < pieces + gi; p += G) {  // the same count for every lane
+        const bool in = p < pieces;
+        const float w = __shfl(wt, in ? p : 0);
+        const float4 v = *reinterpret_cast<const float4 *>(po + (int64_t)(in ? p : 0) * HD + at);
+        if (in) {
+            o[0] = __builtin_fmaf(w, v.x, o[0]);
+            o[1] = __builtin_fmaf(w, v.y, o[1]);
+            o[2] = __builtin_fmaf(w, v.z, o[2]);
+            o[3] = __builtin_fmaf(w, v.w, o[3]);
+        }
     }
-    const bool none = q.before == 0 && tree_sees(a, t, i, q.keys) == 0;
-    T *op = static_cast<T *>(a.out) + (int64_t)t * a.out_row + head * HD + E * lane;
 #pragma unroll
-    for (int e = 0; e < E; ++e) op[e] = (T)(none ? 0.0f : o[e] / l);
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int w = 32; w >= L; w >>= 1) o[e] += __shfl_xor(o[e], w);
+    if (gi != 0) return;
+    const bool none = q.before == 0 && tree_sees(a, t, i, q.keys) == 0;
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+    vec4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (T)(none ? 0.0f : o[e] / l);
+    *reinterpret_cast<vec4 *>(static_cast<T *>(a.out) + (int64_t)t * a.out_row + head * HD + at) = v;
 }
 
 // Launches k_attn<T, HD, WR, KG, TREE> with BR = 32 WR rows per block.
@@ -619,24 +637,28 @@ int launch(const AttnArgs &a, hipStream_t s) {
     return RQ_OK;
 }
 
-// Rows per block.  Fewer where blocks of 128 would leave CUs without work, and
-// for f32, whose blocks take longest (us, 128 rows / 64 / 32: one prompt of 300 tokens,
-// 32/4 heads of 64, 9.2 / 8.2 / 7.8; three of 417, 1000 and 83 in f32 121 / 70 / 92; one of 2048 39.4 /
-// 38.4 / 53.4, of 8192 with 32/8 heads of 128 659 / 790 / 1642).
+// Rows per block: 64 where blocks of 128 would leave CUs without work, in f32, whose
+// blocks take longer, without two blocks (us, 128 rows / 64 / 32: one prompt of 300
+// tokens, 32/4 heads of 64, 9.2 / 8.2 / 7.8, of 2048 39.4 / 38.4 / 53.4, of 8192 with 32/8 heads of 128
+// 570 / 666 / 1487; f32, three of 417, 1000 and 83 87 / 61 / 72, one of 2048 160 / 166 / 195).
 template <typename T, int HD>
 int launch_packed(const AttnArgs &a, int cus, hipStream_t s) {
     const int64_t blocks = cdiv((int64_t)a.tokens * a.n_heads, 128);
-    if (sizeof(T) == 4 || blocks < cus) return launch<T, HD, 2, 2, false>(a, s);
+    if (blocks < (sizeof(T) == 4 ? 2 : 1) * cus) return launch<T, HD, 2, 2, false>(a, s);
     return launch<T, HD, 4, 1, false>(a, s);
 }
 
 // Rows of a tree block (32, 64 or 128 by the rows a sequence may have) and the
-// pieces its keys may be cut into: one block per CU and layer of rows, pieces of
-// four tiles or more (fp16; joining them costs a launch and a pass over their sums).
+// pieces its keys may be cut into: one block per CU and layer of rows.  A cache of
+// a few tiles stays whole: joining pieces costs a launch, about what four tiles take
+// (one token, 513 keys, 8.6 us whole, 9.2 in two; eight trees of 16 over 37 to 2047
+// keys in 4 / 8 / 16 pieces 17.1 / 16.4 / 21.8; 32702 keys, 32/8 heads of 128, in 16 / 32 / 64 41 / 39 / 54).
 int tree_rows(int64_t rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
 int tree_splits(int64_t n_seqs, int64_t n_kv, int64_t rows, int64_t capacity, bool f16) {
-    const int64_t kt = tree_rows(rows) == 1 && f16 ? 128 : 64, heads = std::max<int64_t>(n_seqs * n_kv, 1);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({256 / heads, cdiv(capacity, kt * (f16 ? 4 : 1)), 64}));
+    const bool few = tree_rows(rows) == 1 && f16;  // tiles of 128 keys
+    const int64_t tiles = cdiv(capacity, few ? 128 : 64), heads = std::max<int64_t>(n_seqs * n_kv, 1);
+    if (f16 && tiles <= 5) return 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({256 / heads, f16 && !few ? cdiv(tiles, 2) : tiles, 64}));
 }
 
 template <typename T, int HD>
