@@ -472,6 +472,23 @@ int rq_llama_set_prefill(rq_llama *model, int32_t rows);
  * instantiates it on `stream` (stream capture, no device work) before
  * launching it. */
 int rq_llama_decode(rq_llama *model, int32_t n_steps, rq_stream stream);
+/* One pass over n drafted continuations of the sequence, a tree, in place of
+ * single decode steps (speculative decoding; no reference counterpart).
+ * Draft i is the token tokens[i] after draft parents[i] < i, or after the
+ * sequence's last token for parents[i] = -1 (host arrays; n 0..63, NULL for
+ * n = 0).  All drafts go through the model at once, each attending to the
+ * sequence and its own ancestors (rq_attn_tree over the runner's KV cache).  Then,
+ * from the sequence's last token on, the greedy token is followed as long as it
+ * is a draft of the current one (the first such draft of equal ones); the
+ * followed drafts and the last greedy token join the sequence, which grows by
+ * *accepted + 1 tokens, and their keys and values take their places in the
+ * cache.  The result is what as many rq_llama_decode steps give, up to the
+ * rounding of the kernels that many rows take.  Needs n + 1 free positions
+ * (RQ_ERR_SHAPE otherwise); on an error the sequence is as it was.  The first
+ * call allocates [64, vocab] logits.  Uses the context's GEMM workspace as
+ * rq_llama_prefill does.  Synchronizes. */
+int rq_llama_verify(rq_llama *model, const int32_t *tokens, const int32_t *parents, int32_t n, int32_t *accepted,
+                    rq_stream stream);
 /* Steps run as graph launches (default, use_graph = 1: four steps or one
  * per launch) or as direct kernel launches on the stream (0: for tools that
  * do not trace graphs). */

@@ -156,6 +156,7 @@ _SIGNATURES = {
     "rq_llama_destroy": [_P],
     "rq_llama_prefill": [_P, POINTER(c_int32), c_int32, _P],
     "rq_llama_decode": [_P, c_int32, _P],
+    "rq_llama_verify": [_P, POINTER(c_int32), POINTER(c_int32), c_int32, POINTER(c_int32), _P],
     "rq_qmatmul_lora_workspace": [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, c_int, c_int],
     "rq_qmatmul_lora": [_P, POINTER(rq_qweight), _P, c_int, _P, _P, ctypes.c_int64, _P, c_int, ctypes.c_int64, _P,
                         c_size_t, _P],

@@ -62,6 +62,8 @@ struct rq_llama {
     _Float16 *pxn = nullptr, *pq = nullptr, *patt = nullptr, *ph = nullptr;
     int prefill_cap = 0;   // rows the buffers hold
     int prefill_rows = 0;  // rows per batched chunk; 0: one position at a time through the step graph
+    // drafted trees, allocated by the first rq_llama_verify
+    void *verify = nullptr;
     hipGraph_t graph = nullptr;  // one decode step
     hipGraphExec_t exec = nullptr;
     hipGraph_t graph_k = nullptr;  // kGraphSteps consecutive steps
@@ -576,6 +578,211 @@ int prefill_chunk(rq_llama *md, int p0, int n, bool end, hipStream_t s) {
     return RQ_OK;
 }
 
+// ---- drafted trees ---------------------------------------------------------
+// Row 0 of a pass is the sequence's last token, row i + 1 draft i.  Rows sit in
+// the cache right behind the sequence, row r at position pos + r, whatever their
+// depth; the accepted ones are moved to their places afterwards.
+constexpr int kVerifyRows = 64;
+
+struct VerifyHost {  // uploaded per pass
+    int tokens[kVerifyRows], parents[kVerifyRows], depth[kVerifyRows];
+    uint64_t mask[kVerifyRows];  // the row itself and its ancestors
+    int starts[2], length, pad;
+};
+struct VerifyOut {
+    int accepted, last;        // drafts followed, the row of the last one (0: none)
+    int path[kVerifyRows];     // their rows
+};
+struct VerifyBuffers {
+    VerifyHost *in;
+    VerifyOut *out;
+    int *next;                 // greedy token after each row
+    float *logits;             // [kVerifyRows][vocab]
+    void *work;                // of the attention
+    size_t work_bytes;
+};
+
+// RoPE (kernels.wgsl:60-79) on q and k of row s at position pos + depth[s]; q to
+// fp16 [rows][n_heads][hd], k and v (fp16) to cache position pos + s.
+__global__ __launch_bounds__(NT) void k_rope_tree(const float *__restrict__ qkv, const float2 *__restrict__ rope,
+                                                  const int *__restrict__ depth, int pos, int n_heads, int n_kv, int hd,
+                                                  int max_seq, _Float16 *__restrict__ q, _Float16 *__restrict__ kc,
+                                                  _Float16 *__restrict__ vc) {
+    const int s = blockIdx.x, half = hd / 2;
+    const float *row = qkv + (size_t)s * (n_heads + 2 * n_kv) * hd;
+    const float2 *cs = rope + (size_t)(pos + depth[s]) * half;
+    for (int i = threadIdx.x; i < (n_heads + 2 * n_kv) * half; i += NT) {
+        const int h = i / half, d = i % half;
+        const float a = row[h * hd + d], b = row[h * hd + d + half];
+        const float2 c = cs[d];
+        const bool rot = h < n_heads + n_kv;
+        _Float16 *o = h < n_heads ? q + ((size_t)s * n_heads + h) * hd
+                      : rot ? kc + ((size_t)(h - n_heads) * max_seq + pos + s) * hd
+                            : vc + ((size_t)(h - n_heads - n_kv) * max_seq + pos + s) * hd;
+        o[d] = (_Float16)(rot ? a * c.x - b * c.y : a);
+        o[d + half] = (_Float16)(rot ? a * c.y + b * c.x : b);
+    }
+}
+
+// The greedy token of each row's logits, picked as k_argmax_embed picks it.
+__global__ __launch_bounds__(AT) void k_argmax_rows(const float *__restrict__ logits, int V, int *__restrict__ next) {
+    __shared__ float bv[AT / 64];
+    __shared__ int bi[AT / 64];
+    const float *row = logits + (size_t)blockIdx.x * V;
+    const int t = threadIdx.x;
+    float best = -1e9f;
+    int idx = 0;
+    auto take = [&](float ov, int oi) {
+        if (ov > best || (ov == best && oi < idx)) {
+            best = ov;
+            idx = oi;
+        }
+    };
+    for (int i = t; i < V; i += AT) {
+        const float v = row[i];
+        if (v > best) {  // ascending: the first of equal ones
+            best = v;
+            idx = i;
+        }
+    }
+#pragma unroll
+    for (int w = 32; w > 0; w >>= 1) take(__shfl_xor(best, w), __shfl_xor(idx, w));
+    if ((t & 63) == 0) {
+        bv[t >> 6] = best;
+        bi[t >> 6] = idx;
+    }
+    __syncthreads();
+    if (t == 0) {
+        for (int w = 1; w < AT / 64; ++w) take(bv[w], bi[w]);
+        next[blockIdx.x] = idx;
+    }
+}
+
+// Follows the greedy tokens through the tree, appends them to the sequence and
+// leaves the step state where the decode steps continue.  One block.
+__global__ __launch_bounds__(NT) void k_verify_accept(const VerifyHost *__restrict__ in, int rows, int pos,
+                                                      const int *__restrict__ next, const float *__restrict__ all,
+                                                      int V, const _Float16 *__restrict__ embed, int H,
+                                                      int *__restrict__ tokens, int *__restrict__ pos_p,
+                                                      int *__restrict__ n_prompt_p, float *__restrict__ x,
+                                                      float *__restrict__ logits, VerifyOut *__restrict__ out) {
+    __shared__ int last_s, token_s;
+    if (threadIdx.x == 0) {
+        int cur = 0, n = 0;
+        for (;;) {
+            const int want = next[cur];
+            int child = 0;
+            for (int r = cur + 1; r < rows && !child; ++r)
+                if (in->parents[r] == cur && in->tokens[r] == want) child = r;
+            tokens[pos + n + 1] = want;
+            if (!child) break;
+            out->path[n++] = child;
+            cur = child;
+        }
+        out->accepted = n;
+        out->last = cur;
+        *pos_p = pos + n + 1;
+        *n_prompt_p = pos + n + 1;
+        last_s = cur;
+        token_s = next[cur];
+    }
+    __syncthreads();
+    const _Float16 *row = embed + (size_t)token_s * H;
+    for (int i = threadIdx.x; i < H; i += NT) x[i] = (float)row[i];
+    const float *lr = all + (size_t)last_s * V;
+    for (int i = threadIdx.x; i < V; i += NT) logits[i] = lr[i];
+}
+
+// Moves the accepted rows' keys and values to positions pos + 1, pos + 2, ...:
+// one thread per 16 bytes of a head's row, in path order (a row moves down and
+// no place is written before what lies there was read).
+__global__ __launch_bounds__(NT) void k_verify_compact(const VerifyOut *__restrict__ out, _Float16 *__restrict__ kc,
+                                                       _Float16 *__restrict__ vc, int pos, int hd, int max_seq,
+                                                       int heads) {
+    const int chunks = hd / 8, i = blockIdx.x * NT + threadIdx.x;
+    if (i >= 2 * heads * chunks) return;
+    const int which = i / (heads * chunks), head = i / chunks % heads, c = i % chunks;
+    uint4 *base = reinterpret_cast<uint4 *>((which ? vc : kc) + (size_t)head * max_seq * hd) + c;
+    for (int j = 0; j < out->accepted; ++j) {
+        const int from = out->path[j];
+        if (from != j + 1) base[(size_t)(pos + j + 1) * chunks] = base[(size_t)(pos + from) * chunks];
+    }
+}
+
+// Carves (base non-null) or sizes the buffers of rq_llama_verify.
+size_t verify_buffers(const rq_llama *md, char *base, VerifyBuffers &b) {
+    const rq_llama_config &c = md->cfg;
+    size_t used = 0;
+    auto take = [&](size_t bytes) {
+        char *p = base + used;
+        used += (bytes + 255) & ~size_t(255);
+        return p;
+    };
+    rq_attn at{};
+    at.n_heads = c.n_heads;
+    at.n_kv_heads = c.n_kv_heads;
+    at.head_dim = c.head_dim;
+    at.dtype = RQ_F16;
+    b.work_bytes = 0;  // of any number of rows
+    for (int rows = 1; rows <= kVerifyRows; ++rows)
+        b.work_bytes = std::max(b.work_bytes, rq_attn_tree_workspace(&at, 1, rows, rows, c.max_seq));
+    b.in = reinterpret_cast<VerifyHost *>(take(sizeof(VerifyHost)));
+    b.out = reinterpret_cast<VerifyOut *>(take(sizeof(VerifyOut)));
+    b.next = reinterpret_cast<int *>(take(kVerifyRows * 4));
+    b.logits = reinterpret_cast<float *>(take((size_t)kVerifyRows * c.vocab * 4));
+    b.work = take(b.work_bytes);
+    return used;
+}
+
+// The pass: rows of the tree through every layer at once, the pick, the walk and the cache rows.
+int verify_pass(rq_llama *md, const VerifyBuffers &b, int rows, hipStream_t s) {
+    const rq_llama_config &c = md->cfg;
+    const int H = c.hidden, pos = md->host_pos;
+    const size_t kv_layer = (size_t)c.n_kv_heads * c.max_seq * c.head_dim;
+    const GemmWorkspace ws = gemm_workspace(md->ctx, s);
+    rq_attn at{};
+    at.n_heads = c.n_heads;
+    at.n_kv_heads = c.n_kv_heads;
+    at.head_dim = c.head_dim;
+    at.dtype = RQ_F16;
+    int st;
+    if ((st = launch_embed_rows(b.in->tokens, md->embed, H, md->px, rows, s)) != RQ_OK) return st;
+    for (int l = 0; l < c.n_layers; ++l) {
+        const rq_llama::Layer &L = md->layers[l];
+        _Float16 *kc = md->kc + l * kv_layer, *vc = md->vc + l * kv_layer;
+        if ((st = launch_add_rmsnorm_rows(md->px, l ? md->py : nullptr, L.attn_norm, c.norm_eps, md->pxn, rows, H, s)) ||
+            (st = qmatmul_dispatch(md->ctx, L.qkv, md->pxn, RQ_F16, md->pqkv, RQ_F32, rows, ws, s)))
+            return st;
+        hipLaunchKernelGGL(k_rope_tree, dim3(rows), dim3(NT), 0, s, md->pqkv, md->rope, b.in->depth, pos, c.n_heads,
+                           c.n_kv_heads, c.head_dim, c.max_seq, md->pq, kc, vc);
+        RQ_LAUNCH_CHECK();
+        rq_kv_cache kv{};
+        kv.k = kc;
+        kv.v = vc;
+        kv.n_seqs = 1;
+        kv.capacity = c.max_seq;
+        if ((st = rq_attn_tree(md->ctx, &at, &kv, md->pq, b.in->starts, &b.in->length, b.in->mask, rows, rows, md->patt,
+                               b.work, b.work_bytes, s)) ||
+            (st = qmatmul_dispatch(md->ctx, L.o, md->patt, RQ_F16, md->py, RQ_F32, rows, ws, s)) ||
+            (st = launch_add_rmsnorm_rows(md->px, md->py, L.mlp_norm, c.norm_eps, md->pxn, rows, H, s)) ||
+            (st = swiglu_run(md->ctx, L.gate, L.up, L.down, md->pxn, RQ_F16, md->ph, md->py, RQ_F32, rows, ws, s)))
+            return st;
+    }
+    if ((st = launch_add_rmsnorm_rows(md->px, md->py, md->final_norm, c.norm_eps, md->pxn, rows, H, s)) ||
+        (st = qmatmul_dispatch(md->ctx, md->lm_head, md->pxn, RQ_F16, b.logits, RQ_F32, rows, ws, s)))
+        return st;
+    hipLaunchKernelGGL(k_argmax_rows, dim3(rows), dim3(AT), 0, s, b.logits, c.vocab, b.next);
+    RQ_LAUNCH_CHECK();
+    hipLaunchKernelGGL(k_verify_accept, dim3(1), dim3(NT), 0, s, b.in, rows, pos, b.next, b.logits, c.vocab, md->embed, H,
+                       md->tokens, md->pos, md->n_prompt, md->x, md->logits, b.out);
+    RQ_LAUNCH_CHECK();
+    const int heads = c.n_layers * c.n_kv_heads;  // the layers' caches lie one after another
+    hipLaunchKernelGGL(k_verify_compact, dim3((unsigned)cdiv(2 * heads * (c.head_dim / 8), NT)), dim3(NT), 0, s, b.out,
+                       md->kc, md->vc, pos, c.head_dim, c.max_seq, heads);
+    RQ_LAUNCH_CHECK();
+    return RQ_OK;
+}
+
 // Decode steps per replay of the multi-step graph: the steps are device-driven
 // (position and token live in device memory), so one graph may hold several,
 // which saves the gap between consecutive graph launches (~3-4 us each).
@@ -641,6 +848,7 @@ void release(rq_llama *md) {
     if (md->exec_k) (void)hipGraphExecDestroy(md->exec_k);
     if (md->graph_k) (void)hipGraphDestroy(md->graph_k);
     if (md->owned) (void)hipFree(md->owned);
+    if (md->verify) (void)hipFree(md->verify);
     delete md;
 }
 
@@ -873,6 +1081,56 @@ int rq_llama_decode(rq_llama *md, int32_t n_steps, rq_stream stream) {
     if ((st = run_steps(md, n_steps, s)) != RQ_OK) return st;
     md->host_pos += n_steps;
     md->host_len += n_steps;
+    return RQ_OK;
+}
+
+int rq_llama_verify(rq_llama *md, const int32_t *tokens, const int32_t *parents, int32_t n, int32_t *accepted,
+                    rq_stream stream) {
+    if (!md) return fail(RQ_ERR_INVALID_ARGUMENT, "null runner");
+    RQ_ENTER(md->ctx);
+    if (!accepted || (n > 0 && (!tokens || !parents))) return fail(RQ_ERR_INVALID_ARGUMENT, "null argument");
+    if (n < 0 || n >= kVerifyRows) return fail(RQ_ERR_SHAPE, "%d drafts outside 0..%d", n, kVerifyRows - 1);
+    if (md->host_len == 0) return fail(RQ_ERR_INVALID_ARGUMENT, "no sequence: call rq_llama_prefill first");
+    const int rows = n + 1;
+    if (rows > md->cfg.max_seq - md->host_pos || rows > md->prefill_cap)
+        return fail(RQ_ERR_SHAPE, "%d drafts after position %d exceed max_seq %d", n, md->host_pos, md->cfg.max_seq);
+    VerifyHost in{};
+    in.mask[0] = 1;
+    in.parents[0] = -1;
+    for (int i = 0; i < n; ++i) {
+        if (tokens[i] < 0 || tokens[i] >= md->cfg.vocab)
+            return fail(RQ_ERR_INVALID_ARGUMENT, "token %d at %d outside the vocabulary", tokens[i], i);
+        if (parents[i] < -1 || parents[i] >= i)
+            return fail(RQ_ERR_INVALID_ARGUMENT, "parent %d of draft %d is no earlier draft", parents[i], i);
+        const int p = parents[i] + 1;
+        in.tokens[i + 1] = tokens[i];
+        in.parents[i + 1] = p;
+        in.depth[i + 1] = in.depth[p] + 1;
+        in.mask[i + 1] = in.mask[p] | 1ull << (i + 1);
+    }
+    in.starts[1] = rows;
+    in.length = md->host_pos;
+    VerifyBuffers b{};
+    if (!md->verify) {
+        const size_t bytes = verify_buffers(md, nullptr, b);
+        void *p = nullptr;
+        const hipError_t e = hipMalloc(&p, bytes);
+        if (e != hipSuccess) return fail(RQ_ERR_ALLOC, "hipMalloc(%zu): %s", bytes, hipGetErrorString(e));
+        md->verify = p;
+    }
+    verify_buffers(md, static_cast<char *>(md->verify), b);
+    hipStream_t s = pick(md->ctx, stream);
+    RQ_HIP_TRY(hipMemcpyAsync(b.in, &in, sizeof in, hipMemcpyHostToDevice, s));
+    // row 0: the sequence's last token
+    RQ_HIP_TRY(hipMemcpyAsync(b.in->tokens, md->tokens + md->host_pos, 4, hipMemcpyDeviceToDevice, s));
+    const int st = verify_pass(md, b, rows, s);
+    VerifyOut out{};
+    if (st == RQ_OK) RQ_HIP_TRY(hipMemcpyAsync(&out, b.out, sizeof out, hipMemcpyDeviceToHost, s));
+    RQ_HIP_TRY(hipStreamSynchronize(s));  // (also: `in` may go)
+    if (st != RQ_OK) return st;
+    md->host_pos += out.accepted + 1;
+    md->host_len += out.accepted + 1;
+    *accepted = out.accepted;
     return RQ_OK;
 }
 

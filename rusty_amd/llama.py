@@ -275,6 +275,21 @@ class LlamaRunner:
     def decode(self, n_steps: int, stream=None) -> None:
         call("rq_llama_decode", self.handle, int(n_steps), _stream(stream))
 
+    def verify(self, tokens, parents, stream=None) -> int:
+        """One pass over a drafted tree (``rq_llama_verify``): draft i is
+        ``tokens[i]`` after draft ``parents[i]`` (-1: after the sequence's last
+        token).  Returns how many drafts the greedy picks followed; the
+        sequence grows by one token more than that."""
+        t = np.ascontiguousarray(tokens, dtype=np.int32).ravel()
+        p = np.ascontiguousarray(parents, dtype=np.int32).ravel()
+        if t.size != p.size:
+            raise ValueError("tokens and parents differ in length")
+        ptr = ctypes.POINTER(ctypes.c_int32)
+        accepted = ctypes.c_int32()
+        call("rq_llama_verify", self.handle, t.ctypes.data_as(ptr), p.ctypes.data_as(ptr), int(t.size),
+             ctypes.byref(accepted), _stream(stream))
+        return accepted.value
+
     def set_graph(self, use_graph: bool) -> None:
         """Graph launch per step (default) or direct kernel launches."""
         call("rq_llama_set_graph", self.handle, int(bool(use_graph)))

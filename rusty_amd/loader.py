@@ -181,13 +181,43 @@ class WeightsContext:
             out.append(_widen(np.ascontiguousarray(a), dt).reshape(-1))
         return codes, out[0], out[1]
 
+    def _quantized4_host(self, name: str, q: QuantizationConfig):
+        """4-bit codes as MLX packs them (eight per little-endian U32 word, the
+        first in the low bits: bytes [out, in/2], the even element in the low
+        nibble), scales and biases f32 [out, in/group]."""
+        if q.mode != "affine" or q.bits != 4:
+            raise LoaderError(f"{name}: expected 4-bit affine quantization, got {q.bits}-bit {q.mode}")
+        w, wshape = self.read_bytes(f"{name}.weight")
+        wdt = self._lookup(f"{name}.weight")[1]["dtype"]
+        if len(wshape) != 2 or wdt not in ("U32", "U8"):
+            raise LoaderError(f"{name}.weight: expected packed U32 [out, in/8] or U8 [out, in/2], got {wdt} {wshape}")
+        n_out = wshape[0]
+        codes = np.array(w, copy=True).view(np.uint8).reshape(n_out, -1)
+        k_in = 2 * codes.shape[1]
+        if q.group_size <= 0 or k_in % q.group_size != 0:
+            raise LoaderError(f"{name}: in = {k_in} is not a multiple of group_size {q.group_size}")
+        out = []
+        for part in ("scales", "biases"):
+            a, shape = self.read_bytes(f"{name}.{part}")
+            if int(np.prod(shape)) != n_out * (k_in // q.group_size):
+                raise LoaderError(f"{name}.{part}: {int(np.prod(shape))} values, expected "
+                                  f"{n_out * (k_in // q.group_size)} ([{n_out}, {k_in // q.group_size}])")
+            out.append(_widen(np.ascontiguousarray(a), self._lookup(f"{name}.{part}")[1]["dtype"]).reshape(n_out, -1))
+        return codes, out[0], out[1]
+
     def upload_quantized(self, name: str, ctx: WgpuContext, quant: QuantizationConfig | None = None
                          ) -> QuantizedTensor:
         """`{name}.weight/.scales/.biases` -> a device `QuantizedTensor`
         [out, in] in the reference's affine format, ready for the fused
-        kernels (rusty-loader/src/lib.rs:155-218 without the f32 step)."""
-        codes, s, b = self._quantized_host(name, quant or QuantizationConfig())
+        kernels (rusty-loader/src/lib.rs:155-218 without the f32 step); 4-bit
+        checkpoints of the same layout likewise (the reference reads 8-bit
+        ones only)."""
         g = (quant or QuantizationConfig()).group_size
+        if quant is not None and quant.bits == 4:
+            up = lambda a, dt: UnifiedTensor.new(ctx, a, dtype=dt)  # noqa: E731
+            codes, s, b = self._quantized4_host(name, quant)
+            return QuantizedTensor.from_affine4(up(codes, DType.U8), up(s, DType.FP32), up(b, DType.FP32), g)
+        codes, s, b = self._quantized_host(name, quant or QuantizationConfig())
         return QuantizedTensor.affine(ctx, codes, s, b, group=g)
 
     def upload_dequantized(self, name: str, ctx: WgpuContext, quant: QuantizationConfig | None = None
