@@ -491,7 +491,7 @@ rq::GemmWorkspace rq::gemm_workspace(const rq_ctx *ctx, hipStream_t s) {
 // tuned paths do not serve.
 int rq::qmatmul_dispatch(rq_ctx *ctx, const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dtype yt,
                          int64_t m, const GemmWorkspace &ws, hipStream_t s) {
-    if (w.format == RQ_Q_AFFINE_U4) return launch_linear4(w, x, xt, y, yt, m, s);
+    if (w.format == RQ_Q_AFFINE_U4) return launch_linear4(w, x, xt, y, yt, m, ctx->num_cus, ws, s);
     if (w.k_in > 0) {
         // 1-2 tokens: the VALU dot2 GEMV; 3-16: the MFMA GEMV (measured faster
         // from 3 tokens on, e.g. 4096x4096 m = 4: 7.2 -> 6.3 us); the VALU

@@ -167,7 +167,8 @@ int launch_swiglu_generic(const rq_qweight &gate, const rq_qweight &up, const vo
                           int64_t m, hipStream_t s);
 // 4-bit affine weights (RQ_Q_AFFINE_U4): W to f32, and Y = X . W^T for any m.
 int launch_dequantize4(const rq_qweight &w, float *out, hipStream_t s);
-int launch_linear4(const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dtype yt, int64_t m, hipStream_t s);
+int launch_linear4(const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dtype yt, int64_t m, int num_cus,
+                   const GemmWorkspace &ws, hipStream_t s);
 int launch_silu_mul(const void *g, const void *u, void *h, int64_t n, hipStream_t s);
 // dX[m, k_in] = dY[m, n_out] . deq(W), W dequantized while staged (f32 fma, ascending n_out).
 int launch_qmatmul_dx(const rq_qweight &w, const void *dy, rq_dtype dyt, void *dx, rq_dtype dxt, int64_t m,

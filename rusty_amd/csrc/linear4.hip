@@ -24,6 +24,9 @@ namespace rq {
 namespace {
 
 constexpr int TH = 256;
+// More rows than this: launch_widened (us, 16 at a time / widened: 48 rows, 4096x4096 21 / 35,
+// 11008x4096 45 / 46; 64 rows 28 / 35, 60 / 46)
+constexpr int kRowsBySixteen = 48;
 constexpr uint32_t kOOB = 0x80000000u;  // any offset past a buffer resource reads zero
 
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
@@ -514,6 +517,22 @@ __global__ __launch_bounds__(TH) void k_linear4_generic(const uint8_t *__restric
     }
 }
 
+// 4-bit codes to bytes, 32 of them per thread.
+__global__ __launch_bounds__(TH) void k_widen4(const u32x4 *__restrict__ codes, u32x4 *__restrict__ out, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * TH + threadIdx.x; i < n; i += (int64_t)gridDim.x * TH) {
+        const u32x4 w = codes[i];
+        u32x4 o[2];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t lo = w[e] & 0x0F0F0F0Fu, hi = (w[e] >> 4) & 0x0F0F0F0Fu;
+            o[e / 2][2 * (e % 2)] = __builtin_amdgcn_perm(hi, lo, 0x05010400u);
+            o[e / 2][2 * (e % 2) + 1] = __builtin_amdgcn_perm(hi, lo, 0x07030602u);
+        }
+        out[2 * i] = o[0];
+        out[2 * i + 1] = o[1];
+    }
+}
+
 using DotFn = void (*)(const uint8_t *, const float *, const float *, const void *, void *, int, int, int, int, int);
 
 // The m <= 2 kernel of a shape and the weight rows of its blocks.
@@ -592,12 +611,41 @@ int launch_dequantize4(const rq_qweight &w, float *out, hipStream_t s) {
     return RQ_OK;
 }
 
-int launch_linear4(const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dtype yt, int64_t m, hipStream_t s) {
+// More rows than the kernels above take at once: the codes widened to bytes in the
+// preparation area and the 8-bit GEMM (whose weights are rounded to fp16) on them,
+// where it serves the shape; RQ_ERR_UNSUPPORTED otherwise.
+int launch_widened(const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dtype yt, int64_t m, int num_cus,
+                   const GemmWorkspace &ws, hipStream_t s) {
+    const int64_t N = w.n_out, K = w.k_in;
+    const size_t codes = ((size_t)N * (size_t)K + 255) & ~size_t(255);
+    // (the GEMM lays its scale table, and f32 rows cast to fp16, behind them)
+    if (!ws.prep || K % 64 != 0 || w.group % 64 != 0 || codes > ws.prep_bytes / 4 * 3) return RQ_ERR_UNSUPPORTED;
+    rq_qweight wide = w;
+    wide.codes = ws.prep;
+    wide.format = RQ_Q_AFFINE_U8;
+    wide.prep = nullptr;
+    if (affine_prep_bytes(wide) == 0 || affine_prep_bytes(wide) > (ws.prep_bytes - codes) / 2) return RQ_ERR_UNSUPPORTED;
+    const int64_t chunks = N * K / 32;
+    hipLaunchKernelGGL(k_widen4, dim3((unsigned)std::min<int64_t>(cdiv(chunks, TH), 16384)), dim3(TH), 0, s,
+                       static_cast<const u32x4 *>(w.codes), static_cast<u32x4 *>(ws.prep), chunks);
+    RQ_LAUNCH_CHECK();
+    GemmWorkspace rest = ws;
+    rest.prep = static_cast<char *>(ws.prep) + codes;
+    rest.prep_bytes = ws.prep_bytes - codes;
+    return launch_gemm(wide, x, xt, y, yt, m, num_cus, rest, s);
+}
+
+int launch_linear4(const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dtype yt, int64_t m, int num_cus,
+                   const GemmWorkspace &ws, hipStream_t s) {
     const int64_t N = w.n_out, K = w.k_in;
     const bool xf = xt == RQ_F32, yh = yt == RQ_F16;
     // Chunks of 32 codes in one group each, 16-byte loads, 32-bit offsets into 16 rows of X and of W
     const bool fast = K > 0 && w.group % 32 == 0 && K <= (1 << 24) && grid_ok(N, 64) && aligned(w.codes, 16) && aligned(x, 16);
     if (fast) {
+        if (m > kRowsBySixteen) {
+            const int st = launch_widened(w, x, xt, y, yt, m, num_cus, ws, s);
+            if (st != RQ_ERR_UNSUPPORTED) return st;
+        }
         const size_t xr = (size_t)K * (xf ? 4 : 2), yr = (size_t)N * (yh ? 2 : 4);
         for (int64_t m0 = 0; m0 < m; m0 += 16) {
             const int mc = (int)std::min<int64_t>(16, m - m0);

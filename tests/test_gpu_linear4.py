@@ -102,6 +102,21 @@ def test_rows(ctx, engine, n, k, group, xt, yt):
         check(run(ctx, engine, x, qt, xt, yt), want, tol, f"{m}x{n}x{k}/{group} {xt}->{yt}")
 
 
+@pytest.mark.parametrize("xt,yt", [("f16", "f16"), ("f32", "f32"), ("f16", "f32")])
+@pytest.mark.parametrize("m", [33, 130, 515])
+@pytest.mark.parametrize("n,k,group", [(300, 512, 64), (129, 1088, 64), (72, 640, 128), (100, 512, 32)])
+def test_prompts(ctx, engine, m, n, k, group, xt, yt):
+    """Many rows, on the context's stream (codes widened to bytes where the
+    8-bit GEMM serves the shape) and on a caller's."""
+    g = np.random.default_rng(m + n)
+    w = weight(g, n, k, group)
+    qt = QuantizedTensor.affine4(ctx, *w)
+    x = acts(g, m, k, xt)
+    want, tol = truth(x, w, yt == "f16")
+    check(run(ctx, engine, x, qt, xt, yt), want, tol, f"{m}x{n}x{k}/{group} {xt}->{yt}")
+    check(run(ctx, engine, x, qt, xt, yt, Stream()), want, tol, f"stream {m}x{n}x{k}/{group} {xt}->{yt}")
+
+
 @pytest.mark.parametrize("m", [1, 2, 7, 16, 33])
 def test_without_biases(ctx, engine, m):
     g = np.random.default_rng(m)
