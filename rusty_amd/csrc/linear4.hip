@@ -24,8 +24,8 @@ namespace rq {
 namespace {
 
 constexpr int TH = 256;
-// More rows than this: launch_widened (us, 16 at a time / widened: 48 rows, 4096x4096 21 / 35,
-// 11008x4096 45 / 46; 64 rows 28 / 35, 60 / 46)
+// More rows than this: launch_widened (us, 16 at a time / widened: 48 rows, 4096x4096 22 / 35,
+// 11008x4096 44 / 46, 4096x11008 48 / 47; 64 rows 28 / 35, 60 / 46, 64 / 47; 96 rows 42 / 40, 90 / 56, 97 / 59)
 constexpr int kRowsBySixteen = 48;
 constexpr uint32_t kOOB = 0x80000000u;  // any offset past a buffer resource reads zero
 
