@@ -67,7 +67,9 @@ struct AttnArgs {
     int tokens;
     int wide;     // packed: row tiles per key/value head that the device takes at once
     int splits;   // tree: the most pieces a sequence's keys are cut into
-    float *part;  // splits > 1: sums [tokens][n_heads][splits][dim], then (m, l) [tokens][n_heads][splits]
+    // splits > 1: sums [splits][n_kv][tokens][heads of one][dim] (a block's rows side by side),
+    // then (m, l) [tokens][n_heads][splits]
+    float *part;
     float c;      // |scale| log2 e
     int neg;      // scale < 0: q enters negated
 };
@@ -465,9 +467,17 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
         const int key0 = (first + kt) * KT + kp;
         const uint32_t tb = lds0 + (uint32_t)(kt % NS) * (2 * TILE);
         using All = std::integral_constant<int, TPW>;
-        if (key0 + 32 * TPW <= masked_from) keys(std::false_type{}, All{}, tb, key0);
+        using One = std::integral_constant<int, 1>;
+        if (key0 + 32 * TPW <= masked_from) {
+            keys(std::false_type{}, All{}, tb, key0);
+        } else if constexpr (TREE && TPW > 1) {
+            // (few tiles: one piece at a time, in the registers that the others leave)
+#pragma unroll 1
+            for (int i = 0; i < TPW && key0 + 32 * i < key_end; ++i)
+                keys(std::true_type{}, One{}, tb + (uint32_t)(i * 32 * ROW), key0 + 32 * i);
+        }
         else if (key0 + 32 * (TPW - 1) < key_end) keys(std::true_type{}, All{}, tb, key0);
-        else if (key0 < key_end) keys(std::true_type{}, std::integral_constant<int, 1>{}, tb, key0);
+        else if (key0 < key_end) keys(std::true_type{}, One{}, tb, key0);
     }
     wait_vmcnt<0>();  // no DMA in flight past this point
 
@@ -513,7 +523,7 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
     if (TREE && pieces > 1) {
         if (!live) return;
         const int64_t slot = ((int64_t)(s0 + qi) * a.n_heads + head) * a.splits + piece;
-        float *po = a.part + slot * HD;
+        float *po = a.part + (((int64_t)piece * a.n_kv + g) * a.tokens * grp + (int64_t)(s0 + qi) * grp + (r - qi * grp)) * HD;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -580,7 +590,9 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
     const int per = q.per_piece(KT, a.splits), tiles = (q.keys + KT - 1) / KT;
     const int pieces = (tiles + per - 1) / per;
     if (pieces <= 1) return;  // written by the block that had them all
-    const float *po = a.part + row * a.splits * HD;
+    const int grp = a.n_heads / a.n_kv;
+    const int64_t step = (int64_t)a.tokens * a.n_heads * HD;  // between pieces
+    const float *po = a.part + (((int64_t)(head / grp) * a.tokens + t) * grp + head % grp) * HD;
     const float2 *ml = reinterpret_cast<const float2 *>(a.part + (int64_t)a.tokens * a.n_heads * a.splits * HD) + row * a.splits;
     // lane p has piece p's weight (at most 64 pieces); G pieces are added at once, 16 bytes a lane
     constexpr int L = HD / 4, G = 64 / L;
@@ -598,7 +610,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
     for (int p = gi; p < pieces + gi; p += G) {  // the same count for every lane
         const bool in = p < pieces;
         const float w = __shfl(wt, in ? p : 0);
-        const float4 v = *reinterpret_cast<const float4 *>(po + (int64_t)(in ? p : 0) * HD + at);
+        const float4 v = *reinterpret_cast<const float4 *>(po + (in ? p : 0) * step + at);
         if (in) {
             o[0] = __builtin_fmaf(w, v.x, o[0]);
             o[1] = __builtin_fmaf(w, v.y, o[1]);
