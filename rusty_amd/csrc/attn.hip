@@ -54,6 +54,18 @@ __device__ __forceinline__ float add_halves(float v) {
     return __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y);
 }
 
+// x / d for 0 <= x < 2^31 by one product: m = ceil(2^(31 + b) / d) with 2^b >= d is off by
+// less than 2^b / 2^(31 + b) of 1 / d, so x m / 2^(31 + b) never reaches the next whole number.
+struct Div {
+    uint32_t m, sh;
+    __host__ static Div by(int64_t d) {
+        uint32_t b = 0;
+        while (((int64_t)1 << b) < d) ++b;
+        return {(uint32_t)((((uint64_t)1 << (31 + b)) + (uint64_t)d - 1) / (uint64_t)d), 31 + b};
+    }
+    __device__ __forceinline__ int operator()(int x) const { return (int)(((uint64_t)(uint32_t)x * m) >> sh); }
+};
+
 // What the kernels read; strides in elements.
 struct AttnArgs {
     const void *q, *k, *v;
@@ -72,6 +84,7 @@ struct AttnArgs {
     float *part;
     float c;      // |scale| log2 e
     int neg;      // scale < 0: q enters negated
+    Div by_kv, by_grp, by_seqs, by_rbs, by_wide;  // n_kv, n_heads / n_kv, n_seqs; tree: blocks of a head's rows; packed: wide
 };
 
 __device__ __forceinline__ int seq_start(const AttnArgs &a, int s) { return min(max(a.starts[s], 0), a.tokens); }
@@ -80,7 +93,7 @@ __device__ __forceinline__ int seq_start(const AttnArgs &a, int s) { return min(
 // ascending), and its bounds; x uniform across the wave.  The 64 lanes probe at
 // once: one memory round trip up to 63 sequences, one more per factor of 64.
 template <typename F>
-__device__ __forceinline__ int find_seq(const AttnArgs &a, int64_t x, int *begin, int *end, F at) {
+__device__ __forceinline__ int find_seq(const AttnArgs &a, int x, int *begin, int *end, F at) {
     const int lane = threadIdx.x & 63;
     int lo = 0, n = a.n_seqs;  // the answer is in lo .. lo + n - 1
     while (n > 63) {
@@ -97,20 +110,19 @@ __device__ __forceinline__ int find_seq(const AttnArgs &a, int64_t x, int *begin
     return lo + c;
 }
 
-// Of n drafted positions, those that token t, the i-th of its sequence, sees, as bits.
-__device__ __forceinline__ uint64_t tree_sees(const AttnArgs &a, int t, int i, int n) {
+// Of n drafted positions, those that the i-th token of a sequence sees, as bits; word: its mask, where there is one.
+__device__ __forceinline__ uint64_t tree_sees(const AttnArgs &a, uint64_t word, int i, int n) {
     const uint64_t all = n > 0 ? ~0ull >> (64 - n) : 0;
-    return (a.mask ? a.mask[t] : ~0ull >> (63 - i)) & all;
+    return (a.mask ? word : ~0ull >> (63 - i)) & all;
 }
 
 // One sequence of a tree call: its tokens, and the keys cached before and with them.
 struct TreeSeq {
     int s0, nodes;      // first token, tokens served
     int before, keys;   // cached positions before them; all positions there are
-    __device__ __forceinline__ TreeSeq(const AttnArgs &a, int s) : TreeSeq(a, s, seq_start(a, s), seq_start(a, s + 1)) {}
-    __device__ __forceinline__ TreeSeq(const AttnArgs &a, int s, int begin, int end) : s0(begin) {
+    __device__ __forceinline__ TreeSeq(const AttnArgs &a, int begin, int end, int length) : s0(begin) {
         nodes = min(max(end - begin, 0), a.max_nodes);
-        before = min(max(a.lengths[s], 0), a.capacity);
+        before = min(max(length, 0), a.capacity);
         keys = before + min(nodes, a.capacity - before);
     }
     // tiles of kt keys per piece, for at most `splits` pieces
@@ -124,7 +136,7 @@ template <typename T, int HD, int WR, int KG, bool TREE>
 struct Shape {
     static constexpr int NW = WR * KG;
     static constexpr int ROW = HD * (int)sizeof(T), CH = ROW / 16;
-    static constexpr int KT = KG == 1 ? 64 : 32 * KG;  // keys per tile
+    static constexpr int KT = KG == 1 ? 64 : (WR == 4 ? 64 : 32) * KG;  // keys per tile
     static constexpr int TPW = KT / 32 / KG;           // 32-key pieces of it per wave
     static constexpr int TILE = KT * ROW;              // bytes of one operand's tile
     static constexpr int NS = 6 * TILE <= 49152 ? 3 : 2;
@@ -148,19 +160,18 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wv % WR, kg = wv / WR;
     const int col = lane & 31, hf = lane >> 5;
-    const int grp = a.n_heads / a.n_kv, g = blockIdx.x % a.n_kv;
+    const int grp = a.by_kv(a.n_heads), blk = a.by_kv(blockIdx.x), g = blockIdx.x - blk * a.n_kv;
 
     // the block's sequence, rows and keys
     int s0, nq, r0, nkeys, first = 0, ntiles, pieces = 1, piece = 0, before = 0;
     const char *kb, *vb;  // key 0 of this head
     if constexpr (TREE) {
-        const int rbs = (a.max_nodes * grp + BR - 1) / BR;
-        int b = blockIdx.x / a.n_kv;
-        const int rb = b % rbs;
-        b /= rbs;
-        const int s = b % a.n_seqs;
-        piece = b / a.n_seqs;
-        const TreeSeq q(a, s);
+        const int rbs = (a.max_nodes * grp + BR - 1) / BR, sp = a.by_rbs(blk), rb = blk - sp * rbs;
+        piece = a.by_seqs(sp);
+        const int s = sp - piece * a.n_seqs;
+        int begin = a.starts[s], end = a.starts[s + 1], length = a.lengths[s];
+        asm volatile("" : "+s"(begin), "+s"(end), "+s"(length));  // one wait for the three
+        const TreeSeq q(a, min(max(begin, 0), a.tokens), min(max(end, 0), a.tokens), length);
         s0 = q.s0;
         nq = q.nodes;
         r0 = rb * BR;
@@ -171,7 +182,7 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
         if (r0 >= nq * grp || piece >= pieces) return;
         first = __builtin_amdgcn_readfirstlane(piece * per);
         ntiles = min(per, tiles - piece * per);
-        const int64_t at = s * a.seq_stride + g * a.head_stride;
+        const int64_t at = (int64_t)s * a.seq_stride + g * a.head_stride;
         kb = static_cast<const char *>(a.k) + at * (int64_t)sizeof(T);
         vb = static_cast<const char *>(a.v) + at * (int64_t)sizeof(T);
     } else {
@@ -180,22 +191,23 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
         // The last first, a long prompt's heaviest; every other run of as many as
         // the device takes at once the other way round, so that a CU which got
         // a heavy block gets a light one next.
-        const int total = gridDim.x / a.n_kv, rank = blockIdx.x / a.n_kv, run = rank / a.wide;
-        const int flip = run & 1 ? run * a.wide + min((run + 1) * a.wide, total) - 1 - rank : rank;
-        const int64_t t = total - 1 - flip;
+        // (tokens grp < 2^31: the grid has fewer than 2^32 threads)
+        const int total = a.by_kv(gridDim.x), run = a.by_wide(blk);
+        const int flip = run & 1 ? run * a.wide + min((run + 1) * a.wide, total) - 1 - blk : blk;
+        const int t = total - 1 - flip;
         auto tile0 = [&](int s, int begin) { return (int64_t)begin * grp / BR + s; };
         int end;
         const int s = find_seq(a, t, &s0, &end, tile0);
         nq = max(end - s0, 0);
-        const int64_t row = (t - tile0(s, s0)) * BR;
-        if (row < 0 || row >= (int64_t)nq * grp) return;
+        const int row = (int)(t - tile0(s, s0)) * BR;
+        if (row < 0 || row >= nq * grp) return;
         // rows are counted from the tile's first token on
-        const int skip = (int)(row / grp);
-        r0 = (int)(row - (int64_t)skip * grp);
+        const int skip = a.by_grp(row);
+        r0 = row - skip * grp;
         s0 += skip;
         before = skip;  // tokens of the sequence before token 0 of these
         nq -= skip;
-        nkeys = before + min(nq, (r0 + BR - 1) / grp + 1);
+        nkeys = before + min(nq, a.by_grp(r0 + BR - 1) + 1);
         ntiles = (nkeys + KT - 1) / KT;
         const int64_t seq = (int64_t)(s0 - skip);
         kb = static_cast<const char *>(a.k) + (seq * a.k_row + g * HD) * (int64_t)sizeof(T);
@@ -204,41 +216,6 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
     s0 = __builtin_amdgcn_readfirstlane(s0);
     nkeys = __builtin_amdgcn_readfirstlane(nkeys);
     ntiles = __builtin_amdgcn_readfirstlane(ntiles);
-
-    // this lane's row
-    const int r = r0 + 32 * wr + col, qi = r / grp, head = g * grp + (r - qi * grp);
-    const bool live = qi < nq;
-    const uint64_t see = TREE && live ? tree_sees(a, s0 + qi, qi, nkeys - before) : 0;
-    // of the wave's rows: the last key any of them sees, and the first that some do not
-    const int w_lo = __builtin_amdgcn_readfirstlane((r0 + 32 * wr) / grp);
-    const int w_hi = __builtin_amdgcn_readfirstlane(min((r0 + 32 * wr + 31) / grp, nq - 1));
-    const bool idle = w_lo >= nq;  // no row at all
-    const int key_end = idle ? 0 : TREE ? nkeys : before + w_hi + 1;
-    const int masked_from = idle ? 0 : TREE ? before : before + w_lo + 1;
-    // bit j: whether this lane's row sees key key0 + j
-    auto visible = [&](int key0) -> uint64_t {
-        if constexpr (TREE) {
-            const int d = before - key0;  // keys of these that are cached positions
-            if (d >= 64) return ~0ull;
-            if (d >= 0) return (see << d) | ((1ull << d) - 1);
-            return d > -64 ? see >> -d : 0;
-        } else {
-            const int n = before + qi + 1 - key0;
-            return n >= 64 ? ~0ull : n > 0 ? (1ull << n) - 1 : 0;
-        }
-    };
-
-    uint4 qf[KS];
-    {
-        const char *qp = static_cast<const char *>(a.q) + ((int64_t)(s0 + qi) * a.q_row + head * HD) * (int64_t)sizeof(T);
-        const uint32_t flip = a.neg ? (F16 ? 0x80008000u : 0x80000000u) : 0u;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (live) v = *reinterpret_cast<const uint4 *>(qp + 32 * s + 16 * hf);
-            qf[s] = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
-        }
-    }
 
     // LDS chunk c of row r holds global chunk c ^ f(r)
     auto fk = [](int r) { return F16 && HD == 64 ? (r >> 1) & 7 : r & 15; };
@@ -267,6 +244,43 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
     };
 #pragma unroll
     for (int kt = 0; kt < NS - 1; ++kt) dma(kt);
+
+    // this lane's row
+    const int r = r0 + 32 * wr + col, qi = a.by_grp(r), head = g * grp + (r - qi * grp);
+    const bool live = qi < nq;
+    const uint64_t word = TREE && live && a.mask ? a.mask[s0 + qi] : 0;
+    const uint64_t see = TREE && live ? tree_sees(a, word, qi, nkeys - before) : 0;
+    // of the wave's rows: the last key any of them sees, and the first that some do not
+    const int w_lo = __builtin_amdgcn_readfirstlane(a.by_grp(r0 + 32 * wr));
+    const int w_hi = __builtin_amdgcn_readfirstlane(min(a.by_grp(r0 + 32 * wr + 31), nq - 1));
+    const bool idle = w_lo >= nq;  // no row at all
+    const int key_end = idle ? 0 : TREE ? nkeys : before + w_hi + 1;
+    const int masked_from = idle ? 0 : TREE ? before : before + w_lo + 1;
+    // bit j: whether this lane's row sees key key0 + j
+    auto visible = [&](int key0) -> uint64_t {
+        if constexpr (TREE) {
+            const int d = before - key0;  // keys of these that are cached positions
+            if (d >= 64) return ~0ull;
+            if (d >= 0) return (see << d) | ((1ull << d) - 1);
+            return d > -64 ? see >> -d : 0;
+        } else {
+            const int n = before + qi + 1 - key0;
+            return n >= 64 ? ~0ull : n > 0 ? (1ull << n) - 1 : 0;
+        }
+    };
+
+    // (after the first tiles' loads: the wait for Q is then theirs too)
+    uint4 qf[KS];
+    {
+        const char *qp = static_cast<const char *>(a.q) + ((int64_t)(s0 + qi) * a.q_row + head * HD) * (int64_t)sizeof(T);
+        const uint32_t flip = a.neg ? (F16 ? 0x80008000u : 0x80000000u) : 0u;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (live) v = *reinterpret_cast<const uint4 *>(qp + 32 * s + 16 * hf);
+            qf[s] = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
+        }
+    }
 
     float mc = -__builtin_inff(), l = 0.0f;  // running maximum (scaled), this lane's share of the sum
     floatx16 o[DT];
@@ -306,14 +320,23 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
     auto keys = [&](auto masked_c, auto n_c, uint32_t tb, int key0) {
         constexpr bool MASKED = decltype(masked_c)::value;
         constexpr int N = decltype(n_c)::value;
+        // one piece at a time: K's, then V's, fragments all read ahead of their products,
+        // which otherwise wait for one after another
+        constexpr bool AHEAD = N == 1 && (TREE || KG > 1);
         floatx16 sc[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const floatx16 zero = {};
             sc[i] = zero;
+            u32x4 kr[AHEAD ? KS : 1];
+            if constexpr (AHEAD) {
+#pragma unroll
+                for (int s = 0; s < KS; ++s) kr[s] = *(lds_u32x4 *)(uintptr_t)(tb + ka[s] + (uint32_t)(i * 32 * ROW));
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                const u32x4 kf = *(lds_u32x4 *)(uintptr_t)(tb + ka[s] + (uint32_t)(i * 32 * ROW));
+                const u32x4 kf = AHEAD ? kr[s] : *(lds_u32x4 *)(uintptr_t)(tb + ka[s] + (uint32_t)(i * 32 * ROW));
                 if constexpr (F16) {
                     sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, kf),
                                                                    __builtin_bit_cast(half8, qf[s]), sc[i], 0, 0, 0);
@@ -421,20 +444,35 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
             for (int i = 0; i < N; ++i)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) pf[i][e >> 3][e & 7] = (_Float16)sc[i][e];
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
+            auto read = [&](int d, int i, int s2) {
                 lds_short4 *pa = (lds_short4 *)(uintptr_t)(vt + va[d][0]), *pb = (lds_short4 *)(uintptr_t)(vt + va[d][1]);
+                const uint2 ua =
+                    __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(pa + (2 * i + s2) * 16 * ROW / 8));
+                const uint2 ub =
+                    __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(pb + (2 * i + s2) * 16 * ROW / 8));
+                return __builtin_bit_cast(half8, make_uint4(ua.x, ua.y, ub.x, ub.y));
+            };
+            constexpr int DR = AHEAD ? DT : 1;  // dimensions read at once
 #pragma unroll
-                for (int i = 0; i < N; ++i)
+            for (int d0 = 0; d0 < DT; d0 += DR) {
+                half8 vr[DR][N][2];
+                if constexpr (AHEAD || TREE) {
 #pragma unroll
-                    for (int s2 = 0; s2 < 2; ++s2) {
-                        const uint2 ua = __builtin_bit_cast(
-                            uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(pa + (2 * i + s2) * 16 * ROW / 8));
-                        const uint2 ub = __builtin_bit_cast(
-                            uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(pb + (2 * i + s2) * 16 * ROW / 8));
-                        const half8 vf = __builtin_bit_cast(half8, make_uint4(ua.x, ua.y, ub.x, ub.y));
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[i][s2], o[d], 0, 0, 0);
-                    }
+                    for (int d = 0; d < DR; ++d)
+#pragma unroll
+                        for (int i = 0; i < N; ++i)
+#pragma unroll
+                            for (int s2 = 0; s2 < 2; ++s2) vr[d][i][s2] = read(d0 + d, i, s2);
+                    if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int d = 0; d < DR; ++d)
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+#pragma unroll
+                        for (int s2 = 0; s2 < 2; ++s2)
+                            o[d0 + d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                                AHEAD || TREE ? vr[d][i][s2] : read(d0 + d, i, s2), pf[i][s2], o[d0 + d], 0, 0, 0);
             }
         } else {
             // V's values of 8 keys at a time, all read before the first is used: one by
@@ -567,7 +605,7 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
         constexpr int RPI = 64 / CH;  // rows per store
 #pragma unroll
         for (int i = 0; i < 32 / RPI; ++i) {
-            const int ro = i * RPI + lane / CH, c = lane % CH, rr = r0 + 32 * wr + ro, q2 = rr / grp;
+            const int ro = i * RPI + lane / CH, c = lane % CH, rr = r0 + 32 * wr + ro, q2 = a.by_grp(rr);
             if (q2 >= nq) continue;
             const uint4 v = *reinterpret_cast<const uint4 *>(ol + ro * ROW + (c ^ (ro & 7)) * 16);
             T *op = static_cast<T *>(a.out) + (int64_t)(s0 + q2) * a.out_row + (g * grp + (rr - q2 * grp)) * HD;
@@ -579,24 +617,30 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
 // Joins the pieces of rows whose keys were cut: one wave per (token, head).
 template <typename T, int HD, int KT>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    constexpr int L = HD / 4, G = 64 / L, U = 8;  // pieces added at once, 16 bytes a lane; read ahead of use
+    const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (row >= (int64_t)a.tokens * a.n_heads) return;
     const int t = (int)(row / a.n_heads), head = (int)(row - (int64_t)t * a.n_heads), lane = threadIdx.x & 63;
+    const int grp = a.by_kv(a.n_heads), g = a.by_grp(head), gi = lane / L, at = 4 * (lane % L);
+    const int64_t step = (int64_t)a.tokens * a.n_heads * HD;  // between pieces
+    const float *po = a.part + (((int64_t)g * a.tokens + t) * grp + head - g * grp) * HD + at;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.part + (int64_t)a.tokens * a.n_heads * a.splits * HD) + row * a.splits;
+    // lane p has piece p's weight (at most 64 pieces).  It and the first pieces' sums are
+    // read before it is known how many there are; those past the last go unused.
+    const float2 raw = ml[min(lane, a.splits - 1)];
+    float4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const float4 *>(po + min(gi + u * G, a.splits - 1) * step);
+    const uint64_t word = a.mask ? a.mask[t] : 0;
     int begin, end;
-    const int s = find_seq(a, t, &begin, &end, [](int, int at) { return (int64_t)at; });
-    const TreeSeq q(a, s, begin, end);
+    const int s = find_seq(a, t, &begin, &end, [](int, int at) { return at; });
+    const TreeSeq q(a, begin, end, a.lengths[s]);
     const int i = t - q.s0;
     if (i < 0 || i >= q.nodes) return;
     const int per = q.per_piece(KT, a.splits), tiles = (q.keys + KT - 1) / KT;
     const int pieces = (tiles + per - 1) / per;
     if (pieces <= 1) return;  // written by the block that had them all
-    const int grp = a.n_heads / a.n_kv;
-    const int64_t step = (int64_t)a.tokens * a.n_heads * HD;  // between pieces
-    const float *po = a.part + (((int64_t)(head / grp) * a.tokens + t) * grp + head % grp) * HD;
-    const float2 *ml = reinterpret_cast<const float2 *>(a.part + (int64_t)a.tokens * a.n_heads * a.splits * HD) + row * a.splits;
-    // lane p has piece p's weight (at most 64 pieces); G pieces are added at once, 16 bytes a lane
-    constexpr int L = HD / 4, G = 64 / L;
-    const float2 mine = lane < pieces ? ml[lane] : make_float2(-__builtin_inff(), 0.0f);
+    const float2 mine = lane < pieces ? raw : make_float2(-__builtin_inff(), 0.0f);
     float top = mine.x;
 #pragma unroll
     for (int w = 32; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor(top, w));
@@ -605,17 +649,23 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
     float l = wt * mine.y, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w = 32; w > 0; w >>= 1) l += __shfl_xor(l, w);
-    const int gi = lane / L, at = 4 * (lane % L);
-#pragma unroll 4
-    for (int p = gi; p < pieces + gi; p += G) {  // the same count for every lane
-        const bool in = p < pieces;
-        const float w = __shfl(wt, in ? p : 0);
-        const float4 v = *reinterpret_cast<const float4 *>(po + (in ? p : 0) * step + at);
-        if (in) {
-            o[0] = __builtin_fmaf(w, v.x, o[0]);
-            o[1] = __builtin_fmaf(w, v.y, o[1]);
-            o[2] = __builtin_fmaf(w, v.z, o[2]);
-            o[3] = __builtin_fmaf(w, v.w, o[3]);
+    for (int p0 = 0; p0 < pieces; p0 += U * G) {
+        if (p0 > 0) {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                v[u] = *reinterpret_cast<const float4 *>(po + min(p0 + gi + u * G, pieces - 1) * step);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int p = p0 + gi + u * G;
+            const bool in = p < pieces;
+            const float w = __shfl(wt, in ? p : 0);
+            if (in) {
+                o[0] = __builtin_fmaf(w, v[u].x, o[0]);
+                o[1] = __builtin_fmaf(w, v[u].y, o[1]);
+                o[2] = __builtin_fmaf(w, v[u].z, o[2]);
+                o[3] = __builtin_fmaf(w, v[u].w, o[3]);
+            }
         }
     }
 #pragma unroll
@@ -623,19 +673,24 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
 #pragma unroll
         for (int w = 32; w >= L; w >>= 1) o[e] += __shfl_xor(o[e], w);
     if (gi != 0) return;
-    const bool none = q.before == 0 && tree_sees(a, t, i, q.keys) == 0;
+    const bool none = q.before == 0 && tree_sees(a, word, i, q.keys) == 0;
     typedef T vec4 __attribute__((ext_vector_type(4)));
-    vec4 v;
+    vec4 y;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = (T)(none ? 0.0f : o[e] / l);
-    *reinterpret_cast<vec4 *>(static_cast<T *>(a.out) + (int64_t)t * a.out_row + head * HD + at) = v;
+    for (int e = 0; e < 4; ++e) y[e] = (T)(none ? 0.0f : o[e] / l);
+    *reinterpret_cast<vec4 *>(static_cast<T *>(a.out) + (int64_t)t * a.out_row + head * HD + at) = y;
 }
 
 // Launches k_attn<T, HD, WR, KG, TREE> with BR = 32 WR rows per block.
 template <typename T, int HD, int WR, int KG, bool TREE>
-int launch(const AttnArgs &a, hipStream_t s) {
+int launch(AttnArgs a, hipStream_t s) {
     using SH = Shape<T, HD, WR, KG, TREE>;
     const int64_t grp = a.n_heads / a.n_kv, br = 32 * WR;
+    a.by_kv = Div::by(a.n_kv);
+    a.by_grp = Div::by(grp);
+    a.by_seqs = Div::by(a.n_seqs);
+    a.by_rbs = Div::by(TREE ? cdiv(a.max_nodes * grp, br) : 1);
+    a.by_wide = Div::by(TREE ? 1 : a.wide);
     const int64_t tiles = TREE ? cdiv(a.max_nodes * grp, br) * a.n_seqs * a.splits : (int64_t)a.tokens * grp / br + a.n_seqs;
     if (!grid_ok(tiles * a.n_kv, 64 * SH::NW)) return fail(RQ_ERR_SHAPE, "too many rows for one call");
     hipLaunchKernelGGL((k_attn<T, HD, WR, KG, TREE>), dim3((unsigned)(tiles * a.n_kv)), dim3(64 * SH::NW), 0, s, a);
@@ -660,26 +715,59 @@ int launch_packed(const AttnArgs &a, int cus, hipStream_t s) {
     return launch<T, HD, 4, 1, false>(a, s);
 }
 
-// Rows of a tree block (32, 64 or 128 by the rows a sequence may have) and the
-// pieces its keys may be cut into: one block per CU and layer of rows.  A cache of
-// a few tiles stays whole: joining pieces costs a launch, about what four tiles take
-// (one token, 513 keys, 8.6 us whole, 9.2 in two; eight trees of 16 over 37 to 2047
-// keys in 4 / 8 / 16 pieces 17.1 / 16.4 / 21.8; 32702 keys, 32/8 heads of 128, in 16 / 32 / 64 41 / 39 / 54).
-int tree_rows(int64_t rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
-int tree_splits(int64_t n_seqs, int64_t n_kv, int64_t rows, int64_t capacity, bool f16) {
-    const bool few = tree_rows(rows) == 1 && f16;  // tiles of 128 keys
-    const int64_t tiles = cdiv(capacity, few ? 128 : 64), heads = std::max<int64_t>(n_seqs * n_kv, 1);
-    if (f16 && tiles <= 5) return 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({256 / heads, f16 && !few ? cdiv(tiles, 2) : tiles, 64}));
+// How a tree call is cut: blocks of 32 wr rows and kg groups of keys, the keys of a
+// sequence into at most `splits` pieces, for about kCus blocks at work.  Joining pieces
+// costs a launch and the sums' way to memory and back, so keys are cut only as
+// long as there are too few blocks without (us; rows: of a key/value head):
+//   rows <= 32, tiles of 128 keys: one token, 513 keys, 7.9 whole, 8.9 in 4 pieces.
+//   enough blocks of 128 rows: whole; 16 trees of 64 over 1500 keys, 32/8 heads of 128, 4x2 41.5,
+//     2x4 55.5; 32 of them 4x1 72, 4x2 83.
+//   enough of 64 rows, or half of that and a short cache: whole, 2x4; 8 of these trees 29.5, 4x2 in 2 pieces 36.9; 4 of them 25.6, 26.2 in 4.
+//   few: 64 rows, 2x2, a long axis 128 rows, 4x2, for half the bytes of sums; 2 trees of 32
+//     2x2 in 8 13.6, 4x2 in 16 17.4; one of 64 over 32701 keys 4x2 in 16 55, 2x2 in 16 62, 2x4 in 8 62.
+//   f32, whose blocks are matrix-bound: 4x1 where there are enough, else 2x2 (4 sequences of up to 1501 keys
+//     2x2 in 8 17.0, 4x1 in 16 18.6).
+constexpr int64_t kCus = 256;
+struct TreeShape {
+    int wr, kg, splits;
+};
+TreeShape tree_shape(int64_t n_seqs, int64_t n_kv, int64_t rows, int64_t capacity, bool f16) {
+    const int64_t heads = std::max<int64_t>(n_seqs * n_kv, 1), t64 = cdiv(capacity, 64), t128 = cdiv(capacity, 128);
+    auto cut = [](int64_t blocks, int64_t tiles) {
+        return (int)std::max<int64_t>(1, std::min<int64_t>({kCus / blocks, tiles, 64}));
+    };
+    if (rows <= 32) {
+        if (f16) return {1, 4, t128 <= 5 ? 1 : cut(heads, t128)};
+        return {1, 2, cut(heads, t64)};
+    }
+    const int64_t r64 = heads * cdiv(rows, 64), r128 = heads * cdiv(rows, 128);
+    if (!f16) {
+        if (rows > 64 && r128 >= kCus) return {4, 1, 1};
+        return {2, 2, cut(r64, t64)};
+    }
+    if (rows > 64 && r128 >= kCus) return {4, r128 >= 2 * kCus ? 1 : 2, 1};
+    if (r64 >= 2 * kCus) return {2, 2, 1};
+    if (r64 >= kCus || (2 * r64 >= kCus && t64 <= 40)) return {2, 4, 1};
+    const int few = t64 <= 5 ? 1 : cut(r64, cdiv(t64, 2));
+    if (rows <= 64 || t64 < 8 * few) return {2, 2, few};
+    return {4, 2, cut(r128, t128)};
 }
 
 template <typename T, int HD>
 int launch_tree(const AttnArgs &a, hipStream_t s) {
-    const int wr = tree_rows((int64_t)a.max_nodes * (a.n_heads / a.n_kv));
-    if (wr == 4) return launch<T, HD, 4, 1, true>(a, s);
-    if (wr == 2) return launch<T, HD, 2, 2, true>(a, s);
-    if constexpr (sizeof(T) == 2) return launch<T, HD, 1, 4, true>(a, s);
-    else return launch<T, HD, 1, 2, true>(a, s);
+    constexpr bool F16 = sizeof(T) == 2;
+    const TreeShape sh = tree_shape(a.n_seqs, a.n_kv, (int64_t)a.max_nodes * (a.n_heads / a.n_kv), a.capacity, F16);
+    if (sh.wr == 2) {
+        if constexpr (F16)
+            if (sh.kg == 4) return launch<T, HD, 2, 4, true>(a, s);
+        return launch<T, HD, 2, 2, true>(a, s);
+    }
+    if (sh.wr == 4) {
+        if constexpr (F16)
+            if (sh.kg == 2) return launch<T, HD, 4, 2, true>(a, s);
+        return launch<T, HD, 4, 1, true>(a, s);
+    }
+    return launch<T, HD, 1, F16 ? 4 : 2, true>(a, s);
 }
 
 // The checks both entry points share; fills the strides of a.
@@ -775,8 +863,9 @@ int check_tree(const rq_attn *attn, const rq_kv_cache *cache, const void *q, con
         return fail(RQ_ERR_INVALID_ARGUMENT, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
     if (need > 0 && !aligned(workspace, 16)) return fail(RQ_ERR_UNSUPPORTED, "workspace must be 16-byte aligned");
     a.k_row = a.v_row = (int)pos;
-    a.splits = tree_splits(cache->n_seqs, a.n_kv, (int64_t)max_nodes * (a.n_heads / a.n_kv), cache->capacity,
-                           attn->dtype == RQ_F16);
+    a.splits = tree_shape(cache->n_seqs, a.n_kv, (int64_t)max_nodes * (a.n_heads / a.n_kv), cache->capacity,
+                          attn->dtype == RQ_F16)
+                   .splits;
     a.part = static_cast<float *>(workspace);
     a.q = q;
     a.k = cache->k;
@@ -820,8 +909,9 @@ size_t rq_attn_tree_workspace(const rq_attn *attn, int32_t n_seqs, int64_t token
     if (n_seqs < 1 || tokens < 1 || max_nodes < 1 || max_nodes > kMaxNodes || capacity < 0 ||
         check_attn(attn, tokens, a) != RQ_OK)
         return 0;
-    const int splits = tree_splits(n_seqs, a.n_kv, (int64_t)max_nodes * (a.n_heads / a.n_kv), capacity,
-                                   attn->dtype == RQ_F16);
+    const int splits = tree_shape(n_seqs, a.n_kv, (int64_t)max_nodes * (a.n_heads / a.n_kv), capacity,
+                                  attn->dtype == RQ_F16)
+                           .splits;
     const size_t rows = (size_t)tokens * (size_t)a.n_heads * (size_t)splits;
     return splits > 1 ? (rows * ((size_t)attn->head_dim * 4 + 8) + 15) / 16 * 16 : 0;
 }

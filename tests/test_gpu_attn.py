@@ -266,6 +266,26 @@ def test_tree(ctx, engine, dtype, heads, kv, dim, name):
         check(got, want, tol, f"tree {name} {heads}/{kv}x{dim} {dtype} {'chain' if m is None else ''}")
 
 
+# Few and many sequences, rows and keys: each way in which a call's rows and keys are cut into blocks.
+CUTS = {  # sequences, capacity, most nodes of one, heads, key/value heads, dim
+    "many row tiles": (260, 30, 8, 34, 2, 64), "row tiles": (70, 150, 10, 32, 4, 64), "many small": (130, 40, 9, 16, 4, 64),
+    "half tiles": (33, 300, 20, 16, 4, 128), "half tiles, fewer": (9, 230, 33, 32, 4, 64),
+    "pieces": (3, 1000, 20, 8, 2, 128), "pieces of tiles": (5, 1700, 64, 16, 8, 128), "one long": (1, 20000, 40, 4, 1, 64),
+}
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("name", list(CUTS))
+def test_tree_cuts(ctx, engine, dtype, name):
+    seqs, cap, most, heads, kv, dim = CUTS[name]
+    g = np.random.default_rng(31)
+    nodes = [most] + [int(x) for x in g.integers(0, most + 1, seqs - 1)]
+    lengths = [cap - most] + [int(x) for x in g.integers(0, cap - most + 1, seqs - 1)]
+    q, k, v, mask = tree_inputs(30, lengths, nodes, cap, heads, kv, dim, dtype)
+    want, tol = tree_truth(q, k, v, lengths, nodes, mask, dim ** -0.5, dtype == "f16")
+    check(run_tree(ctx, engine, q, k, v, lengths, nodes, mask, dtype), want, tol, f"tree {name} {dtype}")
+
+
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 def test_tree_masks_that_leave_nothing(ctx, engine, dtype):
     """No cached position and no set bit: zeros.  Bits past the sequence's
