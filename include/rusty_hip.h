@@ -227,8 +227,12 @@ int rq_matmul_at(rq_ctx *ctx, const float *a, const float *b, float *out, int64_
  * fp16-MFMA prefill path), each row scaled first by the power of two that
  * puts its largest magnitude in [2^14, 2^15) and its outputs scaled back, so
  * there too any finite row is served, at fp16 accuracy; it rounds affine
- * weights to fp16 likewise.  On the
- * context's own stream (stream NULL) a GEMM with few tokens splits K over
+ * weights to fp16 likewise.
+ * RQ_Q_AFFINE_U4 weights go 16 rows at a time with exact codes up to m = 48,
+ * f32 rows at f32 accuracy as above; with more rows, on the context's own stream
+ * and with k_in and group multiples of 64, the codes are widened to bytes in the context's
+ * workspace and take the GEMM, at its accuracy, where they fit (48 MiB, k_in n_out bytes).
+ * On the context's own stream (stream NULL) a GEMM with few tokens splits K over
  * more blocks using the context's workspace, so two such calls of one
  * context must not run concurrently (they cannot on one stream); on any
  * other stream it does not split.  A HIP graph captured on the context's
