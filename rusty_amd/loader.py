@@ -1,4 +1,4 @@
-"""MLX affine 8-bit safetensors -> device-resident quantized weights.
+"""MLX affine 8-bit and 4-bit safetensors -> device-resident quantized weights.
 
 Host mirror of the reference's loader (rusty-loader/src/lib.rs): the
 `QuantizationConfig` of a model's config.json (:27-32), `WeightsContext`
@@ -16,7 +16,8 @@ with `load_file` / `get_tensor_info` / `read_bytes` (:95-160) and
   model dtype); they are widened to f32 on the host, exactly.  The reference
   reinterprets their bytes as f32 whatever their dtype (:186-187).
 * `group_size`, `bits` and `mode` are honoured: 8-bit affine codes with any
-  group size dividing `in` (a multiple of 16 for the fast kernels); the
+  group size dividing `in` (a multiple of 16 for the fast kernels), and 4-bit
+  ones, which stay 4-bit on the device (a multiple of 32 there); the
   reference's kernel hard-codes group 64 (kernels.wgsl:395).
 
 The safetensors container is parsed here directly (8-byte little-endian

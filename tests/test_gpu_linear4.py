@@ -172,7 +172,7 @@ def test_degenerate_sizes(ctx, engine):
     assert np.all(Y.to_vec() == 0)
 
 
-@pytest.mark.parametrize("m", [1, 4, 24])
+@pytest.mark.parametrize("m", [1, 4, 24, 130])
 def test_streams_and_graphs(ctx, engine, m):
     g = np.random.default_rng(m + 80)
     w = weight(g, 300, 1024, 64)
@@ -194,7 +194,7 @@ def test_streams_and_graphs(ctx, engine, m):
         ref = run(ctx, engine, x2, qt, "f16", "f32")
 
 
-@pytest.mark.parametrize("m", [1, 2, 6, 16, 40])
+@pytest.mark.parametrize("m", [1, 2, 6, 16, 40, 70])
 @pytest.mark.parametrize("xt", ["f16", "f32"])
 def test_mlp_and_lora(ctx, engine, m, xt):
     """The SwiGLU MLP and the LoRA linear over 4-bit weights."""
