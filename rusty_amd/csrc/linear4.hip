@@ -595,16 +595,19 @@ int launch_mfma(const rq_qweight &w, const void *x, bool xf, void *y, bool yh, i
         else if (w.group % 64 == 0) go(rt, nw, std::integral_constant<int, 2>{}, xfc);
         else go(rt, nw, std::integral_constant<int, 1>{}, xfc);
     };
-    // Waves and row tiles per block, measured (us, 8 rows, 1 tile of 4 waves / 1 of 8 / 2 of 4; f32 rows
-    // in brackets): 4096x4096 6.9 / 6.5 / 9.4 [10.0 / 10.4 / 13.2], 2048x2048 4.9 / 5.2 / 5.8, 4096x11008
-    // in groups of 32 16.9 / 13.5 / 26.6 [24.9 / 21.4 / 35.4], 11008x4096 12.6 / 16.0 / 13.0 (16 rows
-    // 15.9 / 19.2 / 15.4) [21.2 / 28.2 / 25.0], 32000x2048 18.1 / 28.5 / 14.8 [30.9 / 50.2 / 28.6].
+    // Waves and row tiles per block, measured (us, 1 tile of 4 waves / 1 of 8 / 2 of 4; f32 rows in
+    // brackets).  8 rows: 2048x2048 5.0 / 5.3 / 5.7 [6.3 / 6.7 / 7.4], 4096x4096 7.1 / 6.3 / 9.1
+    // [9.4 / 9.1 / 12.3], 4096x11008 in groups of 32 17.1 / 12.7 / 26.4 [23.1 / 19.7 / 32.9], 5632x2048
+    // 6.6 / 6.7 / 6.0 [8.8 / 11.9 / 7.8], 11008x4096 12.1 / 13.3 / 12.7 [19.7 / 24.8 / 18.1], 32000x2048
+    // 18.9 / 20.5 / 13.3 [29.4 / 42.8 / 19.7].  16 rows: 4096x4096 8.2 / 7.9 / 10.3 [12.6 / 11.8 / -],
+    // 5632x2048 8.0 / 9.7 / 7.0, 11008x4096 15.9 / 19.2 / 15.4 [27.8 / 32.2 / 28].
     using I1 = std::integral_constant<int, 1>;
     using I2 = std::integral_constant<int, 2>;
     using I4 = std::integral_constant<int, 4>;
     using I8 = std::integral_constant<int, 8>;
     const int64_t tiles = cdiv(w.n_out, 16);
-    const bool two = tiles >= 1024 || (!xf && m > 8 && tiles > 512), wide = tiles <= 256 && w.k_in > (xf ? 4096 : 2048);
+    const bool two = tiles >= 1024 || (tiles > 256 && (xf ? m <= 8 : m > 8 || tiles <= 512));
+    const bool wide = tiles <= 256 && w.k_in > 2048;
     auto by_shape = [&](auto xfc) {
         if (two) by_group(I2{}, I4{}, xfc);
         else if (wide) by_group(I1{}, I8{}, xfc);
