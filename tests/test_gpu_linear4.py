@@ -102,6 +102,44 @@ def test_rows(ctx, engine, n, k, group, xt, yt):
         check(run(ctx, engine, x, qt, xt, yt), want, tol, f"{m}x{n}x{k}/{group} {xt}->{yt}")
 
 
+@pytest.mark.parametrize("xt", ["f16", "f32"])
+@pytest.mark.parametrize("n,k,group", SHAPES + [(4133, 320, 64), (9000, 256, 32), (16411, 128, 64), (37, 20480, 32),
+                                                (4133, 17408, 32)], ids=lambda v: str(v))
+def test_whole_numbers(ctx, engine, n, k, group, xt):
+    """Activations, scales and biases of small whole numbers: every sum, in any
+    order and with the codes offset by 16, stays a whole number below
+    3 * 4 * 31 * 20480 < 2^24, so results are exact -- no element lost or taken twice."""
+    g = np.random.default_rng(n + k + 7)
+    u = g.integers(0, 16, (n, k), dtype=np.uint8)
+    s = 2.0 ** g.integers(0, 3, (n, k // group)) * g.choice([-1, 1], (n, k // group))
+    b = g.integers(-8, 9, s.shape).astype(np.float64)
+    qt = QuantizedTensor.affine4(ctx, u, s, b, group)
+    at = np.unique(g.integers(0, n, 200))
+    W = u[at] * np.repeat(s[at], group, 1) + np.repeat(b[at], group, 1)
+    for m in (1, 2, 3, 7, 8, 9, 15, 16, 18, 60):
+        x = g.integers(-3, 4, (m, k)).astype(KIND[xt][0])
+        got = run(ctx, engine, x, qt, xt, "f32")
+        assert np.array_equal(got[:, at], x.astype(np.float64) @ W.T), m
+
+
+@pytest.mark.parametrize("xt", ["f16", "f32"])
+@pytest.mark.parametrize("n,k,group", [(4133, 320, 64), (9000, 256, 32), (16411, 128, 64), (37, 20480, 32),
+                                       (4133, 17408, 32), (16411, 1056, 32)])
+def test_tall_and_long(ctx, engine, n, k, group, xt):
+    """Weights of many rows (two row tiles per block) and of more than 512
+    groups per row; some rows of each are checked."""
+    g = np.random.default_rng(n + k)
+    u, s, b, _ = w = weight(g, n, k, group)
+    qt = QuantizedTensor.affine4(ctx, *w)
+    at = np.unique(np.concatenate([np.arange(40), n // 2 + np.arange(40), n - 1 - np.arange(40)]) % n)
+    for m in (2, 3, 8, 9, 16, 18):
+        x = acts(g, m, k, xt)
+        want, tol = truth(x, (u[at], s[at], b[at], group), False)
+        got = run(ctx, engine, x, qt, xt, "f32")
+        assert np.isfinite(got).all() and np.count_nonzero(got == 7.0) <= 1
+        check(got[:, at], want, tol, f"{m}x{n}x{k}/{group} {xt}")
+
+
 @pytest.mark.parametrize("xt,yt", [("f16", "f16"), ("f32", "f32"), ("f16", "f32")])
 @pytest.mark.parametrize("m", [33, 130, 515])
 @pytest.mark.parametrize("n,k,group", [(300, 512, 64), (129, 1088, 64), (72, 640, 128), (100, 512, 32)])
