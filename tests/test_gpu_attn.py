@@ -286,6 +286,48 @@ def test_tree_cuts(ctx, engine, dtype, name):
     check(run_tree(ctx, engine, q, k, v, lengths, nodes, mask, dtype), want, tol, f"tree {name} {dtype}")
 
 
+# With q = 0 every weight is 1, and whole values below 9 have exact sums: a result is a
+# mean with one rounding of 1 / l, one of the product and the output's own, so a key
+# lost or taken twice among thousands shows.
+def check_means(got, sums, counts, f16, what):
+    want = sums / np.maximum(counts, 1)
+    check(got, want, ((2.0 ** -11 if f16 else U) + 3 * U) * np.abs(want) + (2.0 ** -25 if f16 else 0.0), what)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 1, 64), (4, 2, 128)])
+@pytest.mark.parametrize("lengths", [[1], [5, 0, 70, 1], [1000, 3], [129] * 9, [2500]], ids=str)
+def test_packed_takes_every_key_once(ctx, engine, dtype, heads, kv, dim, lengths):
+    starts = np.concatenate([[0], np.cumsum(lengths)])
+    q, k, v = packed_inputs(3, int(starts[-1]), heads, kv, dim, dtype)
+    v = np.random.default_rng(4).integers(-8, 9, v.shape).astype(v.dtype)
+    got = run_packed(ctx, engine, 0 * q, k, v, starts, dtype)
+    sums = np.concatenate([np.cumsum(v[a:b].astype(np.float64), 0) for a, b in zip(starts, starts[1:])])
+    counts = np.concatenate([np.arange(1, n + 1) for n in lengths])[:, None, None]
+    check_means(got, np.repeat(sums, heads // kv, 1), counts, dtype == "f16", f"means {lengths[:3]} {dtype}")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("name", list(CUTS))
+def test_tree_takes_every_key_once(ctx, engine, dtype, name):
+    seqs, cap, most, heads, kv, dim = CUTS[name]
+    g = np.random.default_rng(41)
+    nodes = [most] + [int(x) for x in g.integers(0, most + 1, seqs - 1)]
+    lengths = [cap - most] + [int(x) for x in g.integers(0, cap - most + 1, seqs - 1)]
+    q, k, v, mask = tree_inputs(42, lengths, nodes, cap, heads, kv, dim, dtype)
+    v = g.integers(-8, 9, v.shape).astype(v.dtype)
+    got = run_tree(ctx, engine, 0 * q, k, v, lengths, nodes, mask, dtype)
+    sums, counts, t = np.zeros(q.shape), np.zeros((len(q), 1, 1)), 0
+    for s, (length, n) in enumerate(zip(lengths, nodes)):
+        cached = v[s, :, :length].sum(1, dtype=np.float64)
+        for i in range(n):
+            seen = [j for j in range(n) if int(mask[t]) >> j & 1]
+            sums[t] = np.repeat(cached + v[s][:, [length + j for j in seen]].sum(1, dtype=np.float64), heads // kv, 0)
+            counts[t] = length + len(seen)
+            t += 1
+    check_means(got, sums, counts, dtype == "f16", f"means {name} {dtype}")
+
+
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 def test_tree_masks_that_leave_nothing(ctx, engine, dtype):
     """No cached position and no set bit: zeros.  Bits past the sequence's
