@@ -66,6 +66,24 @@ struct Div {
     __device__ __forceinline__ int operator()(int x) const { return (int)(((uint64_t)(uint32_t)x * m) >> sh); }
 };
 
+// Sum and maximum over the wave's 64 lanes of values >= 0.
+template <typename F>
+__device__ __forceinline__ int wave_join(int v, F f) {
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false));  // lanes 1, 2, 4, 8 before in the row of 16
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false));
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false));
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false));
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));  // the row before, the half before
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));
+    return __builtin_amdgcn_readlane(v, 63);
+}
+__device__ __forceinline__ int wave_sum(int v) {
+    return wave_join(v, [](int a, int b) { return a + b; });
+}
+__device__ __forceinline__ int wave_max(int v) {
+    return wave_join(v, [](int a, int b) { return max(a, b); });
+}
+
 // What the kernels read; strides in elements.
 struct AttnArgs {
     const void *q, *k, *v;
@@ -77,6 +95,7 @@ struct AttnArgs {
     int k_row, v_row;                 // between a head's consecutive keys
     int n_heads, n_kv, n_seqs, capacity, max_nodes;
     int tokens;
+    int ranked;   // packed: blocks in order of their work
     int wide;     // packed: row tiles per key/value head that the device takes at once
     int splits;   // tree: the most pieces a sequence's keys are cut into
     // splits > 1: sums [splits][n_kv][tokens][heads of one][dim] (a block's rows side by side),
@@ -186,21 +205,46 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
         kb = static_cast<const char *>(a.k) + at * (int64_t)sizeof(T);
         vb = static_cast<const char *>(a.v) + at * (int64_t)sizeof(T);
     } else {
-        // Row tiles of the sequences, one after another: sequence s has the
-        // indexes from starts[s] grp / BR + s on, at least as many as it needs.
-        // The last first, a long prompt's heaviest; every other run of as many as
-        // the device takes at once the other way round, so that a CU which got
-        // a heavy block gets a light one next.
-        // (tokens grp < 2^31: the grid has fewer than 2^32 threads)
-        const int total = a.by_kv(gridDim.x), run = a.by_wide(blk);
-        const int flip = run & 1 ? run * a.wide + min((run + 1) * a.wide, total) - 1 - blk : blk;
-        const int t = total - 1 - flip;
-        auto tile0 = [&](int s, int begin) { return (int64_t)begin * grp / BR + s; };
-        int end;
-        const int s = find_seq(a, t, &s0, &end, tile0);
-        nq = max(end - s0, 0);
-        const int row = (int)(t - tile0(s, s0)) * BR;
-        if (row < 0 || row >= nq * grp) return;
+        int row;
+        // every other run of as many blocks as the device takes at once goes the other way
+        // round, so that a CU which got a heavy block gets a light one next
+        const int run = a.by_wide(blk);
+        auto turned = [&](int total) { return run & 1 ? run * a.wide + min((run + 1) * a.wide, total) - 1 - blk : blk; };
+        if (a.ranked) {
+            // row tiles of all sequences (at most 64) by the keys they take, the most first
+            const int b0 = seq_start(a, min(lane, a.n_seqs)), b1 = seq_start(a, min(lane + 1, a.n_seqs));
+            const int mine = (int)((uint32_t)(max(b1 - b0, 0) * grp + BR - 1) / BR);  // tiles of sequence `lane`
+            const int total = wave_sum(mine);
+            if (blk >= total) return;
+            const int rank = turned(total);
+            // its place in its sequence: the last that more than `rank` tiles reach; `above` tiles lie past it
+            int lo = 0, hi = wave_max(mine), above = 0;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2, c = wave_sum(max(mine - mid, 0));
+                if (c > rank) {
+                    lo = mid;
+                } else {
+                    hi = mid;
+                    above = c;
+                }
+            }
+            const uint64_t has = __builtin_amdgcn_ballot_w64(mine > lo);
+            const int nth = __builtin_amdgcn_mbcnt_hi((uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0));
+            const int s = __builtin_ctzll(__builtin_amdgcn_ballot_w64(mine > lo && nth == rank - above));
+            s0 = __builtin_amdgcn_readlane(b0, s);
+            nq = __builtin_amdgcn_readlane(b1, s) - s0;
+            row = lo * BR;
+        } else {
+            // one sequence after another, its last tile first: sequence s has the indexes from
+            // starts[s] grp / BR + s on, at least as many as it needs (tokens grp < 2^31: the grid has fewer than 2^32 threads)
+            const int total = a.by_kv(gridDim.x), t = total - 1 - turned(total);
+            auto tile0 = [&](int s, int begin) { return (int64_t)begin * grp / BR + s; };
+            int end;
+            const int s = find_seq(a, t, &s0, &end, tile0);
+            nq = max(end - s0, 0);
+            row = (int)(t - tile0(s, s0)) * BR;
+            if (row < 0 || row >= nq * grp) return;
+        }
         // rows are counted from the tile's first token on
         const int skip = a.by_grp(row);
         r0 = row - skip * grp;
@@ -208,6 +252,9 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
         before = skip;  // tokens of the sequence before token 0 of these
         nq -= skip;
         nkeys = before + min(nq, a.by_grp(r0 + BR - 1) + 1);
+        // (per lane: where the compiler knows it uniform it keeps 16 more registers through the
+        // tiles, and head_dim 128 spills: 8192 tokens 550 -> 620 us)
+        asm volatile("" : "+v"(nq));
         ntiles = (nkeys + KT - 1) / KT;
         const int64_t seq = (int64_t)(s0 - skip);
         kb = static_cast<const char *>(a.k) + (seq * a.k_row + g * HD) * (int64_t)sizeof(T);
@@ -689,8 +736,8 @@ int launch(AttnArgs a, hipStream_t s) {
     a.by_kv = Div::by(a.n_kv);
     a.by_grp = Div::by(grp);
     a.by_seqs = Div::by(a.n_seqs);
-    a.by_rbs = Div::by(TREE ? cdiv(a.max_nodes * grp, br) : 1);
     a.by_wide = Div::by(TREE ? 1 : a.wide);
+    a.by_rbs = Div::by(TREE ? cdiv(a.max_nodes * grp, br) : 1);
     const int64_t tiles = TREE ? cdiv(a.max_nodes * grp, br) * a.n_seqs * a.splits : (int64_t)a.tokens * grp / br + a.n_seqs;
     if (!grid_ok(tiles * a.n_kv, 64 * SH::NW)) return fail(RQ_ERR_SHAPE, "too many rows for one call");
     hipLaunchKernelGGL((k_attn<T, HD, WR, KG, TREE>), dim3((unsigned)(tiles * a.n_kv)), dim3(64 * SH::NW), 0, s, a);
@@ -708,11 +755,16 @@ int launch(AttnArgs a, hipStream_t s) {
 // blocks take longer, without two blocks (us, 128 rows / 64 / 32: one prompt of 300
 // tokens, 32/4 heads of 64, 9.2 / 8.2 / 7.8, of 2048 39.4 / 38.4 / 53.4, of 8192 with 32/8 heads of 128
 // 570 / 666 / 1487; f32, three of 417, 1000 and 83 87 / 61 / 72, one of 2048 160 / 166 / 195).
+// Blocks are ranked by their work where some have to wait for others and the sequences
+// fit a wave's lanes (9 prompts of 1 to 1047 tokens, 32/4 heads of 64, in the order of the tokens
+// 31.4, ranked 26-28; in one round of blocks the search only costs, 5 prompts of 1 to 64 4.9 / 5.2).
 template <typename T, int HD>
-int launch_packed(const AttnArgs &a, int cus, hipStream_t s) {
+int launch_packed(AttnArgs a, int cus, hipStream_t s) {
     const int64_t blocks = cdiv((int64_t)a.tokens * a.n_heads, 128);
-    if (blocks < (sizeof(T) == 4 ? 2 : 1) * cus) return launch<T, HD, 2, 2, false>(a, s);
-    return launch<T, HD, 4, 1, false>(a, s);
+    const bool half = blocks < (sizeof(T) == 4 ? 2 : 1) * cus;
+    a.wide = std::max(1, cus / a.n_kv);
+    a.ranked = a.n_seqs > 1 && a.n_seqs <= 64 && (half ? 2 : 1) * blocks > cus;
+    return half ? launch<T, HD, 2, 2, false>(a, s) : launch<T, HD, 4, 1, false>(a, s);
 }
 
 // How a tree call is cut: blocks of 32 wr rows and kg groups of keys, the keys of a
@@ -897,7 +949,6 @@ int rq_attn_packed(rq_ctx *ctx, const rq_attn *attn, const void *q, const void *
     if (st != RQ_OK || !run) return st;
     hipStream_t s = pick(ctx, stream);
     const int cus = ctx->num_cus;
-    a.wide = std::max(1, cus / a.n_kv);
     if (attn->dtype == RQ_F16)
         return attn->head_dim == 64 ? launch_packed<_Float16, 64>(a, cus, s) : launch_packed<_Float16, 128>(a, cus, s);
     return attn->head_dim == 64 ? launch_packed<float, 64>(a, cus, s) : launch_packed<float, 128>(a, cus, s);
