@@ -96,7 +96,7 @@ struct AttnArgs {
     int n_heads, n_kv, n_seqs, capacity, max_nodes;
     int tokens;
     int ranked;   // packed: blocks in order of their work
-    int wide;     // packed: row tiles per key/value head that the device takes at once
+    int wide;     // packed: row tiles per key/value head between turns of their order
     int splits;   // tree: the most pieces a sequence's keys are cut into
     // splits > 1: sums [splits][n_kv][tokens][heads of one][dim] (a block's rows side by side),
     // then (m, l) [tokens][n_heads][splits]
@@ -206,8 +206,8 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
         vb = static_cast<const char *>(a.v) + at * (int64_t)sizeof(T);
     } else {
         int row;
-        // every other run of as many blocks as the device takes at once goes the other way
-        // round, so that a CU which got a heavy block gets a light one next
+        // every other run of `wide` tiles, as many as the device takes at once, the other way round:
+        // a CU which got a heavy one gets a light one next
         const int run = a.by_wide(blk);
         auto turned = [&](int total) { return run & 1 ? run * a.wide + min((run + 1) * a.wide, total) - 1 - blk : blk; };
         if (a.ranked) {
@@ -751,18 +751,22 @@ int launch(AttnArgs a, hipStream_t s) {
     return RQ_OK;
 }
 
-// Rows per block: 64 where blocks of 128 would leave CUs without work, in f32, whose
-// blocks take longer, without two blocks (us, 128 rows / 64 / 32: one prompt of 300
-// tokens, 32/4 heads of 64, 9.2 / 8.2 / 7.8, of 2048 39.4 / 38.4 / 53.4, of 8192 with 32/8 heads of 128
-// 570 / 666 / 1487; f32, three of 417, 1000 and 83 87 / 61 / 72, one of 2048 160 / 166 / 195).
+// Rows per block: 64 where blocks of 128 would leave CUs without work, or are the tiles of one long prompt,
+// in f32, whose blocks take longer, without two blocks (us, 128 rows / 64: one prompt of 300
+// tokens, 32/4 heads of 64, 8.0 / 7.2, of 1200 21.8 / 18.2, of 2048 36.4 / 33.8, of 3000 57.8 / 60.9, three
+// of 700, 800 and 500 18.3 / 20.5, one of 8192 with 32/8 heads of 128 557 / 641; f32, three of 417, 1000
+// and 83 87 / 59, one of 2048 158 / 166).
 // Blocks are ranked by their work where some have to wait for others and the sequences
 // fit a wave's lanes (9 prompts of 1 to 1047 tokens, 32/4 heads of 64, in the order of the tokens
-// 31.4, ranked 26-28; in one round of blocks the search only costs, 5 prompts of 1 to 64 4.9 / 5.2).
+// 31.4, ranked 28; in one round of blocks the search only costs, 5 prompts of 1 to 64 4.9 / 5.2).
+// Every other run of them is turned round in f32 only (one prompt of 2048 158, in order 206; fp16 560 / 545
+// for 8192 tokens).
 template <typename T, int HD>
 int launch_packed(AttnArgs a, int cus, hipStream_t s) {
+    constexpr bool F16 = sizeof(T) == 2;
     const int64_t blocks = cdiv((int64_t)a.tokens * a.n_heads, 128);
-    const bool half = blocks < (sizeof(T) == 4 ? 2 : 1) * cus;
-    a.wide = std::max(1, cus / a.n_kv);
+    const bool half = blocks < (F16 ? 1 : 2) * cus || (F16 && a.n_seqs == 1 && blocks <= 2 * cus);
+    a.wide = F16 ? 1 << 30 : std::max(1, cus / a.n_kv);
     a.ranked = a.n_seqs > 1 && a.n_seqs <= 64 && (half ? 2 : 1) * blocks > cus;
     return half ? launch<T, HD, 2, 2, false>(a, s) : launch<T, HD, 4, 1, false>(a, s);
 }
