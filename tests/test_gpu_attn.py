@@ -294,9 +294,13 @@ def check_means(got, sums, counts, f16, what):
     check(got, want, ((2.0 ** -11 if f16 else U) + 3 * U) * np.abs(want) + (2.0 ** -25 if f16 else 0.0), what)
 
 
+RAGGED = [int(x) for x in np.random.default_rng(5).integers(0, 60, 65)]
+
+
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
-@pytest.mark.parametrize("heads,kv,dim", [(8, 1, 64), (4, 2, 128)])
-@pytest.mark.parametrize("lengths", [[1], [5, 0, 70, 1], [1000, 3], [129] * 9, [2500]], ids=str)
+@pytest.mark.parametrize("heads,kv,dim", [(8, 1, 64), (4, 2, 128), (32, 4, 64), (24, 3, 128)])
+@pytest.mark.parametrize("lengths", [[1], [5, 0, 70, 1], [1000, 3], [129] * 9, [2500], [300, 290], RAGGED[:64], RAGGED,
+                                     [0, 700, 1, 300, 0, 530, 64], [1, 2, 1500]], ids=lambda v: str(v[:7]))
 def test_packed_takes_every_key_once(ctx, engine, dtype, heads, kv, dim, lengths):
     starts = np.concatenate([[0], np.cumsum(lengths)])
     q, k, v = packed_inputs(3, int(starts[-1]), heads, kv, dim, dtype)
