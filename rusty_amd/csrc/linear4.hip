@@ -107,6 +107,8 @@ __device__ __forceinline__ void split8(floatx4 a, floatx4 b, int sh, u32x4 &hi, 
 // meet in LDS; a wave then finishes whole (row, token) sums.
 // XF: f32 rows; each chunk of a row is scaled by the power of two that puts its
 // largest magnitude in [2^14, 2^15) and carried as two fp16 terms.
+// One row: 4096x4096 4.8 us (one launch's first bytes and end bound it), 32000x2048 8.9,
+// 4.6 TB/s (HBM).
 template <int M, int CPT, int TPR, int R, bool XF>
 __global__ __launch_bounds__(TH) void k_linear4_dot(const uint8_t *__restrict__ W, const float *__restrict__ scales,
                                                     const float *__restrict__ biases, const void *__restrict__ X,
@@ -249,7 +251,8 @@ __global__ __launch_bounds__(TH) void k_linear4_dot(const uint8_t *__restrict__ 
 // Scales and biases go through LDS too, whole rows of them first (they lie one
 // after another), as (s, b - 16 s): read by each lane in place they touch 16 cache
 // lines per load, which bounded the kernel (8 rows, 11008x4096 in groups of 64 21.2 us,
-// 12.6 this way; 4096x11008 in groups of 32 32.3, 16.9).  Rows longer than kSegGroups groups take several rounds.
+// 12.6 this way; 4096x11008 in groups of 32 32.3, 16.9; of 5.6 and 6.8 that the bytes need.  What
+// is left is the loads of X, which every block reads whole, about 4 and 8 us).  Rows longer than kSegGroups groups take several rounds.
 // XF: f32 rows as two fp16 terms; a batch whose sums are not finite (values past
 // fp16's range) is multiplied again, each row scaled by a power of two.
 constexpr int kSegGroups = 512;
@@ -533,7 +536,7 @@ __global__ __launch_bounds__(TH) void k_linear4_generic(const uint8_t *__restric
     }
 }
 
-// 4-bit codes to bytes, 32 of them per thread.
+// 4-bit codes to bytes, 32 of them per thread (bound by its 1.5 bytes per code: 4096x4096 about 5 us).
 __global__ __launch_bounds__(TH) void k_widen4(const u32x4 *__restrict__ codes, u32x4 *__restrict__ out, int64_t n) {
     for (int64_t i = (int64_t)blockIdx.x * TH + threadIdx.x; i < n; i += (int64_t)gridDim.x * TH) {
         const u32x4 w = codes[i];
