@@ -536,7 +536,7 @@ __global__ __launch_bounds__(TH) void k_linear4_generic(const uint8_t *__restric
     }
 }
 
-// 4-bit codes to bytes, 32 of them per thread (bound by its 1.5 bytes per code: 4096x4096 about 5 us).
+// 4-bit codes to bytes, 32 of them per thread (bound by its 1.5 bytes per code: 4096x4096 9 us, 11008x4096 15.5, 4.4 TB/s).
 __global__ __launch_bounds__(TH) void k_widen4(const u32x4 *__restrict__ codes, u32x4 *__restrict__ out, int64_t n) {
     for (int64_t i = (int64_t)blockIdx.x * TH + threadIdx.x; i < n; i += (int64_t)gridDim.x * TH) {
         const u32x4 w = codes[i];
