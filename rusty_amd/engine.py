@@ -482,7 +482,9 @@ class ComputeEngine:
         [tokens, n_heads, head_dim], the cache k and v [n_seqs, n_kv_heads,
         capacity, head_dim] (``strides``: elements between sequences, heads and
         positions where it is laid out otherwise), ``starts`` I32 [n_seqs + 1],
-        ``lengths`` I32 [n_seqs], ``mask`` U64 [tokens] or None (chains)."""
+        ``lengths`` I32 [n_seqs], ``mask`` U64 [tokens] or None (chains).
+        Without a ``workspace`` the call allocates one where it needs it; a
+        captured call is given its own, which lives as long as the graph."""
         if len(q.shape) != 3 or len(k.shape) != 4 or k.shape != v.shape or out.shape != q.shape \
                 or k.shape[3] != q.shape[2]:
             raise ValueError(f"q {q.shape} / out {out.shape}: expected [tokens, heads, dim]; k {k.shape} / v {v.shape}: "
