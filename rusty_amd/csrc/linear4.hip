@@ -286,8 +286,9 @@ __global__ __launch_bounds__(NW * 64) void k_linear4_mfma(const uint8_t *__restr
 
     struct Batch {
         u32x4 w[RT][2], x[XF ? 2 * XL : XL];
-        int g;  // the batch's first group, from the segment's
+        int g, r;  // the batch's first k: its group, from the segment's, and how far into it (in 32 k)
     };
+    const int g32 = group / 32;
     floatx4 acc[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -317,7 +318,8 @@ __global__ __launch_bounds__(NW * 64) void k_linear4_mfma(const uint8_t *__restr
             int bb = bi + rot;
             bb -= bb >= nb ? nb : 0;
             const uint32_t k0 = (uint32_t)kbeg + (uint32_t)bb * 256u;
-            b.g = bb * 256 / group;
+            b.g = bb * 8 / g32;
+            b.r = bb * 8 - b.g * g32;
 #pragma unroll
             for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -341,6 +343,16 @@ __global__ __launch_bounds__(NW * 64) void k_linear4_mfma(const uint8_t *__restr
         auto mma = [&](const Batch &b) {
             uint32_t u[RT][8];
             float2 sv[RT][NG];
+            // the groups of the batch's NG pieces of GS * 32 k, which divide a group: a group
+            // may start and end anywhere in a batch (96, 192, ...)
+            int gi[NG], at = b.g, in = b.r;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                gi[g] = min(at, sg - 1);
+                in += GS;
+                at += in == g32;
+                in = in == g32 ? 0 : in;
+            }
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
                 uint8_t *wl = wt[wave][i];
@@ -353,10 +365,7 @@ __global__ __launch_bounds__(NW * 64) void k_linear4_mfma(const uint8_t *__restr
                 // not stored: any place inside sc does)
                 const int r = min(16 * i + fr, rows - 1);
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    const int gi = b.g + g * GS * 32 / group;
-                    sv[i][g] = sc[r * pitch + min(gi, sg - 1)];
-                }
+                for (int g = 0; g < NG; ++g) sv[i][g] = sc[r * pitch + gi[g]];
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     u[i][j] = *reinterpret_cast<const uint32_t *>(wl + fr * 128 + ((j ^ (fr & 7)) << 4) + 4 * q);
