@@ -83,9 +83,21 @@ __device__ __forceinline__ u32x4 turn8(u32x4 x) {
     return y;
 }
 
+// The largest v of the four lanes l % 16, l % 16 + 16, ... (EIGHT: of the eight l % 8, l % 8 + 8, ...).
+template <bool EIGHT>
+__device__ __forceinline__ float row_max(float v) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+    const unsigned p0 = p[0], p1 = p[1];
+    v = fmaxf(__builtin_bit_cast(float, p0), __builtin_bit_cast(float, p1));
+    const auto q = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+    const unsigned q0 = q[0], q1 = q[1];
+    v = fmaxf(__builtin_bit_cast(float, q0), __builtin_bit_cast(float, q1));
+    return EIGHT ? fmaxf(v, dpp<0x128>(v)) : v;
+}
+
 // 8 f32 values (a, b) times 2^-sh -> hi = fp16(v), lo = fp16(v - hi) in the
-// codes' pair order: hi + lo is v to about 2^-22 relative while |v| stays inside
-// fp16's range.
+// codes' pair order: hi + lo is the scaled v to 2^-22 relative from 2^-3 to fp16's largest, and
+// to 2^-25 below.
 template <bool SC>
 __device__ __forceinline__ void split8(floatx4 a, floatx4 b, int sh, u32x4 &hi, u32x4 &lo) {
 #pragma unroll
@@ -253,8 +265,11 @@ __global__ __launch_bounds__(TH) void k_linear4_dot(const uint8_t *__restrict__ 
 // lines per load, which bounded the kernel (8 rows, 11008x4096 in groups of 64 21.2 us,
 // 12.6 this way; 4096x11008 in groups of 32 32.3, 16.9; of 5.6 and 6.8 that the bytes need.  What
 // is left is the loads of X, which every block reads whole, about 4 and 8 us).  Rows longer than kSegGroups groups take several rounds.
-// XF: f32 rows as two fp16 terms; a batch whose sums are not finite (values past
-// fp16's range) is multiplied again, each row scaled by a power of two.
+// XF: f32 rows as two fp16 terms.  In a batch where a row's largest magnitude is past fp16's range or
+// below 1 (whose low terms reach fp16's subnormals, an error of 2^-25 whatever the row's size)
+// every row is scaled by a power of two, so that each keeps f32 accuracy.  Looking at the batch first costs
+// 5 % (13 rows 4096x11008 25.7 -> 27.5 us in a graph, 8 rows 11008x4096 19.5 -> 20.3), a scaled one 3 % more; scaling
+// them all 28.3 and 21.9; multiplying first and again where needed spills (37).
 constexpr int kSegGroups = 512;
 
 // M8: up to 8 rows, where half of the lanes would load nothing: lanes 8-15 of each 16 take the
@@ -413,30 +428,17 @@ __global__ __launch_bounds__(NW * 64) void k_linear4_mfma(const uint8_t *__restr
                 }
             };
             if constexpr (XF) {
-                floatx4 old[RT];
+                float top = 0.0f;  // the row's largest magnitude in the batch
 #pragma unroll
-                for (int i = 0; i < RT; ++i) old[i] = acc[i];
-                run(std::false_type{}, 0);
-                bool bad = false;
-#pragma unroll
-                for (int i = 0; i < RT; ++i)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) bad = bad || !__builtin_isfinite(acc[i][r]);
-                if (__builtin_amdgcn_ballot_w64(bad) != 0) {
-                    float amax = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 2 * XL; ++i) {
-                        const floatx4 f = __builtin_bit_cast(floatx4, b.x[i]);
-                        amax = fmaxf(fmaxf(fmaxf(amax, fabsf(f.x)), fmaxf(fabsf(f.y), fabsf(f.z))), fabsf(f.w));
-                    }
-                    amax = fmaxf(amax, __shfl_xor(amax, 16));  // the four lanes of a row
-                    amax = fmaxf(amax, __shfl_xor(amax, 32));
-                    if constexpr (M8) amax = fmaxf(amax, __shfl_xor(amax, 8));
-                    const int sh = __builtin_amdgcn_frexp_expf(amax) - 15;
-#pragma unroll
-                    for (int i = 0; i < RT; ++i) acc[i] = old[i];
-                    run(std::true_type{}, sh);
+                for (int i = 0; i < 2 * XL; ++i) {
+                    const floatx4 f = __builtin_bit_cast(floatx4, b.x[i]);
+                    top = fmaxf(fmaxf(fmaxf(top, fabsf(f.x)), fmaxf(fabsf(f.y), fabsf(f.z))), fabsf(f.w));
                 }
+                top = row_max<M8>(top);
+                // sh puts it in [2^14, 2^15) (2^-126 at most, so that the power is a normal number)
+                if (__builtin_amdgcn_ballot_w64(top > 65504.0f || (top < 1.0f && top > 0.0f)))
+                    run(std::true_type{}, max(__builtin_amdgcn_frexp_expf(top) - 15, -126));
+                else run(std::false_type{}, 0);
             } else {
                 run(std::false_type{}, 0);
             }

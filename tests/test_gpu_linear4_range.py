@@ -1,0 +1,73 @@
+"""4-bit Linears at the ends of their types' range.
+
+Tolerance as in test_gpu_linear4.py without its fp16 term, |dy| <= ((K / 32 +
+64) u + 2^-21) S and half a step of the output: the two fp16 terms of an f32
+activation keep 2^-22 of it, or 2^-25 of the largest of its row in their
+256 k, which is added here as 2^-23 (two such errors, a factor 2 spare) of
+that largest value times the weights' sizes.
+"""
+import numpy as np
+import pytest
+from test_gpu_linear4 import KIND, U, acts, check, parts, run, truth, weight
+
+from rusty_amd import QuantizedTensor
+
+pytestmark = pytest.mark.gpu
+
+
+def tight(x, w, y_f16):
+    """truth() of 16 rows at a time: exact codes, f32 rows as two terms."""
+    p = [truth(x[i:i + 16], w, y_f16) for i in range(0, len(x), 16)]
+    return np.concatenate([a for a, _ in p]), np.concatenate([b for _, b in p])
+
+
+def peaks(x, S):
+    """sum over k of S[n, k] times the largest |x| of the row in the 256 k around k."""
+    out = np.zeros((x.shape[0], S.shape[0]))
+    for k in range(0, x.shape[1], 256):
+        out += np.abs(x[:, k:k + 256]).max(1, keepdims=True).astype(np.float64) * S[:, k:k + 256].sum(1)
+    return out
+
+
+@pytest.mark.parametrize("std", [1.0, 0.3, 1e-2, 1e-3, 1e-4, 1e-6, 1e-20, 1e-37])
+@pytest.mark.parametrize("n,k,group", [(70, 1024, 64), (19, 20480, 128), (600, 320, 32)], ids=lambda v: str(v))
+def test_small_f32_rows(ctx, engine, n, k, group, std):
+    """f32 rows of any magnitude keep f32 accuracy in 1 to 48 rows: the error is relative to the row."""
+    g = np.random.default_rng(k)
+    w = weight(g, n, k, group)
+    qt = QuantizedTensor.affine4(ctx, *w)
+    S = parts(w)[1]
+    for m in (1, 2, 3, 8, 9, 16, 17, 40):
+        x = acts(g, m, k, "f32", std)
+        want, tol = tight(x, w, False)
+        tol = tol + 2.0 ** -23 * peaks(x, S) / 16 + 2.0 ** -149 * k  # (peaks: every element at its row's largest)
+        check(run(ctx, engine, x, qt, "f32", "f32"), want, tol, f"std {std} {m}x{n}x{k}")
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 8, 13, 16])
+def test_small_rows_typical_error(ctx, engine, m):
+    """The rms error relative to the rms of S x: f32 rounding of K / 32 sums and 2^-22 of the activations stay below
+    2^-20 of the typical size at any magnitude (a row rounded to fp16's subnormals: 1e-5 and more at 1e-3)."""
+    g = np.random.default_rng(m + 9)
+    w = weight(g, 96, 2048, 64)
+    qt = QuantizedTensor.affine4(ctx, *w)
+    S = parts(w)[1]
+    for std in (1.0, 1e-2, 1e-3, 1e-4, 1e-5):
+        x = acts(g, m, 2048, "f32", std)
+        want, _ = tight(x, w, False)
+        err = run(ctx, engine, x, qt, "f32", "f32") - want
+        size = np.sqrt((x.astype(np.float64) ** 2) @ (S ** 2).T)
+        r = float(np.sqrt((err ** 2).mean()) / np.sqrt((size ** 2).mean()))
+        print(f"[m {m} std {std}] rms {r:.2e}", flush=True)
+        assert r < 2.0 ** -20
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 8, 9, 16, 33])
+@pytest.mark.parametrize("xt", ["f16", "f32"])
+def test_tiny_fp16_rows(ctx, engine, m, xt):
+    """Values of fp16's subnormals are exact activations, in either type."""
+    g = np.random.default_rng(m + 21)
+    w = weight(g, 40, 512, 64)
+    x = (g.integers(-64, 65, (m, 512)) * 2.0 ** -24).astype(KIND[xt][0])
+    want, tol = tight(x, w, False)
+    check(run(ctx, engine, x, w, xt, "f32"), want, tol, f"subnormal m={m} {xt}")
