@@ -2,15 +2,16 @@
 
 Tolerance as in test_gpu_linear4.py without its fp16 term, |dy| <= ((K / 32 +
 64) u + 2^-21) S and half a step of the output: the two fp16 terms of an f32
-activation keep 2^-22 of it, or 2^-25 of the largest of its row in their
-256 k, which is added here as 2^-23 (two such errors, a factor 2 spare) of
-that largest value times the weights' sizes.
+activation are it to 2^-22, or where the row's largest magnitude in the 256 k
+is 1 or more (or else scaled to 2^14 and more) to 2^-25 of that, half the
+spacing of fp16's subnormals: 2^-25 of the largest times the weights' sizes.
 """
 import numpy as np
 import pytest
 from test_gpu_linear4 import KIND, U, acts, check, parts, run, truth, weight
 
 from rusty_amd import QuantizedTensor
+from rusty_amd.hiprt import Stream
 
 pytestmark = pytest.mark.gpu
 
@@ -40,7 +41,7 @@ def test_small_f32_rows(ctx, engine, n, k, group, std):
     for m in (1, 2, 3, 8, 9, 16, 17, 40):
         x = acts(g, m, k, "f32", std)
         want, tol = tight(x, w, False)
-        tol = tol + 2.0 ** -23 * peaks(x, S) / 16 + 2.0 ** -149 * k  # (peaks: every element at its row's largest)
+        tol = tol + 2.0 ** -25 * peaks(x, S) + 2.0 ** -149 * k
         check(run(ctx, engine, x, qt, "f32", "f32"), want, tol, f"std {std} {m}x{n}x{k}")
 
 
@@ -71,3 +72,16 @@ def test_tiny_fp16_rows(ctx, engine, m, xt):
     x = (g.integers(-64, 65, (m, 512)) * 2.0 ** -24).astype(KIND[xt][0])
     want, tol = tight(x, w, False)
     check(run(ctx, engine, x, w, xt, "f32"), want, tol, f"subnormal m={m} {xt}")
+
+
+@pytest.mark.parametrize("xt,yt", [("f16", "f16"), ("f32", "f32"), ("f16", "f32")])
+@pytest.mark.parametrize("n,k,group", [(300, 512, 64), (72, 640, 128), (100, 512, 32)], ids=lambda v: str(v))
+def test_sixteen_at_a_time(ctx, engine, n, k, group, xt, yt):
+    """17 to 48 rows, and any number on a caller's stream or in groups of 32, keep the codes exact."""
+    g = np.random.default_rng(n + k)
+    w = weight(g, n, k, group)
+    qt = QuantizedTensor.affine4(ctx, *w)
+    for m, stream in ((17, None), (33, None), (48, None), (49, Stream()), (130, Stream())) + (((130, None),) if group == 32 else ()):
+        x = acts(g, m, k, xt)
+        want, tol = tight(x, w, yt == "f16")
+        check(run(ctx, engine, x, qt, xt, yt, stream), want, tol, f"{m}x{n}x{k}/{group} {xt}->{yt}")
