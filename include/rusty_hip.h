@@ -231,7 +231,8 @@ int rq_matmul_at(rq_ctx *ctx, const float *a, const float *b, float *out, int64_
  * RQ_Q_AFFINE_U4 weights go 16 rows at a time with exact codes up to m = 48,
  * f32 rows at f32 accuracy whatever their magnitude (two fp16 terms again, scaled
  * per 32 values of a row for one or two rows of up to 16384, else per row and 256 k where
- * needed); with more rows, on the context's own stream
+ * needed), and the infinities and NaN that x w has (an output that is not finite
+ * is summed again term by term, so such rows take longer); with more rows, on the context's own stream
  * and with k_in and group multiples of 64, the codes are widened to bytes in the context's
  * workspace and take the GEMM, at its accuracy, where they fit (48 MiB, k_in n_out bytes).
  * On the context's own stream (stream NULL) a GEMM with few tokens splits K over

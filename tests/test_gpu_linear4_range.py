@@ -85,3 +85,48 @@ def test_sixteen_at_a_time(ctx, engine, n, k, group, xt, yt):
         x = acts(g, m, k, xt)
         want, tol = tight(x, w, yt == "f16")
         check(run(ctx, engine, x, qt, xt, yt, stream), want, tol, f"{m}x{n}x{k}/{group} {xt}->{yt}")
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 8, 9, 16, 33])
+@pytest.mark.parametrize("big", [1e36, 1e37])
+def test_sums_that_fit_while_their_parts_do_not(ctx, engine, m, big):
+    """f32 rows whose products with 16 + u pass f32's range though the result does not."""
+    g = np.random.default_rng(m)
+    w = weight(g, 48, 512, 64)
+    x = np.clip(acts(g, m, 512, "f32"), -3, 3) * np.float32(big)
+    want, tol = tight(x, w, False)
+    assert np.abs(want).max() < 1e38
+    check(run(ctx, engine, x, w, "f32", "f32"), want, tol, f"{big} m={m}")
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 8, 9, 16, 20, 60])
+@pytest.mark.parametrize("xt", ["f16", "f32"])
+@pytest.mark.parametrize("n,k,group", [(37, 320, 32), (300, 512, 64), (20, 20480, 64), (50, 360, 24)], ids=lambda v: str(v))
+def test_infinities_and_nan(ctx, engine, n, k, group, m, xt):
+    """An infinite activation gives the infinity of x w, whatever the other terms; NaN, and infinities of both signs or
+    against a zero weight, give NaN; other rows keep their values."""
+    if m > 48 and group % 64 == 0 and xt == "f32":
+        pytest.skip("the 8-bit GEMM's f32 rows")
+    g = np.random.default_rng(n + m)
+    u, s, b, _ = w = weight(g, n, k, group)
+    s[:, 0], b[:, 0], u[3, 2] = 2.0 ** -6, -2.0 ** -4, 4  # W[3, 2] = 0
+    u[:, 1] |= 8
+    x = acts(g, m, k, xt)
+    x[0, k - 1] = np.inf
+    if m > 2:
+        x[1, 5], x[2, 2] = np.nan, -np.inf
+    if m > 8:
+        x[7, 1], x[7, 0], x[8, 1] = np.inf, 0.0, -np.inf
+    W = parts(w)[0]
+    with np.errstate(invalid="ignore"):
+        want = np.stack([(x[i].astype(np.float64) * W).sum(1) for i in range(m)])
+    for stream in (None, Stream()) if m in (3, 60) else (None,):
+        got = run(ctx, engine, x, w, xt, "f32", stream).astype(np.float64)
+        assert np.array_equal(np.isnan(got), np.isnan(want))
+        assert np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+        ok = np.isfinite(want).all(1)
+        if ok.any():
+            ref, tol = truth(x[ok], w, False) if m > 48 else tight(x[ok], w, False)
+            if m > 48:  # (the fp16 term of truth() past 16 rows)
+                tol = tol + 2.0 ** -10 * np.abs(x[ok].astype(np.float64)) @ np.abs(W).T
+            check(got[ok], ref, tol, f"beside {m}x{n}x{k} {xt}")
