@@ -56,6 +56,11 @@ class DType(enum.Enum):
         return self.np.itemsize
 
 
+# Array types that UnifiedTensor.new keeps; numbers of any other become FP32.
+# I32 and U64 buffers (offsets, lengths, masks) are asked for by name.
+_INFERRED = {d.value: d for d in (DType.FP32, DType.FP16, DType.I8, DType.U8, DType.U32)}
+
+
 def _prod(shape: Sequence[int]) -> int:
     n = 1
     for s in shape:
@@ -129,7 +134,7 @@ class UnifiedTensor:
             dtype: DType | None = None) -> "UnifiedTensor":
         arr = np.asarray(data)
         if dtype is None:
-            dtype = DType(arr.dtype.type) if arr.dtype.type in {d.value for d in DType} else DType.FP32
+            dtype = _INFERRED.get(arr.dtype.type, DType.FP32)
         arr = np.ascontiguousarray(arr, dtype=dtype.np)
         shape = tuple(arr.shape) if shape is None else tuple(shape)
         if _prod(shape) != arr.size:
