@@ -491,7 +491,8 @@ int rq_llama_decode(rq_llama *model, int32_t n_steps, rq_stream stream);
  * *accepted + 1 tokens, and their keys and values take their places in the
  * cache.  The result is what as many rq_llama_decode steps give, up to the
  * rounding of the kernels that many rows take.  Needs n + 1 free positions
- * (RQ_ERR_SHAPE otherwise); on an error the sequence is as it was.  The first
+ * (RQ_ERR_SHAPE otherwise); on an error the sequence is as it was (unless the device
+ * itself fails under the pass, after which no call works).  The first
  * call allocates [64, vocab] logits.  Uses the context's GEMM workspace as
  * rq_llama_prefill does.  Synchronizes. */
 int rq_llama_verify(rq_llama *model, const int32_t *tokens, const int32_t *parents, int32_t n, int32_t *accepted,

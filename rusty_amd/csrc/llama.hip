@@ -63,7 +63,7 @@ struct rq_llama {
     int prefill_cap = 0;   // rows the buffers hold
     int prefill_rows = 0;  // rows per batched chunk; 0: one position at a time through the step graph
     // drafted trees, allocated by the first rq_llama_verify
-    void *verify = nullptr;
+    void *verify = nullptr, *pinned = nullptr;
     hipGraph_t graph = nullptr;  // one decode step
     hipGraphExec_t exec = nullptr;
     hipGraph_t graph_k = nullptr;  // kGraphSteps consecutive steps
@@ -593,6 +593,10 @@ struct VerifyOut {
     int accepted, last;        // drafts followed, the row of the last one (0: none)
     int path[kVerifyRows];     // their rows
 };
+struct VerifyPinned {  // host memory that the copies of a pass in flight use
+    VerifyHost in;
+    VerifyOut out;
+};
 struct VerifyBuffers {
     VerifyHost *in;
     VerifyOut *out;
@@ -658,38 +662,38 @@ __global__ __launch_bounds__(AT) void k_argmax_rows(const float *__restrict__ lo
     }
 }
 
-// Follows the greedy tokens through the tree, appends them to the sequence and
-// leaves the step state where the decode steps continue.  One block.
-__global__ __launch_bounds__(NT) void k_verify_accept(const VerifyHost *__restrict__ in, int rows, int pos,
+// Follows the greedy tokens through the tree.
+__global__ void k_verify_walk(const VerifyHost *__restrict__ in, int rows, const int *__restrict__ next,
+                              VerifyOut *__restrict__ out) {
+    int cur = 0, n = 0;
+    for (;;) {
+        const int want = next[cur];
+        int child = 0;
+        for (int r = cur + 1; r < rows && !child; ++r)
+            if (in->parents[r] == cur && in->tokens[r] == want) child = r;
+        if (!child) break;
+        out->path[n++] = child;
+        cur = child;
+    }
+    out->accepted = n;
+    out->last = cur;
+}
+
+// Appends the followed tokens and the last greedy one to the sequence and leaves the step
+// state where the decode steps continue.  The pass's only writes to what decode steps,
+// further passes and read-outs see, launched last: an error before it leaves the sequence as it was.
+__global__ __launch_bounds__(NT) void k_verify_commit(const VerifyOut *__restrict__ out, int pos,
                                                       const int *__restrict__ next, const float *__restrict__ all,
                                                       int V, const _Float16 *__restrict__ embed, int H,
                                                       int *__restrict__ tokens, int *__restrict__ pos_p,
                                                       int *__restrict__ n_prompt_p, float *__restrict__ x,
-                                                      float *__restrict__ logits, VerifyOut *__restrict__ out) {
-    __shared__ int last_s, token_s;
-    if (threadIdx.x == 0) {
-        int cur = 0, n = 0;
-        for (;;) {
-            const int want = next[cur];
-            int child = 0;
-            for (int r = cur + 1; r < rows && !child; ++r)
-                if (in->parents[r] == cur && in->tokens[r] == want) child = r;
-            tokens[pos + n + 1] = want;
-            if (!child) break;
-            out->path[n++] = child;
-            cur = child;
-        }
-        out->accepted = n;
-        out->last = cur;
-        *pos_p = pos + n + 1;
-        *n_prompt_p = pos + n + 1;
-        last_s = cur;
-        token_s = next[cur];
-    }
-    __syncthreads();
-    const _Float16 *row = embed + (size_t)token_s * H;
+                                                      float *__restrict__ logits) {
+    const int n = out->accepted, last = out->last, token = next[last];
+    for (int i = threadIdx.x; i <= n; i += NT) tokens[pos + i + 1] = next[i ? out->path[i - 1] : 0];
+    if (threadIdx.x == 0) *pos_p = *n_prompt_p = pos + n + 1;
+    const _Float16 *row = embed + (size_t)token * H;
     for (int i = threadIdx.x; i < H; i += NT) x[i] = (float)row[i];
-    const float *lr = all + (size_t)last_s * V;
+    const float *lr = all + (size_t)last * V;
     for (int i = threadIdx.x; i < V; i += NT) logits[i] = lr[i];
 }
 
@@ -734,7 +738,8 @@ size_t verify_buffers(const rq_llama *md, char *base, VerifyBuffers &b) {
     return used;
 }
 
-// The pass: rows of the tree through every layer at once, the pick, the walk and the cache rows.
+// The pass: rows of the tree through every layer at once, the pick, the walk and the cache rows,
+// all of them behind the sequence's.
 int verify_pass(rq_llama *md, const VerifyBuffers &b, int rows, hipStream_t s) {
     const rq_llama_config &c = md->cfg;
     const int H = c.hidden, pos = md->host_pos;
@@ -773,8 +778,7 @@ int verify_pass(rq_llama *md, const VerifyBuffers &b, int rows, hipStream_t s) {
         return st;
     hipLaunchKernelGGL(k_argmax_rows, dim3(rows), dim3(AT), 0, s, b.logits, c.vocab, b.next);
     RQ_LAUNCH_CHECK();
-    hipLaunchKernelGGL(k_verify_accept, dim3(1), dim3(NT), 0, s, b.in, rows, pos, b.next, b.logits, c.vocab, md->embed, H,
-                       md->tokens, md->pos, md->n_prompt, md->x, md->logits, b.out);
+    hipLaunchKernelGGL(k_verify_walk, dim3(1), dim3(1), 0, s, b.in, rows, b.next, b.out);
     RQ_LAUNCH_CHECK();
     const int heads = c.n_layers * c.n_kv_heads;  // the layers' caches lie one after another
     hipLaunchKernelGGL(k_verify_compact, dim3((unsigned)cdiv(2 * heads * (c.head_dim / 8), NT)), dim3(NT), 0, s, b.out,
@@ -849,6 +853,7 @@ void release(rq_llama *md) {
     if (md->graph_k) (void)hipGraphDestroy(md->graph_k);
     if (md->owned) (void)hipFree(md->owned);
     if (md->verify) (void)hipFree(md->verify);
+    if (md->pinned) (void)hipHostFree(md->pinned);
     delete md;
 }
 
@@ -1084,6 +1089,12 @@ int rq_llama_decode(rq_llama *md, int32_t n_steps, rq_stream stream) {
     return RQ_OK;
 }
 
+static int g_verify_fail = 0;
+
+// For the tests, no part of the C ABI: rq_llama_verify calls return an error in place of this step of
+// the pass (0: none).
+void rusty_verify_fail_at(int step) { g_verify_fail = step; }
+
 int rq_llama_verify(rq_llama *md, const int32_t *tokens, const int32_t *parents, int32_t n, int32_t *accepted,
                     rq_stream stream) {
     if (!md) return fail(RQ_ERR_INVALID_ARGUMENT, "null runner");
@@ -1092,7 +1103,7 @@ int rq_llama_verify(rq_llama *md, const int32_t *tokens, const int32_t *parents,
     if (n < 0 || n >= kVerifyRows) return fail(RQ_ERR_SHAPE, "%d drafts outside 0..%d", n, kVerifyRows - 1);
     if (md->host_len == 0) return fail(RQ_ERR_INVALID_ARGUMENT, "no sequence: call rq_llama_prefill first");
     const int rows = n + 1;
-    if (rows > md->cfg.max_seq - md->host_pos || rows > md->prefill_cap)
+    if (rows > md->cfg.max_seq - md->host_pos)  // (so the prompt buffers hold the rows, too)
         return fail(RQ_ERR_SHAPE, "%d drafts after position %d exceed max_seq %d", n, md->host_pos, md->cfg.max_seq);
     VerifyHost in{};
     in.mask[0] = 1;
@@ -1113,24 +1124,51 @@ int rq_llama_verify(rq_llama *md, const int32_t *tokens, const int32_t *parents,
     VerifyBuffers b{};
     if (!md->verify) {
         const size_t bytes = verify_buffers(md, nullptr, b);
-        void *p = nullptr;
-        const hipError_t e = hipMalloc(&p, bytes);
+        void *p = nullptr, *h = nullptr;
+        hipError_t e = hipMalloc(&p, bytes);
         if (e != hipSuccess) return fail(RQ_ERR_ALLOC, "hipMalloc(%zu): %s", bytes, hipGetErrorString(e));
+        e = hipHostMalloc(&h, sizeof(VerifyPinned), hipHostMallocDefault);
+        if (e != hipSuccess) {
+            (void)hipFree(p);
+            return fail(RQ_ERR_ALLOC, "hipHostMalloc(%zu): %s", sizeof(VerifyPinned), hipGetErrorString(e));
+        }
         md->verify = p;
+        md->pinned = h;
     }
     verify_buffers(md, static_cast<char *>(md->verify), b);
+    VerifyPinned *host = static_cast<VerifyPinned *>(md->pinned);
+    host->in = in;
     hipStream_t s = pick(md->ctx, stream);
-    RQ_HIP_TRY(hipMemcpyAsync(b.in, &in, sizeof in, hipMemcpyHostToDevice, s));
-    // row 0: the sequence's last token
-    RQ_HIP_TRY(hipMemcpyAsync(b.in->tokens, md->tokens + md->host_pos, 4, hipMemcpyDeviceToDevice, s));
-    const int st = verify_pass(md, b, rows, s);
-    VerifyOut out{};
-    if (st == RQ_OK) RQ_HIP_TRY(hipMemcpyAsync(&out, b.out, sizeof out, hipMemcpyDeviceToHost, s));
-    RQ_HIP_TRY(hipStreamSynchronize(s));  // (also: `in` may go)
+    const rq_llama_config &c = md->cfg;
+    // step i of the pass, or the error that a test asked for in its place
+    auto step = [](int i, auto f) -> int { return i == g_verify_fail ? fail(RQ_ERR_HIP, "step %d of a pass", i) : f(); };
+    int st;
+    (void)((st = step(1, [&]() -> int {
+                RQ_HIP_TRY(hipMemcpyAsync(b.in, &host->in, sizeof in, hipMemcpyHostToDevice, s));
+                return RQ_OK;
+            })) ||
+           (st = step(2, [&]() -> int {  // row 0: the sequence's last token
+                RQ_HIP_TRY(hipMemcpyAsync(b.in->tokens, md->tokens + md->host_pos, 4, hipMemcpyDeviceToDevice, s));
+                return RQ_OK;
+            })) ||
+           (st = step(3, [&]() -> int { return verify_pass(md, b, rows, s); })) ||
+           (st = step(4, [&]() -> int {
+                RQ_HIP_TRY(hipMemcpyAsync(&host->out, b.out, sizeof host->out, hipMemcpyDeviceToHost, s));
+                return RQ_OK;
+            })) ||
+           (st = step(5, [&]() -> int {
+                hipLaunchKernelGGL(k_verify_commit, dim3(1), dim3(NT), 0, s, b.out, md->host_pos, b.next, b.logits,
+                                   c.vocab, md->embed, c.hidden, md->tokens, md->pos, md->n_prompt, md->x, md->logits);
+                RQ_LAUNCH_CHECK();
+                return RQ_OK;
+            })));
+    // (after an error, too: nothing of this pass runs on behind the calls that follow)
+    const hipError_t e = hipStreamSynchronize(s);
     if (st != RQ_OK) return st;
-    md->host_pos += out.accepted + 1;
-    md->host_len += out.accepted + 1;
-    *accepted = out.accepted;
+    if (e != hipSuccess) return fail(RQ_ERR_HIP, "hipStreamSynchronize: %s", hipGetErrorString(e));
+    md->host_pos += host->out.accepted + 1;
+    md->host_len += host->out.accepted + 1;
+    *accepted = host->out.accepted;
     return RQ_OK;
 }
 
