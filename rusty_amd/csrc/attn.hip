@@ -668,8 +668,10 @@ __global__ __launch_bounds__(64 * WR * KG, 2) void k_attn(AttnArgs a) {
 }
 
 // Joins the pieces of rows whose keys were cut: one wave per (token, head).
+// Such a sequence has cached positions, which every row sees: drafted keys alone are one tile.
 template <typename T, int HD, int KT>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
+    static_assert(KT >= kMaxNodes, "a cut sequence has cached positions");
     constexpr int L = HD / 4, G = 64 / L, U = 8;  // pieces added at once, 16 bytes a lane; read ahead of use
     const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (row >= (int64_t)a.tokens * a.n_heads) return;
@@ -684,7 +686,6 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
     float4 v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const float4 *>(po + min(gi + u * G, a.splits - 1) * step);
-    const uint64_t word = a.mask ? a.mask[t] : 0;
     int begin, end;
     const int s = find_seq(a, t, &begin, &end, [](int, int at) { return at; });
     const TreeSeq q(a, begin, end, a.lengths[s]);
@@ -726,11 +727,10 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
 #pragma unroll
         for (int w = 32; w >= L; w >>= 1) o[e] += __shfl_xor(o[e], w);
     if (gi != 0) return;
-    const bool none = q.before == 0 && tree_sees(a, word, i, q.keys) == 0;
     typedef T vec4 __attribute__((ext_vector_type(4)));
     vec4 y;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = (T)(none ? 0.0f : o[e] / l);
+    for (int e = 0; e < 4; ++e) y[e] = (T)(o[e] / l);
     *reinterpret_cast<vec4 *>(static_cast<T *>(a.out) + (int64_t)t * a.out_row + head * HD + at) = y;
 }
 
