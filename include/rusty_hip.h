@@ -381,7 +381,7 @@ typedef struct rq_kv_cache {
     const void *k, *v;
     int64_t seq_stride, head_stride, pos_stride;
     int32_t n_seqs;
-    int32_t capacity;  /* positions per sequence */
+    int32_t capacity;  /* positions per sequence, at most 2^31 - 1025 */
 } rq_kv_cache;
 
 /* Attention of drafted tokens (a tree per sequence) over the cache.  Sequence

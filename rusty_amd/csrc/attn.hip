@@ -40,6 +40,7 @@ namespace rq {
 namespace {
 
 constexpr int kMaxNodes = 64;
+constexpr int kMaxPositions = 0x7fffffff - 1024;  // a sequence's positions rounded up to tiles stay below 2^31
 constexpr int64_t kMaxRow = (int64_t)1 << 21;  // elements of a row stride: a tile's offsets stay below 2^31 bytes
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -897,6 +898,7 @@ int check_tree(const rq_attn *attn, const rq_kv_cache *cache, const void *q, con
     if (!cache) return fail(RQ_ERR_INVALID_ARGUMENT, "null cache");
     if (max_nodes < 1 || max_nodes > kMaxNodes) return fail(RQ_ERR_SHAPE, "max_nodes %d outside 1..%d", max_nodes, kMaxNodes);
     if (cache->n_seqs < 0 || cache->capacity < 0) return fail(RQ_ERR_SHAPE, "negative cache size");
+    if (cache->capacity > kMaxPositions) return fail(RQ_ERR_SHAPE, "capacity %d above %d", cache->capacity, kMaxPositions);
     const int64_t hd = attn->head_dim, unit = attn->dtype == RQ_F16 ? 8 : 4, most = (int64_t)1 << 40;
     a.seq_stride = cache->seq_stride;
     a.head_stride = cache->head_stride;
@@ -967,7 +969,7 @@ int rq_attn_packed(rq_ctx *ctx, const rq_attn *attn, const void *q, const void *
 size_t rq_attn_tree_workspace(const rq_attn *attn, int32_t n_seqs, int64_t tokens, int32_t max_nodes,
                               int32_t capacity) {
     AttnArgs a{};
-    if (n_seqs < 1 || tokens < 1 || max_nodes < 1 || max_nodes > kMaxNodes || capacity < 0 ||
+    if (n_seqs < 1 || tokens < 1 || max_nodes < 1 || max_nodes > kMaxNodes || capacity < 0 || capacity > kMaxPositions ||
         check_attn(attn, tokens, a) != RQ_OK)
         return 0;
     const int splits = tree_shape(n_seqs, a.n_kv, (int64_t)max_nodes * (a.n_heads / a.n_kv), capacity,
