@@ -285,7 +285,9 @@ int rq_qmatmul_lora_ex(rq_ctx *ctx, const rq_qweight *w, const void *x, rq_dtype
  * h: caller workspace of 2*m*I fp16 values; on return its first m*I hold the
  * activated intermediate silu(g)*u (rounded to fp16).  For m <= 16 with fp16
  * activations and per-row int8 weights, gate and up are read in one fused
- * pass with the silu*mul epilogue. */
+ * pass with the silu*mul epilogue.  With a 4-bit gate or up (any m) g and u
+ * are rounded to fp16 before silu(g)*u; past its range silu of a negative gate
+ * is 0 and of a positive one infinite. */
 int rq_mlp_swiglu(rq_ctx *ctx, const rq_qweight *gate, const rq_qweight *up, const rq_qweight *down, const void *x,
                   rq_dtype x_dtype, void *h, void *y, rq_dtype y_dtype, int64_t m, rq_stream stream);
 

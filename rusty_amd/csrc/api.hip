@@ -543,7 +543,9 @@ int rq::swiglu_run(rq_ctx *ctx, const rq_qweight &gate, const rq_qweight &up, co
     if (I == 0) return qmatmul_dispatch(ctx, down, h, RQ_F16, y, y_dtype, m, ws, s);
     if (gate.format == RQ_Q_AFFINE_U4 || up.format == RQ_Q_AFFINE_U4) {
         // 4-bit gate or up: two products into the two halves of the workspace,
-        // then h = silu(g) * u in place over the first half
+        // then h = silu(g) * u in place over the first half.  The workspace holds
+        // g and u in 16 bits: half an fp16 step of each (2^-11 of g, times at most 1.1 of
+        // silu's slope, and 2^-11 of u), next to h's own rounding.
         _Float16 *g = static_cast<_Float16 *>(h), *u = g + m * I;
         int st = qmatmul_dispatch(ctx, gate, x, x_dtype, g, RQ_F16, m, ws, s);
         if (st == RQ_OK) st = qmatmul_dispatch(ctx, up, x, x_dtype, u, RQ_F16, m, ws, s);

@@ -108,11 +108,15 @@ __global__ __launch_bounds__(TH) void k_swiglu_generic(rq_qweight gate, rq_qweig
     }
 }
 
+// silu of a gate that was rounded to fp16: one below fp16's range arrives as -inf, whose -inf / inf is
+// NaN where the gate's own silu is 0.
+__device__ __forceinline__ float silu_of_half(_Float16 v) { return (float)v < -65504.0f ? 0.0f : silu((float)v); }
+
 // h = silu(g) * u elementwise on fp16 (the prefill SwiGLU epilogue).
 __global__ __launch_bounds__(TH) void k_silu_mul(const _Float16 *__restrict__ G, const _Float16 *__restrict__ U,
                                                  _Float16 *__restrict__ H, int64_t n) {
     for (int64_t i = (int64_t)blockIdx.x * TH + threadIdx.x; i < n; i += (int64_t)gridDim.x * TH)
-        H[i] = (_Float16)(silu((float)G[i]) * (float)U[i]);
+        H[i] = (_Float16)(silu_of_half(G[i]) * (float)U[i]);
 }
 
 // The same, 8 values per thread per step (16-byte loads and stores).
@@ -123,7 +127,7 @@ __global__ __launch_bounds__(TH) void k_silu_mul8(const uint4 *__restrict__ G, c
         const half8_t g = __builtin_bit_cast(half8_t, G[i]), u = __builtin_bit_cast(half8_t, U[i]);
         half8_t h;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = (_Float16)(silu((float)g[e]) * (float)u[e]);
+        for (int e = 0; e < 8; ++e) h[e] = (_Float16)(silu_of_half(g[e]) * (float)u[e]);
         H[i] = __builtin_bit_cast(uint4, h);
     }
 }

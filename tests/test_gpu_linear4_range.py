@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 from test_gpu_linear4 import KIND, U, acts, check, parts, run, truth, weight
 
-from rusty_amd import QuantizedTensor
+from rusty_amd import DType, QuantizedTensor, UnifiedTensor
 from rusty_amd.hiprt import Stream
 
 pytestmark = pytest.mark.gpu
@@ -130,3 +130,22 @@ def test_infinities_and_nan(ctx, engine, n, k, group, m, xt):
             if m > 48:  # (the fp16 term of truth() past 16 rows)
                 tol = tol + 2.0 ** -10 * np.abs(x[ok].astype(np.float64)) @ np.abs(W).T
             check(got[ok], ref, tol, f"beside {m}x{n}x{k} {xt}")
+
+
+@pytest.mark.parametrize("m", [1, 2, 6, 16, 40])
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_mlp_of_a_saturated_gate(ctx, engine, m, sign):
+    """A gate past fp16's range: silu of a large negative one is 0, of a large positive one infinite in fp16."""
+    g = np.random.default_rng(m)
+    H, I = 256, 64
+    one = np.ones((I, H // 64), np.float32)
+    gate = (np.full((I, H), 8, np.uint8), sign * 50 * one, None, 64)
+    up = (np.full((I, H), 8, np.uint8), 1e-3 * one, None, 64)
+    down = weight(g, H, I, 64)
+    X = UnifiedTensor.new(ctx, np.ones((m, H)), dtype=DType.FP16)
+    Y = UnifiedTensor.empty(ctx, [m, H], DType.FP32)
+    h = engine.mlp_swiglu(ctx, X, *[QuantizedTensor.affine4(ctx, *w) for w in (gate, up, down)], Y)
+    h = h.to_vec().ravel()[:m * I].astype(np.float64)
+    assert np.all(h == (np.inf if sign > 0 else 0.0))
+    if sign < 0:
+        assert np.all(Y.to_vec() == 0)
