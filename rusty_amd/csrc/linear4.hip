@@ -287,26 +287,27 @@ __global__ __launch_bounds__(TH) void k_linear4_dot(const uint8_t *__restrict__ 
 // one is multiplied.  The waves' sums meet in LDS.
 // Scales and biases go through LDS too, whole rows of them first (they lie one
 // after another), as (s, b - 16 s): read by each lane in place they touch 16 cache
-// lines per load, which bounded the kernel (8 rows, 11008x4096 in groups of 64 21.2 us,
-// 12.6 this way; 4096x11008 in groups of 32 32.3, 16.9; of 5.6 and 6.8 that the bytes need.  What
-// is left is the loads of X, which every block reads whole, about 4 and 8 us).  Rows longer than kSegGroups groups take several rounds.
+// lines per load, which bounded the kernel (this step alone, 8 rows: 11008x4096 in groups of 64 21.2 ->
+// 12.6 us, 4096x11008 in groups of 32 32.3 -> 16.9).  What is left above the bytes' 5.6 and 6.8 us
+// is the loads of X, which every block reads whole, and the expansion of the codes (the table of
+// shapes at launch_mfma has today's times).  Rows longer than kSegGroups groups take several rounds.
 // XF: f32 rows as two fp16 terms.  In a batch where a row's largest magnitude is past fp16's range or
 // below 1 (whose low terms reach fp16's subnormals, an error of 2^-25 whatever the row's size)
-// every row is scaled by a power of two, so that each keeps f32 accuracy.  Looking at the batch first costs
-// 5 % (13 rows 4096x11008 25.7 -> 27.5 us in a graph, 8 rows 11008x4096 19.5 -> 20.3), a scaled one 3 % more; scaling
-// them all 28.3 and 21.9; multiplying first and again where needed spills (37).
+// every row is scaled by a power of two, so that each keeps f32 accuracy.  Looking at the batch first
+// costs up to 7 % (us in a graph, without / with: 8 rows 11008x4096 18.8 / 19.3, 16 rows 27.8 / 28.9, 13 rows
+// 4096x11008 25.7 / 27.5), a scaled batch 3 % more, scaling them all 28.3 for the last; multiplying first
+// and again where needed spills (37).  Two waves per SIMD are asked for where they fit: with 16 rows and
+// one tile the compiler otherwise takes 262 registers and one wave (16 rows 11008x4096 37.4 us, 28.9 with two).
 constexpr int kSegGroups = 512;
 
 // M8: up to 8 rows, where half of the lanes would load nothing: lanes 8-15 of each 16 take the
 // next 32 k of rows 0-7 instead, whole cache lines per load and half the loads, and a
 // rotation by 8 lanes brings those to their place (result rows 8-15 mix both and go unused;
-// 8 rows 11008x4096 13.4 -> 12.7 us, f32 32000x2048 29.1 -> 19.8).
+// this step alone, 8 rows: 11008x4096 13.4 -> 12.7 us, f32 32000x2048 29.1 -> 19.8).
 template <int RT, int NW, int GS, bool XF, bool M8>
-__global__ __launch_bounds__(NW * 64) void k_linear4_mfma(const uint8_t *__restrict__ W,
-                                                          const float *__restrict__ scales,
-                                                          const float *__restrict__ biases,
-                                                          const void *__restrict__ X, void *__restrict__ Y, int y_f16,
-                                                          int m_act, int N, int K, int group) {
+__global__ __launch_bounds__(NW * 64, RT == 1 || M8 ? 2 : 1) void k_linear4_mfma(
+    const uint8_t *__restrict__ W, const float *__restrict__ scales, const float *__restrict__ biases,
+    const void *__restrict__ X, void *__restrict__ Y, int y_f16, int m_act, int N, int K, int group) {
     constexpr int NG = 8 / GS, NT = NW * 64;  // groups of a batch, threads
     __shared__ floatx4 red[NW][RT][64];
     __shared__ __attribute__((aligned(16))) uint8_t wt[NW][RT][16 * 128];
@@ -651,12 +652,14 @@ int launch_mfma(const rq_qweight &w, const void *x, bool xf, void *y, bool yh, i
         else if (w.group % 64 == 0) go(rt, nw, std::integral_constant<int, 2>{}, xfc);
         else go(rt, nw, std::integral_constant<int, 1>{}, xfc);
     };
-    // Waves and row tiles per block, measured (us, 1 tile of 4 waves / 1 of 8 / 2 of 4; f32 rows in
-    // brackets).  8 rows: 2048x2048 5.0 / 5.3 / 5.7 [6.3 / 6.7 / 7.4], 4096x4096 7.1 / 6.3 / 9.1
-    // [9.4 / 9.1 / 12.3], 4096x11008 in groups of 32 17.1 / 12.7 / 26.4 [23.1 / 19.7 / 32.9], 5632x2048
-    // 6.6 / 6.7 / 6.0 [8.8 / 11.9 / 7.8], 11008x4096 12.1 / 13.3 / 12.7 [19.7 / 24.8 / 18.1], 32000x2048
-    // 18.9 / 20.5 / 13.3 [29.4 / 42.8 / 19.7].  16 rows: 4096x4096 8.2 / 7.9 / 10.3 [12.6 / 11.8 / -],
-    // 5632x2048 8.0 / 9.7 / 7.0, 11008x4096 15.9 / 19.2 / 15.4 [27.8 / 32.2 / 28].
+    // Waves and row tiles per block, measured (us in a graph, 1 tile of 4 waves / 1 of 8 / 2 of 4; f32 rows in
+    // brackets).  8 rows: 2048x2048 4.6 / 4.8 / 5.6 [6.3 / 6.1 / 7.4], 4096x4096 7.0 / 7.0 / 8.6
+    // [10.1 / 10.0 / 12.5], 4096x11008 in groups of 32 18.1 / 14.3 / 25.9 [25.8 / 21.8 / 33.3], 5632x2048
+    // 6.2 / 7.0 / 6.0 [9.0 / 11.7 / 8.0], 11008x4096 12.5 / 14.5 / 13.2 [21.0 / 26.8 / 19.2], 32000x2048
+    // 17.3 / 23.2 / 14.2 [30.5 / 44.0 / 21.2].  16 rows: 4096x4096 7.9 / 7.8 / 10.2 [13.2 / 12.5 / 15.4],
+    // 4096x11008 19.3 / 17.6 / 28.6 [30.6 / 28.2 / 39.1], 5632x2048 7.7 / 9.5 / 7.0 [11.7 / 14.6 / 9.7],
+    // 11008x4096 16.3 / 19.6 / 16.1 [28.9 / 34.3 / 29.6], 32000x2048 23.4 / 32.5 / 18.2 [39.8 / 55.2 / 35.3].
+    // (f32 past 8 rows keeps one tile below 1024: right at 688 tiles, 2 us off at 352.)
     using I1 = std::integral_constant<int, 1>;
     using I2 = std::integral_constant<int, 2>;
     using I4 = std::integral_constant<int, 4>;
