@@ -765,7 +765,7 @@ int launch(AttnArgs a, hipStream_t s) {
 // and 83 87 / 59, one of 2048 158 / 166).
 // Blocks are ranked by their work where some have to wait for others and the sequences
 // fit a wave's lanes (9 prompts of 1 to 1047 tokens, 32/4 heads of 64, in the order of the tokens
-// 31.4, ranked 28; in one round of blocks the search only costs, 5 prompts of 1 to 64 4.9 / 5.2).
+// 31.4, ranked 28 when this was chosen, 26 to 27 now; in one round of blocks the search only costs, 5 prompts of 1 to 64 4.9 / 5.2).
 // Every other run of them is turned round in f32 only (one prompt of 2048 158, in order 206; fp16 560 / 545
 // for 8192 tokens).
 template <typename T, int HD>

@@ -142,8 +142,8 @@ __device__ __forceinline__ float by_terms(const uint8_t *W, const float *scales,
 // meet in LDS; a wave then finishes whole (row, token) sums.
 // XF: f32 rows; each chunk of a row is scaled by the power of two that puts its
 // largest magnitude in [2^14, 2^15) and carried as two fp16 terms.
-// One row: 4096x4096 4.8 us (one launch's first bytes and end bound it), 32000x2048 8.9,
-// 4.6 TB/s (HBM).
+// One row: 4096x4096 4.5 us in a graph (one launch's first bytes and end bound it), 32000x2048 9.0,
+// 4.5 TB/s (HBM).
 template <int M, int CPT, int TPR, int R, bool XF>
 __global__ __launch_bounds__(TH) void k_linear4_dot(const uint8_t *__restrict__ W, const float *__restrict__ scales,
                                                     const float *__restrict__ biases, const void *__restrict__ X,
