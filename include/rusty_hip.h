@@ -234,7 +234,8 @@ int rq_matmul_at(rq_ctx *ctx, const float *a, const float *b, float *out, int64_
  * needed), and the infinities and NaN that x w has (an output that is not finite
  * is summed again term by term, so such rows take longer); with more rows, on the context's own stream
  * and with k_in and group multiples of 64, the codes are widened to bytes in the context's
- * workspace and take the GEMM, at its accuracy, where they fit (48 MiB, k_in n_out bytes).
+ * workspace and take the GEMM, at its accuracy (an f32 row with an infinity is
+ * NaN there), where they fit (48 MiB, k_in n_out bytes).
  * On the context's own stream (stream NULL) a GEMM with few tokens splits K over
  * more blocks using the context's workspace, so two such calls of one
  * context must not run concurrently (they cannot on one stream); on any

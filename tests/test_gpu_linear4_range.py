@@ -104,9 +104,7 @@ def test_sums_that_fit_while_their_parts_do_not(ctx, engine, m, big):
 @pytest.mark.parametrize("n,k,group", [(37, 320, 32), (300, 512, 64), (20, 20480, 64), (50, 360, 24)], ids=lambda v: str(v))
 def test_infinities_and_nan(ctx, engine, n, k, group, m, xt):
     """An infinite activation gives the infinity of x w, whatever the other terms; NaN, and infinities of both signs or
-    against a zero weight, give NaN; other rows keep their values."""
-    if m > 48 and group % 64 == 0 and xt == "f32":
-        pytest.skip("the 8-bit GEMM's f32 rows")
+    against a zero weight, give NaN (f32 rows of the 8-bit GEMM all NaN); other rows keep their values."""
     g = np.random.default_rng(n + m)
     u, s, b, _ = w = weight(g, n, k, group)
     s[:, 0], b[:, 0], u[3, 2] = 2.0 ** -6, -2.0 ** -4, 4  # W[3, 2] = 0
@@ -122,8 +120,11 @@ def test_infinities_and_nan(ctx, engine, n, k, group, m, xt):
         want = np.stack([(x[i].astype(np.float64) * W).sum(1) for i in range(m)])
     for stream in (None, Stream()) if m in (3, 60) else (None,):
         got = run(ctx, engine, x, w, xt, "f32", stream).astype(np.float64)
-        assert np.array_equal(np.isnan(got), np.isnan(want))
-        assert np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+        if m > 48 and group % 64 == 0 and xt == "f32" and stream is None:
+            assert np.isnan(got[~np.isfinite(want)]).all()  # the 8-bit GEMM scales f32 rows by their largest value
+        else:
+            assert np.array_equal(np.isnan(got), np.isnan(want))
+            assert np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
         ok = np.isfinite(want).all(1)
         if ok.any():
             ref, tol = truth(x[ok], w, False) if m > 48 else tight(x[ok], w, False)
