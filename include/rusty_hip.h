@@ -279,6 +279,37 @@ int rq_qmatmul_lora_ex(rq_ctx *ctx, const rq_qweight *w, const void *x, rq_dtype
                        const float *lora_b, int64_t rank, void *y, rq_dtype y_dtype, int64_t m, unsigned flags,
                        void *workspace, size_t workspace_bytes, rq_stream stream);
 
+/* Y = X . deq(W)^T with an adapter per row: a batch of tokens of many
+ * requests, each with a fine-tuned adapter of its own beside the shared weight
+ * (the reference has one adapter per Linear, rusty-graph/src/lib.rs:69-83):
+ *   Y[t] = X[t] . deq(W)^T + factors[i] (X[t] . A_i^T) . B_i,  i = ids[t],
+ * nothing added where i is no adapter (outside 0..n_adapters-1).  ids: device
+ * int32[m], in any order; rows of one adapter side by side are fastest.  The
+ * adapter's products are summed in f32 (with fp16 X and adapters, exact
+ * products), the weight's as rq_qmatmul's in f32; Y is rounded once.  Any k_in,
+ * n_out and rank are served; 16-byte loads are taken where k_in (for X and A)
+ * and n_out (for B and Y) are multiples of 8 elements and the pointers 16-byte
+ * aligned.  A row's result does not depend on the other rows' adapters, whatever they
+ * hold.  workspace: rq_qmatmul_loras_workspace(...) bytes, 256-byte aligned, one
+ * per call in flight (a captured call keeps its own); Y overlaps no input.
+ * Uses the context's GEMM workspace as rq_qmatmul does. */
+typedef struct rq_lora_set {
+    const void *a;         /* device [n_adapters][rank][k_in]: the reference's A transposed */
+    const void *b;         /* device [n_adapters][rank][n_out]                   */
+    const float *factors;  /* device [n_adapters] (alpha / rank), NULL: all 1    */
+    const int32_t *ranks;  /* device [n_adapters]: rows of A and B that an adapter
+                            * has (0..rank, clamped; the others are not read), NULL: rank */
+    int32_t n_adapters;
+    int32_t rank;          /* 1..256                                             */
+    int32_t dtype;         /* rq_dtype of a and b                                */
+    int32_t reserved;      /* 0                                                  */
+} rq_lora_set;
+size_t rq_qmatmul_loras_workspace(const rq_lora_set *set, int64_t m, int64_t k_in, int64_t n_out, rq_dtype x_dtype,
+                                  rq_dtype y_dtype);
+int rq_qmatmul_loras(rq_ctx *ctx, const rq_qweight *w, const rq_lora_set *set, const int32_t *ids, const void *x,
+                     rq_dtype x_dtype, void *y, rq_dtype y_dtype, int64_t m, void *workspace, size_t workspace_bytes,
+                     rq_stream stream);
+
 /* MLP::forward (rusty-graph/src/lib.rs:317-323):
  * y = down( silu(x . gate^T) * (x . up^T) ), silu(v) = v / (1 + exp(-v))
  * (kernels.wgsl:104-113; the elementwise product kernels.wgsl:146-151).
@@ -405,6 +436,105 @@ size_t rq_attn_tree_workspace(const rq_attn *attn, int32_t n_seqs, int64_t token
 int rq_attn_tree(rq_ctx *ctx, const rq_attn *attn, const rq_kv_cache *cache, const void *q, const int32_t *starts,
                  const int32_t *lengths, const uint64_t *mask, int64_t tokens, int32_t max_nodes, void *out,
                  void *workspace, size_t workspace_bytes, rq_stream stream);
+
+/* ---- rotary positions -------------------------------------------------------
+ * The first rot_dim elements of a head are turned in pairs (a, b) by the angle
+ * t = position * freqs[i] (radians, i the pair):
+ *   out_a = magnitude (x_a cos t - x_b sin t),  out_b = magnitude (x_b cos t + x_a sin t),
+ * the others are copied.  RQ_ROPE_HALF pairs (i, i + rot_dim / 2) as the
+ * reference does (kernels.wgsl:60-79, there with one position for all tokens), RQ_ROPE_INTERLEAVED (2 i, 2 i + 1).  Angles
+ * are formed in 64 bits, so far positions lose nothing; the rest is f32, rounded once. */
+typedef enum rq_rope_layout { RQ_ROPE_HALF = 0, RQ_ROPE_INTERLEAVED = 1 } rq_rope_layout;
+typedef struct rq_rope {
+    const double *freqs;  /* device [rot_dim / 2]                               */
+    int32_t head_dim;     /* 2..1024                                            */
+    int32_t rot_dim;      /* even, 2..head_dim                                  */
+    int32_t layout;       /* rq_rope_layout                                     */
+    float magnitude;      /* 1 where nothing else is asked for                  */
+} rq_rope;
+
+/* The frequencies theta^(-2i / rot_dim), and how they are scaled for contexts
+ * `factor` times as long as the trained one (of `trained` positions):
+ *  RQ_ROPE_LINEAR : all divided by factor (positions interpolated);
+ *  RQ_ROPE_STRETCH: theta * factor^(rot_dim / (rot_dim - 2)) for theta, so that the
+ *                   slowest pair's is divided by factor and the fastest's kept;
+ *  RQ_ROPE_BANDS  : by the turns n = trained f / 2 pi a pair makes within the
+ *                   trained context: below `low` divided, above `high` kept,
+ *                   linear in n between them;
+ *  RQ_ROPE_RAMP   : likewise, but linear in the pair's index between the pairs
+ *                   (rounded outwards) that make `high` and `low` turns; and the
+ *                   magnitude is 0.1 ln(factor) + 1. */
+typedef enum rq_rope_scaling {
+    RQ_ROPE_PLAIN = 0,
+    RQ_ROPE_LINEAR = 1,
+    RQ_ROPE_STRETCH = 2,
+    RQ_ROPE_BANDS = 3,
+    RQ_ROPE_RAMP = 4
+} rq_rope_scaling;
+typedef struct rq_rope_config {
+    double theta;     /* base, > 1 (10000 in the reference)                     */
+    double factor;    /* >= 1; PLAIN: not used                                  */
+    double trained;   /* BANDS and RAMP: positions, > 0                         */
+    double low, high; /* BANDS and RAMP: 0 < low < high                         */
+    int32_t scaling;  /* rq_rope_scaling                                        */
+    int32_t rot_dim;  /* even, 2..1024                                          */
+} rq_rope_config;
+/* Fills freqs (HOST, rot_dim / 2 values, to be copied to the device once) and
+ * *magnitude.  Host arithmetic; no device is used. */
+int rq_rope_frequencies(const rq_rope_config *config, double *freqs, float *magnitude);
+
+/* x and out: [tokens][n_heads][head_dim] of dtype, the heads of a token side by
+ * side, x_row and out_row elements between tokens (0: packed).  positions:
+ * device int32[tokens], of any sign.  out may be x (with the same row stride;
+ * the elements past rot_dim are then not touched) and overlaps it no other way.
+ * flags: RQ_ROPE_BACKWARD gives the gradient of x from that of out: the turn by -t. */
+#define RQ_ROPE_BACKWARD 1u
+int rq_rope_rows(rq_ctx *ctx, const rq_rope *rope, const void *x, int64_t x_row, const int32_t *positions,
+                 int64_t tokens, int32_t n_heads, rq_dtype dtype, void *out, int64_t out_row, unsigned flags,
+                 rq_stream stream);
+
+/* ---- a paged KV cache --------------------------------------------------------
+ * Position p of sequence s and KV head g at k + page * page_stride +
+ * g * head_stride + (p % page_size) * pos_stride (elements; all three 0:
+ * [n_pages][n_kv_heads][page_size][head_dim]), v alike, with
+ * page = table[s * table_row + p / page_size] (table_row 0: max_pages).  An entry
+ * outside 0..n_pages-1 names no page: its positions hold nothing.  Strides are
+ * multiples of 16 bytes; n_seqs times the capacity (max_pages * page_size) is at most 2^34. */
+typedef struct rq_kv_pages {
+    void *k, *v;
+    const int32_t *table;  /* device                                            */
+    int64_t page_stride, head_stride, pos_stride;
+    int64_t table_row;
+    int32_t n_seqs;
+    int32_t max_pages;     /* per sequence; max_pages * page_size <= 2^31 - 1025 */
+    int32_t n_pages;       /* in the pool                                       */
+    int32_t page_size;     /* positions, a power of two up to 65536             */
+} rq_kv_pages;
+
+/* Rotary positions and the cache's new rows in one pass, between the q/k/v
+ * product and the attention (Attention::forward, rusty-graph/src/lib.rs:205-246,
+ * for one sequence): out = q turned, and each token's k turned and its v copied to
+ * position positions[t] of its sequence.  q, k, v, out: rows of attn's heads
+ * (attn->scale is not used; rope->head_dim is attn->head_dim); out may be q.
+ * starts (device int32[n_seqs + 1], as in rq_attn_packed): sequence s is tokens
+ * starts[s] .. starts[s+1]-1; NULL: token t is all of sequence t.  Tokens of no
+ * sequence are left out whole: their rows of out stay as they were.  A token whose
+ * position is negative, past the capacity or in no page is turned but not cached.
+ * No two tokens of a call have one position. */
+int rq_rope_append(rq_ctx *ctx, const rq_rope *rope, const rq_attn *attn, const rq_kv_pages *cache, const void *q,
+                   const void *k, const void *v, const int32_t *starts, const int32_t *positions, int64_t tokens,
+                   void *out, rq_stream stream);
+
+/* Attention of one new token per sequence over the cache (a decode step of many
+ * sequences): row s of q sees the positions 0 .. lengths[s]-1 of sequence s
+ * (device int32[n_seqs], clamped to 0..capacity; the token's own position is the
+ * last of them, already cached) that lie in a page, and gets zeros if there are none.
+ * Arithmetic as in rq_attn_tree; of attn, k_row and v_row are not used.
+ * workspace: rq_attn_paged_workspace(...) bytes, 16-byte aligned, one per call in
+ * flight (a captured call keeps its own). */
+size_t rq_attn_paged_workspace(const rq_attn *attn, const rq_kv_pages *cache);
+int rq_attn_paged(rq_ctx *ctx, const rq_attn *attn, const rq_kv_pages *cache, const void *q, const int32_t *lengths,
+                  void *out, void *workspace, size_t workspace_bytes, rq_stream stream);
 
 /* ---- int8-weight Llama greedy decode ------------------------------------
  * LlamaModel::forward (rusty-graph/src/lib.rs:420-436) over LlamaBlock

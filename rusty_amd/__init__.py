@@ -5,7 +5,8 @@ ABI of ``include/rusty_hip.h``); this package is its host-side mirror of the
 reference's ``ComputeEngine`` surface.
 """
 from ._lib import RqError, header_symbols, lib  # noqa: F401
-from .engine import ComputeEngine, Context, DType, QuantizedTensor, UnifiedTensor, WgpuContext  # noqa: F401
+from .engine import (ComputeEngine, Context, DType, LoraSet, PagedCache, QuantizedTensor, Rope,  # noqa: F401
+                     UnifiedTensor, WgpuContext)
 
-__all__ = ["ComputeEngine", "Context", "DType", "QuantizedTensor", "RqError", "UnifiedTensor", "WgpuContext",
-           "header_symbols", "lib"]
+__all__ = ["ComputeEngine", "Context", "DType", "LoraSet", "PagedCache", "QuantizedTensor", "Rope", "RqError",
+           "UnifiedTensor", "WgpuContext", "header_symbols", "lib"]

@@ -30,6 +30,14 @@ RQ_Q_AFFINE_U8 = 1
 RQ_Q_AFFINE_U4 = 2
 RQ_AFFINE_FMA = 1
 RQ_LORA_TREE = 1
+RQ_ROPE_HALF = 0
+RQ_ROPE_INTERLEAVED = 1
+RQ_ROPE_PLAIN = 0
+RQ_ROPE_LINEAR = 1
+RQ_ROPE_STRETCH = 2
+RQ_ROPE_BANDS = 3
+RQ_ROPE_RAMP = 4
+RQ_ROPE_BACKWARD = 1
 
 
 class rq_qweight(ctypes.Structure):
@@ -69,6 +77,57 @@ class rq_kv_cache(ctypes.Structure):
         ("pos_stride", c_int64),
         ("n_seqs", c_int32),
         ("capacity", c_int32),
+    ]
+
+
+class rq_kv_pages(ctypes.Structure):
+    _fields_ = [
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("table", c_void_p),
+        ("page_stride", c_int64),
+        ("head_stride", c_int64),
+        ("pos_stride", c_int64),
+        ("table_row", c_int64),
+        ("n_seqs", c_int32),
+        ("max_pages", c_int32),
+        ("n_pages", c_int32),
+        ("page_size", c_int32),
+    ]
+
+
+class rq_rope(ctypes.Structure):
+    _fields_ = [
+        ("freqs", c_void_p),
+        ("head_dim", c_int32),
+        ("rot_dim", c_int32),
+        ("layout", c_int32),
+        ("magnitude", ctypes.c_float),
+    ]
+
+
+class rq_rope_config(ctypes.Structure):
+    _fields_ = [
+        ("theta", ctypes.c_double),
+        ("factor", ctypes.c_double),
+        ("trained", ctypes.c_double),
+        ("low", ctypes.c_double),
+        ("high", ctypes.c_double),
+        ("scaling", c_int32),
+        ("rot_dim", c_int32),
+    ]
+
+
+class rq_lora_set(ctypes.Structure):
+    _fields_ = [
+        ("a", c_void_p),
+        ("b", c_void_p),
+        ("factors", c_void_p),
+        ("ranks", c_void_p),
+        ("n_adapters", c_int32),
+        ("rank", c_int32),
+        ("dtype", c_int32),
+        ("reserved", c_int32),
     ]
 
 
@@ -152,6 +211,14 @@ _SIGNATURES = {
     "rq_attn_tree_workspace": [POINTER(rq_attn), c_int32, c_int64, c_int32, c_int32],
     "rq_attn_tree": [_P, POINTER(rq_attn), POINTER(rq_kv_cache), _P, _P, _P, _P, c_int64, c_int32, _P, _P, c_size_t,
                      _P],
+    "rq_rope_frequencies": [POINTER(rq_rope_config), POINTER(ctypes.c_double), POINTER(ctypes.c_float)],
+    "rq_rope_rows": [_P, POINTER(rq_rope), _P, c_int64, _P, c_int64, c_int32, c_int, _P, c_int64, c_uint32, _P],
+    "rq_rope_append": [_P, POINTER(rq_rope), POINTER(rq_attn), POINTER(rq_kv_pages), _P, _P, _P, _P, _P, c_int64, _P, _P],
+    "rq_attn_paged_workspace": [POINTER(rq_attn), POINTER(rq_kv_pages)],
+    "rq_attn_paged": [_P, POINTER(rq_attn), POINTER(rq_kv_pages), _P, _P, _P, _P, c_size_t, _P],
+    "rq_qmatmul_loras_workspace": [POINTER(rq_lora_set), c_int64, c_int64, c_int64, c_int, c_int],
+    "rq_qmatmul_loras": [_P, POINTER(rq_qweight), POINTER(rq_lora_set), _P, _P, c_int, _P, c_int, c_int64, _P, c_size_t,
+                         _P],
     "rq_llama_create": [_P, POINTER(rq_llama_config), POINTER(rq_llama_weights), POINTER(c_void_p)],
     "rq_llama_destroy": [_P],
     "rq_llama_prefill": [_P, POINTER(c_int32), c_int32, _P],
@@ -172,7 +239,8 @@ _SIGNATURES = {
 _RESTYPES = {"rq_status_string": c_char_p, "rq_last_error": c_char_p, "rq_qmatmul_lora_workspace": c_size_t,
              "rq_qmatmul_lora_ex_workspace": c_size_t, "rq_qweight_prep_bytes": c_size_t,
              "rq_qweight_dx_table_bytes": c_size_t, "rq_qmatmul_dx_mfma_workspace": c_size_t,
-             "rq_attn_tree_workspace": c_size_t}
+             "rq_attn_tree_workspace": c_size_t, "rq_attn_paged_workspace": c_size_t,
+             "rq_qmatmul_loras_workspace": c_size_t}
 
 
 class RqError(RuntimeError):

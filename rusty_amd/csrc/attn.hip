@@ -833,8 +833,9 @@ int launch_tree(const AttnArgs &a, hipStream_t s) {
     return launch<T, HD, 1, F16 ? 4 : 2, true>(a, s);
 }
 
-// The checks both entry points share; fills the strides of a.
-int check_attn(const rq_attn *at, int64_t tokens, AttnArgs &a) {
+}  // namespace
+
+int check_attn_rows(const rq_attn *at, int64_t tokens, AttnRows *r) {
     if (!at) return fail(RQ_ERR_INVALID_ARGUMENT, "null attention descriptor");
     if (at->dtype != RQ_F16 && at->dtype != RQ_F32) return fail(RQ_ERR_INVALID_ARGUMENT, "dtype must be RQ_F16 or RQ_F32");
     if (at->reserved != 0) return fail(RQ_ERR_INVALID_ARGUMENT, "reserved field must be 0");
@@ -852,17 +853,33 @@ int check_attn(const rq_attn *at, int64_t tokens, AttnArgs &a) {
         return fail(RQ_ERR_SHAPE, "row strides must hold a row and be at most 2^21 elements");
     if (qr % unit || orow % unit || kr % unit || vr % unit)
         return fail(RQ_ERR_UNSUPPORTED, "row strides must be multiples of 16 bytes");
-    a.q_row = qr;
-    a.out_row = orow;
-    a.k_row = (int)kr;
-    a.v_row = (int)vr;
+    r->q = qr;
+    r->out = orow;
+    r->k = kr;
+    r->v = vr;
+    const float scale = at->scale != 0.0f ? at->scale : 1.0f / sqrtf((float)at->head_dim);
+    r->neg = scale < 0.0f;
+    // (not below the normal numbers: a hidden key's -inf times c stays -inf)
+    r->c = (float)std::min(std::max(fabs((double)scale) * 1.4426950408889634, 1.2e-38), 3.4e38);
+    return RQ_OK;
+}
+
+namespace {
+
+// The checks both entry points share; fills the strides of a.
+int check_attn(const rq_attn *at, int64_t tokens, AttnArgs &a) {
+    AttnRows r;
+    const int st = check_attn_rows(at, tokens, &r);
+    if (st != RQ_OK) return st;
+    a.q_row = r.q;
+    a.out_row = r.out;
+    a.k_row = (int)r.k;
+    a.v_row = (int)r.v;
     a.n_heads = at->n_heads;
     a.n_kv = at->n_kv_heads;
     a.tokens = (int)tokens;
-    const float scale = at->scale != 0.0f ? at->scale : 1.0f / sqrtf((float)at->head_dim);
-    a.neg = scale < 0.0f;
-    // (not below the normal numbers: a hidden key's -inf times c stays -inf)
-    a.c = (float)std::min(std::max(fabs((double)scale) * 1.4426950408889634, 1.2e-38), 3.4e38);
+    a.neg = r.neg;
+    a.c = r.c;
     a.splits = 1;
     return RQ_OK;
 }

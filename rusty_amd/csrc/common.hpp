@@ -207,6 +207,15 @@ int swiglu_run(rq_ctx *ctx, const rq_qweight &gate, const rq_qweight &up, const 
 // reported by that entry point, not by context creation.
 void noalloc_init(int device);
 
+// The checks of an attention descriptor that every attention entry point shares: row strides in
+// elements, c = |scale| log2 e, and whether q enters negated.
+struct AttnRows {
+    int64_t q, k, v, out;
+    float c;
+    int neg;
+};
+int check_attn_rows(const rq_attn *at, int64_t tokens, AttnRows *r);
+
 enum MatmulVariant { MM_AB = 0, MM_ABT = 1, MM_ATB = 2 };
 
 }  // namespace rq

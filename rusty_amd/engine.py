@@ -14,6 +14,7 @@ reference (rusty-backend)        here
 ``matmul``  lib.rs:4403          :meth:`ComputeEngine.matmul`
 ``matmul_bt``  lib.rs:4299       :meth:`ComputeEngine.matmul_bt`
 ``matmul_at``  lib.rs:4351       :meth:`ComputeEngine.matmul_at`
+``rope`` (kernels.wgsl:60)       :meth:`ComputeEngine.rope`
 (none: weights are f32)          :class:`QuantizedTensor`, :meth:`ComputeEngine.qmatmul`
 ==============================  ==================================================
 
@@ -46,6 +47,7 @@ class DType(enum.Enum):
     U32 = np.uint32
     I32 = np.int32
     U64 = np.uint64
+    FP64 = np.float64
 
     @property
     def np(self):
@@ -57,7 +59,7 @@ class DType(enum.Enum):
 
 
 # Array types that UnifiedTensor.new keeps; numbers of any other become FP32.
-# I32 and U64 buffers (offsets, lengths, masks) are asked for by name.
+# I32, U64 and FP64 buffers (offsets, lengths, masks, frequencies) are asked for by name.
 _INFERRED = {d.value: d for d in (DType.FP32, DType.FP16, DType.I8, DType.U8, DType.U32)}
 
 
@@ -209,6 +211,16 @@ class QuantizedTensor:
                    None, n, k, _lib.RQ_Q_ROWWISE_I8, 0)
 
     @classmethod
+    def from_rowwise(cls, codes: UnifiedTensor, scales: UnifiedTensor) -> "QuantizedTensor":
+        """The same from device tensors: I8 [n_out, k_in] and FP32 [n_out]."""
+        if codes.dtype is not DType.I8 or scales.dtype is not DType.FP32 or len(codes.shape) != 2:
+            raise ValueError("codes must be I8 [n_out, k_in], scales FP32")
+        n, k = codes.shape
+        if scales.numel != n:
+            raise ValueError(f"{n}x{k} weight needs {n} scales")
+        return cls(codes, scales, None, n, k, _lib.RQ_Q_ROWWISE_I8, 0)
+
+    @classmethod
     def affine(cls, ctx: WgpuContext, u: np.ndarray, scales: np.ndarray, biases: np.ndarray | None,
                group: int = 64, prepare: bool = True) -> "QuantizedTensor":
         """The reference's affine format: unsigned codes ``u[n_out, k_in]``,
@@ -228,6 +240,20 @@ class QuantizedTensor:
         if prepare:
             qt.prepare(ctx)
         return qt
+
+    @classmethod
+    def from_affine(cls, codes: UnifiedTensor, scales: UnifiedTensor, biases: UnifiedTensor | None,
+                    group: int = 64) -> "QuantizedTensor":
+        """The same from device tensors: U8 [n_out, k_in], f32 scales and biases of
+        consecutive groups (:meth:`prepare` builds the prefill GEMM's table)."""
+        if codes.dtype is not DType.U8 or len(codes.shape) != 2 or scales.dtype is not DType.FP32 \
+                or (biases is not None and biases.dtype is not DType.FP32):
+            raise ValueError("codes must be U8 [n_out, k_in], scales and biases FP32")
+        n, k = codes.shape
+        need = -(-n * k // group) if group > 0 else 0
+        if group <= 0 or scales.numel < need or (biases is not None and biases.numel < need):
+            raise ValueError(f"{n}x{k} weight with group {group} needs {need} scales/biases")
+        return cls(codes, scales, biases, n, k, _lib.RQ_Q_AFFINE_U8, group)
 
     @classmethod
     def affine4(cls, ctx: WgpuContext, u: np.ndarray, scales: np.ndarray, biases: np.ndarray | None,
@@ -295,6 +321,112 @@ class QuantizedTensor:
         return rq_qweight(self.codes.ptr, self.scales.ptr, self.biases.ptr if self.biases is not None else None,
                           self.n_out, self.k_in, self.format, self.group,
                           self.prep.ptr if self.prep is not None else None)
+
+
+class Rope:
+    """How rotary positions turn a head: the frequencies on the device, and what
+    of the head they turn (rq_rope, rq_rope_config).
+
+    ``layout`` "half" pairs (i, i + rot_dim / 2) as the reference does,
+    "interleaved" (2 i, 2 i + 1).  ``scaling`` for contexts ``factor`` times the
+    ``trained`` one: "none", "linear", "stretch", "bands" or "ramp" (the last two
+    with ``low`` and ``high`` turns within the trained context).  ``frequencies``
+    (radians per position, rot_dim / 2 values) in place of all that."""
+
+    LAYOUTS = {"half": _lib.RQ_ROPE_HALF, "interleaved": _lib.RQ_ROPE_INTERLEAVED}
+    SCALINGS = {"none": _lib.RQ_ROPE_PLAIN, "linear": _lib.RQ_ROPE_LINEAR, "stretch": _lib.RQ_ROPE_STRETCH,
+                "bands": _lib.RQ_ROPE_BANDS, "ramp": _lib.RQ_ROPE_RAMP}
+
+    def __init__(self, ctx: WgpuContext, head_dim: int, rot_dim: int | None = None, layout: str = "half",
+                 theta: float = 10000.0, scaling: str = "none", factor: float = 1.0, trained: float = 0.0,
+                 low: float = 1.0, high: float = 32.0, frequencies=None, magnitude: float | None = None):
+        rot_dim = head_dim if rot_dim is None else rot_dim
+        if layout not in self.LAYOUTS or scaling not in self.SCALINGS:
+            raise ValueError(f"layout {layout!r} / scaling {scaling!r}: expected one of {list(self.LAYOUTS)} / "
+                             f"{list(self.SCALINGS)}")
+        if frequencies is None:
+            frequencies, own = self.frequencies_of(rot_dim, theta, scaling, factor, trained, low, high)
+        else:
+            frequencies, own = np.ascontiguousarray(frequencies, dtype=np.float64), 1.0
+            if frequencies.shape != (rot_dim // 2,):
+                raise ValueError(f"rot_dim {rot_dim} has {rot_dim // 2} frequencies")
+        self.frequencies = UnifiedTensor.new(ctx, frequencies, dtype=DType.FP64)
+        self.head_dim, self.rot_dim = head_dim, rot_dim
+        self.descriptor = _lib.rq_rope(self.frequencies.ptr, head_dim, rot_dim, self.LAYOUTS[layout],
+                                       own if magnitude is None else magnitude)
+
+    @classmethod
+    def frequencies_of(cls, rot_dim: int, theta: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                       trained: float = 0.0, low: float = 1.0, high: float = 32.0) -> tuple[np.ndarray, float]:
+        """(frequencies, magnitude) of rq_rope_frequencies."""
+        c = _lib.rq_rope_config(theta, factor, trained, low, high, cls.SCALINGS[scaling], rot_dim)
+        f = (ctypes.c_double * max(rot_dim // 2, 1))()
+        m = ctypes.c_float()
+        call("rq_rope_frequencies", ctypes.byref(c), f, ctypes.byref(m))
+        return np.array(f[:], dtype=np.float64), m.value
+
+
+class PagedCache:
+    """Keys and values of many sequences in pages (rq_kv_pages): ``k`` and ``v``
+    [n_pages, n_kv_heads, page_size, head_dim] (``order`` "heads") or
+    [n_pages, page_size, n_kv_heads, head_dim] ("positions"), ``table`` I32
+    [n_seqs, max_pages]: the page of each sequence's positions p with p / page_size
+    the column, -1 where there is none.  ``strides``: elements between pages, heads
+    and positions where they are laid out otherwise."""
+
+    def __init__(self, k: UnifiedTensor, v: UnifiedTensor, table: UnifiedTensor, order: str = "heads",
+                 strides: Sequence[int] | None = None):
+        if order not in ("heads", "positions"):
+            raise ValueError(f"order {order!r}: expected 'heads' or 'positions'")
+        if len(k.shape) != 4 or k.shape != v.shape or k.dtype is not v.dtype or len(table.shape) != 2 \
+                or table.dtype is not DType.I32:
+            raise ValueError(f"k {k.shape} / v {v.shape}: expected [n_pages, heads, positions, dim] of one type; table "
+                             f"{table.shape}: expected I32 [n_seqs, max_pages]")
+        self.k, self.v, self.table, self.dtype = k, v, table, k.dtype
+        n_pages, a, b, self.head_dim = k.shape
+        self.n_kv, page = (a, b) if order == "heads" else (b, a)
+        if strides is None:
+            strides = (0, 0, 0) if order == "heads" else (page * self.n_kv * self.head_dim, self.head_dim,
+                                                          self.n_kv * self.head_dim)
+        self.n_seqs, max_pages = table.shape
+        self.descriptor = _lib.rq_kv_pages(k.ptr, v.ptr, table.ptr, *strides, 0, self.n_seqs, max_pages, n_pages, page)
+
+
+class LoraSet:
+    """Adapters of one Linear, for rows that each name one (rq_lora_set): ``a``
+    [n_adapters, rank, k_in] (the reference's A transposed) and ``b`` [n_adapters,
+    rank, n_out], both FP16 or both FP32, ``factors`` FP32 [n_adapters] (alpha / rank; None:
+    1), ``ranks`` I32 [n_adapters] where some have fewer rows than ``rank``."""
+
+    def __init__(self, a: UnifiedTensor, b: UnifiedTensor, factors: UnifiedTensor | None = None,
+                 ranks: UnifiedTensor | None = None):
+        if len(a.shape) != 3 or len(b.shape) != 3 or a.shape[:2] != b.shape[:2] or a.dtype not in _XDT \
+                or b.dtype is not a.dtype:
+            raise ValueError(f"a {a.shape} / b {b.shape}: expected [n_adapters, rank, k_in] and [n_adapters, rank, n_out] "
+                             "of one type")
+        n = a.shape[0]
+        if (factors is not None and (factors.dtype is not DType.FP32 or factors.numel != n)) \
+                or (ranks is not None and (ranks.dtype is not DType.I32 or ranks.numel != n)):
+            raise ValueError("factors FP32 [n_adapters] and ranks I32 [n_adapters] do not match")
+        self.a, self.b, self.factors, self.ranks = a, b, factors, ranks
+        self.descriptor = _lib.rq_lora_set(a.ptr, b.ptr, factors.ptr if factors is not None else None,
+                                           ranks.ptr if ranks is not None else None, n, a.shape[1], _XDT[a.dtype], 0)
+
+    @classmethod
+    def stack(cls, ctx: WgpuContext, adapters, factors=None, dtype: DType = DType.FP16) -> "LoraSet":
+        """From host arrays as the reference holds them: pairs (A [k_in, rank],
+        B [rank, n_out]), whose ranks may differ."""
+        ranks = [a.shape[1] for a, _ in adapters]
+        k, n, rank = adapters[0][0].shape[0], adapters[0][1].shape[1], max(max(ranks), 1)
+        a = np.zeros((len(adapters), rank, k), dtype.np)
+        b = np.zeros((len(adapters), rank, n), dtype.np)
+        for i, (x, y) in enumerate(adapters):
+            if x.shape != (k, ranks[i]) or y.shape != (ranks[i], n):
+                raise ValueError(f"adapter {i}: A {x.shape} / B {y.shape} do not match [{k}, rank] / [rank, {n}]")
+            a[i, :ranks[i]], b[i, :ranks[i]] = x.T, y
+        T = lambda v, d: UnifiedTensor.new(ctx, v, dtype=d)  # noqa: E731
+        return cls(T(a, dtype), T(b, dtype), None if factors is None else T(factors, DType.FP32),
+                   T(ranks, DType.I32) if min(ranks) < rank else None)
 
 
 _XDT = {DType.FP32: _lib.RQ_F32, DType.FP16: _lib.RQ_F16}
@@ -413,6 +545,42 @@ class ComputeEngine:
                  out.ptr, _XDT[out.dtype], m, workspace.ptr, workspace.numel * workspace.dtype.itemsize,
                  _stream(stream))
 
+    def qmatmul_loras(self, ctx: WgpuContext, x: UnifiedTensor, w: QuantizedTensor, adapters: LoraSet,
+                      ids: UnifiedTensor, out: UnifiedTensor, workspace: UnifiedTensor | None = None,
+                      stream=None) -> None:
+        """``out[t] = x[t] . deq(w)^T + factors[i] (x[t] . A_i^T) . B_i`` with i =
+        ``ids[t]`` (I32 [m] on the device; none for i < 0): a batch of tokens of many
+        requests, each with its own adapter (rq_qmatmul_loras).  Without a
+        ``workspace`` the call allocates one; a captured call is given its own,
+        which lives as long as the graph."""
+        m = self._check_loras(x, w, adapters, out)
+        if ids.dtype is not DType.I32 or ids.numel != m:
+            raise ValueError(f"ids must be I32 [{m}]")
+        if workspace is None:
+            workspace = self.qmatmul_loras_workspace(ctx, x, w, adapters, out)
+        d = w.descriptor()
+        call("rq_qmatmul_loras", ctx.handle, ctypes.byref(d), ctypes.byref(adapters.descriptor), ids.ptr, x.ptr,
+             _XDT[x.dtype], out.ptr, _XDT[out.dtype], m, workspace.ptr, workspace.nbytes, _stream(stream))
+
+    def qmatmul_loras_workspace(self, ctx: WgpuContext, x: UnifiedTensor, w: QuantizedTensor, adapters: LoraSet,
+                                out: UnifiedTensor) -> UnifiedTensor:
+        """A workspace for ``qmatmul_loras`` calls of these shapes (one per call in flight)."""
+        m = self._check_loras(x, w, adapters, out)
+        need = int(_lib.lib().rq_qmatmul_loras_workspace(ctypes.byref(adapters.descriptor), m, w.k_in, w.n_out,
+                                                         _XDT[x.dtype], _XDT[out.dtype]))
+        return UnifiedTensor.empty(ctx, [max(need, 1)], DType.U8)
+
+    @staticmethod
+    def _check_loras(x, w, adapters, out) -> int:
+        if x.dtype not in _XDT or out.dtype not in _XDT:
+            raise ValueError("x and out must be FP16 or FP32")
+        m = x.numel // w.k_in if w.k_in else x.shape[0]
+        if x.numel != m * w.k_in or out.numel != m * w.n_out or adapters.a.shape[2] != w.k_in \
+                or adapters.b.shape[2] != w.n_out:
+            raise ValueError(f"x {x.shape} / A {adapters.a.shape} / B {adapters.b.shape} / out {out.shape} do not match "
+                             f"weight [{w.n_out}, {w.k_in}]")
+        return m
+
     def qmatmul_dx(self, ctx: WgpuContext, dy: UnifiedTensor, w: QuantizedTensor, dx: UnifiedTensor,
                    stream=None, mfma: bool = False, workspace: UnifiedTensor | None = None) -> None:
         """Input gradient of ``qmatmul`` with the weight frozen:
@@ -514,6 +682,74 @@ class ComputeEngine:
         """A workspace for ``attn_tree`` calls of these shapes (one per call in flight)."""
         a = _attn(q, k, k, q, k.shape[1], None)
         need = int(_lib.lib().rq_attn_tree_workspace(ctypes.byref(a), k.shape[0], q.shape[0], max_nodes, k.shape[2]))
+        return UnifiedTensor.empty(ctx, [max(need, 1)], DType.U8)
+
+
+    # ---- rotary positions, paged caches ----------------------------------------
+    def rope(self, ctx: WgpuContext, x: UnifiedTensor, rope: Rope, positions: UnifiedTensor,
+             out: UnifiedTensor | None = None, backward: bool = False, x_row: int | None = None,
+             out_row: int | None = None, stream=None) -> None:
+        """``out = x`` [tokens, heads, head_dim] with each head turned by its token's
+        position (kernels.wgsl:60-79, which has one position for all; rq_rope_rows), in
+        place without ``out``.  ``positions`` I32 [tokens].  ``backward``: the gradient of
+        x from that of out.  ``*_row``: elements between the rows of consecutive tokens."""
+        if out is None:
+            out, out_row = x, x_row
+        if len(x.shape) != 3 or out.shape != x.shape or x.shape[2] != rope.head_dim or x.dtype not in _XDT \
+                or out.dtype is not x.dtype:
+            raise ValueError(f"x {x.shape} / out {out.shape}: expected [tokens, heads, {rope.head_dim}], FP16 or FP32")
+        tokens, heads, _ = x.shape
+        if positions.dtype is not DType.I32 or positions.numel != tokens:
+            raise ValueError(f"positions must be I32 [{tokens}]")
+        call("rq_rope_rows", ctx.handle, ctypes.byref(rope.descriptor), x.ptr, x_row or 0, positions.ptr, tokens, heads,
+             _XDT[x.dtype], out.ptr, out_row or 0, _lib.RQ_ROPE_BACKWARD if backward else 0, _stream(stream))
+
+    def rope_append(self, ctx: WgpuContext, q: UnifiedTensor, k: UnifiedTensor, v: UnifiedTensor, rope: Rope,
+                    positions: UnifiedTensor, cache: PagedCache, out: UnifiedTensor, starts: UnifiedTensor | None = None,
+                    q_row: int | None = None, k_row: int | None = None, v_row: int | None = None,
+                    out_row: int | None = None, stream=None) -> None:
+        """``out = q`` turned by position, ``k`` turned and ``v`` copied into the cache's
+        pages (rq_rope_append): q and out [tokens, n_heads, dim], k and v
+        [tokens, n_kv_heads, dim], ``positions`` I32 [tokens], each within its
+        sequence.  ``starts`` I32 [n_seqs + 1]: sequence s is tokens starts[s] ..
+        starts[s+1]-1; without, token t is all of sequence t."""
+        if len(q.shape) != 3 or k.shape != (q.shape[0], cache.n_kv, cache.head_dim) or v.shape != k.shape \
+                or out.shape != q.shape or q.shape[2] != cache.head_dim or cache.dtype is not q.dtype:
+            raise ValueError(f"q {q.shape} / k {k.shape} / v {v.shape} / out {out.shape}: expected [tokens, heads, dim] of "
+                             f"the cache's {cache.n_kv} heads of {cache.head_dim} and its type")
+        tokens = q.shape[0]
+        if positions.dtype is not DType.I32 or positions.numel != tokens or (
+                starts is not None and (starts.dtype is not DType.I32 or starts.numel != cache.n_seqs + 1)):
+            raise ValueError("positions I32 [tokens] and starts I32 [n_seqs + 1] do not match")
+        a = _attn(q, k, v, out, cache.n_kv, None)
+        a.q_row, a.k_row, a.v_row, a.out_row = q_row or 0, k_row or 0, v_row or 0, out_row or 0
+        call("rq_rope_append", ctx.handle, ctypes.byref(rope.descriptor), ctypes.byref(a), ctypes.byref(cache.descriptor),
+             q.ptr, k.ptr, v.ptr, starts.ptr if starts is not None else None, positions.ptr, tokens, out.ptr,
+             _stream(stream))
+
+    def attn_paged(self, ctx: WgpuContext, q: UnifiedTensor, cache: PagedCache, lengths: UnifiedTensor,
+                   out: UnifiedTensor, scale: float | None = None, workspace: UnifiedTensor | None = None,
+                   q_row: int | None = None, out_row: int | None = None, stream=None) -> None:
+        """Attention of one new token per sequence over a paged cache
+        (rq_attn_paged): q and out [n_seqs, n_heads, head_dim], ``lengths`` I32
+        [n_seqs], the token itself included.  Without a ``workspace`` the call
+        allocates one; a captured call is given its own, which lives as long as the
+        graph."""
+        if len(q.shape) != 3 or out.shape != q.shape or q.shape[0] != cache.n_seqs or q.shape[2] != cache.head_dim:
+            raise ValueError(f"q {q.shape} / out {out.shape}: expected [{cache.n_seqs}, heads, {cache.head_dim}]")
+        if lengths.dtype is not DType.I32 or lengths.numel != cache.n_seqs:
+            raise ValueError(f"lengths must be I32 [{cache.n_seqs}]")
+        a = _attn(q, cache.k, cache.v, out, cache.n_kv, scale)
+        a.q_row, a.out_row = q_row or 0, out_row or 0
+        if workspace is None:
+            workspace = self.attn_paged_workspace(ctx, q, cache)
+        call("rq_attn_paged", ctx.handle, ctypes.byref(a), ctypes.byref(cache.descriptor), q.ptr, lengths.ptr, out.ptr,
+             workspace.ptr, workspace.nbytes, _stream(stream))
+
+    def attn_paged_workspace(self, ctx: WgpuContext, q: UnifiedTensor, cache: PagedCache) -> UnifiedTensor:
+        """A workspace for ``attn_paged`` calls of these shapes (one per call in flight)."""
+        a = _attn(q, cache.k, cache.v, q, cache.n_kv, None)
+        need = int(_lib.lib().rq_attn_paged_workspace(ctypes.byref(a), ctypes.byref(cache.descriptor)))
         return UnifiedTensor.empty(ctx, [max(need, 1)], DType.U8)
 
 
