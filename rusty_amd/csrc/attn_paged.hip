@@ -39,10 +39,8 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int NW = 4;         // waves per block
-constexpr int NS = 2;         // units of a wave's ring
 constexpr int64_t kCus = 256;
-constexpr int kMinRun = NW;   // units: one per wave
+constexpr int kCounterStride = 32;  // of the context's arrival counters, a line each
 
 struct PagedArgs {
     const char *q;
@@ -52,10 +50,16 @@ struct PagedArgs {
     Pages pages;
     int n_heads, n_kv, grp, rbs;  // grp: query heads of a key/value head, in rbs blocks of 16
     int runs;                     // blocks that the units are dealt to
-    float *part;                  // sums [2 runs][n_kv][grp][dim], then (m, l) [2 runs][n_kv][grp]
+    float *part;                  // sums [2 runs][n_heads][dim], then (m, l) [2 runs][n_heads]
+    int *counters;                // a cut sequence's arrived pieces, zero between launches; null: k_paged_join joins
     float c;                      // |scale| log2 e
     int neg;                      // scale < 0
 };
+
+constexpr int NW = 8;  // waves per block
+constexpr int TH = 64 * NW;
+// Blocks per CU that the rings (8 or 16 KiB a wave) leave room for.
+constexpr int blocks_per_cu(int hd) { return hd == 64 ? 2 : 1; }
 
 template <typename T, int HD>
 struct PShape {
@@ -64,7 +68,7 @@ struct PShape {
     static constexpr int ROW = HD * (int)sizeof(T), CH = ROW / 16;
     static constexpr int TILE = KT * ROW;             // bytes of K or V of a unit
     static constexpr int RPU = 1024 / ROW, UN = TILE / 1024;  // rows per DMA instruction, instructions
-    static constexpr int RING = NS * 2 * TILE;        // of a wave
+    static constexpr int RING = 2 * TILE;             // of a wave
     static constexpr int PAD = HD + 4;                // floats between rows of the joined sums
     static_assert(16 * PAD * 4 <= RING, "the partial sums reuse the ring");
 };
@@ -83,7 +87,7 @@ __device__ __forceinline__ float join4(float v, F f) {
 // DMA of 16 bytes per lane from 64-bit addresses: LDS[lds_addr + 16 * lane] = *p (see dma16).
 __device__ __forceinline__ void dma16_at(const char *p, uint32_t lds_addr) {
     const uint32_t l = __builtin_amdgcn_readfirstlane(lds_addr);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(l), "v"(p) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" : : "s"(l), "v"(p) : "memory", "m0");
 }
 
 __device__ __forceinline__ int clamped(const PagedArgs &a, int s) { return min(max(a.lengths[s], 0), a.pages.capacity()); }
@@ -93,79 +97,145 @@ __device__ __forceinline__ int units_of(int length) {
 }
 
 __device__ __forceinline__ int scan_add(int v) {  // inclusive, over the wave
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int w = 1; w < 64; w <<= 1) {
-        const int o = __shfl_up(v, w);
-        v += lane >= w ? o : 0;
-    }
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // lanes 1, 2, 4, 8 before in the row of 16
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // the row before, the half before
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
     return v;
 }
 
-// Units of all sequences, and of those before sequence `upto`.
-template <int KT>
-__device__ __forceinline__ int total_units(const PagedArgs &a, int upto, int *before) {
-    const int lane = threadIdx.x & 63;
-    int all = 0, some = 0;
-    for (int s = lane; s < a.pages.n_seqs; s += 64) {
-        const int u = units_of<KT>(clamped(a, s));
-        all += u;
-        some += s < upto ? u : 0;
-    }
-#pragma unroll
-    for (int w = 32; w > 0; w >>= 1) {
-        all += __shfl_xor(all, w);
-        some += __shfl_xor(some, w);
-    }
-    *before = __builtin_amdgcn_readfirstlane(some);
-    return __builtin_amdgcn_readfirstlane(all);
-}
+__device__ __forceinline__ int run_length(const PagedArgs &a, int total) { return max(NW, (total + a.runs - 1) / a.runs); }
 
-// The sequence that unit x (below the total) belongs to, and its first unit.  Whole wave, x uniform.
-template <int KT>
-__device__ __forceinline__ int find_unit(const PagedArgs &a, int x, int *first) {
-    const int lane = threadIdx.x & 63;
-    int lo = 0, n = a.pages.n_seqs, t0 = 0;  // in sequences lo .. lo + n - 1, whose units begin at t0
-    for (;;) {
-        const int m = (n + 63) / 64;  // sequences of a lane
-        int u = 0;
-        for (int j = 0; j < m; ++j) {
-            const int i = lane * m + j;
-            if (i < n) u += units_of<KT>(clamped(a, lo + i));
+// Where a run lies: the units of all sequences, of a run, its own x0 .. x1 - 1, and 64 (`held`) sequences
+// from `base` on, lane l's units begin .. end - 1 and its length; the run's first unit is among them.
+// Whole wave, `run` uniform.  Up to 64 sequences take one trip for the lengths, one more per factor of 64.
+template <typename T, int HD>
+struct Where {
+    static constexpr int KT = PShape<T, HD>::KT;
+    int total, len, x0, x1;
+    int base, held, length, begin, end;
+    bool none;  // the run is past all units
+    __device__ __forceinline__ Where(const PagedArgs &a, int run) {
+        const int lane = threadIdx.x & 63;
+        int lo = 0, n = a.pages.n_seqs, t0 = 0;  // in sequences lo .. lo + n - 1, whose units begin at t0
+        for (bool first = true;; first = false) {
+            const int m = (n + 63) / 64;  // sequences of a lane
+            int u = 0;
+            length = 0;
+            for (int j = 0; j < m; ++j) {
+                const int i = lane * m + j;
+                if (i < n) {
+                    length = clamped(a, lo + i);
+                    u += units_of<KT>(length);
+                }
+            }
+            const int upto = scan_add(u);
+            if (first) {
+                total = __builtin_amdgcn_readlane(upto, 63);
+                len = run_length(a, total);
+                const int64_t x = (int64_t)run * len;
+                none = x >= total;
+                if (none) return;
+                x0 = (int)x;
+                x1 = x0 + min(len, total - x0);
+            }
+            begin = t0 + upto - u;
+            end = t0 + upto;
+            if (m == 1) break;
+            const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(end > x0) | 1ull << 63);
+            t0 = __builtin_amdgcn_readlane(begin, l);
+            lo += l * m;
+            n = min(m, n - l * m);
         }
-        const int upto = scan_add(u);
-        const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(t0 + upto > x) | 1ull << 63);
-        t0 += __builtin_amdgcn_readlane(upto - u, l);
-        lo += l * m;
-        n = min(m, n - l * m);
-        if (m == 1) break;
+        base = lo;
+        held = n;
     }
-    *first = t0;
-    return lo;
+    // The 64 sequences from the one whose units begin at x on, the next after those held.
+    __device__ __forceinline__ void next(const PagedArgs &a, int x) {
+        const int lane = threadIdx.x & 63;
+        base += held;
+        held = min(64, a.pages.n_seqs - base);
+        length = lane < held ? clamped(a, base + lane) : 0;
+        const int u = lane < held ? units_of<KT>(length) : 0;
+        end = x + scan_add(u);
+        begin = end - u;
+    }
+};
+
+// Device-coherent stores and loads (sc1): the blocks of a sequence may sit on different XCDs.
+__device__ __forceinline__ void store_part(__amdgpu_buffer_rsrc_t r, uint32_t at, floatx4 v) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, at, 0, 16);
 }
 
-__device__ __forceinline__ int run_length(const PagedArgs &a, int total) { return max(kMinRun, (total + a.runs - 1) / a.runs); }
+// One row's pieces joined: piece p's (m, l) at ml + stride p / HD * 2, its sums at part + stride p (float
+// indexes of slot 0; piece 0 lies one slot further: a sequence's first piece is a run's last part).
+// Pieces first, first + step, ... < pieces.
+template <int HD>
+struct Joined {
+    float top = -__builtin_inff(), l = 0.0f;
+    floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    __device__ __forceinline__ void add(float m, float wl, floatx4 v) {
+        const float t = fmaxf(top, m), base = t == -__builtin_inff() ? 0.0f : t;
+        const float w0 = __builtin_amdgcn_exp2f(top - base), w1 = __builtin_amdgcn_exp2f(m - base);
+        l = __builtin_fmaf(w1, wl, w0 * l);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(w1, v[e], w0 * o[e]);
+        top = t;
+    }
+    // (head, 4 dims at `at`) of the sequence whose first run is b0
+    __device__ __forceinline__ void read(const PagedArgs &a, __amdgpu_buffer_rsrc_t r, int b0, int pieces, int head, int at,
+                                         int first, int step) {
+        constexpr int U = 8;  // pieces read at once
+        const uint32_t mls = (uint32_t)(2 * a.runs * a.n_heads) * (HD * 4);
+        for (int p0 = first; p0 < pieces; p0 += U * step) {
+            floatx4 v[U];
+            float2 ml[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int p = min(p0 + u * step, pieces - 1), slot = 2 * (b0 + p) + (p == 0 ? 1 : 0);
+                const uint32_t row = (uint32_t)(slot * a.n_heads + head);
+                v[u] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(r, row * (HD * 4) + at * 4, 0, 16));
+                ml[u] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(r, mls + row * 8, 0, 16));
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (p0 + u * step < pieces) add(ml[u].x, ml[u].y, v[u]);
+        }
+    }
+};
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t part_rsrc(const PagedArgs &a, int hd) {
+    return make_rsrc(a.part, (uint32_t)(2 * a.runs * a.n_heads) * (uint32_t)(hd * 4 + 8));
+}
+
+template <typename T>
+__device__ __forceinline__ void write_out(const PagedArgs &a, int s, int64_t at, float top, float l, floatx4 o) {
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+    vec4 y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = (T)(top == -__builtin_inff() ? 0.0f : o[i] / l);
+    *reinterpret_cast<vec4 *>(a.out + s * a.out_row + at * (int)sizeof(T)) = y;
+}
 
 template <typename T, int HD>
-__global__ __launch_bounds__(64 * NW, 1) void k_attn_paged(PagedArgs a) {
+__global__ __launch_bounds__(TH, 2 * blocks_per_cu(HD)) void k_attn_paged(PagedArgs a) {
     using SH = PShape<T, HD>;
     constexpr bool F16 = SH::F16;
     constexpr int KT = SH::KT, ROW = SH::ROW, CH = SH::CH, TILE = SH::TILE, RPU = SH::RPU, UN = SH::UN;
     constexpr int DT = HD / 16, KS = F16 ? HD / 32 : HD / 16;  // 16-dim tiles; 16-byte pieces of a row per lane
     __shared__ __attribute__((aligned(1024))) unsigned char lds[NW * SH::RING];
     __shared__ float joined[2][NW][16];
+    __shared__ int last[2];
 
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, qt = lane >> 4;
     const int per_run = a.n_kv * a.rbs;
     const int run = blockIdx.x / per_run, rest = blockIdx.x - run * per_run, g = rest / a.rbs, rb = rest - g * a.rbs;
-    int dummy;
-    const int total = total_units<KT>(a, 0, &dummy), len = run_length(a, total);
-    const int64_t x0l = (int64_t)run * len;
-    if (x0l >= total) return;
-    const int x0 = (int)x0l, x1 = (int)min(x0l + len, (int64_t)total);
-    int t0, s = __builtin_amdgcn_readfirstlane(find_unit<KT>(a, x0, &t0));
-    t0 = __builtin_amdgcn_readfirstlane(t0);
+    Where<T, HD> where(a, run);
+    if (where.none) return;
+    const int x0 = where.x0, x1 = where.x1, len = where.len;
 
     const int rows = min(16, a.grp - 16 * rb), head0 = g * a.grp + 16 * rb;  // of this block
     const char *kb = a.pages.k + g * a.pages.head_stride, *vb = a.pages.v + g * a.pages.head_stride;
@@ -201,19 +271,41 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_paged(PagedArgs a) {
     typedef __attribute__((address_space(3))) short4v lds_short4;
     typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 
-    while (t0 < x1) {
-        const int length = __builtin_amdgcn_readfirstlane(clamped(a, s)), units = units_of<KT>(length);
-        // this part: units ua .. ub - 1 of the sequence, and of them this wave's
-        const int ua = max(x0 - t0, 0), ub = min(x1 - t0, units);
-        const int per = (ub - ua + NW - 1) / NW;
-        const int w0 = min(ua + wv * per, ub), n = length > 0 ? min(w0 + per, ub) - w0 : 0;
+    // Sequences that other blocks have parts of, too: at most the first and the last of the run.
+    int cuts = 0, cut_s[2] = {0, 0}, cut_begin[2] = {0, 0}, cut_end[2] = {1, 1};
+
+    for (int x = x0; x < x1;) {
+        if (x >= __builtin_amdgcn_readlane(where.end, 63)) where.next(a, x);
+        // This round's parts: lane l's of its sequence, units from .. from + mine - 1 of the flat order, to waves
+        // until - need .. until - 1, per units each; as many parts as find waves, with per up to twice an equal share.
+        const int from = max(where.begin, x), mine = max(min(where.end, x1) - from, 0);
+        int per = (x1 - x + NW - 1) / NW, need = 0, until = 0;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            need = (mine + per - 1) / per;
+            until = scan_add(need);
+            if (t == 1 || __builtin_amdgcn_readlane(until, 63) <= NW) break;
+            per *= 2;
+        }
+        const uint64_t dealt = __builtin_amdgcn_ballot_w64(mine > 0 && until <= NW);  // a run of lanes, not empty
+        const int l0 = __builtin_ctzll(dealt), l1 = 63 - __builtin_clzll(dealt);
+        x = min(__builtin_amdgcn_readlane(where.end, l1), x1);
+        // this wave's (the last waves may have none)
+        const uint64_t past = __builtin_amdgcn_ballot_w64(until > wv) & dealt;
+        const int pl = past ? __builtin_ctzll(past) : l0;
+        const int ms = where.base + pl, length = __builtin_amdgcn_readlane(where.length, pl);
+        const int waves = __builtin_amdgcn_readlane(need, pl), wave0 = __builtin_amdgcn_readlane(until, pl) - waves;
+        const int sb = __builtin_amdgcn_readlane(where.begin, pl), se = __builtin_amdgcn_readlane(where.end, pl);
+        const int pf = __builtin_amdgcn_readlane(from, pl), pm = __builtin_amdgcn_readlane(mine, pl);
+        const int w0 = pf - sb + (wv - wave0) * per;  // its first unit within the sequence
+        const int n = past && length > 0 ? min(per, pm - (wv - wave0) * per) : 0;
 
         // the pages' entries, lane l's of page p0 + l, and the queries: one trip
         int p0 = (w0 * KT) >> a.pages.shift;
-        int entry = a.pages.page(s, p0 + lane);
+        int entry = a.pages.page(ms, p0 + lane);
         u32x4 qf[KS];
         {
-            const char *qp = a.q + s * a.q_row + (int64_t)(head0 + min(col, rows - 1)) * ROW;
+            const char *qp = a.q + ms * a.q_row + (int64_t)(head0 + min(col, rows - 1)) * ROW;
             const uint32_t flip = a.neg ? (F16 ? 0x80008000u : 0x80000000u) : 0u;
 #pragma unroll
             for (int j = 0; j < KS; ++j) {
@@ -224,38 +316,36 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_paged(PagedArgs a) {
         }
         asm volatile("" : "+v"(entry));
 
-        // unit w0 + i into its place; keys that lie in no page read another row's bytes
-        auto dma = [&](int i) {
+        // The offsets of unit w0 + i's rows, and which of its keys are seen, as bits; keys that lie in
+        // no page read another row's bytes.
+        int64_t rowat[UN];
+        uint32_t bits = 0;
+        auto locate = [&](int i) {
             const int key0 = (w0 + i) * KT;
             if (((key0 + KT - 1) >> a.pages.shift) - p0 > 63) {
                 p0 = key0 >> a.pages.shift;
-                entry = a.pages.page(s, p0 + lane);
+                entry = a.pages.page(ms, p0 + lane);
                 asm volatile("" : "+v"(entry));
             }
-            const uint32_t base = lds0 + (uint32_t)(i % NS) * (2 * TILE);
 #pragma unroll
             for (int u = 0; u < UN; ++u) {
                 const int key = key0 + u * RPU + lane / CH;
                 const int e = max(__shfl(entry, (key >> a.pages.shift) - p0), 0);
-                const int64_t at = e * a.pages.page_stride + (int64_t)(key & page_mask) * a.pages.pos_stride;
-                dma16_at(kb + at + koff[u], base + (uint32_t)u * 1024u);
-                dma16_at(vb + at + voff[u], base + (uint32_t)TILE + (uint32_t)u * 1024u);
+                rowat[u] = e * a.pages.page_stride + (int64_t)(key & page_mask) * a.pages.pos_stride;
             }
-        };
-        // which keys of unit w0 + i are seen, as bits (after its dma: the entries are those of its pages)
-        auto seen = [&](int i) -> uint32_t {
-            const int key = (w0 + i) * KT + (lane & (KT - 1));
+            const int key = key0 + (lane & (KT - 1));
             const int e = __shfl(entry, (key >> a.pages.shift) - p0);
-            return (uint32_t)__builtin_amdgcn_ballot_w64(lane < KT && key < length && e >= 0);
+            bits = (uint32_t)__builtin_amdgcn_ballot_w64(lane < KT && key < length && e >= 0);
         };
-        uint32_t sees[NS];
+        auto dma = [&](const char *from, const int *off, uint32_t to) {
 #pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            sees[i] = 0;
-            if (i < n) {
-                dma(i);
-                sees[i] = seen(i);
-            }
+            for (int u = 0; u < UN; ++u) dma16_at(from + rowat[u] + off[u], to + (uint32_t)u * 1024u);
+        };
+        const uint32_t kt = lds0, vt = lds0 + (uint32_t)TILE;
+        if (n > 0) {
+            locate(0);
+            dma(kb, koff, kt);
+            dma(vb, voff, vt);
         }
 
         float mc = -__builtin_inff(), l = 0.0f;  // running maximum (scaled), this lane's share of the sum
@@ -264,25 +354,21 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_paged(PagedArgs a) {
         for (int d = 0; d < DT; ++d) o[d] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
         bool any = false;
 
-        auto unit = [&](uint32_t tb, uint32_t bits) {
+        for (int i = 0; i < per; ++i) {
+            if (i > 0) __builtin_amdgcn_s_barrier();  // (for an even pace: older waves' loads go first)
+            if (i >= n) continue;
             constexpr uint32_t ALL = KT == 32 ? 0xffffffffu : 0xffffu;
             constexpr int NT = KT / 16;
-            any = any || bits != 0;
-            if (bits != ALL) {
-                // V's rows of keys that are not seen: zeros, whatever the bytes were
-#pragma unroll
-                for (int u = 0; u < UN; ++u)
-                    if (!(bits >> (u * RPU + lane / CH) & 1))
-                        *(lds_u32x4 *)(uintptr_t)(tb + TILE + (uint32_t)(u * 1024 + lane * 16)) = u32x4{0, 0, 0, 0};
-                wait_lgkm0();
-            }
+            const uint32_t sees = bits;
+            any = any || sees != 0;
+            wait_vmcnt<UN>();  // K has landed, V may not have
             floatx4 sc[NT];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 sc[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int j = 0; j < KS; ++j) {
-                    const u32x4 kf = *(lds_u32x4 *)(uintptr_t)(tb + ka[j] + (uint32_t)(16 * t * ROW));
+                    const u32x4 kf = *(lds_u32x4 *)(uintptr_t)(kt + ka[j] + (uint32_t)(16 * t * ROW));
                     if constexpr (F16) {
                         sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, kf),
                                                                        __builtin_bit_cast(half8, qf[j]), sc[t], 0, 0, 0);
@@ -293,12 +379,17 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_paged(PagedArgs a) {
                     }
                 }
             }
-            if (bits != ALL) {
+            wait_lgkm0();  // K has been read: the next unit's may take its place
+            if (i + 1 < n) {
+                locate(i + 1);
+                dma(kb, koff, kt);
+            }
+            if (sees != ALL) {
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        sc[t][e] = bits >> (16 * t + 4 * qt + e) & 1 ? sc[t][e] : -__builtin_inff();
+                        sc[t][e] = sees >> (16 * t + 4 * qt + e) & 1 ? sc[t][e] : -__builtin_inff();
             }
             float mt = sc[0][0];
 #pragma unroll
@@ -323,7 +414,16 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_paged(PagedArgs a) {
                     sc[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][e], a.c, off));
                     l += sc[t][e];
                 }
-            const uint32_t vt = tb + TILE;
+            if (i + 1 < n) wait_vmcnt<UN>();
+            else wait_vmcnt<0>();
+            if (sees != ALL) {
+                // V's rows of keys that are not seen: zeros, whatever the bytes were
+#pragma unroll
+                for (int u = 0; u < UN; ++u)
+                    if (!(sees >> (u * RPU + lane / CH) & 1))
+                        *(lds_u32x4 *)(uintptr_t)(vt + (uint32_t)(u * 1024 + lane * 16)) = u32x4{0, 0, 0, 0};
+                wait_lgkm0();
+            }
             if constexpr (F16) {
                 half8 pf;
 #pragma unroll
@@ -349,18 +449,8 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_paged(PagedArgs a) {
                             o[4 * h + i] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], sc[0][e], o[4 * h + i], 0, 0, 0);
                     }
             }
-        };
-        for (int i = 0; i < n; ++i) {
-            if (i + 1 < n) wait_vmcnt<2 * UN>();
-            else wait_vmcnt<0>();
-            const uint32_t bits = sees[0];
-            sees[0] = sees[1];
-            unit(lds0 + (uint32_t)(i % NS) * (2 * TILE), bits);
-            wait_lgkm0();  // (the unit has been read)
-            if (i + NS < n) {
-                dma(i + NS);
-                sees[1] = seen(i + NS);
-            }
+            wait_lgkm0();  // V has been read
+            if (i + 1 < n) dma(vb, voff, vt);
         }
         l = join4(l, [](float x, float y) { return x + y; });
         // -inf as the maximum means no key at all: keys whose scores are all -inf give NaN, as 0 / 0
@@ -368,15 +458,15 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_paged(PagedArgs a) {
 
         // the waves' sums through their rings
         __syncthreads();
-        float *mine = reinterpret_cast<float *>(lds + wv * SH::RING) + col * SH::PAD;
+        float *put = reinterpret_cast<float *>(lds + wv * SH::RING) + col * SH::PAD;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             if constexpr (F16) {
-                *reinterpret_cast<floatx4 *>(mine + 16 * d + 4 * qt) = o[d];
+                *reinterpret_cast<floatx4 *>(put + 16 * d + 4 * qt) = o[d];
             } else {
                 // row r of instruction (h, i): dim 64 h + 4 (4 qt + r) + i
 #pragma unroll
-                for (int r = 0; r < 4; ++r) mine[64 * (d / 4) + 16 * qt + 4 * r + d % 4] = o[d][r];
+                for (int r = 0; r < 4; ++r) put[64 * (d / 4) + 16 * qt + 4 * r + d % 4] = o[d][r];
             }
         }
         if (qt == 0) {
@@ -384,101 +474,134 @@ __global__ __launch_bounds__(64 * NW, 1) void k_attn_paged(PagedArgs a) {
             joined[1][wv][col] = l;
         }
         __syncthreads();
-        const bool cut = t0 < x0 || t0 + units > x1;
-        const int slot = 2 * run + (t0 < x0 ? 0 : 1);
-        for (int e = threadIdx.x; e < rows * (HD / 4); e += 64 * NW) {
+        const auto rp = part_rsrc(a, HD);
+        const bool cut = sb < x0 || se > x1;
+        const int slot = 2 * run + (sb < x0 ? 0 : 1);
+        // the part's waves join it
+        for (int e = past ? (wv - wave0) * 64 + lane : rows * (HD / 4); e < rows * (HD / 4); e += waves * 64) {
             const int row = e / (HD / 4), at = 4 * (e % (HD / 4));
-            float top = joined[0][0][row];
-#pragma unroll
-            for (int w = 1; w < NW; ++w) top = fmaxf(top, joined[0][w][row]);
-            const float base = top == -__builtin_inff() ? 0.0f : top;
-            float sum = 0.0f;
-            floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                const float wt = __builtin_amdgcn_exp2f(joined[0][w][row] - base);
-                const floatx4 x = *reinterpret_cast<const floatx4 *>(reinterpret_cast<const float *>(lds + w * SH::RING) + row * SH::PAD + at);
-                sum = __builtin_fmaf(wt, joined[1][w][row], sum);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(wt, x[i], v[i]);
+            Joined<HD> j;
+            for (int w = wave0; w < wave0 + waves; ++w)
+                j.add(joined[0][w][row], joined[1][w][row],
+                      *reinterpret_cast<const floatx4 *>(reinterpret_cast<const float *>(lds + w * SH::RING) + row * SH::PAD + at));
+            if (!cut) {
+                write_out<T>(a, ms, (int64_t)(head0 + row) * HD + at, j.top, j.l, j.o);
+                continue;
             }
-            if (cut) {
-                const int64_t r = ((int64_t)slot * a.n_kv + g) * a.grp + 16 * rb + row;
-                *reinterpret_cast<floatx4 *>(a.part + r * HD + at) = v;
-                if (at == 0)
-                    reinterpret_cast<float2 *>(a.part + (int64_t)2 * a.runs * a.n_kv * a.grp * HD)[r] = make_float2(top, sum);
-            } else {
-                typedef T vec4 __attribute__((ext_vector_type(4)));
-                vec4 y;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = (T)(top == -__builtin_inff() ? 0.0f : v[i] / sum);
-                *reinterpret_cast<vec4 *>(a.out + s * a.out_row + ((int64_t)(head0 + row) * HD + at) * (int)sizeof(T)) = y;
+            const uint32_t r = (uint32_t)(slot * a.n_heads + head0 + row);
+            store_part(rp, r * (HD * 4) + at * 4, j.o);
+            if (at == 0) {
+                typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+                __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, make_float2(j.top, j.l)), rp,
+                                                      (uint32_t)(2 * a.runs * a.n_heads) * (HD * 4) + r * 8, 0, 16);
             }
         }
-        __syncthreads();  // the ring is free again
-        t0 += units;
-        ++s;
+        // its cut sequences: one that began before the run, one that goes on behind it
+        const int fb = __builtin_amdgcn_readlane(where.begin, l0), fe = __builtin_amdgcn_readlane(where.end, l0);
+        const int lb = __builtin_amdgcn_readlane(where.begin, l1), le = __builtin_amdgcn_readlane(where.end, l1);
+        if (fb < x0) {
+            cut_s[0] = where.base + l0;
+            cut_begin[0] = fb;
+            cut_end[0] = fe;
+            cuts = 1;
+        }
+        if (le > x1 && lb >= x0) {
+            cut_s[cuts] = where.base + l1;
+            cut_begin[cuts] = lb;
+            cut_end[cuts] = le;
+            ++cuts;
+        }
+        __syncthreads();  // the rings are free again
+    }
+    if (!cuts || !a.counters) return;
+
+    // The block that arrives last joins a sequence's pieces, in their order.  Stores and loads are
+    // device-coherent (sc1), a store's acknowledgement says that it is visible, and the barrier that all of
+    // the block's are, before the relaxed atomic counts them; the loads follow its result.  No block waits for another.
+    auto first_run = [&](int i) { return cut_begin[i] / len; };
+    auto pieces_of = [&](int i) { return (cut_end[i] - 1) / len - first_run(i) + 1; };
+    auto counter = [&](int i) { return a.counters + ((int64_t)first_run(i) * per_run + rest) * kCounterStride; };
+    wait_vmcnt<0>();
+    __syncthreads();
+    if ((int)threadIdx.x < cuts) {
+        const int i = threadIdx.x;
+        last[i] = __hip_atomic_fetch_add(i ? counter(1) : counter(0), 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                  (i ? pieces_of(1) : pieces_of(0)) - 1;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (i >= cuts || !last[i]) continue;
+        if (threadIdx.x == 0) __hip_atomic_store(counter(i), 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const auto rp = part_rsrc(a, HD);
+        const int E = rows * (HD / 4), groups = max(1, TH / E);  // threads of all dims, pieces side by side
+        for (int e0 = 0; e0 < E; e0 += TH) {
+            const int gi = groups > 1 ? (int)threadIdx.x / E : 0;
+            const int e = groups > 1 ? (int)threadIdx.x - gi * E : e0 + (int)threadIdx.x;
+            const bool in = gi < groups && e < E;
+            const int row = e / (HD / 4), at = 4 * (e % (HD / 4));
+            Joined<HD> j;
+            if (in) j.read(a, rp, first_run(i), pieces_of(i), head0 + row, at, gi, groups);
+            if (groups > 1) {
+                float *x = reinterpret_cast<float *>(lds) + threadIdx.x * 8;
+                __syncthreads();
+                *reinterpret_cast<floatx4 *>(x) = j.o;
+                x[4] = j.top;
+                x[5] = j.l;
+                __syncthreads();
+                if (in && gi == 0)
+                    for (int k = 1; k < groups; ++k) {
+                        const float *y = reinterpret_cast<const float *>(lds) + (k * E + e) * 8;
+                        j.add(y[4], y[5], *reinterpret_cast<const floatx4 *>(y));
+                    }
+            }
+            if (in && gi == 0) write_out<T>(a, cut_s[i], (int64_t)(head0 + row) * HD + at, j.top, j.l, j.o);
+        }
     }
 }
 
-// Joins the pieces of sequences that more than one block had: one wave per (sequence, head).
+// The same in a launch of its own, where the context's counters may not be used: one wave per (sequence, head).
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a) {
     constexpr int KT = PShape<T, HD>::KT, L = HD / 4, G = 64 / L;  // lanes of a piece, pieces side by side
     const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (row >= (int64_t)a.pages.n_seqs * a.n_heads) return;
     const int s = (int)(row / a.n_heads), head = (int)(row - (int64_t)s * a.n_heads), lane = threadIdx.x & 63;
-    int t0;
-    const int total = total_units<KT>(a, s, &t0), len = run_length(a, total);
-    const int t1 = t0 + units_of<KT>(clamped(a, s));
+    int all = 0, before = 0;
+    for (int i = lane; i < a.pages.n_seqs; i += 64) {
+        const int u = units_of<KT>(clamped(a, i));
+        all += u;
+        before += i < s ? u : 0;
+    }
+    const int total = __builtin_amdgcn_readlane(scan_add(all), 63), t0 = __builtin_amdgcn_readlane(scan_add(before), 63);
+    const int len = run_length(a, total), t1 = t0 + units_of<KT>(clamped(a, s));
     const int b0 = t0 / len, pieces = (t1 - 1) / len - b0 + 1;
     if (pieces <= 1) return;  // written by the block that had them all
     const int gi = lane / L, at = 4 * (lane % L);
-    // piece p's row: the part that a run begins with, but for the first, unless the run begins with the sequence
-    auto place = [&](int p) { return (int64_t)(2 * (b0 + p) + (p == 0 ? 1 : 0)) * a.n_heads + head; };
-    const float2 *ml = reinterpret_cast<const float2 *>(a.part + (int64_t)2 * a.runs * a.n_heads * HD);
-    float top = -__builtin_inff();
-    for (int p = lane; p < pieces; p += 64) top = fmaxf(top, ml[place(p)].x);
-#pragma unroll
-    for (int w = 32; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor(top, w));
-    const float base = top == -__builtin_inff() ? 0.0f : top;
-    float l = 0.0f;
-    floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int p = gi; p < pieces; p += G) {
-        const float2 m = ml[place(p)];
-        const floatx4 v = *reinterpret_cast<const floatx4 *>(a.part + place(p) * HD + at);
-        const float w = __builtin_amdgcn_exp2f(m.x - base);
-        l = __builtin_fmaf(w, m.y, l);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(w, v[e], o[e]);
-    }
+    Joined<HD> j;
+    j.read(a, part_rsrc(a, HD), b0, pieces, head, at, gi, G);
 #pragma unroll
     for (int w = 32; w >= L; w >>= 1) {
-        l += __shfl_xor(l, w);
+        floatx4 o;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], w);
+        for (int e = 0; e < 4; ++e) o[e] = __shfl_xor(j.o[e], w);
+        j.add(__shfl_xor(j.top, w), __shfl_xor(j.l, w), o);
     }
-    if (gi != 0) return;
-    typedef T vec4 __attribute__((ext_vector_type(4)));
-    vec4 y;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = (T)(top == -__builtin_inff() ? 0.0f : o[e] / l);
-    *reinterpret_cast<vec4 *>(a.out + s * a.out_row + ((int64_t)head * HD + at) * (int)sizeof(T)) = y;
+    if (gi == 0) write_out<T>(a, s, (int64_t)head * HD + at, j.top, j.l, j.o);
 }
 
 // Blocks that the units are dealt to, per key/value head and 16 rows: as many as the device holds at once.
 int paged_runs(int n_heads, int n_kv, int head_dim) {
-    const int64_t rbs = cdiv(n_heads / n_kv, 16), blocks = kCus * (head_dim == 64 ? 2 : 1);
-    return (int)std::max<int64_t>(1, blocks / (n_kv * rbs));
+    return (int)std::max<int64_t>(1, blocks_per_cu(head_dim) * kCus / (n_kv * cdiv(n_heads / n_kv, 16)));
 }
 
 template <typename T, int HD>
 int launch(PagedArgs a, hipStream_t s) {
     const int64_t blocks = (int64_t)a.runs * a.n_kv * a.rbs, rows = cdiv((int64_t)a.pages.n_seqs * a.n_heads, 4);
-    if (!grid_ok(blocks, 64 * NW) || !grid_ok(rows, 256)) return fail(RQ_ERR_SHAPE, "too many rows for one call");
-    hipLaunchKernelGGL((k_attn_paged<T, HD>), dim3((unsigned)blocks), dim3(64 * NW), 0, s, a);
+    if (!grid_ok(blocks, TH) || !grid_ok(rows, 256)) return fail(RQ_ERR_SHAPE, "too many rows for one call");
+    hipLaunchKernelGGL((k_attn_paged<T, HD>), dim3((unsigned)blocks), dim3(TH), 0, s, a);
     RQ_LAUNCH_CHECK();
-    if (a.runs > 1) {
+    if (a.runs > 1 && !a.counters) {
         hipLaunchKernelGGL((k_paged_join<T, HD>), dim3((unsigned)rows), dim3(256), 0, s, a);
         RQ_LAUNCH_CHECK();
     }
@@ -594,6 +717,8 @@ int rq_attn_paged(rq_ctx *ctx, const rq_attn *attn, const rq_kv_pages *cache, co
     const int st = check_paged(attn, cache, q, lengths, out, workspace, workspace_bytes, a, run);
     if (st != RQ_OK || !run) return st;
     hipStream_t s = pick(ctx, stream);
+    const GemmWorkspace ws = gemm_workspace(ctx, s);
+    if (ws.counters && a.runs * a.n_kv * a.rbs <= ws.n_counters) a.counters = ws.counters;
     if (attn->dtype == RQ_F16) return attn->head_dim == 64 ? launch<_Float16, 64>(a, s) : launch<_Float16, 128>(a, s);
     return attn->head_dim == 64 ? launch<float, 64>(a, s) : launch<float, 128>(a, s);
 }

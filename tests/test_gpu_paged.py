@@ -273,3 +273,23 @@ def test_refusals(ctx, engine):
                 lambda: engine.attn_paged(ctx, dev(ctx, q[:1]), cache, L, dev(ctx, q[:1]))):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("heads,kv,dim,lengths,page", [(8, 2, 64, [9000, 5, 130, 700], 64), (16, 1, 128, [3000, 2000], 16),
+                                                       (40, 2, 64, [2500], 8), (6, 6, 128, [900, 800, 0, 700], 32)])
+def test_on_a_callers_stream(ctx, engine, dtype, heads, kv, dim, lengths, page):
+    """Cut sequences on another stream than the context's, where their pieces are joined by a launch of its own."""
+    stream = Stream()
+    q, pools, table, rows = make(13, lengths, heads, kv, dim, page, "heads", dtype)
+    want, tol = truth(q, rows, 1 / np.sqrt(dim), dtype == "f16")
+    kind = KIND[dtype][1]
+    cache = PagedCache(dev(ctx, pools[0], kind), dev(ctx, pools[1], kind), dev(ctx, table, DType.I32))
+    Q, out, L = dev(ctx, q, kind), dev(ctx, np.full(q.shape, 7.0), kind), dev(ctx, np.array(lengths, np.int32), DType.I32)
+    work = engine.attn_paged_workspace(ctx, Q, cache)
+    call("rq_memset", ctx.handle, work.ptr, 0xFF, work.nbytes, None)
+    ctx.sync()
+    for _ in range(2):
+        engine.attn_paged(ctx, Q, cache, L, out, workspace=work, stream=stream.h)
+        stream.synchronize()
+        check(out.to_vec(), want, tol, f"caller's stream {lengths} {dtype}")
