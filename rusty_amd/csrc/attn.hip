@@ -61,18 +61,6 @@ __device__ __forceinline__ float add_halves(float v) {
     return __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y);
 }
 
-// x / d for 0 <= x < 2^31 by one product: m = ceil(2^(31 + b) / d) with 2^b >= d is off by
-// less than 2^b / 2^(31 + b) of 1 / d, so x m / 2^(31 + b) never reaches the next whole number.
-struct Div {
-    uint32_t m, sh;
-    __host__ static Div by(int64_t d) {
-        uint32_t b = 0;
-        while (((int64_t)1 << b) < d) ++b;
-        return {(uint32_t)((((uint64_t)1 << (31 + b)) + (uint64_t)d - 1) / (uint64_t)d), 31 + b};
-    }
-    __device__ __forceinline__ int operator()(int x) const { return (int)(((uint64_t)(uint32_t)x * m) >> sh); }
-};
-
 // Sum and maximum over the wave's 64 lanes of values >= 0.
 template <typename F>
 __device__ __forceinline__ int wave_join(int v, F f) {

@@ -54,6 +54,7 @@ struct PagedArgs {
     int *counters;                // a cut sequence's arrived pieces, zero between launches; null: k_paged_join joins
     float c;                      // |scale| log2 e
     int neg;                      // scale < 0
+    Div by_runs;
 };
 
 constexpr int NW = 8;  // waves per block
@@ -69,6 +70,7 @@ struct PShape {
     static constexpr int TILE = KT * ROW;             // bytes of K or V of a unit
     static constexpr int RPU = 1024 / ROW, UN = TILE / 1024;  // rows per DMA instruction, instructions
     static constexpr int RING = 2 * TILE;             // of a wave
+    static constexpr int L = HD / 4;                  // lanes of a row of sums
     static constexpr int PAD = HD + 4;                // floats between rows of the joined sums
     static_assert(16 * PAD * 4 <= RING, "the partial sums reuse the ring");
 };
@@ -84,10 +86,18 @@ __device__ __forceinline__ float join4(float v, F f) {
     return f(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
 }
 
-// DMA of 16 bytes per lane from 64-bit addresses: LDS[lds_addr + 16 * lane] = *p (see dma16).
+// DMA of 16 bytes per lane (see dma16), not to be kept: every key is read once.  LDS[lds_addr + 16 * lane] = *p
+// of each lane's own address, or base[voff] with a uniform base.
 __device__ __forceinline__ void dma16_at(const char *p, uint32_t lds_addr) {
     const uint32_t l = __builtin_amdgcn_readfirstlane(lds_addr);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" : : "s"(l), "v"(p) : "memory", "m0");
+}
+__device__ __forceinline__ void dma16_from(uint64_t base, uint32_t voff, uint32_t lds_addr) {
+    const uint32_t l = __builtin_amdgcn_readfirstlane(lds_addr);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+                 :
+                 : "s"(l), "v"(voff), "s"(base)
+                 : "memory", "m0");
 }
 
 __device__ __forceinline__ int clamped(const PagedArgs &a, int s) { return min(max(a.lengths[s], 0), a.pages.capacity()); }
@@ -106,7 +116,7 @@ __device__ __forceinline__ int scan_add(int v) {  // inclusive, over the wave
     return v;
 }
 
-__device__ __forceinline__ int run_length(const PagedArgs &a, int total) { return max(NW, (total + a.runs - 1) / a.runs); }
+__device__ __forceinline__ int run_length(const PagedArgs &a, int total) { return max(NW, a.by_runs(total + a.runs - 1)); }
 
 // Where a run lies: the units of all sequences, of a run, its own x0 .. x1 - 1, and 64 (`held`) sequences
 // from `base` on, lane l's units begin .. end - 1 and its length; the run's first unit is among them.
@@ -169,29 +179,37 @@ __device__ __forceinline__ void store_part(__amdgpu_buffer_rsrc_t r, uint32_t at
     __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, at, 0, 16);
 }
 
-// One row's pieces joined: piece p's (m, l) at ml + stride p / HD * 2, its sums at part + stride p (float
-// indexes of slot 0; piece 0 lies one slot further: a sequence's first piece is a run's last part).
-// Pieces first, first + step, ... < pieces.
-template <int HD>
+// Pieces of one row joined: their maximum, sum, and 4 dims of their sums.
 struct Joined {
     float top = -__builtin_inff(), l = 0.0f;
     floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    __device__ __forceinline__ void add(float m, float wl, floatx4 v) {
-        const float t = fmaxf(top, m), base = t == -__builtin_inff() ? 0.0f : t;
-        const float w0 = __builtin_amdgcn_exp2f(top - base), w1 = __builtin_amdgcn_exp2f(m - base);
-        l = __builtin_fmaf(w1, wl, w0 * l);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(w1, v[e], w0 * o[e]);
+    // The maximum rises to t: returns what new pieces' maxima are taken relative to.
+    __device__ __forceinline__ float rise(float t) {
+        t = fmaxf(top, t);
+        const float base = t == -__builtin_inff() ? 0.0f : t, w = __builtin_amdgcn_exp2f(top - base);
         top = t;
+        l *= w;
+        o *= w;
+        return base;
     }
-    // (head, 4 dims at `at`) of the sequence whose first run is b0
+    __device__ __forceinline__ void add(float m, float wl, floatx4 v, float base) {
+        const float w = __builtin_amdgcn_exp2f(m - base);
+        l = __builtin_fmaf(w, wl, l);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(w, v[e], o[e]);
+    }
+    // Pieces first, first + step, ... < pieces of a sequence whose first run is b0 (that run's last part: slot
+    // 2 b0 + 1; then the first part of each), head `head`, dims `at` ..; HD of them in a row.
+    template <int HD>
     __device__ __forceinline__ void read(const PagedArgs &a, __amdgpu_buffer_rsrc_t r, int b0, int pieces, int head, int at,
                                          int first, int step) {
-        constexpr int U = 8;  // pieces read at once
+        constexpr int U = 4;  // pieces read at once
         const uint32_t mls = (uint32_t)(2 * a.runs * a.n_heads) * (HD * 4);
+#pragma unroll 1
         for (int p0 = first; p0 < pieces; p0 += U * step) {
             floatx4 v[U];
             float2 ml[U];
+            float t = -__builtin_inff();
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int p = min(p0 + u * step, pieces - 1), slot = 2 * (b0 + p) + (p == 0 ? 1 : 0);
@@ -200,8 +218,11 @@ struct Joined {
                 ml[u] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(r, mls + row * 8, 0, 16));
             }
 #pragma unroll
+            for (int u = 0; u < U; ++u) t = fmaxf(t, ml[u].x);  // (one read twice does not tell)
+            const float base = rise(t);
+#pragma unroll
             for (int u = 0; u < U; ++u)
-                if (p0 + u * step < pieces) add(ml[u].x, ml[u].y, v[u]);
+                if (p0 + u * step < pieces) add(ml[u].x, ml[u].y, v[u], base);
         }
     }
 };
@@ -219,11 +240,12 @@ __device__ __forceinline__ void write_out(const PagedArgs &a, int s, int64_t at,
     *reinterpret_cast<vec4 *>(a.out + s * a.out_row + at * (int)sizeof(T)) = y;
 }
 
-template <typename T, int HD>
+// Block (key/value head, 16 of its query heads, run).  WIDE: the rows of a DMA instruction lie in one page.
+template <typename T, int HD, bool WIDE>
 __global__ __launch_bounds__(TH, 2 * blocks_per_cu(HD)) void k_attn_paged(PagedArgs a) {
     using SH = PShape<T, HD>;
     constexpr bool F16 = SH::F16;
-    constexpr int KT = SH::KT, ROW = SH::ROW, CH = SH::CH, TILE = SH::TILE, RPU = SH::RPU, UN = SH::UN;
+    constexpr int KT = SH::KT, ROW = SH::ROW, CH = SH::CH, TILE = SH::TILE, RPU = SH::RPU, UN = SH::UN, L = SH::L;
     constexpr int DT = HD / 16, KS = F16 ? HD / 32 : HD / 16;  // 16-dim tiles; 16-byte pieces of a row per lane
     __shared__ __attribute__((aligned(1024))) unsigned char lds[NW * SH::RING];
     __shared__ float joined[2][NW][16];
@@ -231,8 +253,7 @@ __global__ __launch_bounds__(TH, 2 * blocks_per_cu(HD)) void k_attn_paged(PagedA
 
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, qt = lane >> 4;
-    const int per_run = a.n_kv * a.rbs;
-    const int run = blockIdx.x / per_run, rest = blockIdx.x - run * per_run, g = rest / a.rbs, rb = rest - g * a.rbs;
+    const int g = blockIdx.x, rb = blockIdx.y, run = blockIdx.z;
     Where<T, HD> where(a, run);
     if (where.none) return;
     const int x0 = where.x0, x1 = where.x1, len = where.len;
@@ -247,12 +268,14 @@ __global__ __launch_bounds__(TH, 2 * blocks_per_cu(HD)) void k_attn_paged(PagedA
         if (!F16) return 0;
         return HD == 64 ? (((r >> 1) & 1) << 2) ^ (((r >> 2) & 1) << 1) : ((r & 3) << 2) ^ (((r >> 2) & 1) << 1);
     };
-    int koff[UN], voff[UN];  // this lane's 16 bytes within its row of each DMA instruction
+    // this lane's 16 bytes within its row of each DMA instruction (WIDE: within its rows)
+    uint32_t koff[UN], voff[UN];
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
         const int row = u * RPU + lane / CH, c = lane % CH;
-        koff[u] = (c ^ fk(row)) * 16;
-        voff[u] = (c ^ fv(row)) * 16;
+        const uint32_t at = WIDE ? (uint32_t)(lane / CH) * (uint32_t)a.pages.pos_stride : 0u;
+        koff[u] = at + (uint32_t)((c ^ fk(row)) * 16);
+        voff[u] = at + (uint32_t)((c ^ fv(row)) * 16);
     }
     const uint32_t lds0 = lds_addr(&lds[0]) + (uint32_t)(wv * SH::RING);
     uint32_t ka[KS];
@@ -282,7 +305,9 @@ __global__ __launch_bounds__(TH, 2 * blocks_per_cu(HD)) void k_attn_paged(PagedA
         int per = (x1 - x + NW - 1) / NW, need = 0, until = 0;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            need = (mine + per - 1) / per;
+            need = 0;  // mine / per rounded up, as far as it tells
+#pragma unroll
+            for (int k = 0; k <= NW; ++k) need += (uint32_t)mine > (uint32_t)k * (uint32_t)per ? 1 : 0;
             until = scan_add(need);
             if (t == 1 || __builtin_amdgcn_readlane(until, 63) <= NW) break;
             per *= 2;
@@ -320,26 +345,38 @@ __global__ __launch_bounds__(TH, 2 * blocks_per_cu(HD)) void k_attn_paged(PagedA
         // no page read another row's bytes.
         int64_t rowat[UN];
         uint32_t bits = 0;
+        int64_t pageat = (int64_t)max(entry, 0) * a.pages.page_stride;
         auto locate = [&](int i) {
             const int key0 = (w0 + i) * KT;
             if (((key0 + KT - 1) >> a.pages.shift) - p0 > 63) {
                 p0 = key0 >> a.pages.shift;
                 entry = a.pages.page(ms, p0 + lane);
                 asm volatile("" : "+v"(entry));
+                pageat = (int64_t)max(entry, 0) * a.pages.page_stride;
             }
 #pragma unroll
             for (int u = 0; u < UN; ++u) {
-                const int key = key0 + u * RPU + lane / CH;
-                const int e = max(__shfl(entry, (key >> a.pages.shift) - p0), 0);
-                rowat[u] = e * a.pages.page_stride + (int64_t)(key & page_mask) * a.pages.pos_stride;
+                if constexpr (WIDE) {
+                    const int key = key0 + u * RPU, p = (key >> a.pages.shift) - p0;
+                    const uint64_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)pageat, p);
+                    const uint64_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(pageat >> 32), p);
+                    rowat[u] = (int64_t)((hi << 32 | lo) + (uint64_t)((uint32_t)(key & page_mask) * (uint32_t)a.pages.pos_stride));
+                } else {
+                    const int key = key0 + u * RPU + lane / CH;
+                    const int e = max(__shfl(entry, (key >> a.pages.shift) - p0), 0);
+                    rowat[u] = e * a.pages.page_stride + (int64_t)(key & page_mask) * a.pages.pos_stride;
+                }
             }
             const int key = key0 + (lane & (KT - 1));
             const int e = __shfl(entry, (key >> a.pages.shift) - p0);
             bits = (uint32_t)__builtin_amdgcn_ballot_w64(lane < KT && key < length && e >= 0);
         };
-        auto dma = [&](const char *from, const int *off, uint32_t to) {
+        auto dma = [&](const char *from, const uint32_t *off, uint32_t to) {
 #pragma unroll
-            for (int u = 0; u < UN; ++u) dma16_at(from + rowat[u] + off[u], to + (uint32_t)u * 1024u);
+            for (int u = 0; u < UN; ++u) {
+                if constexpr (WIDE) dma16_from((uint64_t)from + (uint64_t)rowat[u], off[u], to + (uint32_t)u * 1024u);
+                else dma16_at(from + rowat[u] + off[u], to + (uint32_t)u * 1024u);
+            }
         };
         const uint32_t kt = lds0, vt = lds0 + (uint32_t)TILE;
         if (n > 0) {
@@ -478,12 +515,15 @@ __global__ __launch_bounds__(TH, 2 * blocks_per_cu(HD)) void k_attn_paged(PagedA
         const bool cut = sb < x0 || se > x1;
         const int slot = 2 * run + (sb < x0 ? 0 : 1);
         // the part's waves join it
-        for (int e = past ? (wv - wave0) * 64 + lane : rows * (HD / 4); e < rows * (HD / 4); e += waves * 64) {
-            const int row = e / (HD / 4), at = 4 * (e % (HD / 4));
-            Joined<HD> j;
+        for (int e = past ? (wv - wave0) * 64 + lane : rows * L; e < rows * L; e += waves * 64) {
+            const int row = e / L, at = 4 * (e % L);
+            float t = -__builtin_inff();
+            for (int w = wave0; w < wave0 + waves; ++w) t = fmaxf(t, joined[0][w][row]);
+            Joined j;
+            const float base = j.rise(t);
             for (int w = wave0; w < wave0 + waves; ++w)
                 j.add(joined[0][w][row], joined[1][w][row],
-                      *reinterpret_cast<const floatx4 *>(reinterpret_cast<const float *>(lds + w * SH::RING) + row * SH::PAD + at));
+                      *reinterpret_cast<const floatx4 *>(reinterpret_cast<const float *>(lds + w * SH::RING) + row * SH::PAD + at), base);
             if (!cut) {
                 write_out<T>(a, ms, (int64_t)(head0 + row) * HD + at, j.top, j.l, j.o);
                 continue;
@@ -506,10 +546,13 @@ __global__ __launch_bounds__(TH, 2 * blocks_per_cu(HD)) void k_attn_paged(PagedA
             cuts = 1;
         }
         if (le > x1 && lb >= x0) {
-            cut_s[cuts] = where.base + l1;
-            cut_begin[cuts] = lb;
-            cut_end[cuts] = le;
-            ++cuts;
+            const int i = cuts++;  // (selects: an index that is not known would put the arrays in memory)
+            cut_s[0] = i == 0 ? where.base + l1 : cut_s[0];
+            cut_begin[0] = i == 0 ? lb : cut_begin[0];
+            cut_end[0] = i == 0 ? le : cut_end[0];
+            cut_s[1] = where.base + l1;
+            cut_begin[1] = lb;
+            cut_end[1] = le;
         }
         __syncthreads();  // the rings are free again
     }
@@ -518,45 +561,49 @@ __global__ __launch_bounds__(TH, 2 * blocks_per_cu(HD)) void k_attn_paged(PagedA
     // The block that arrives last joins a sequence's pieces, in their order.  Stores and loads are
     // device-coherent (sc1), a store's acknowledgement says that it is visible, and the barrier that all of
     // the block's are, before the relaxed atomic counts them; the loads follow its result.  No block waits for another.
-    auto first_run = [&](int i) { return cut_begin[i] / len; };
-    auto pieces_of = [&](int i) { return (cut_end[i] - 1) / len - first_run(i) + 1; };
-    auto counter = [&](int i) { return a.counters + ((int64_t)first_run(i) * per_run + rest) * kCounterStride; };
     wait_vmcnt<0>();
     __syncthreads();
+    auto mine_of = [&](int i, int &seq, int &b0, int &pieces) {
+        const int begin = i ? cut_begin[1] : cut_begin[0], end = i ? cut_end[1] : cut_end[0];
+        seq = i ? cut_s[1] : cut_s[0];
+        b0 = begin / len;
+        pieces = (end - 1) / len - b0 + 1;
+        return a.counters + (((int64_t)b0 * a.n_kv + g) * a.rbs + rb) * kCounterStride;
+    };
     if ((int)threadIdx.x < cuts) {
-        const int i = threadIdx.x;
-        last[i] = __hip_atomic_fetch_add(i ? counter(1) : counter(0), 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-                  (i ? pieces_of(1) : pieces_of(0)) - 1;
+        int seq, b0, pieces;
+        int *counter = mine_of(threadIdx.x, seq, b0, pieces);
+        const bool all = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == pieces - 1;
+        last[threadIdx.x] = all;
+        if (all) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        if (i >= cuts || !last[i]) continue;
-        if (threadIdx.x == 0) __hip_atomic_store(counter(i), 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const auto rp = part_rsrc(a, HD);
-        const int E = rows * (HD / 4), groups = max(1, TH / E);  // threads of all dims, pieces side by side
-        for (int e0 = 0; e0 < E; e0 += TH) {
-            const int gi = groups > 1 ? (int)threadIdx.x / E : 0;
-            const int e = groups > 1 ? (int)threadIdx.x - gi * E : e0 + (int)threadIdx.x;
-            const bool in = gi < groups && e < E;
-            const int row = e / (HD / 4), at = 4 * (e % (HD / 4));
-            Joined<HD> j;
-            if (in) j.read(a, rp, first_run(i), pieces_of(i), head0 + row, at, gi, groups);
-            if (groups > 1) {
-                float *x = reinterpret_cast<float *>(lds) + threadIdx.x * 8;
-                __syncthreads();
-                *reinterpret_cast<floatx4 *>(x) = j.o;
-                x[4] = j.top;
-                x[5] = j.l;
-                __syncthreads();
-                if (in && gi == 0)
-                    for (int k = 1; k < groups; ++k) {
-                        const float *y = reinterpret_cast<const float *>(lds) + (k * E + e) * 8;
-                        j.add(y[4], y[5], *reinterpret_cast<const floatx4 *>(y));
-                    }
-            }
-            if (in && gi == 0) write_out<T>(a, cut_s[i], (int64_t)(head0 + row) * HD + at, j.top, j.l, j.o);
+#pragma unroll 1
+    for (int i = 0; i < cuts; ++i) {
+        if (!last[i]) continue;
+        int seq, b0, pieces;
+        mine_of(i, seq, b0, pieces);
+        // threads: 4 dims of a row each, and as many pieces side by side as that leaves room for
+        const int lr = rows > 8 ? 4 : rows > 4 ? 3 : rows > 2 ? 2 : rows > 1 ? 1 : 0;
+        const int sub = threadIdx.x / L, row = sub & ((1 << lr) - 1), gi = sub >> lr, groups = (TH / L) >> lr, at = 4 * (threadIdx.x % L);
+        Joined j;
+        if (row < rows) j.read<HD>(a, part_rsrc(a, HD), b0, pieces, head0 + row, at, gi, groups);
+        float *x = reinterpret_cast<float *>(lds) + threadIdx.x * 8;
+        __syncthreads();  // the last sequence's have been read
+        *reinterpret_cast<floatx4 *>(x) = j.o;
+        x[4] = j.top;
+        x[5] = j.l;
+        __syncthreads();
+        if (gi != 0 || row >= rows) continue;
+        const int used = min(groups, pieces);
+        float t = -__builtin_inff();
+        for (int k = 1; k < used; ++k) t = fmaxf(t, x[k * (8 * L << lr) + 4]);
+        const float base = j.rise(t);
+        for (int k = 1; k < used; ++k) {
+            const float *y = x + k * (8 * L << lr);
+            j.add(y[4], y[5], *reinterpret_cast<const floatx4 *>(y), base);
         }
+        write_out<T>(a, seq, (int64_t)(head0 + row) * HD + at, j.top, j.l, j.o);
     }
 }
 
@@ -578,14 +625,15 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a) {
     const int b0 = t0 / len, pieces = (t1 - 1) / len - b0 + 1;
     if (pieces <= 1) return;  // written by the block that had them all
     const int gi = lane / L, at = 4 * (lane % L);
-    Joined<HD> j;
-    j.read(a, part_rsrc(a, HD), b0, pieces, head, at, gi, G);
+    Joined j;
+    j.read<HD>(a, part_rsrc(a, HD), b0, pieces, head, at, gi, G);
 #pragma unroll
     for (int w = 32; w >= L; w >>= 1) {
         floatx4 o;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = __shfl_xor(j.o[e], w);
-        j.add(__shfl_xor(j.top, w), __shfl_xor(j.l, w), o);
+        const float m = __shfl_xor(j.top, w), l = __shfl_xor(j.l, w);
+        j.add(m, l, o, j.rise(m));
     }
     if (gi == 0) write_out<T>(a, s, (int64_t)head * HD + at, j.top, j.l, j.o);
 }
@@ -597,9 +645,17 @@ int paged_runs(int n_heads, int n_kv, int head_dim) {
 
 template <typename T, int HD>
 int launch(PagedArgs a, hipStream_t s) {
-    const int64_t blocks = (int64_t)a.runs * a.n_kv * a.rbs, rows = cdiv((int64_t)a.pages.n_seqs * a.n_heads, 4);
-    if (!grid_ok(blocks, TH) || !grid_ok(rows, 256)) return fail(RQ_ERR_SHAPE, "too many rows for one call");
-    hipLaunchKernelGGL((k_attn_paged<T, HD>), dim3((unsigned)blocks), dim3(TH), 0, s, a);
+    using SH = PShape<T, HD>;
+    const int64_t rows = cdiv((int64_t)a.pages.n_seqs * a.n_heads, 4);
+    if (!grid_ok(a.n_kv, TH) || a.rbs > 65535 || !grid_ok(rows, 256)) return fail(RQ_ERR_SHAPE, "too many rows for one call");
+    a.by_runs = Div::by(a.runs);
+    const dim3 grid((unsigned)a.n_kv, (unsigned)a.rbs, (unsigned)a.runs);
+    // (offsets within a page and within the rows of a DMA instruction in 32 bits)
+    const int64_t page = (int64_t)1 << a.pages.shift;
+    if (page >= SH::RPU && page * a.pages.pos_stride < ((int64_t)1 << 31))
+        hipLaunchKernelGGL((k_attn_paged<T, HD, true>), grid, dim3(TH), 0, s, a);
+    else
+        hipLaunchKernelGGL((k_attn_paged<T, HD, false>), grid, dim3(TH), 0, s, a);
     RQ_LAUNCH_CHECK();
     if (a.runs > 1 && !a.counters) {
         hipLaunchKernelGGL((k_paged_join<T, HD>), dim3((unsigned)rows), dim3(256), 0, s, a);

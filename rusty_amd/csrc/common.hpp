@@ -62,6 +62,18 @@ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // HIP launches fewer than 2^32 threads along a grid dimension.
 inline bool grid_ok(int64_t blocks, int64_t threads) { return blocks * threads < ((int64_t)1 << 32); }
 
+// x / d for 0 <= x < 2^31 by one product: m = ceil(2^(31 + b) / d) with 2^b >= d is off by
+// less than 2^b / 2^(31 + b) of 1 / d, so x m / 2^(31 + b) never reaches the next whole number.
+struct Div {
+    uint32_t m, sh;
+    __host__ static Div by(int64_t d) {
+        uint32_t b = 0;
+        while (((int64_t)1 << b) < d) ++b;
+        return {(uint32_t)((((uint64_t)1 << (31 + b)) + (uint64_t)d - 1) / (uint64_t)d), 31 + b};
+    }
+    __device__ __forceinline__ int operator()(int x) const { return (int)(((uint64_t)(uint32_t)x * m) >> sh); }
+};
+
 // Launchers implemented in the kernel translation units.  Arguments are
 // validated by the C-ABI layer before these are called.
 int launch_dequantize(const uint32_t *in, size_t n_words, float *out, size_t n_out, hipStream_t s);
