@@ -116,7 +116,12 @@ __device__ __forceinline__ int scan_add(int v) {  // inclusive, over the wave
     return v;
 }
 
-__device__ __forceinline__ int run_length(const PagedArgs &a, int total) { return max(NW, a.by_runs(total + a.runs - 1)); }
+// A run's units: an equal share, at least 12; and a sequence of up to so many units is not cut, the run
+// that it begins in has all of it.  Shorter runs and more cuts cost joining, longer ones the waves' turns (us, 48
+// chats of 37 to 2047 keys, 32/4 heads of 64 / one sequence of 513: at least 8, all cut 12.9 / 7.9, up to 16
+// whole 12.6 / 7.9; 12, up to 24 whole 12.5 / 7.3; 24, up to 24 whole 14.2 / 7.1).
+__device__ __forceinline__ int run_length(const PagedArgs &a, int total) { return max(12, a.by_runs(total + a.runs - 1)); }
+__device__ __forceinline__ int whole_units(int len) { return min(2 * len, 24); }
 
 // Where a run lies: the units of all sequences, of a run, its own x0 .. x1 - 1, and 64 (`held`) sequences
 // from `base` on, lane l's units begin .. end - 1 and its length; the run's first unit is among them.
@@ -242,7 +247,7 @@ __device__ __forceinline__ void write_out(const PagedArgs &a, int s, int64_t at,
 
 // Block (key/value head, 16 of its query heads, run).  WIDE: the rows of a DMA instruction lie in one page.
 template <typename T, int HD, bool WIDE>
-__global__ __launch_bounds__(TH, 2 * blocks_per_cu(HD)) void k_attn_paged(PagedArgs a) {
+__global__ __launch_bounds__(TH, NW * blocks_per_cu(HD) / 4) void k_attn_paged(PagedArgs a) {
     using SH = PShape<T, HD>;
     constexpr bool F16 = SH::F16;
     constexpr int KT = SH::KT, ROW = SH::ROW, CH = SH::CH, TILE = SH::TILE, RPU = SH::RPU, UN = SH::UN, L = SH::L;
@@ -297,12 +302,21 @@ __global__ __launch_bounds__(TH, 2 * blocks_per_cu(HD)) void k_attn_paged(PagedA
     // Sequences that other blocks have parts of, too: at most the first and the last of the run.
     int cuts = 0, cut_s[2] = {0, 0}, cut_begin[2] = {0, 0}, cut_end[2] = {1, 1};
 
+    const int whole = whole_units(len);
     for (int x = x0; x < x1;) {
-        if (x >= __builtin_amdgcn_readlane(where.end, 63)) where.next(a, x);
+        const int held_end = __builtin_amdgcn_readlane(where.end, 63);
+        if (x >= held_end) where.next(a, held_end);
         // This round's parts: lane l's of its sequence, units from .. from + mine - 1 of the flat order, to waves
         // until - need .. until - 1, per units each; as many parts as find waves, with per up to twice an equal share.
-        const int from = max(where.begin, x), mine = max(min(where.end, x1) - from, 0);
-        int per = (x1 - x + NW - 1) / NW, need = 0, until = 0;
+        const bool entire = where.end - where.begin <= whole;
+        const int from = max(where.begin, x);
+        const int mine = max((entire ? (where.begin >= x0 && where.begin < x1 ? where.end : 0) : min(where.end, x1)) - from, 0);
+        const int share = (__builtin_amdgcn_readlane(scan_add(mine), 63) + NW - 1) / NW;
+        if (share == 0) {  // (what is held began in another run)
+            x = __builtin_amdgcn_readlane(where.end, 63);
+            continue;
+        }
+        int per = share, need = 0, until = 0;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             need = 0;  // mine / per rounded up, as far as it tells
@@ -314,7 +328,7 @@ __global__ __launch_bounds__(TH, 2 * blocks_per_cu(HD)) void k_attn_paged(PagedA
         }
         const uint64_t dealt = __builtin_amdgcn_ballot_w64(mine > 0 && until <= NW);  // a run of lanes, not empty
         const int l0 = __builtin_ctzll(dealt), l1 = 63 - __builtin_clzll(dealt);
-        x = min(__builtin_amdgcn_readlane(where.end, l1), x1);
+        x = __builtin_amdgcn_readlane(from + mine, l1);
         // this wave's (the last waves may have none)
         const uint64_t past = __builtin_amdgcn_ballot_w64(until > wv) & dealt;
         const int pl = past ? __builtin_ctzll(past) : l0;
@@ -512,7 +526,7 @@ __global__ __launch_bounds__(TH, 2 * blocks_per_cu(HD)) void k_attn_paged(PagedA
         }
         __syncthreads();
         const auto rp = part_rsrc(a, HD);
-        const bool cut = sb < x0 || se > x1;
+        const bool cut = se - sb > whole && (sb < x0 || se > x1);
         const int slot = 2 * run + (sb < x0 ? 0 : 1);
         // the part's waves join it
         for (int e = past ? (wv - wave0) * 64 + lane : rows * L; e < rows * L; e += waves * 64) {
@@ -539,13 +553,13 @@ __global__ __launch_bounds__(TH, 2 * blocks_per_cu(HD)) void k_attn_paged(PagedA
         // its cut sequences: one that began before the run, one that goes on behind it
         const int fb = __builtin_amdgcn_readlane(where.begin, l0), fe = __builtin_amdgcn_readlane(where.end, l0);
         const int lb = __builtin_amdgcn_readlane(where.begin, l1), le = __builtin_amdgcn_readlane(where.end, l1);
-        if (fb < x0) {
+        if (fe - fb > whole && fb < x0) {
             cut_s[0] = where.base + l0;
             cut_begin[0] = fb;
             cut_end[0] = fe;
             cuts = 1;
         }
-        if (le > x1 && lb >= x0) {
+        if (le - lb > whole && le > x1 && lb >= x0) {
             const int i = cuts++;  // (selects: an index that is not known would put the arrays in memory)
             cut_s[0] = i == 0 ? where.base + l1 : cut_s[0];
             cut_begin[0] = i == 0 ? lb : cut_begin[0];
@@ -623,7 +637,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a) {
     const int total = __builtin_amdgcn_readlane(scan_add(all), 63), t0 = __builtin_amdgcn_readlane(scan_add(before), 63);
     const int len = run_length(a, total), t1 = t0 + units_of<KT>(clamped(a, s));
     const int b0 = t0 / len, pieces = (t1 - 1) / len - b0 + 1;
-    if (pieces <= 1) return;  // written by the block that had them all
+    if (pieces <= 1 || t1 - t0 <= whole_units(len)) return;  // written by the block that had them all
     const int gi = lane / L, at = 4 * (lane % L);
     Joined j;
     j.read<HD>(a, part_rsrc(a, HD), b0, pieces, head, at, gi, G);
