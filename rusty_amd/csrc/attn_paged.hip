@@ -86,20 +86,6 @@ __device__ __forceinline__ float join4(float v, F f) {
     return f(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
 }
 
-// DMA of 16 bytes per lane (see dma16), not to be kept: every key is read once.  LDS[lds_addr + 16 * lane] = *p
-// of each lane's own address, or base[voff] with a uniform base.
-__device__ __forceinline__ void dma16_at(const char *p, uint32_t lds_addr) {
-    const uint32_t l = __builtin_amdgcn_readfirstlane(lds_addr);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" : : "s"(l), "v"(p) : "memory", "m0");
-}
-__device__ __forceinline__ void dma16_from(uint64_t base, uint32_t voff, uint32_t lds_addr) {
-    const uint32_t l = __builtin_amdgcn_readfirstlane(lds_addr);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
-                 :
-                 : "s"(l), "v"(voff), "s"(base)
-                 : "memory", "m0");
-}
-
 __device__ __forceinline__ int clamped(const PagedArgs &a, int s) { return min(max(a.lengths[s], 0), a.pages.capacity()); }
 template <int KT>
 __device__ __forceinline__ int units_of(int length) {

@@ -1,5 +1,6 @@
 // Buffer resources and global -> LDS DMA for gfx950 (CDNA4), shared by the
-// kernels that stage operands through LDS rings (gemm.hip, matmul_f32.hip, prefill.hip, attn.hip).
+// kernels that stage operands through LDS rings (gemm.hip, matmul_f32.hip, prefill.hip, attn.hip,
+// attn_paged.hip, loras.hip).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -41,7 +42,7 @@ __device__ __forceinline__ uint32_t lds_addr(T *p) {
 // base (one wait state before the load, as the ISA requires).  The compiler
 // reserves M0 and warns that the "m0" clobber is not honoured (-Winline-asm):
 // that is safe only while nothing else in these kernels holds a value in M0
-// across a DMA, and in the device assembly of gemm.hip, matmul_f32.hip, prefill.hip and attn.hip the
+// across a DMA, and in the device assembly of gemm.hip, matmul_f32.hip, prefill.hip, attn.hip, attn_paged.hip and loras.hip the
 // only instructions naming M0 are these moves (each directly before its load).
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint32_t lds_addr, uint32_t voff) {
     const uint32_t l = __builtin_amdgcn_readfirstlane(lds_addr);
@@ -57,6 +58,25 @@ __device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t r, uint32_t lds_addr
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
                  :
                  : "s"(l), "v"(voff), "s"(r)
+                 : "memory", "m0");
+}
+
+// DMA of 16 bytes per lane from memory of any size, for data that is read once (nt: not kept in the caches):
+// LDS[lds_addr + 16 * lane] = *p of each lane's own address, or base[voff] with a uniform base.
+__device__ __forceinline__ void dma16_at(const char *p, uint32_t lds_addr) {
+    const uint32_t l = __builtin_amdgcn_readfirstlane(lds_addr);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" : : "s"(l), "v"(p) : "memory", "m0");
+}
+// The same for data that other blocks read, too.
+__device__ __forceinline__ void dma16_kept(const char *p, uint32_t lds_addr) {
+    const uint32_t l = __builtin_amdgcn_readfirstlane(lds_addr);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(l), "v"(p) : "memory", "m0");
+}
+__device__ __forceinline__ void dma16_from(uint64_t base, uint32_t voff, uint32_t lds_addr) {
+    const uint32_t l = __builtin_amdgcn_readfirstlane(lds_addr);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+                 :
+                 : "s"(l), "v"(voff), "s"(base)
                  : "memory", "m0");
 }
 

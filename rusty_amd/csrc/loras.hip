@@ -20,6 +20,7 @@
 #include <type_traits>
 
 #include "common.hpp"
+#include "lds_dma.hpp"
 
 namespace rq {
 namespace {
@@ -28,17 +29,21 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxRank = 256;
-constexpr int kSlice = 1024;  // k of a k_loras_in block: 256 a wave
+// Rows of a k_loras_in block, in tiles of 16: one tile while rows are few, else four, so that A's rows are read
+// less often.  And its k, a quarter per wave: as much as the registers hold of X and of 32 rows of A.
+constexpr int64_t kFewRows = 64;
+constexpr int slice(bool f16, int tiles) { return (f16 ? 1024 : 512) / (tiles > 1 ? 2 : 1); }
 
 struct LoraArgs {
     const void *x, *a, *b;
     const float *factors;
     const int *ids, *ranks;
-    float *part;        // [m][slices][rank]
+    float *part;        // [m][slices][ranks4]: X . A_i^T, a sum per slice of k
     const float *main;  // [m][n]
     void *y;
     int64_t m, k, n;
     int n_adapters, rank, slices;
+    int ranks4;         // rank rounded up to 4
 };
 
 // The adapter of row t, -1 for none.
@@ -70,170 +75,308 @@ __device__ __forceinline__ D load_n(const S *p, int64_t e, int64_t end) {
     return r;
 }
 
-// Block (tile, slice, z): 16 rows, kSlice of k; of the tile's distinct adapters every gridDim.z-th.
-template <typename X, typename A, bool VEC>
+// Block (TM tiles of 16 rows, slice of k, z): of the rows' distinct adapters every gridDim.z-th, 16 RT of their
+// rows at once.  X is asked for at once.
+template <typename X, typename A, int TM, int RT, bool VEC>
 __global__ __launch_bounds__(256) void k_loras_in(LoraArgs p) {
     constexpr bool F16 = sizeof(X) == 2 && sizeof(A) == 2;
-    constexpr int N = F16 ? 8 : 4, STEP = 4 * N, STEPS = 256 / STEP;  // k a lane, an instruction, of a wave
+    constexpr int N = F16 ? 8 : 4, STEP = 4 * N, WAVE = slice(F16, TM) / 4, STEPS = WAVE / STEP;  // k a lane, an instruction, of a wave
     typedef std::conditional_t<F16, half8, floatx4> frag;
-    __shared__ float sums[4][16][17];
+    __shared__ float sums[4][16 * TM][16 * RT + 1];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, col = lane & 15, qt = lane >> 4;
-    const int64_t t0 = (int64_t)blockIdx.x * 16, row = min(t0 + col, p.m - 1);
-    const int64_t k0 = (int64_t)blockIdx.y * kSlice + wv * 256 + N * qt;
-    const int mine = t0 + col < p.m ? adapter_of(p, t0 + col) : -1;
-    uint64_t left = __builtin_amdgcn_ballot_w64(lane < 16 && mine >= 0);
-    if (!left) return;
-    const X *xr = static_cast<const X *>(p.x) + row * p.k;
-    frag xf[STEPS];
+    const int64_t t0 = (int64_t)blockIdx.x * 16 * TM;
+    const int64_t k0 = (int64_t)blockIdx.y * slice(F16, TM) + wv * WAVE + N * qt;
+    const int id = adapter_of(p, min(t0 + lane, p.m - 1));
+    frag xf[TM][STEPS];
 #pragma unroll
-    for (int j = 0; j < STEPS; ++j) xf[j] = load_n<X, N, VEC, frag>(xr, k0 + j * STEP, p.k);
+    for (int u = 0; u < TM; ++u) {
+        const X *xr = static_cast<const X *>(p.x) + min(t0 + 16 * u + col, p.m - 1) * p.k;
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j) xf[u][j] = load_n<X, N, VEC, frag>(xr, k0 + j * STEP, p.k);
+    }
+    const int mine = lane < 16 * TM && t0 + lane < p.m ? id : -1;
+    uint64_t left = __builtin_amdgcn_ballot_w64(mine >= 0);
     for (int z = 0; left; ++z) {
         const int i = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
-        const uint64_t same = __builtin_amdgcn_ballot_w64(mine == i) & left;
+        const uint64_t same = __builtin_amdgcn_ballot_w64(mine == i);
         left &= ~same;
         if (z % (int)gridDim.z != (int)blockIdx.z) continue;
         const int rank = rank_of(p, i);
-        for (int r0 = 0; r0 < rank; r0 += 16) {
-            const A *ar = static_cast<const A *>(p.a) + ((int64_t)i * p.rank + min(r0 + col, rank - 1)) * p.k;
-            floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-            frag af[STEPS];
+        const A *a = static_cast<const A *>(p.a) + (int64_t)i * p.rank * p.k;
+#pragma unroll 1
+        for (int r0 = 0; r0 < rank; r0 += 16 * RT) {
+            frag af[RT][STEPS];
 #pragma unroll
-            for (int j = 0; j < STEPS; ++j) af[j] = load_n<A, N, VEC, frag>(ar, k0 + j * STEP, p.k);
+            for (int u = 0; u < RT; ++u) {
+                const A *ar = a + (int64_t)min(r0 + 16 * u + col, rank - 1) * p.k;
 #pragma unroll
-            for (int j = 0; j < STEPS; ++j) {
-                if constexpr (F16) {
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(xf[j], af[j], acc, 0, 0, 0);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(xf[j][e], af[j][e], acc, 0, 0, 0);
-                }
+                for (int j = 0; j < STEPS; ++j) af[u][j] = load_n<A, N, VEC, frag>(ar, k0 + j * STEP, p.k);
             }
             __syncthreads();  // the last sums have been read
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sums[wv][4 * qt + e][col] = acc[e];
+            for (int t = 0; t < TM; ++t)
+#pragma unroll
+                for (int u = 0; u < RT; ++u) {
+                    floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int j = 0; j < STEPS; ++j) {
+                        if constexpr (F16) {
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(xf[t][j], af[u][j], acc, 0, 0, 0);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(xf[t][j][e], af[u][j][e], acc, 0, 0, 0);
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sums[wv][16 * t + 4 * qt + e][16 * u + col] = acc[e];
+                }
             __syncthreads();
-            const int tr = threadIdx.x >> 4, r = threadIdx.x & 15;  // one (row, r) a thread
-            if ((same >> tr & 1) && r0 + r < rank)
-                p.part[((t0 + tr) * p.slices + blockIdx.y) * p.rank + r0 + r] =
-                    (sums[0][tr][r] + sums[1][tr][r]) + (sums[2][tr][r] + sums[3][tr][r]);
+#pragma unroll
+            for (int e = 0; e < TM * RT; ++e) {
+                const int tr = (e / RT) * 16 + (threadIdx.x >> 4), r = 16 * (e % RT) + (threadIdx.x & 15);
+                if ((same >> tr & 1) && r0 + r < p.ranks4)
+                    p.part[((t0 + tr) * p.slices + blockIdx.y) * p.ranks4 + r0 + r] =
+                        r0 + r < rank ? (sums[0][tr][r] + sums[1][tr][r]) + (sums[2][tr][r] + sums[3][tr][r]) : 0.0f;
+            }
         }
     }
 }
 
-// The row's t times its factor into ts[0 .. rank), the slices summed in order; whole block of TH threads or wave.
-template <int TH>
-__device__ __forceinline__ void sum_slices(const LoraArgs &p, int64_t t, int i, int rank, int thread, float *ts) {
-    const float f = p.factors ? p.factors[i] : 1.0f;
-    for (int r = thread; r < rank; r += TH) {
-        const float *q = p.part + t * p.slices * p.rank + r;
-        float s = 0.0f;
-        for (int j = 0; j < p.slices; ++j) s += q[(int64_t)j * p.rank];
-        ts[r] = f * s;
-    }
-}
-
-// Few rows: block (row, stretch of 2048 columns).
+// Few rows: block (row, stretch of 2048 columns).  What does not wait for t is asked for first.
 template <typename B, typename Y, bool VEC>
 __global__ __launch_bounds__(256) void k_loras_out_row(LoraArgs p) {
     typedef float floatx8 __attribute__((ext_vector_type(8)));
-    __shared__ float ts[kMaxRank];
+    typedef B vecb __attribute__((ext_vector_type(8)));
+    constexpr int RC = sizeof(B) == 2 ? 16 : 8;  // rows of B at once
     const int64_t t = blockIdx.x, c = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 8;
-    const int i = adapter_of(p, t), rank = i < 0 ? 0 : rank_of(p, i);
-    if (rank > 0) sum_slices<256>(p, t, i, rank, threadIdx.x, ts);
-    __syncthreads();
-    if (c >= p.n) return;
-    floatx8 acc = {};
+    const int i = adapter_of(p, t);
+    const floatx8 main = load_n<float, 8, VEC, floatx8>(p.main + t * p.n, c, p.n);
+    const int rank = i < 0 ? 0 : rank_of(p, i);
     const B *b = static_cast<const B *>(p.b) + (int64_t)max(i, 0) * p.rank * p.n;
-#pragma unroll 8
-    for (int r = 0; r < rank; ++r) {
-        const floatx8 v = load_n<B, 8, VEC, floatx8>(b + (int64_t)r * p.n, c, p.n);
-        const float s = ts[r];
+    const float f = p.factors && i >= 0 ? p.factors[i] : 1.0f;
+    const int lane = threadIdx.x & 63, u0 = lane & 15;
+    floatx8 acc = {};
+#pragma unroll 1
+    for (int r0 = 0; r0 < rank; r0 += RC) {
+        vecb bv[RC];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] = __builtin_fmaf(s, v[e], acc[e]);
+        for (int u = 0; u < RC; ++u) bv[u] = load_n<B, 8, VEC, vecb>(b + (int64_t)min(r0 + u, rank - 1) * p.n, c, r0 + u < rank ? p.n : 0);
+        // t of r0 + lane % 16: the wave's four rows of lanes take every fourth slice
+        float s = 0.0f;
+        if (u0 < RC && r0 + u0 < rank)
+            for (int j = lane >> 4; j < p.slices; j += 4) s += p.part[(t * p.slices + j) * p.ranks4 + r0 + u0];
+        s += __shfl_xor(s, 16);
+        s += __shfl_xor(s, 32);
+        s *= f;
+#pragma unroll
+        for (int u = 0; u < RC; ++u) {
+            const float su = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s), u));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] = __builtin_fmaf(su, (float)bv[u][e], acc[e]);
+        }
     }
-    const float *main = p.main + t * p.n;
-    const floatx8 v = load_n<float, 8, VEC, floatx8>(main, c, p.n);
+    if (c >= p.n) return;
     Y *y = static_cast<Y *>(p.y) + t * p.n;
     typedef Y vec __attribute__((ext_vector_type(8)));
     if constexpr (VEC) {
         vec o;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = (Y)(v[e] + acc[e]);
+        for (int e = 0; e < 8; ++e) o[e] = (Y)(main[e] + acc[e]);
         *reinterpret_cast<vec *>(y + c) = o;
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-            if (c + e < p.n) y[c + e] = (Y)(v[e] + acc[e]);
+            if (c + e < p.n) y[c + e] = (Y)(main[e] + acc[e]);
     }
 }
 
-// Many rows: block (16 rows, stretch of 4 x 16 V columns), a wave 16 V columns.
-template <typename B, typename Y, bool VEC>
+// Many rows: block (16 rows, stretch of 256 columns), a wave 64 of them: B^T . t^T on the matrix instructions, so
+// that a lane gets 16 columns side by side of one row (row i of instruction v is column 16 (i / 4) + 4 v + i % 4).
+// Bound by the shared product's way in and Y's out.  A load that is waited for alone costs 1 to 2 us here, so all
+// that a tile with one adapter of up to 32 ranks reads is asked for together, and what B and the shared product take
+// waits in LDS (DMA): few registers, many waves.  Further adapters and ranks take turns with two buffers of 32 (f32 B: 16) ranks.
+// fp16 B: t, scaled by a power of two per row, is two fp16 terms (off by at most 2^-22), two instructions of 32 ranks
+// a 16 columns, B's fragments by transposing LDS reads; f32 instructions of 4 ranks took 3 us longer at 2048 x 4096, rank 32.
+__host__ __device__ constexpr int out_ranks(int rank) { return (rank + 31) / 32 * 32; }
+template <typename B, typename Y>
 __global__ __launch_bounds__(256) void k_loras_out(LoraArgs p) {
-    constexpr int V = 16 / (int)sizeof(B);  // columns of a lane: V instructions, column col of the v-th is V col + v
-    typedef float vecf __attribute__((ext_vector_type(V)));
-    __shared__ float ts[16][kMaxRank + 4];
-    __shared__ int id[16];
+    constexpr bool F16 = sizeof(B) == 2;
+    constexpr int R = F16 ? 32 : 16;  // ranks of a step
+    constexpr int CH = 64 * (int)sizeof(B) / 16, RPU = 64 / CH, UN = R / RPU;  // B: 16-byte pieces of a row, rows of a DMA
+    typedef short short4v __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) short4v lds_short4;
+    __shared__ __attribute__((aligned(16))) floatx4 main[4][16][16];       // [wave][row][16-byte piece ^ row]
+    __shared__ __attribute__((aligned(16))) B bs[4][2][R][64];             // [wave][buffer][rank][column]
+    extern __shared__ __attribute__((aligned(16))) float ts[];             // [16][out_ranks + 4]: t, fp16 B: its two terms side by side
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, col = lane & 15, qt = lane >> 4;
-    const int64_t t0 = (int64_t)blockIdx.x * 16, c = ((int64_t)blockIdx.y * 4 + wv) * 16 * V + V * col;
-    for (int tr = wv; tr < 16; tr += 4) {
-        const int64_t t = t0 + tr;
-        const int i = t < p.m ? adapter_of(p, t) : -1, rank = i < 0 ? 0 : rank_of(p, i);
-        for (int r = rank + lane; r < ((p.rank + 3) & ~3); r += 64) ts[tr][r] = 0.0f;
-        if (rank > 0) sum_slices<64>(p, t, i, rank, lane, ts[tr]);
-        if (lane == 0) id[tr] = i;
-    }
-    __syncthreads();
-    const int mine = id[col];
-    uint64_t left = __builtin_amdgcn_ballot_w64(lane < 16 && mine >= 0);
-    vecf out[4];  // rows 4 qt + e
+    const int64_t t0 = (int64_t)blockIdx.x * 16, c0 = ((int64_t)blockIdx.y * 4 + wv) * 64;
+    const int ranks = out_ranks(p.rank), row4 = ranks + 4;
+    int mine = t0 + col < p.m ? adapter_of(p, t0 + col) : -1;
+    asm volatile("" : "+v"(mine));  // (waited for here: later the wait would be for the DMA, too)
+    const uint64_t all = __builtin_amdgcn_ballot_w64(lane < 16 && mine >= 0);
+    // steps: R ranks of one adapter
+    struct Step {
+        int i, rank, r0;
+        uint64_t same, left;  // its rows; those of the adapters after it
+    };
+    auto adapter = [&](uint64_t left) {
+        Step s;
+        s.i = __builtin_amdgcn_readlane(mine, left ? __builtin_ctzll(left) : 0);
+        s.same = __builtin_amdgcn_ballot_w64(mine == s.i) & left;
+        s.left = left & ~s.same;
+        s.rank = left ? rank_of(p, s.i) : 0;
+        s.r0 = 0;
+        return s;
+    };
+    auto after = [&](Step s) {
+        s.r0 += R;
+        return s.r0 < s.rank ? s : adapter(s.left);
+    };
+    auto fetch = [&](const Step &s, int buffer) {
+        const int64_t c = min(c0 + lane % CH * (16 / (int)sizeof(B)), p.n - 16 / (int)sizeof(B));
+        const B *b = static_cast<const B *>(p.b) + (int64_t)s.i * p.rank * p.n + c;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) out[e] = {};
-    while (left) {
-        const int i = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
-        const uint64_t same = __builtin_amdgcn_ballot_w64(mine == i) & left;
-        left &= ~same;
-        const int rank = rank_of(p, i);
-        const B *b = static_cast<const B *>(p.b) + (int64_t)i * p.rank * p.n;
-        floatx4 acc[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) acc[v] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-        for (int r0 = 0; r0 < rank; r0 += 4) {
-            const int r = r0 + qt;
-            const vecf bv = load_n<B, V, VEC, vecf>(b + (int64_t)min(r, rank - 1) * p.n, c, r < rank ? p.n : 0);
-            const float s = ts[col][r];
-#pragma unroll
-            for (int v = 0; v < V; ++v) acc[v] = __builtin_amdgcn_mfma_f32_16x16x4f32(s, bv[v], acc[v], 0, 0, 0);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (same >> (4 * qt + e) & 1)
-#pragma unroll
-                for (int v = 0; v < V; ++v) out[e][v] = acc[v][e];
-    }
-    if (c >= p.n) return;
+        for (int u = 0; u < UN; ++u)
+            dma16_kept(reinterpret_cast<const char *>(b + (int64_t)min(s.r0 + u * RPU + lane / CH, max(s.rank - 1, 0)) * p.n),
+                       lds_addr(&bs[wv][buffer][u * RPU][0]));
+    };
+    Step s = adapter(all);
+    if (all) fetch(s, 0);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const int64_t t = t0 + 4 * qt + e;
-        if (t >= p.m) return;
-        const vecf v = load_n<float, V, VEC, vecf>(p.main + t * p.n, c, p.n);
-        Y *y = static_cast<Y *>(p.y) + t * p.n;
-        typedef Y vec __attribute__((ext_vector_type(V)));
-        if constexpr (VEC) {
-            vec o;
+        const int r = 4 * e + qt;
+        dma16_at(reinterpret_cast<const char *>(p.main + min(t0 + r, p.m - 1) * p.n + min(c0 + 4 * (col ^ r), p.n - 4)),
+                 lds_addr(&main[wv][4 * e][0]));
+    }
+    {
+        // t, 16 threads a row, 4 ranks each: the slices summed in order, times the factor; of rows without an
+        // adapter not written, and not used
+        const int tr = threadIdx.x >> 4, u = threadIdx.x & 15, i = __shfl(mine, tr);
+        float *to = ts + tr * row4;
+        float most = 0.0f;
+        if (i >= 0) {
+            const float f = p.factors ? p.factors[i] : 1.0f;
+            for (int r = 4 * u; r < ranks; r += 64) {
+                const float *q = p.part + (t0 + tr) * p.slices * p.ranks4 + r;
+                floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (r < p.ranks4) {
+#pragma unroll 8
+                    for (int j = 0; j < p.slices; ++j) v += *reinterpret_cast<const floatx4 *>(q + (int64_t)j * p.ranks4);
+                }
+                const int rank = rank_of(p, i);
 #pragma unroll
-            for (int i = 0; i < V; ++i) o[i] = (Y)(v[i] + out[e][i]);
-            *reinterpret_cast<vec *>(y + c) = o;
-        } else {
+                for (int e = 0; e < 4; ++e) {
+                    v[e] = r + e < rank ? f * v[e] : 0.0f;
+                    most = fmaxf(most, fabsf(v[e]));
+                }
+                *reinterpret_cast<floatx4 *>(to + r) = v;
+            }
+        }
+        if constexpr (F16) {
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (c + i < p.n) y[c + i] = (Y)(v[i] + out[e][i]);
+            for (int w = 1; w < 16; w <<= 1) most = fmaxf(most, __shfl_xor(most, w));
+            // the largest in [2^14, 2^15) (a row of zeros, or that is not finite, as it is)
+            const int e = most > 0.0f && most < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+            if (u == 0) to[ranks] = __builtin_ldexpf(1.0f, -e);
+            if (i >= 0)
+                for (int r = 4 * u; r < ranks; r += 64) {
+                    const floatx4 v = *reinterpret_cast<const floatx4 *>(to + r);
+                    typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+                    half4 hi, lo;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float x = __builtin_ldexpf(v[k], e);
+                        hi[k] = (_Float16)x;
+                        lo[k] = __builtin_isfinite((float)hi[k]) ? (_Float16)(x - (float)hi[k]) : (_Float16)0.0f;
+                    }
+                    // (8 ranks: 16 bytes of first terms, 16 of second)
+                    half4 *h = reinterpret_cast<half4 *>(to + r / 8 * 8) + r / 4 % 2;
+                    __builtin_amdgcn_wave_barrier();  // (both halves of the 8 have been read by these lanes)
+                    h[0] = hi;
+                    h[2] = lo;
+                }
         }
     }
+    __syncthreads();
+    floatx4 out[4], acc[4];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) out[v] = acc[v] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    wait_vmcnt<0>();
+    for (int k = 0; s.same; ++k) {
+        const Step next = after(s);
+        if (next.same) {
+            wait_lgkm0();  // (the buffer has been read)
+            fetch(next, (k + 1) & 1);
+            if (k > 0) wait_vmcnt<UN>();
+        } else if (k > 0) {
+            wait_vmcnt<0>();
+        }
+        const int count = min(s.rank - s.r0, R);  // of these ranks, those that the adapter has
+        const B *b = &bs[wv][k & 1][0][0];
+        if constexpr (F16) {
+            if (count < R) {
+                // (what lies past the rank is another rank's, and may be infinite)
+#pragma unroll
+                for (int u = 0; u < UN; ++u)
+                    if (u * RPU + lane / CH >= count)
+                        *reinterpret_cast<half8 *>(&bs[wv][k & 1][u * RPU + lane / CH][lane % CH * 8]) = half8{};
+                wait_lgkm0();
+            }
+            const half8 *t = reinterpret_cast<const half8 *>(ts + col * row4 + s.r0 + 8 * qt);
+            const half8 hi = t[0], lo = t[1];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                // 16 lanes take 4 ranks x 4 x 4 columns; each gets one column's 4 ranks
+                lds_short4 *a = (lds_short4 *)(uintptr_t)(lds_addr(b) + (uint32_t)((8 * qt + col / 4) * 128 + (col & 3) * 32 + v * 8));
+                const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(a));
+                const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(a + 4 * 128 / 8));
+                const half8 bt = __builtin_bit_cast(half8, make_uint4(x.x, x.y, y.x, y.y));
+                acc[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bt, hi, acc[v], 0, 0, 0);
+                acc[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bt, lo, acc[v], 0, 0, 0);
+            }
+        } else {
+            float bv[R / 4][4], tv[R / 4];  // (all read before the first is used)
+#pragma unroll
+            for (int u = 0; u < R / 4; ++u) {
+                const int r = 4 * u + qt;
+                tv[u] = ts[col * row4 + s.r0 + r];
+#pragma unroll
+                for (int v = 0; v < 4; ++v) bv[u][v] = r < count ? (float)b[r * 64 + 16 * (col / 4) + 4 * v + col % 4] : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < R / 4; ++u)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) acc[v] = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[u][v], tv[u], acc[v], 0, 0, 0);
+        }
+        if (next.i != s.i || !next.same) {
+            const bool has = s.same >> col & 1;
+            const float scale = F16 ? ts[col * row4 + ranks] : 1.0f;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) out[v][e] = has ? acc[v][e] * scale : out[v][e];
+                acc[v] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+        }
+        s = next;
+    }
+    const int64_t t = t0 + col, c = c0 + 16 * qt;
+    if (t >= p.m) return;
+    Y *y = static_cast<Y *>(p.y) + t * p.n + c;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // 8 columns
+        if (c + 8 * h >= p.n) break;
+        const floatx4 a0 = main[wv][col][(4 * qt + 2 * h) ^ col] + out[2 * h], a1 = main[wv][col][(4 * qt + 2 * h + 1) ^ col] + out[2 * h + 1];
+        typedef Y vec8 __attribute__((ext_vector_type(8)));
+        vec8 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            o[e] = (Y)a0[e];
+            o[4 + e] = (Y)a1[e];
+        }
+        *reinterpret_cast<vec8 *>(y + 8 * h) = o;
+    }
 }
-
-constexpr int64_t kRowForm = 64;  // rows that k_loras_out_row serves
 
 int check_set(const rq_lora_set *s) {
     if (!s) return fail(RQ_ERR_INVALID_ARGUMENT, "null adapter set");
@@ -244,7 +387,8 @@ int check_set(const rq_lora_set *s) {
     return RQ_OK;
 }
 
-int64_t slices_of(int64_t k) { return std::max<int64_t>(1, cdiv(k, kSlice)); }
+int64_t slices_of(int64_t m, int64_t k, bool f16) { return std::max<int64_t>(1, cdiv(k, slice(f16, m > kFewRows ? 4 : 1))); }
+int64_t ranks4_of(int rank) { return (rank + 3) / 4 * 4; }
 
 int check_loras(const rq_qweight *w, const rq_lora_set *set, const int32_t *ids, const void *x, rq_dtype xt, void *y,
                 rq_dtype yt, int64_t m, void *workspace, size_t workspace_bytes, LoraArgs &p, bool &run) {
@@ -258,7 +402,7 @@ int check_loras(const rq_qweight *w, const rq_lora_set *set, const int32_t *ids,
     const int64_t K = w->k_in, N = w->n_out;
     int64_t t;
     if (!mul_ok(m, K * 4, &t) || !mul_ok(m, N * 4, &t) || K > ((int64_t)1 << 40) || N > ((int64_t)1 << 40) ||
-        !mul_ok((int64_t)set->n_adapters * set->rank, std::max(K, N) * 4, &t) || !mul_ok(m, slices_of(K) * set->rank * 4, &t))
+        !mul_ok((int64_t)set->n_adapters * set->rank, std::max(K, N) * 4, &t) || !mul_ok(m, slices_of(m, K, false) * ranks4_of(set->rank) * 4, &t))
         return fail(RQ_ERR_SHAPE, "shape overflows");
     if (m == 0 || N == 0) return RQ_OK;
     if (!y || (K > 0 && !x) || !ids) return fail(RQ_ERR_INVALID_ARGUMENT, "null pointer");
@@ -283,7 +427,8 @@ int check_loras(const rq_qweight *w, const rq_lora_set *set, const int32_t *ids,
     p.n = N;
     p.n_adapters = set->n_adapters;
     p.rank = set->rank;
-    p.slices = (int)slices_of(K);
+    p.ranks4 = (int)ranks4_of(set->rank);
+    p.slices = (int)slices_of(m, K, xt == RQ_F16 && set->dtype == RQ_F16);
     // workspace: the shared product in f32, where y is not that already, then the partial sums
     char *ws = static_cast<char *>(workspace);
     p.main = yt == RQ_F32 ? static_cast<float *>(y) : reinterpret_cast<float *>(ws);
@@ -298,43 +443,48 @@ int by_type(int dtype, F f) {
 }
 
 int run_in(const LoraArgs &p, rq_dtype xt, int at, int num_cus, hipStream_t s) {
-    const int64_t tiles = cdiv(p.m, 16);
-    // A tile's adapters side by side while blocks are few.
+    const bool few = p.m <= kFewRows;
+    const int64_t blocks = cdiv(p.m, few ? 16 : 64);
+    // A block's adapters side by side while blocks are few.
     const int64_t z = std::max<int64_t>(
-        1, std::min<int64_t>({16, p.m, (int64_t)p.n_adapters, 4 * num_cus / std::max<int64_t>(1, tiles * p.slices)}));
-    if (!grid_ok(tiles, 256) || p.slices > 65535) return fail(RQ_ERR_SHAPE, "too many rows or inputs for one call");
-    const dim3 grid((unsigned)tiles, (unsigned)p.slices, (unsigned)z);
+        1, std::min<int64_t>({few ? 16 : 64, p.m, (int64_t)p.n_adapters, num_cus / (blocks * p.slices)}));
+    if (!grid_ok(blocks, 256) || p.slices > 65535) return fail(RQ_ERR_SHAPE, "too many rows or inputs for one call");
+    const dim3 grid((unsigned)blocks, (unsigned)p.slices, (unsigned)z);
     const int n = xt == RQ_F16 && at == RQ_F16 ? 8 : 4, xs = xt == RQ_F16 ? 2 : 4, as = at == RQ_F16 ? 2 : 4;
     const bool vec = p.k % n == 0 && aligned(p.x, n * xs) && aligned(p.a, n * as);
     return by_type(xt, [&](auto *x) {
         return by_type(at, [&](auto *a) {
             using X = std::remove_pointer_t<decltype(x)>;
             using A = std::remove_pointer_t<decltype(a)>;
-            if (vec) hipLaunchKernelGGL((k_loras_in<X, A, true>), grid, dim3(256), 0, s, p);
-            else hipLaunchKernelGGL((k_loras_in<X, A, false>), grid, dim3(256), 0, s, p);
+            auto go = [&](auto tm, auto rt) {
+                constexpr int TM = decltype(tm)::value, RT = decltype(rt)::value;
+                if (vec) hipLaunchKernelGGL((k_loras_in<X, A, TM, RT, true>), grid, dim3(256), 0, s, p);
+                else hipLaunchKernelGGL((k_loras_in<X, A, TM, RT, false>), grid, dim3(256), 0, s, p);
+            };
+            using One = std::integral_constant<int, 1>;
+            using Two = std::integral_constant<int, 2>;
+            using Four = std::integral_constant<int, 4>;
+            if (few) p.rank <= 16 ? go(One{}, One{}) : go(One{}, Two{});
+            else p.rank <= 16 ? go(Four{}, One{}) : go(Four{}, Two{});
             RQ_LAUNCH_CHECK();
             return (int)RQ_OK;
         });
     });
 }
 
+// Few rows, or columns that 16-byte pieces do not divide: a row per block; else 16.
 int run_out(const LoraArgs &p, int bt, rq_dtype yt, hipStream_t s) {
-    const bool vec = p.n % 8 == 0 && aligned(p.b, 16) && aligned(p.y, 16);
+    const bool vec = p.n % 8 == 0 && aligned(p.b, 16) && aligned(p.y, 16), rows = p.m <= kFewRows || !vec;
+    const int64_t bx = rows ? p.m : cdiv(p.m, 16), by = cdiv(p.n, rows ? 2048 : 256);
+    if (!grid_ok(bx, 256) || by > 65535) return fail(RQ_ERR_SHAPE, "too many rows or outputs for one call");
+    const dim3 grid((unsigned)bx, (unsigned)by);
     return by_type(bt, [&](auto *b) {
         return by_type(yt, [&](auto *y) {
             using B = std::remove_pointer_t<decltype(b)>;
             using Y = std::remove_pointer_t<decltype(y)>;
-            const bool rows = p.m <= kRowForm;
-            const int64_t bx = rows ? p.m : cdiv(p.m, 16), by = cdiv(p.n, rows ? 2048 : 64 * (16 / (int)sizeof(B)));
-            if (!grid_ok(bx, 256) || by > 65535) return fail(RQ_ERR_SHAPE, "too many rows or outputs for one call");
-            const dim3 grid((unsigned)bx, (unsigned)by);
-            if (rows) {
-                if (vec) hipLaunchKernelGGL((k_loras_out_row<B, Y, true>), grid, dim3(256), 0, s, p);
-                else hipLaunchKernelGGL((k_loras_out_row<B, Y, false>), grid, dim3(256), 0, s, p);
-            } else {
-                if (vec) hipLaunchKernelGGL((k_loras_out<B, Y, true>), grid, dim3(256), 0, s, p);
-                else hipLaunchKernelGGL((k_loras_out<B, Y, false>), grid, dim3(256), 0, s, p);
-            }
+            if (!rows) hipLaunchKernelGGL((k_loras_out<B, Y>), grid, dim3(256), 16 * (out_ranks(p.rank) + 4) * sizeof(float), s, p);
+            else if (vec) hipLaunchKernelGGL((k_loras_out_row<B, Y, true>), grid, dim3(256), 0, s, p);
+            else hipLaunchKernelGGL((k_loras_out_row<B, Y, false>), grid, dim3(256), 0, s, p);
             RQ_LAUNCH_CHECK();
             return (int)RQ_OK;
         });
@@ -350,10 +500,11 @@ extern "C" {
 
 size_t rq_qmatmul_loras_workspace(const rq_lora_set *set, int64_t m, int64_t k_in, int64_t n_out, rq_dtype x_dtype,
                                   rq_dtype y_dtype) {
-    (void)x_dtype;
     int64_t part, main = 0, t;
-    if (check_set(set) != RQ_OK || m < 1 || k_in < 0 || n_out < 1 || !mul_ok(m, slices_of(k_in), &part) ||
-        !mul_ok(part, 4 * set->rank, &part) || !mul_ok(m, n_out, &t) || !mul_ok(t, 4, &t))
+    if (check_set(set) != RQ_OK || m < 1 || k_in < 0 || n_out < 1 ||
+        !mul_ok(m, slices_of(m, k_in, x_dtype == RQ_F16 && set->dtype == RQ_F16), &part) ||
+        !mul_ok(part, 4 * ranks4_of(set->rank), &part) ||
+        !mul_ok(m, n_out, &t) || !mul_ok(t, 4, &t))
         return 0;
     if (y_dtype != RQ_F32) main = (t + 255) / 256 * 256;
     return (size_t)main + (size_t)part;
