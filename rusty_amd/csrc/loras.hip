@@ -31,7 +31,7 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 constexpr int kMaxRank = 256;
 // Rows of a k_loras_in block, in tiles of 16: one tile while rows are few, else four, so that A's rows are read
 // less often.  And its k, a quarter per wave: as much as the registers hold of X and of 32 rows of A.
-constexpr int64_t kFewRows = 64;
+constexpr int64_t kFewRows = 256;
 constexpr int slice(bool f16, int tiles) { return (f16 ? 1024 : 512) / (tiles > 1 ? 2 : 1); }
 
 struct LoraArgs {

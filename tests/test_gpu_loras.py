@@ -102,34 +102,34 @@ TYPES = [("f16", "f16", "f16"), ("f32", "f32", "f32"), ("f16", "f32", "f32"), ("
 
 
 @pytest.mark.parametrize("x_t,y_t,a_t", TYPES)
-@pytest.mark.parametrize("m", [1, 2, 3, 15, 16, 17, 48, 64, 65, 130])
-@pytest.mark.parametrize("rank", [1, 4, 16, 21])
+@pytest.mark.parametrize("m", [1, 2, 3, 15, 16, 17, 48, 64, 65, 256, 257, 330])
+@pytest.mark.parametrize("rank", [1, 4, 16, 21, 40])
 def test_rows_and_ranks(ctx, engine, x_t, y_t, a_t, m, rank):
     case(ctx, engine, m + rank, m, 256, 512, 5, rank, "rowwise8", x_t, y_t, a_t)
 
 
 @pytest.mark.parametrize("x_t,y_t,a_t", TYPES)
 @pytest.mark.parametrize("n,k", [(1, 1), (5, 7), (8, 64), (100, 100), (2056, 1032), (40, 2500), (333, 1024), (4100, 8)])
-@pytest.mark.parametrize("m", [3, 70])
+@pytest.mark.parametrize("m", [3, 70, 270])
 def test_odd_sizes(ctx, engine, x_t, y_t, a_t, n, k, m):
     case(ctx, engine, n + k, m, n, k, 3, 9, "rowwise8", x_t, y_t, a_t)
 
 
 @pytest.mark.parametrize("form", ["rowwise8", "affine8", "affine4"])
-@pytest.mark.parametrize("m", [1, 8, 33, 200])
+@pytest.mark.parametrize("m", [1, 8, 33, 200, 400])
 def test_weights(ctx, engine, form, m):
     case(ctx, engine, m, m, 512, 1024, 6, 16, form, "f16", "f16", "f16")
 
 
 @pytest.mark.parametrize("x_t,y_t,a_t", TYPES)
-@pytest.mark.parametrize("m", [7, 90])
+@pytest.mark.parametrize("m", [7, 90, 300])
 @pytest.mark.parametrize("rank", [16, 100, 256])
 def test_adapters_of_other_ranks(ctx, engine, x_t, y_t, a_t, m, rank):
     """What lies past an adapter's rank is not read; rank 0 adds nothing."""
     case(ctx, engine, rank, m, 136, 264, 9, rank, "rowwise8", x_t, y_t, a_t, some_ranks=True)
 
 
-@pytest.mark.parametrize("m", [20, 100])
+@pytest.mark.parametrize("m", [20, 100, 290])
 @pytest.mark.parametrize("kind", ["one", "none", "foreign", "every", "runs"])
 def test_ids(ctx, engine, m, kind):
     """One adapter, none, numbers of none (below zero, past the set), a new one each row, runs across tiles."""
@@ -139,7 +139,7 @@ def test_ids(ctx, engine, m, kind):
 
 
 @pytest.mark.parametrize("x_t,y_t,a_t", TYPES)
-@pytest.mark.parametrize("m", [16, 80])
+@pytest.mark.parametrize("m", [16, 80, 280])
 def test_foreign_adapters_do_not_reach_a_row(ctx, engine, x_t, y_t, a_t, m):
     """Adapters of infinities and NaN: their rows have them, the others' bits are those without them."""
     g = np.random.default_rng(2)
@@ -155,12 +155,12 @@ def test_foreign_adapters_do_not_reach_a_row(ctx, engine, x_t, y_t, a_t, m):
     assert np.array_equal(got[other], clean[other]) and np.all(np.isnan(got[~other]))
     x[ids == 1] = np.nan  # rows of NaN likewise
     got = run(ctx, engine, x, w, a, b, f, ids, None, x_t, y_t, a_t)
-    if not (x_t == "f32" and 2 < m <= 16):  # (rows of one tile share a power of two there)
+    if not (x_t == "f32" and 2 < m <= 16):  # (the shared product's rows of one tile have a power of two in common there)
         assert np.array_equal(got[other], clean[other])
 
 
 @pytest.mark.parametrize("x_t,y_t,a_t", TYPES)
-@pytest.mark.parametrize("m", [9, 77])
+@pytest.mark.parametrize("m", [9, 77, 273])
 def test_whole_numbers_are_exact(ctx, engine, x_t, y_t, a_t, m):
     """Small whole numbers: every sum is exact, so every value is."""
     g = np.random.default_rng(3)
@@ -218,7 +218,7 @@ def test_graph_and_stream(ctx, engine):
     w, w64 = weight(ctx, g, 256, 512, "rowwise8")
     a, b = adapters(g, 4, 16, 512, 256, "f16")
     s = LoraSet(dev(ctx, a), dev(ctx, b))
-    for m in (5, 100):
+    for m in (5, 100, 300):
         x = g.standard_normal((m, 512)).astype(np.float16)
         X, I = dev(ctx, x), dev(ctx, np.zeros(m, np.int32), DType.I32)
         outs = [dev(ctx, np.zeros((m, 256), np.float16)) for _ in range(2)]
@@ -251,3 +251,33 @@ def test_refusals(ctx, engine):
                 lambda: engine.qmatmul_loras(ctx, X, w, s, I, X)):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("m", [4, 300])
+@pytest.mark.parametrize("exp", [-60, -20, 14, 40])
+def test_large_and_small_products(ctx, engine, m, exp):
+    """x . A_i^T far outside fp16's range, and far below it, in rows side by side: f32 adapters and fp16
+    ones keep f32 accuracy whatever t's magnitude."""
+    g = np.random.default_rng(8)
+    k, n, rank, count = 256, 128, 24, 4
+    w = QuantizedTensor.rowwise(ctx, np.zeros((n, k), np.int8), np.ones(n, np.float32))
+    a, b = adapters(g, count, rank, k, n, "f16")
+    f = np.array([1.0, 2.0 ** exp, 2.0 ** (exp // 2), -1.0], np.float32)
+    x = g.standard_normal((m, k)).astype(np.float16)
+    ids = np.arange(m) % count
+    want, tol = truth(x, np.zeros((n, k)), a, b, f, ids, [rank] * count, "f32", False)
+    check(run(ctx, engine, x, w, a, b, f, ids, None, "f16", "f32", "f16"), want, tol, f"factors 2^{exp}")
+
+
+def test_infinite_products(ctx, engine):
+    """t beyond f32: the row's results are what plain f32 arithmetic gives, infinite, the others' unchanged."""
+    g = np.random.default_rng(9)
+    k, n, m = 64, 64, 300
+    w = QuantizedTensor.rowwise(ctx, np.zeros((n, k), np.int8), np.ones(n, np.float32))
+    a, b = np.ones((2, 8, k), np.float16), np.ones((2, 8, n), np.float16)
+    f = np.array([1.0, 3e38], np.float32)
+    x = np.full((m, k), 4.0, np.float16)
+    ids = np.arange(m) % 2
+    for rows in (m, 8):
+        got = run(ctx, engine, x[:rows], w, a, b, f, ids[:rows], None, "f16", "f32", "f16")
+        assert np.all(got[0::2] == 8 * 256.0) and np.all(got[1::2] == np.inf)
