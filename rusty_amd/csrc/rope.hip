@@ -10,7 +10,9 @@
 // a token share its rot / 2 angles.  A block takes a few whole tokens: it asks
 // for its first elements, forms the tokens' (cos, sin) once into LDS -- the angle
 // in 64 bits, reduced to a fraction of a turn there, then f32 functions -- and turns
-// the elements, up to 16 bytes a load.
+// the elements, 16 bytes a load at any alignment: where a head's parts are no
+// whole number of such pieces, the last one overlaps the one before it, unless the call
+// works in place (4096 tokens of 32 heads of 128, 86 of them turned, fp16: element by element 34 us, so 13.6).
 #include <math.h>
 
 #include <algorithm>
@@ -39,6 +41,7 @@ struct RopeArgs {
     int n_q, n_kv;         // heads of q; APPEND: of k and of v
     int turned, units;     // of a head: units that are turned, all units
     int adjacent;          // V = 1: pairs side by side
+    Div by_token, by_units;  // units of a token, of a head
     float magnitude, sign;
 };
 
@@ -61,12 +64,11 @@ __device__ __forceinline__ int seq_of(const int *starts, int n_seqs, int64_t tok
     return c >= 0 && (past >> (c + 1) & 1) ? lo + c : -1;
 }
 
-// A unit is V consecutive elements (INTER) or V pairs as two vectors (otherwise: of a head's halves; where
-// nothing is aligned V = 1 and, `adjacent`, of two elements side by side); units past `turned` are one vector
-// (INTER) or two side by side, the last maybe one, that are copied.
+// A unit is V consecutive elements (INTER) or V pairs as two vectors (otherwise: of a head's halves; V = 1 and
+// `adjacent`, of two elements side by side).  Units past `turned` are up to V elements that are copied.
 template <typename T, int V, bool INTER, bool APPEND>
 __global__ __launch_bounds__(TH) void k_rope(RopeArgs a) {
-    typedef T vec __attribute__((ext_vector_type(V)));
+    typedef T vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
     extern __shared__ float2 cs[];  // [tokens][rot / 2]
     __shared__ int64_t place[APPEND ? TH : 1];  // a token's offset in the cache; -1: not cached, -2: no sequence
     const int64_t t0 = (int64_t)blockIdx.x * a.per_block;
@@ -77,26 +79,27 @@ __global__ __launch_bounds__(TH) void k_rope(RopeArgs a) {
     const int part = (total + (int)gridDim.y - 1) / (int)gridDim.y;
     const int first = (int)blockIdx.y * part, end = min(first + part, total);
 
+    const int rest = a.hd - a.rot;
     struct Unit {
         int token, head, pair, e0, e1;  // its first pair, the elements of its two vectors; e1 < 0: one vector
-        bool turn;
+        bool turn, part;                // part: fewer than V elements, to the head's end
     };
     auto unit = [&](int u) {
         Unit r;
-        r.token = u / per_token;
+        r.token = a.by_token(u);
         const int w = u - r.token * per_token;
-        r.head = w / a.units;
+        r.head = a.by_units(w);
         const int i = w - r.head * a.units;
         r.turn = i < a.turned;
-        if constexpr (INTER) {
-            r.pair = i * (V / 2);
-            r.e0 = i * V;
+        const bool adjacent = V == 1 && a.adjacent;
+        r.pair = INTER ? min(i * (V / 2), half - V / 2) : min(i * V, half - V);
+        r.e0 = INTER || adjacent ? 2 * r.pair : r.pair;
+        r.e1 = INTER ? -1 : r.e0 + (adjacent ? 1 : half);
+        r.part = false;
+        if (!r.turn) {
+            r.part = rest < V;
+            r.e0 = r.part ? a.rot : a.rot + min((i - a.turned) * V, rest - V);
             r.e1 = -1;
-        } else {
-            const bool adjacent = V == 1 && a.adjacent;
-            r.pair = i * V;
-            r.e0 = r.turn ? (adjacent ? 2 * i : i * V) : a.rot + (i - a.turned) * 2 * V;
-            r.e1 = r.turn ? r.e0 + (adjacent ? 1 : half) : (r.e0 + V < a.hd ? r.e0 + V : -1);
         }
         if (APPEND && r.head >= a.n_q + a.n_kv) r.turn = false;  // v
         return r;
@@ -115,6 +118,12 @@ __global__ __launch_bounds__(TH) void k_rope(RopeArgs a) {
             if (u >= end) break;
             const Unit r = unit(u);
             const T *p = reinterpret_cast<const T *>(source(r));
+            if (V > 1 && r.part) {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (e < rest) x[i][e] = p[r.e0 + e];
+                continue;
+            }
             x[i] = *reinterpret_cast<const vec *>(p + r.e0);
             if constexpr (!INTER)
                 if (r.e1 >= 0) y[i] = *reinterpret_cast<const vec *>(p + r.e1);
@@ -177,6 +186,12 @@ __global__ __launch_bounds__(TH) void k_rope(RopeArgs a) {
                 }
             }
             T *d = reinterpret_cast<T *>(to);
+            if (V > 1 && r.part) {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (e < rest) d[r.e0 + e] = p[e];
+                continue;
+            }
             *reinterpret_cast<vec *>(d + r.e0) = p;
             if constexpr (!INTER)
                 if (r.e1 >= 0) *reinterpret_cast<vec *>(d + r.e1) = q;
@@ -184,26 +199,24 @@ __global__ __launch_bounds__(TH) void k_rope(RopeArgs a) {
     }
 }
 
-// Elements per vector: the widest power of two up to 16 bytes that divides what `bits` holds
-// (the heads, halves and strides in elements, the addresses in elements).
-int width(uint64_t bits, int size) {
-    int v = 16 / size;
-    while (v > 1 && bits % v) v /= 2;
-    return v;
-}
-
+// Launches the kernel over vectors of V elements, up to 16 bytes: of what is turned (HALF: of its half) whole pieces
+// in place, else one at least (the last may overlap).
 template <typename T, bool APPEND>
-int launch(RopeArgs a, bool inter, int v, bool copies, hipStream_t s) {
-    const int half = a.rot / 2, rest = copies ? a.hd - a.rot : 0;
+int launch(RopeArgs a, bool inter, bool in_place, hipStream_t s) {
+    const int half = a.rot / 2, span = inter ? a.rot : half, rest = in_place && !APPEND ? 0 : a.hd - a.rot;
+    int v = 16 / (int)sizeof(T);
+    while (v > 1 && (in_place ? span % v != 0 : span < v)) v /= 2;
     a.adjacent = inter && v == 1;
     if (v == 1) inter = false;
-    a.turned = (inter ? a.rot : half) / v;
-    a.units = a.turned + (inter ? rest / v : (int)cdiv(rest, 2 * v));
+    a.turned = (int)cdiv(inter ? a.rot : half, v);
+    a.units = a.turned + (int)cdiv(rest, v);
     const int64_t heads = APPEND ? a.n_q + 2 * (int64_t)a.n_kv : a.n_q, units = heads * a.units;
     if (units > 0x7fffffff / TH) return fail(RQ_ERR_SHAPE, "too many heads");
     // Tokens per block: a thousand units, as long as that leaves a block for every CU.
     int64_t per = std::max<int64_t>(1, std::min({U * TH / units, (int64_t)kMaxAngles / half, (int64_t)TH, cdiv(a.tokens, 512)}));
     a.per_block = (int)per;
+    a.by_token = Div::by(units);
+    a.by_units = Div::by(a.units);
     const int64_t blocks = cdiv(a.tokens, per);
     // few tokens: a token's units over several blocks
     const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(cdiv(per * units, TH), 512 / blocks));
@@ -252,8 +265,7 @@ void fill_rope(const rq_rope &r, RopeArgs &a) {
 
 // rq_rope_rows' arguments; a is complete where there is work (*run).
 int check_rows(const rq_rope *rope, const void *x, int64_t x_row, const int32_t *positions, int64_t tokens,
-               int32_t n_heads, rq_dtype dtype, const void *out, int64_t out_row, unsigned flags, RopeArgs &a, int &v,
-               bool &run) {
+               int32_t n_heads, rq_dtype dtype, const void *out, int64_t out_row, unsigned flags, RopeArgs &a, bool &run) {
     run = false;
     const int st = check_rope(rope);
     if (st != RQ_OK) return st;
@@ -280,10 +292,6 @@ int check_rows(const rq_rope *rope, const void *x, int64_t x_row, const int32_t 
     a.tokens = tokens;
     a.n_q = n_heads;
     if (flags & RQ_ROPE_BACKWARD) a.sign = -1.0f;
-    const uint64_t pair = rope->layout == RQ_ROPE_INTERLEAVED ? rope->rot_dim : rope->rot_dim / 2;
-    v = width(pair | (uint64_t)rope->head_dim | (uint64_t)xr | (uint64_t)orow | reinterpret_cast<uintptr_t>(x) / size |
-                  reinterpret_cast<uintptr_t>(out) / size,
-              size);
     run = true;
     return RQ_OK;
 }
@@ -291,7 +299,7 @@ int check_rows(const rq_rope *rope, const void *x, int64_t x_row, const int32_t 
 // rq_rope_append's arguments likewise.
 int check_append(const rq_rope *rope, const rq_attn *attn, const rq_kv_pages *cache, const void *q, const void *k,
                  const void *v, const int32_t *starts, const int32_t *positions, int64_t tokens, const void *out,
-                 RopeArgs &a, int &vw, bool &run) {
+                 RopeArgs &a, bool &run) {
     run = false;
     int st = check_rope(rope);
     if (st != RQ_OK) return st;
@@ -323,8 +331,6 @@ int check_append(const rq_rope *rope, const rq_attn *attn, const rq_kv_pages *ca
     a.tokens = tokens;
     a.n_q = attn->n_heads;
     a.n_kv = attn->n_kv_heads;
-    // (heads, rows and strides are multiples of 16 bytes)
-    vw = width(rope->layout == RQ_ROPE_INTERLEAVED ? rope->rot_dim : rope->rot_dim / 2, size);
     run = true;
     return RQ_OK;
 }
@@ -373,13 +379,12 @@ int rq_rope_rows(rq_ctx *ctx, const rq_rope *rope, const void *x, int64_t x_row,
                  rq_stream stream) {
     RQ_ENTER(ctx);
     RopeArgs a{};
-    int v = 1;
     bool run;
-    const int st = check_rows(rope, x, x_row, positions, tokens, n_heads, dtype, out, out_row, flags, a, v, run);
+    const int st = check_rows(rope, x, x_row, positions, tokens, n_heads, dtype, out, out_row, flags, a, run);
     if (st != RQ_OK || !run) return st;
-    const bool inter = rope->layout == RQ_ROPE_INTERLEAVED, copies = x != out;
+    const bool inter = rope->layout == RQ_ROPE_INTERLEAVED, in_place = x == out;
     hipStream_t s = pick(ctx, stream);
-    return dtype == RQ_F16 ? launch<_Float16, false>(a, inter, v, copies, s) : launch<float, false>(a, inter, v, copies, s);
+    return dtype == RQ_F16 ? launch<_Float16, false>(a, inter, in_place, s) : launch<float, false>(a, inter, in_place, s);
 }
 
 int rq_rope_append(rq_ctx *ctx, const rq_rope *rope, const rq_attn *attn, const rq_kv_pages *cache, const void *q,
@@ -387,13 +392,12 @@ int rq_rope_append(rq_ctx *ctx, const rq_rope *rope, const rq_attn *attn, const 
                    void *out, rq_stream stream) {
     RQ_ENTER(ctx);
     RopeArgs a{};
-    int vw = 1;
     bool run;
-    const int st = check_append(rope, attn, cache, q, k, v, starts, positions, tokens, out, a, vw, run);
+    const int st = check_append(rope, attn, cache, q, k, v, starts, positions, tokens, out, a, run);
     if (st != RQ_OK || !run) return st;
-    const bool inter = rope->layout == RQ_ROPE_INTERLEAVED;
+    const bool inter = rope->layout == RQ_ROPE_INTERLEAVED, in_place = q == out;
     hipStream_t s = pick(ctx, stream);
-    return attn->dtype == RQ_F16 ? launch<_Float16, true>(a, inter, vw, true, s) : launch<float, true>(a, inter, vw, true, s);
+    return attn->dtype == RQ_F16 ? launch<_Float16, true>(a, inter, in_place, s) : launch<float, true>(a, inter, in_place, s);
 }
 
 // For the tests, no part of the C ABI: the argument checks alone (attn NULL: rq_rope_rows').  Host arithmetic.
@@ -401,10 +405,9 @@ int rusty_rope_check(const rq_rope *rope, const rq_attn *attn, const rq_kv_pages
                      const void *v, int64_t x_row, const int32_t *starts, const int32_t *positions, int64_t tokens,
                      int32_t n_heads, int dtype, const void *out, int64_t out_row, unsigned flags) {
     RopeArgs a{};
-    int w = 1;
     bool run;
-    return attn ? check_append(rope, attn, cache, q, k, v, starts, positions, tokens, out, a, w, run)
-                : check_rows(rope, q, x_row, positions, tokens, n_heads, (rq_dtype)dtype, out, out_row, flags, a, w, run);
+    return attn ? check_append(rope, attn, cache, q, k, v, starts, positions, tokens, out, a, run)
+                : check_rows(rope, q, x_row, positions, tokens, n_heads, (rq_dtype)dtype, out, out_row, flags, a, run);
 }
 
 }  // extern "C"
