@@ -22,9 +22,9 @@ def get(ctx, base, offset, shape):
 
 
 @pytest.mark.parametrize("n_pages,page,strides", [(40000, 512, (0, 0, 0)), (3, 16, (1 << 31, 1 << 29, 1 << 24)),
-                                                  (3, 64, (128, 64, 1 << 25))], ids=["far pages", "far rows", "pages within rows"])
+                                                  (3, 64, (128, 64, 1 << 26))], ids=["far pages", "far rows", "pages within rows"])
 def test_far(ctx, engine, n_pages, page, strides):
-    """A pool of 5 GiB of K (V beside it in the same memory): the last page and others past 4 GiB."""
+    """A pool of 4 to 8 GiB (K and V in one memory): the last page, or its last rows, lie past 4 GiB."""
     kv, dim = 2, 64
     ps, hs, xs = strides if any(strides) else (page * kv * dim, page * dim, dim)
     size = 2 * ((n_pages - 1) * ps + (kv - 1) * hs + (page - 1) * xs + dim)
