@@ -29,8 +29,8 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxRank = 256;
-// Rows of a k_loras_in block, in tiles of 16: one tile while rows are few, else four, so that A's rows are read
-// less often.  And its k, a quarter per wave: as much as the registers hold of X and of 32 rows of A.
+// Rows of a k_loras_in block, in tiles of 16: one tile while rows are few, else two, so that A's rows are read
+// less often (2048 rows, rank 32: one 12.6 us, two 9.4, four 10.6).  And its k, a quarter per wave: as much as the registers hold of X and of 32 rows of A.
 constexpr int64_t kFewRows = 256;
 constexpr int slice(bool f16, int tiles) { return (f16 ? 1024 : 512) / (tiles > 1 ? 2 : 1); }
 
@@ -194,7 +194,8 @@ __global__ __launch_bounds__(256) void k_loras_out_row(LoraArgs p) {
 // that a lane gets 16 columns side by side of one row (row i of instruction v is column 16 (i / 4) + 4 v + i % 4).
 // Bound by the shared product's way in and Y's out.  A load that is waited for alone costs 1 to 2 us here, so all
 // that a tile with one adapter of up to 32 ranks reads is asked for together, and what B and the shared product take
-// waits in LDS (DMA): few registers, many waves.  Further adapters and ranks take turns with two buffers of 32 (f32 B: 16) ranks.
+// waits in LDS (DMA): few registers, many waves.  B's buffers hold 32 ranks (f32 B: 16); with more ranks there are two,
+// else further adapters wait for their turn with one (2048 x 11008, rank 16: two buffers 45 us, one 40).
 // fp16 B: t, scaled by a power of two per row, is two fp16 terms (off by at most 2^-22), two instructions of 32 ranks
 // a 16 columns, B's fragments by transposing LDS reads; f32 instructions of 4 ranks took 3 us longer at 2048 x 4096, rank 32.
 __host__ __device__ constexpr int out_ranks(int rank) { return (rank + 31) / 32 * 32; }
@@ -206,11 +207,12 @@ __global__ __launch_bounds__(256) void k_loras_out(LoraArgs p) {
     typedef short short4v __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) short4v lds_short4;
     __shared__ __attribute__((aligned(16))) floatx4 main[4][16][16];       // [wave][row][16-byte piece ^ row]
-    __shared__ __attribute__((aligned(16))) B bs[4][2][R][64];             // [wave][buffer][rank][column]
-    extern __shared__ __attribute__((aligned(16))) float ts[];             // [16][out_ranks + 4]: t, fp16 B: its two terms side by side
+    // [16][out_ranks + 4]: t, fp16 B: its two terms side by side; then B [wave][buffer][rank][column]
+    extern __shared__ __attribute__((aligned(16))) float ts[];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, col = lane & 15, qt = lane >> 4;
     const int64_t t0 = (int64_t)blockIdx.x * 16, c0 = ((int64_t)blockIdx.y * 4 + wv) * 64;
-    const int ranks = out_ranks(p.rank), row4 = ranks + 4;
+    const int ranks = out_ranks(p.rank), row4 = ranks + 4, buffers = p.rank > R ? 2 : 1;
+    B *bs = reinterpret_cast<B *>(ts + 16 * row4) + wv * buffers * (R * 64);
     int mine = t0 + col < p.m ? adapter_of(p, t0 + col) : -1;
     asm volatile("" : "+v"(mine));  // (waited for here: later the wait would be for the DMA, too)
     const uint64_t all = __builtin_amdgcn_ballot_w64(lane < 16 && mine >= 0);
@@ -238,7 +240,7 @@ __global__ __launch_bounds__(256) void k_loras_out(LoraArgs p) {
 #pragma unroll
         for (int u = 0; u < UN; ++u)
             dma16_kept(reinterpret_cast<const char *>(b + (int64_t)min(s.r0 + u * RPU + lane / CH, max(s.rank - 1, 0)) * p.n),
-                       lds_addr(&bs[wv][buffer][u * RPU][0]));
+                       lds_addr(bs + (buffer * R + u * RPU) * 64));
     };
     Step s = adapter(all);
     if (all) fetch(s, 0);
@@ -304,7 +306,7 @@ __global__ __launch_bounds__(256) void k_loras_out(LoraArgs p) {
     wait_vmcnt<0>();
     for (int k = 0; s.same; ++k) {
         const Step next = after(s);
-        if (next.same) {
+        if (next.same && buffers == 2) {
             wait_lgkm0();  // (the buffer has been read)
             fetch(next, (k + 1) & 1);
             if (k > 0) wait_vmcnt<UN>();
@@ -312,14 +314,14 @@ __global__ __launch_bounds__(256) void k_loras_out(LoraArgs p) {
             wait_vmcnt<0>();
         }
         const int count = min(s.rank - s.r0, R);  // of these ranks, those that the adapter has
-        const B *b = &bs[wv][k & 1][0][0];
+        B *b = bs + (buffers == 2 ? k & 1 : 0) * (R * 64);
         if constexpr (F16) {
             if (count < R) {
                 // (what lies past the rank is another rank's, and may be infinite)
 #pragma unroll
                 for (int u = 0; u < UN; ++u)
                     if (u * RPU + lane / CH >= count)
-                        *reinterpret_cast<half8 *>(&bs[wv][k & 1][u * RPU + lane / CH][lane % CH * 8]) = half8{};
+                        *reinterpret_cast<half8 *>(b + (u * RPU + lane / CH) * 64 + lane % CH * 8) = half8{};
                 wait_lgkm0();
             }
             const half8 *t = reinterpret_cast<const half8 *>(ts + col * row4 + s.r0 + 8 * qt);
@@ -358,6 +360,10 @@ __global__ __launch_bounds__(256) void k_loras_out(LoraArgs p) {
                 acc[v] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
             }
         }
+        if (next.same && buffers == 1) {
+            wait_lgkm0();
+            fetch(next, 0);
+        }
         s = next;
     }
     const int64_t t = t0 + col, c = c0 + 16 * qt;
@@ -387,7 +393,7 @@ int check_set(const rq_lora_set *s) {
     return RQ_OK;
 }
 
-int64_t slices_of(int64_t m, int64_t k, bool f16) { return std::max<int64_t>(1, cdiv(k, slice(f16, m > kFewRows ? 4 : 1))); }
+int64_t slices_of(int64_t m, int64_t k, bool f16) { return std::max<int64_t>(1, cdiv(k, slice(f16, m > kFewRows ? 2 : 1))); }
 int64_t ranks4_of(int rank) { return (rank + 3) / 4 * 4; }
 
 int check_loras(const rq_qweight *w, const rq_lora_set *set, const int32_t *ids, const void *x, rq_dtype xt, void *y,
@@ -444,10 +450,10 @@ int by_type(int dtype, F f) {
 
 int run_in(const LoraArgs &p, rq_dtype xt, int at, int num_cus, hipStream_t s) {
     const bool few = p.m <= kFewRows;
-    const int64_t blocks = cdiv(p.m, few ? 16 : 64);
+    const int64_t blocks = cdiv(p.m, few ? 16 : 32);
     // A block's adapters side by side while blocks are few.
     const int64_t z = std::max<int64_t>(
-        1, std::min<int64_t>({few ? 16 : 64, p.m, (int64_t)p.n_adapters, num_cus / (blocks * p.slices)}));
+        1, std::min<int64_t>({few ? 16 : 32, p.m, (int64_t)p.n_adapters, num_cus / (blocks * p.slices)}));
     if (!grid_ok(blocks, 256) || p.slices > 65535) return fail(RQ_ERR_SHAPE, "too many rows or inputs for one call");
     const dim3 grid((unsigned)blocks, (unsigned)p.slices, (unsigned)z);
     const int n = xt == RQ_F16 && at == RQ_F16 ? 8 : 4, xs = xt == RQ_F16 ? 2 : 4, as = at == RQ_F16 ? 2 : 4;
@@ -463,9 +469,8 @@ int run_in(const LoraArgs &p, rq_dtype xt, int at, int num_cus, hipStream_t s) {
             };
             using One = std::integral_constant<int, 1>;
             using Two = std::integral_constant<int, 2>;
-            using Four = std::integral_constant<int, 4>;
             if (few) p.rank <= 16 ? go(One{}, One{}) : go(One{}, Two{});
-            else p.rank <= 16 ? go(Four{}, One{}) : go(Four{}, Two{});
+            else p.rank <= 16 ? go(Two{}, One{}) : go(Two{}, Two{});
             RQ_LAUNCH_CHECK();
             return (int)RQ_OK;
         });
@@ -482,7 +487,9 @@ int run_out(const LoraArgs &p, int bt, rq_dtype yt, hipStream_t s) {
         return by_type(yt, [&](auto *y) {
             using B = std::remove_pointer_t<decltype(b)>;
             using Y = std::remove_pointer_t<decltype(y)>;
-            if (!rows) hipLaunchKernelGGL((k_loras_out<B, Y>), grid, dim3(256), 16 * (out_ranks(p.rank) + 4) * sizeof(float), s, p);
+            const int r = sizeof(B) == 2 ? 32 : 16;
+            const size_t lds = 16 * (out_ranks(p.rank) + 4) * sizeof(float) + (p.rank > r ? 2 : 1) * (size_t)(4 * r * 64) * sizeof(B);
+            if (!rows) hipLaunchKernelGGL((k_loras_out<B, Y>), grid, dim3(256), lds, s, p);
             else if (vec) hipLaunchKernelGGL((k_loras_out_row<B, Y, true>), grid, dim3(256), 0, s, p);
             else hipLaunchKernelGGL((k_loras_out_row<B, Y, false>), grid, dim3(256), 0, s, p);
             RQ_LAUNCH_CHECK();
