@@ -15,14 +15,24 @@
 // units of KT (a sequence has at least one), laid one behind another, are dealt
 // out in equal runs to as many blocks as the device holds at once, so a batch of one
 // long and many short sequences fills it.  The lengths are on the device, so
-// every block finds its run from them (a wave sums them).  A block
-// takes the parts of its run, one sequence each, in turn; its four waves
-// take quarters of a part and join through LDS; a sequence that ends in another
-// block than it began leaves partial sums that k_paged_join joins.
+// every block finds its run from them (a wave scans them).  A block deals the parts
+// of its run, one sequence each, to its eight waves, which join through LDS; a
+// sequence that several blocks have parts of is joined by the one that arrives
+// last (the context's counters, on its own stream), or by a launch of its own.
 //
-// Each wave streams its keys through a ring of its own in LDS (DMA, two units,
-// no block barrier): the pages' entries lie in its lanes, 64 at a time, and each lane
-// forms the address of its own 16 bytes, so pages may be of any size and order.
+// Each wave streams its units through a place of its own in LDS (DMA, no block
+// barrier needed), K's next unit under way as soon as K has been read, V's as V
+// has.  The pages' entries lie in a wave's lanes, 64 at a time; the rows of a DMA
+// instruction share a page and their address is formed on the scalar unit, but for pages
+// smaller than that.
+//
+// Times (us; the bytes at the rate of a plain read of as much, 6.9 TB/s): six sequences
+// of up to 32701 keys, 32/8 heads of 128, 67 (55); f32, seven of up to 3001, 16/16 heads of 128, 25.8
+// (16); 48 chats of 37 to 2047 keys, 32/4 heads of 64, 12.5 (3.6); one of 513 7.2.  What is left is
+// latency: about 1 us each for the launch, the lengths, a page's entry, the first keys, and 3 for a join (the
+// stores' acknowledgement, the counter, the pieces); and that blocks of one size are not done at one time (the
+// first of six long sequences' at 50 us, the last at 61).  Loads that leave the caches alone (nt) took 10 % off the
+// long calls, one block of eight waves per CU over two of four 2 %, waves in step (s_barrier) 3 %.
 #include <math.h>
 
 #include <algorithm>
@@ -40,6 +50,7 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int64_t kCus = 256;
+constexpr int kMaxSeqs = 65536;  // (every block scans the lengths)
 constexpr int kCounterStride = 32;  // of the context's arrival counters, a line each
 
 struct PagedArgs {
@@ -607,26 +618,22 @@ __global__ __launch_bounds__(TH, NW * blocks_per_cu(HD) / 4) void k_attn_paged(P
     }
 }
 
-// The same in a launch of its own, where the context's counters may not be used: one wave per (sequence, head).
+// The same in a launch of its own, where the context's counters may not be used: block (four heads, run b + 1) joins
+// the sequence that is cut where that run begins, if it is not cut before.  One wave per head.
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a) {
-    constexpr int KT = PShape<T, HD>::KT, L = HD / 4, G = 64 / L;  // lanes of a piece, pieces side by side
-    const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (row >= (int64_t)a.pages.n_seqs * a.n_heads) return;
-    const int s = (int)(row / a.n_heads), head = (int)(row - (int64_t)s * a.n_heads), lane = threadIdx.x & 63;
-    int all = 0, before = 0;
-    for (int i = lane; i < a.pages.n_seqs; i += 64) {
-        const int u = units_of<KT>(clamped(a, i));
-        all += u;
-        before += i < s ? u : 0;
-    }
-    const int total = __builtin_amdgcn_readlane(scan_add(all), 63), t0 = __builtin_amdgcn_readlane(scan_add(before), 63);
-    const int len = run_length(a, total), t1 = t0 + units_of<KT>(clamped(a, s));
-    const int b0 = t0 / len, pieces = (t1 - 1) / len - b0 + 1;
-    if (pieces <= 1 || t1 - t0 <= whole_units(len)) return;  // written by the block that had them all
+    constexpr int L = HD / 4, G = 64 / L;  // lanes of a piece, pieces side by side
+    const int head = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), b = blockIdx.y, lane = threadIdx.x & 63;
+    if (head >= a.n_heads) return;
+    const Where<T, HD> where(a, b + 1);
+    if (where.none) return;
+    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(where.end > where.x0) | 1ull << 63);
+    const int begin = __builtin_amdgcn_readlane(where.begin, l), end = __builtin_amdgcn_readlane(where.end, l);
+    if (begin >= where.x0 || begin / where.len != b || end - begin <= whole_units(where.len)) return;
+    const int pieces = (end - 1) / where.len - b + 1;
     const int gi = lane / L, at = 4 * (lane % L);
     Joined j;
-    j.read<HD>(a, part_rsrc(a, HD), b0, pieces, head, at, gi, G);
+    j.read<HD>(a, part_rsrc(a, HD), b, pieces, head, at, gi, G);
 #pragma unroll
     for (int w = 32; w >= L; w >>= 1) {
         floatx4 o;
@@ -635,7 +642,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a) {
         const float m = __shfl_xor(j.top, w), l = __shfl_xor(j.l, w);
         j.add(m, l, o, j.rise(m));
     }
-    if (gi == 0) write_out<T>(a, s, (int64_t)head * HD + at, j.top, j.l, j.o);
+    if (gi == 0) write_out<T>(a, where.base + l, (int64_t)head * HD + at, j.top, j.l, j.o);
 }
 
 // Blocks that the units are dealt to, per key/value head and 16 rows: as many as the device holds at once.
@@ -646,8 +653,7 @@ int paged_runs(int n_heads, int n_kv, int head_dim) {
 template <typename T, int HD>
 int launch(PagedArgs a, hipStream_t s) {
     using SH = PShape<T, HD>;
-    const int64_t rows = cdiv((int64_t)a.pages.n_seqs * a.n_heads, 4);
-    if (!grid_ok(a.n_kv, TH) || a.rbs > 65535 || !grid_ok(rows, 256)) return fail(RQ_ERR_SHAPE, "too many rows for one call");
+    // (n_kv and n_heads are at most 65536, rbs 4096, runs 512)
     a.by_runs = Div::by(a.runs);
     const dim3 grid((unsigned)a.n_kv, (unsigned)a.rbs, (unsigned)a.runs);
     // (offsets within a page and within the rows of a DMA instruction in 32 bits)
@@ -658,7 +664,7 @@ int launch(PagedArgs a, hipStream_t s) {
         hipLaunchKernelGGL((k_attn_paged<T, HD, false>), grid, dim3(TH), 0, s, a);
     RQ_LAUNCH_CHECK();
     if (a.runs > 1 && !a.counters) {
-        hipLaunchKernelGGL((k_paged_join<T, HD>), dim3((unsigned)rows), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_paged_join<T, HD>), dim3((unsigned)cdiv(a.n_heads, 4), (unsigned)a.runs - 1), dim3(256), 0, s, a);
         RQ_LAUNCH_CHECK();
     }
     return RQ_OK;
@@ -673,6 +679,7 @@ int check_paged(const rq_attn *attn, const rq_kv_pages *cache, const void *q, co
     if (st != RQ_OK) return st;
     if ((st = check_pages(cache, attn, &a.pages)) != RQ_OK) return st;
     if (cache->n_seqs == 0) return RQ_OK;
+    if (cache->n_seqs > kMaxSeqs) return fail(RQ_ERR_SHAPE, "more than %d sequences in one call", kMaxSeqs);
     if (!q || !lengths || !out) return fail(RQ_ERR_INVALID_ARGUMENT, "null pointer");
     if (!aligned(q, 16) || !aligned(out, 16) || !aligned(lengths, 4))
         return fail(RQ_ERR_UNSUPPORTED, "pointers must be 16-byte aligned");

@@ -7,15 +7,21 @@
 // once.  Small batches are bound by the launches and by the weight's bytes, which
 // each used adapter adds (k_in + n_out) rank elements to; prompts by the shared product.
 //
-// k_loras_in: 16 rows of X are the rows of a matrix instruction, 16 rows of A_i its
+// k_loras_in: rows of X are the rows of a matrix instruction, 16 rows of A_i its
 // columns, k runs along both (16-byte loads, no LDS).  Rows of a tile may have
-// different adapters: each one's product is formed for all 16 rows and
+// different adapters: each one's product is formed for all its rows and
 // kept for its own, so nothing a foreign adapter holds reaches a row.
 //
 // k_loras_out has two forms.  Few rows: a block takes one row and a stretch of
 // columns, its lanes 8 columns each, the adapter's rank one fma at a time -- no work
-// on foreign rows.  Many: a wave takes 16 rows and 16 V columns on the f32 matrix
-// instructions (t keeps its f32 bits), a B fragment of V columns a load.
+// on foreign rows.  Many: a wave takes 16 rows and 64 columns on the matrix
+// instructions, an adapter of theirs after another (f32 B: f32 instructions; fp16 B:
+// t as two fp16 terms).
+//
+// Measured (us, 4096 x 4096; X . A / shared product / t . B; the bytes at 6.9 TB/s, the products at 1157
+// TFLOP/s): one row, 8-bit rows, rank 16: 3.3 / 4.7 / 2.7 (2.5); 61 rows of 11 adapters, 4-bit groups,
+// f32 rows, rank 32: 5.0 / 16.8 / 3.9 (4.9); 2048 rows, 8-bit, rank 32: 9.4 / 66 / 18.9 (60).  One launch for X . A and
+// the shared product of a few rows took 8 us where the two take 6.1.
 #include <algorithm>
 #include <type_traits>
 
@@ -29,9 +35,13 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxRank = 256;
-// Rows of a k_loras_in block, in tiles of 16: one tile while rows are few, else two, so that A's rows are read
-// less often (2048 rows, rank 32: one 12.6 us, two 9.4, four 10.6).  And its k, a quarter per wave: as much as the registers hold of X and of 32 rows of A.
+constexpr int kMaxSide = 65535 * 256;  // m, k_in, n_out
+// Up to so many rows k_loras_in takes one tile of 16 rows a block (more blocks), else two, so that A's rows are
+// read less often (2048 rows, rank 32: one 12.6 us, two 9.4, four 10.6), and the output a row a block, else 16:
+// 4096 x 4096, all three launches, row / tile: 128 rows of 64 adapters of rank 16 23.7 / 35.7 us, of one 20.3 / 21.8;
+// 256 of 64 32.2 / 43.3, of one 24.6 / 25.7, of rank 64 32.4 / 29.5; 512 of one 35.6 / 35.9, of rank 64 46.6 / 40.4.
 constexpr int64_t kFewRows = 256;
+// A block's k, a quarter per wave: as much as the registers hold of X and of 32 rows of A.
 constexpr int slice(bool f16, int tiles) { return (f16 ? 1024 : 512) / (tiles > 1 ? 2 : 1); }
 
 struct LoraArgs {
@@ -269,7 +279,7 @@ __global__ __launch_bounds__(256) void k_loras_out(LoraArgs p) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     v[e] = r + e < rank ? f * v[e] : 0.0f;
-                    most = fmaxf(most, fabsf(v[e]));
+                    most = fmaxf(most, __builtin_isfinite(v[e]) ? fabsf(v[e]) : 0.0f);
                 }
                 *reinterpret_cast<floatx4 *>(to + r) = v;
             }
@@ -277,8 +287,8 @@ __global__ __launch_bounds__(256) void k_loras_out(LoraArgs p) {
         if constexpr (F16) {
 #pragma unroll
             for (int w = 1; w < 16; w <<= 1) most = fmaxf(most, __shfl_xor(most, w));
-            // the largest in [2^14, 2^15) (a row of zeros, or that is not finite, as it is)
-            const int e = most > 0.0f && most < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+            // the largest that is finite in [2^14, 2^15)
+            const int e = most > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
             if (u == 0) to[ranks] = __builtin_ldexpf(1.0f, -e);
             if (i >= 0)
                 for (int r = 4 * u; r < ranks; r += 64) {
@@ -404,12 +414,11 @@ int check_loras(const rq_qweight *w, const rq_lora_set *set, const int32_t *ids,
     if ((st = check_set(set)) != RQ_OK) return st;
     if ((xt != RQ_F16 && xt != RQ_F32) || (yt != RQ_F16 && yt != RQ_F32))
         return fail(RQ_ERR_INVALID_ARGUMENT, "dtype must be RQ_F16 or RQ_F32");
-    if (m < 0 || m > 0x7fffffff) return fail(RQ_ERR_SHAPE, "m outside 0..2^31-1");
     const int64_t K = w->k_in, N = w->n_out;
+    // (every grid fits, and every size 64 bits)
+    if (m < 0 || m > kMaxSide || K > kMaxSide || N > kMaxSide) return fail(RQ_ERR_SHAPE, "m, k_in and n_out go up to %d", kMaxSide);
     int64_t t;
-    if (!mul_ok(m, K * 4, &t) || !mul_ok(m, N * 4, &t) || K > ((int64_t)1 << 40) || N > ((int64_t)1 << 40) ||
-        !mul_ok((int64_t)set->n_adapters * set->rank, std::max(K, N) * 4, &t) || !mul_ok(m, slices_of(m, K, false) * ranks4_of(set->rank) * 4, &t))
-        return fail(RQ_ERR_SHAPE, "shape overflows");
+    if (!mul_ok((int64_t)set->n_adapters * set->rank, std::max(K, N) * 4, &t)) return fail(RQ_ERR_SHAPE, "shape overflows");
     if (m == 0 || N == 0) return RQ_OK;
     if (!y || (K > 0 && !x) || !ids) return fail(RQ_ERR_INVALID_ARGUMENT, "null pointer");
     if (set->n_adapters > 0 && ((K > 0 && !set->a) || !set->b)) return fail(RQ_ERR_INVALID_ARGUMENT, "null adapter pointer");
@@ -454,7 +463,6 @@ int run_in(const LoraArgs &p, rq_dtype xt, int at, int num_cus, hipStream_t s) {
     // A block's adapters side by side while blocks are few.
     const int64_t z = std::max<int64_t>(
         1, std::min<int64_t>({few ? 16 : 32, p.m, (int64_t)p.n_adapters, num_cus / (blocks * p.slices)}));
-    if (!grid_ok(blocks, 256) || p.slices > 65535) return fail(RQ_ERR_SHAPE, "too many rows or inputs for one call");
     const dim3 grid((unsigned)blocks, (unsigned)p.slices, (unsigned)z);
     const int n = xt == RQ_F16 && at == RQ_F16 ? 8 : 4, xs = xt == RQ_F16 ? 2 : 4, as = at == RQ_F16 ? 2 : 4;
     const bool vec = p.k % n == 0 && aligned(p.x, n * xs) && aligned(p.a, n * as);
@@ -481,7 +489,6 @@ int run_in(const LoraArgs &p, rq_dtype xt, int at, int num_cus, hipStream_t s) {
 int run_out(const LoraArgs &p, int bt, rq_dtype yt, hipStream_t s) {
     const bool vec = p.n % 8 == 0 && aligned(p.b, 16) && aligned(p.y, 16), rows = p.m <= kFewRows || !vec;
     const int64_t bx = rows ? p.m : cdiv(p.m, 16), by = cdiv(p.n, rows ? 2048 : 256);
-    if (!grid_ok(bx, 256) || by > 65535) return fail(RQ_ERR_SHAPE, "too many rows or outputs for one call");
     const dim3 grid((unsigned)bx, (unsigned)by);
     return by_type(bt, [&](auto *b) {
         return by_type(yt, [&](auto *y) {
@@ -507,14 +514,10 @@ extern "C" {
 
 size_t rq_qmatmul_loras_workspace(const rq_lora_set *set, int64_t m, int64_t k_in, int64_t n_out, rq_dtype x_dtype,
                                   rq_dtype y_dtype) {
-    int64_t part, main = 0, t;
-    if (check_set(set) != RQ_OK || m < 1 || k_in < 0 || n_out < 1 ||
-        !mul_ok(m, slices_of(m, k_in, x_dtype == RQ_F16 && set->dtype == RQ_F16), &part) ||
-        !mul_ok(part, 4 * ranks4_of(set->rank), &part) ||
-        !mul_ok(m, n_out, &t) || !mul_ok(t, 4, &t))
-        return 0;
-    if (y_dtype != RQ_F32) main = (t + 255) / 256 * 256;
-    return (size_t)main + (size_t)part;
+    if (check_set(set) != RQ_OK || m < 1 || k_in < 0 || n_out < 1 || m > kMaxSide || k_in > kMaxSide || n_out > kMaxSide) return 0;
+    const int64_t part = m * slices_of(m, k_in, x_dtype == RQ_F16 && set->dtype == RQ_F16) * 4 * ranks4_of(set->rank);
+    const int64_t main = y_dtype != RQ_F32 ? (m * n_out * 4 + 255) / 256 * 256 : 0;
+    return (size_t)(main + part);
 }
 
 int rq_qmatmul_loras(rq_ctx *ctx, const rq_qweight *w, const rq_lora_set *set, const int32_t *ids, const void *x,

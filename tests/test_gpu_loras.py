@@ -281,3 +281,16 @@ def test_infinite_products(ctx, engine):
     for rows in (m, 8):
         got = run(ctx, engine, x[:rows], w, a, b, f, ids[:rows], None, "f16", "f32", "f16")
         assert np.all(got[0::2] == 8 * 256.0) and np.all(got[1::2] == np.inf)
+
+
+@pytest.mark.parametrize("m", [8, 300])
+def test_infinite_beside_large(ctx, engine, m):
+    """A t with an infinite entry (one rank's sum is past f32) and entries past fp16's range: columns where the
+    infinite entry's B is 1 are infinite, whatever the sign of the finite one's, and no NaN appears."""
+    k, n = 64, 64
+    w = QuantizedTensor.rowwise(ctx, np.zeros((n, k), np.int8), np.ones(n, np.float32))
+    a, b = np.full((1, 2, k), 6e4, np.float16), np.ones((1, 2, n), np.float16)
+    a[0, 1], b[0, 1, ::2] = 1e-3, -1.0
+    x = np.full((m, k), 1e34, np.float32)  # 1e34 6e4 > 3.4e38 > 64 1e34 1e-3 > 65504
+    got = run(ctx, engine, x, w, a, b, None, np.zeros(m, int), None, "f32", "f32", "f16")
+    assert np.all(got == np.inf)

@@ -3,7 +3,7 @@ derived in test_gpu_attn.py (the same arithmetic, the keys in pages)."""
 import numpy as np
 import pytest
 
-from rusty_amd import DType, PagedCache, UnifiedTensor
+from rusty_amd import DType, PagedCache, QuantizedTensor, UnifiedTensor
 from rusty_amd._lib import call
 from rusty_amd.hiprt import Graph, Stream
 from test_gpu_attn import KIND, attend, check
@@ -293,3 +293,38 @@ def test_on_a_callers_stream(ctx, engine, dtype, heads, kv, dim, lengths, page):
         engine.attn_paged(ctx, Q, cache, L, out, workspace=work, stream=stream.h)
         stream.synchronize()
         check(out.to_vec(), want, tol, f"caller's stream {lengths} {dtype}")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_graphs_on_the_contexts_stream(ctx, engine, dtype):
+    """Two calls captured on the context's own stream, whose cut sequences are joined through the context's counters,
+    with workspaces of their own: replayed in turn, with a product that uses the same counters and eager calls between."""
+    n = [4000, 40, 2500]
+    q, pools, table, rows = make(14, n, 8, 2, 64, 16, "heads", dtype)
+    kind = KIND[dtype][1]
+    cache = PagedCache(dev(ctx, pools[0], kind), dev(ctx, pools[1], kind), dev(ctx, table, DType.I32))
+    Q, L = dev(ctx, q, kind), dev(ctx, np.zeros(3, np.int32), DType.I32)
+    outs = [dev(ctx, np.full(q.shape, 7.0), kind) for _ in range(3)]
+    works = [engine.attn_paged_workspace(ctx, Q, cache) for _ in range(3)]
+    g = np.random.default_rng(15)
+    w = QuantizedTensor.rowwise(ctx, g.integers(-127, 128, (512, 4096)).astype(np.int8), np.full(512, 0.01, np.float32))
+    X = dev(ctx, g.standard_normal((64, 4096)).astype(np.float16))
+    Y = [dev(ctx, np.zeros((64, 512), np.float32)) for _ in range(2)]
+    engine.qmatmul(ctx, X, w, Y[0])
+    first = Y[0].to_vec()
+    ctx.sync()
+    graphs = [Graph(ctx.stream, lambda i=i: engine.attn_paged(ctx, Q, cache, L, outs[i], workspace=works[i])) for i in range(2)]
+    for lengths in ([4000, 40, 2500], [1, 0, 2], [3999, 1, 700], [33, 40, 2500]):
+        h = np.array(lengths, np.int32)
+        call("rq_memcpy_h2d", ctx.handle, L.ptr, h.ctypes.data, h.nbytes, None)
+        ctx.sync()
+        want, tol = truth(q, [[r[:, :m] for r in rows[s]] for s, m in enumerate(lengths)], 1 / 8, dtype == "f16")
+        graphs[0].launch()
+        engine.qmatmul(ctx, X, w, Y[1])
+        graphs[1].launch()
+        engine.attn_paged(ctx, Q, cache, L, outs[2], workspace=works[2])
+        eager = outs[2].to_vec()
+        check(eager, want, tol, f"eager {lengths}")
+        for o in outs[:2]:
+            assert np.array_equal(o.to_vec(), eager)
+        assert np.array_equal(Y[1].to_vec(), first)

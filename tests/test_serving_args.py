@@ -51,6 +51,17 @@ def paged(a=attn(), c=pages(), q=P, lengths=P, out=P, work=P, work_bytes=WS):
     return _fn("rusty_paged_check", [p, p, p, p, p, p, ctypes.c_size_t])(ref(a), ref(c), q, lengths, out, work, work_bytes)
 
 
+def test_limits():
+    """Sizes up to the documented ones are taken, one past them refused before anything is launched."""
+    assert paged(c=pages(n_seqs=65536)) == 0 and paged(c=pages(n_seqs=65537)) == SHAPE
+    assert append(c=pages(n_seqs=65537)) == 0
+    most = (1 << 24) - 256
+    for kw in (dict(m=most), dict(w=weight(n=most)), dict(w=weight(k=most))):
+        assert loras(work_bytes=1 << 62, **kw) == 0
+    for kw in (dict(m=most + 1), dict(w=weight(n=most + 1)), dict(w=weight(k=most + 128))):
+        assert loras(work_bytes=1 << 62, **kw) == SHAPE
+
+
 # ---- rotary rows -------------------------------------------------------------------
 
 
