@@ -26,6 +26,7 @@ from __future__ import annotations
 
 import ctypes
 import enum
+import math
 from dataclasses import dataclass
 from typing import Sequence
 
@@ -49,13 +50,14 @@ class DType(enum.Enum):
     U64 = np.uint64
     FP64 = np.float64
 
+    def __init__(self, value):
+        self.itemsize = np.dtype(value).itemsize
+
+    __hash__ = object.__hash__  # members are singletons; Enum's own hashes the name, in Python, at every look-up
+
     @property
     def np(self):
         return np.dtype(self.value)
-
-    @property
-    def itemsize(self) -> int:
-        return self.np.itemsize
 
 
 # Array types that UnifiedTensor.new keeps; numbers of any other become FP32.
@@ -148,7 +150,7 @@ class UnifiedTensor:
 
     @property
     def numel(self) -> int:
-        return _prod(self.shape)
+        return math.prod(self.shape)
 
     @property
     def nbytes(self) -> int:
@@ -574,8 +576,9 @@ class ComputeEngine:
     def _check_loras(x, w, adapters, out) -> int:
         if x.dtype not in _XDT or out.dtype not in _XDT:
             raise ValueError("x and out must be FP16 or FP32")
-        m = x.numel // w.k_in if w.k_in else x.shape[0]
-        if x.numel != m * w.k_in or out.numel != m * w.n_out or adapters.a.shape[2] != w.k_in \
+        n = x.numel
+        m = n // w.k_in if w.k_in else x.shape[0]
+        if n != m * w.k_in or out.numel != m * w.n_out or adapters.a.shape[2] != w.k_in \
                 or adapters.b.shape[2] != w.n_out:
             raise ValueError(f"x {x.shape} / A {adapters.a.shape} / B {adapters.b.shape} / out {out.shape} do not match "
                              f"weight [{w.n_out}, {w.k_in}]")
