@@ -87,6 +87,18 @@ int launch_matmul_f32(int variant, const float *a, const float *b, float *out, i
 int launch_matmul_f32_ah(const _Float16 *a, const float *b, float *out, int64_t m, int64_t k, int64_t n, int num_cus,
                          hipStream_t s);
 int launch_gemv_decode(const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dtype yt, int m, hipStream_t s);
+// What an adapter per row (rq_qmatmul_loras) adds to a decode GEMV's rows: of row t, whose adapter is
+// i = ids[t], the sums part[t][slices][rank rounded up to 4] of X . A_i^T, and the adapters' B.
+struct LoraDecode {
+    const void *b = nullptr;  // [n_adapters][rank][n_out] of RQ_F16 or RQ_F32
+    const float *factors = nullptr, *part = nullptr;
+    const int *ids = nullptr, *ranks = nullptr;
+    int n_adapters = 0, rank = 0, slices = 0, f16 = 0;
+};
+// m <= 2: launch_gemv_decode with the adapters' products added before y is rounded; RQ_ERR_UNSUPPORTED where
+// that does not serve (or an adapter's B spans 2 GiB).
+int launch_gemv_decode_loras(const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dtype yt, int m,
+                             const LoraDecode &ld, hipStream_t s);
 // m = 1..4 decode GEMV that adds its result into an f32 y (y += X . deq(W)^T):
 // the residual connection fused into the projection's epilogue.
 int launch_gemv_decode_add(const rq_qweight &w, const void *x, float *y, int m, hipStream_t s);

@@ -100,6 +100,9 @@ __device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
 // b cos, angle pos * theta^(-2d/hd) from the table at the step's position
 // (kernels.wgsl:60-79) -- and writes q (f32) to rd.q, k (rotated) and v
 // (fp16) into the caches at that position (rusty-graph/src/lib.rs:235-246).
+// LORA (m <= 2, the plain row): an adapter per row (ld).  A row's t = factor X . A^T lies in lanes (rank r in
+// lane r % 64), as do the B of the output that the wave finishes, asked for behind the weights; their
+// product is summed over the wave beside the weight's own.
 // XF (no NORM / SA): the activations are f32 (Xf).  Each 16-value chunk of a
 // row is scaled by a power of two 2^-e that puts its largest magnitude in
 // [2^14, 2^15) (exact), every scaled value is split into two fp16 terms
@@ -107,7 +110,8 @@ __device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
 // and the chunk's partial sums are multiplied back by 2^e: any finite f32
 // row is carried without overflowing fp16, and small values keep f32
 // accuracy instead of fp16's subnormal spacing.
-template <int M, int CPT, int TPR, int R, int FMT, bool SWI, bool NORM, int SA = 0, bool XF = false, bool ROPE = false>
+template <int M, int CPT, int TPR, int R, int FMT, bool SWI, bool NORM, int SA = 0, bool XF = false, bool ROPE = false,
+          bool LORA = false>
 __global__ __launch_bounds__(DT) void k_gemv_decode(const uint8_t *__restrict__ W, const float *__restrict__ scales,
                                                     const float *__restrict__ biases,
                                                     const uint8_t *__restrict__ W2, const float *__restrict__ scales2,
@@ -115,10 +119,11 @@ __global__ __launch_bounds__(DT) void k_gemv_decode(const uint8_t *__restrict__ 
                                                     const _Float16 *__restrict__ X, const float *__restrict__ Xf,
                                                     const _Float16 *__restrict__ NW, float eps,
                                                     void *__restrict__ Yv, int ymode, int m_act, int N, int K,
-                                                    int group, int attn_hd, RopeDecode rd) {
+                                                    int group, int attn_hd, RopeDecode rd, LoraDecode ld) {
     static_assert(!NORM || M == 1, "the fused norm serves one activation row");
     static_assert(SA == 0 || (M == 1 && !NORM && !SWI), "the attention combine serves one activation row");
     static_assert(!XF || (!NORM && SA == 0), "f32 activations replace the plain fp16 row");
+    static_assert(!LORA || (M <= 2 && !SWI && !NORM && SA == 0 && !ROPE), "an adapter per row of the plain product");
     static_assert(!ROPE || (NORM && !SWI), "the rotary epilogue serves the normed q/k/v projection");
     constexpr int RP = DT / TPR;
     constexpr int ROWS = R * RP;
@@ -337,6 +342,47 @@ __global__ __launch_bounds__(DT) void k_gemv_decode(const uint8_t *__restrict__ 
             if constexpr (ROPE) off = c < C && lr < rows_here ? (uint32_t)wrow(lr) * (uint32_t)K + (uint32_t)c * 16 : kOOB;
             w[r][j] = bload<2>(r < R ? rw : rw2, off);
         }
+    // LORA: the first 8 slices of t's and B's ranks lane, lane + 64, ... (one each), t 0 past the rank
+    constexpr int TS = 8;
+    float tq[LORA ? TS : 1], bq[LORA ? NTW : 1], lora[LORA ? NTW : 1];
+    int lrank[LORA ? M : 1];
+    float lfactor[LORA ? M : 1];
+    int64_t lbase[LORA ? M : 1];
+    // task i of this wave is of row lm (M = 1, 2: the same for all), output lrow(i)
+    const int lwave = __builtin_amdgcn_readfirstlane(wave), lm = M == 2 ? lwave & 1 : 0;
+    auto lrow = [&](int i) { return min(row0 + min(lwave + (DT / 64) * i, TASKS - 1) / M, N - 1); };
+    auto of_lm = [&](const auto &v) {
+        const auto a = v[0], b = v[LORA ? M - 1 : 0];  // (values: a choice between places would put them in memory)
+        return lm ? b : a;
+    };
+    const int ranks4 = LORA ? (ld.rank + 3) / 4 * 4 : 0, bsize = LORA && ld.f16 ? 2 : 4;
+    auto b_of = [&](int r, int row) {
+        const int rank = of_lm(lrank);
+        const auto rb = make_rsrc(static_cast<const char *>(ld.b) + of_lm(lbase), (uint32_t)rank * (uint32_t)N * (uint32_t)bsize);
+        const uint32_t off = r < rank ? ((uint32_t)r * (uint32_t)N + (uint32_t)row) * (uint32_t)bsize : kOOB;
+        if (ld.f16) return (float)__builtin_bit_cast(_Float16, __builtin_amdgcn_raw_buffer_load_b16(rb, off, 0, 0));
+        return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rb, off, 0, 0));
+    };
+    auto t_of = [&](int r, int j) {
+        const auto rt = make_rsrc(ld.part + (size_t)lm * ld.slices * ranks4, (uint32_t)(ld.slices * ranks4) * 4u);
+        const bool live = r < of_lm(lrank) && j < ld.slices;
+        return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rt, live ? (uint32_t)(j * ranks4 + r) * 4u : kOOB, 0, 0));
+    };
+    if constexpr (LORA) {
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            const int i = m < m_act ? ld.ids[m] : -1;
+            const bool has = (uint32_t)i < (uint32_t)ld.n_adapters;
+            const int own = has && ld.ranks ? ld.ranks[i] : ld.rank;
+            lrank[m] = has ? min(max(own, 0), ld.rank) : 0;
+            lfactor[m] = has && ld.factors ? ld.factors[i] : 1.0f;
+            lbase[m] = has ? (int64_t)i * ld.rank * N * bsize : 0;
+        }
+#pragma unroll
+        for (int j = 0; j < TS; ++j) tq[j] = t_of(lane, j);
+#pragma unroll
+        for (int i = 0; i < NTW; ++i) bq[i] = b_of(lane, lrow(i));
+    }
     if constexpr (ROPE) {
 #pragma unroll
         for (int i = 0; i < NPW; ++i) {
@@ -524,6 +570,22 @@ __global__ __launch_bounds__(DT) void k_gemv_decode(const uint8_t *__restrict__ 
             part[(r / R) * TASKS + ((r % R) * RP + rp) * M + m][tt] = v;
         }
     }
+    if constexpr (LORA) {
+        const float f = of_lm(lfactor);
+        const int rank = of_lm(lrank);
+        float tl = 0.0f;
+#pragma unroll
+        for (int j = 0; j < TS; ++j) tl += tq[j];
+        for (int j = TS; j < ld.slices; ++j) tl += t_of(lane, j);
+#pragma unroll
+        for (int i = 0; i < NTW; ++i) lora[i] = lane < rank ? f * tl * bq[i] : 0.0f;
+        for (int r = lane + 64; r - lane < rank; r += 64) {
+            float v = 0.0f;
+            for (int j = 0; j < ld.slices; ++j) v += t_of(r, j);
+#pragma unroll
+            for (int i = 0; i < NTW; ++i) lora[i] = r < rank ? __builtin_fmaf(f * v, b_of(r, lrow(i)), lora[i]) : lora[i];
+        }
+    }
     __syncthreads();
 
     if constexpr (ROPE) {
@@ -577,10 +639,12 @@ __global__ __launch_bounds__(DT) void k_gemv_decode(const uint8_t *__restrict__ 
         }
         const float tot = wave_total(v);
         const float tot2 = SWI ? wave_total(v2) : 0.0f;
+        const float lo = LORA ? wave_total(lora[i_t]) : 0.0f;
         const int rin = task / M, m = task % M;
         const int row = row0 + rin;
         if (lane == 0 && rin < rows_here && m < m_act) {
             float y = FMT == 0 ? tot * srow[i_t] : tot;
+            if constexpr (LORA) y += lo;
             if constexpr (SWI) y = silu(y) * (FMT == 0 ? tot2 * srow2[i_t] : tot2);
             const size_t o = (size_t)m * N + row;
             if (ymode == kYF16) reinterpret_cast<_Float16 *>(Yv)[o] = (_Float16)y;
@@ -592,7 +656,7 @@ __global__ __launch_bounds__(DT) void k_gemv_decode(const uint8_t *__restrict__ 
 
 using DecodeFn = void (*)(const uint8_t *, const float *, const float *, const uint8_t *, const float *,
                           const float *, const _Float16 *, const float *, const _Float16 *, float, void *, int, int, int, int, int,
-                          int, RopeDecode);
+                          int, RopeDecode, LoraDecode);
 
 // A kernel instance and the rows per row group (R) it was compiled for; the
 // grid is derived from the same R.
@@ -600,8 +664,9 @@ struct Decode {
     DecodeFn fn;
     int r;
 };
-template <int M, int CPT, int TPR, int R, int FMT, bool SWI, bool NORM, int SA = 0, bool XF = false, bool ROPE = false>
-constexpr Decode inst() { return {&k_gemv_decode<M, CPT, TPR, R, FMT, SWI, NORM, SA, XF, ROPE>, R}; }
+template <int M, int CPT, int TPR, int R, int FMT, bool SWI, bool NORM, int SA = 0, bool XF = false, bool ROPE = false,
+          bool LORA = false>
+constexpr Decode inst() { return {&k_gemv_decode<M, CPT, TPR, R, FMT, SWI, NORM, SA, XF, ROPE, LORA>, R}; }
 
 // Rows per row group, measured on MI355X with the weights streamed from HBM:
 //  m = 1:
@@ -633,7 +698,33 @@ constexpr Decode inst() { return {&k_gemv_decode<M, CPT, TPR, R, FMT, SWI, NORM,
 // combine of sa partials per head; xf (m <= 2, no norm / sa) f32 activations:
 // 0 for fp16, else the rows per block for f32 rows (m = 1: 2, 4 or 8; m = 2: 4 or 8).
 template <int M, int CPT, int TPR, int FMT>
-Decode pick_fmt(bool swi, bool norm, bool tall, int sa, int xf, bool rope) {
+Decode pick_lora(bool tall, int xf) {
+    if constexpr (M == 1) {
+        constexpr int RP = FMT == 0 && CPT >= 2 ? 4 : 2;
+        if (FMT == 0 && tall)
+            return xf ? inst<1, CPT, TPR, 8, FMT, false, false, 0, true, false, true>()
+                      : inst<1, CPT, TPR, 8, FMT, false, false, 0, false, false, true>();
+        if constexpr (TPR == 256) {
+            if (xf == 8) return inst<1, CPT, TPR, 8, FMT, false, false, 0, true, false, true>();
+            if (xf == 4) return inst<1, CPT, TPR, 4, FMT, false, false, 0, true, false, true>();
+            if (xf) return inst<1, CPT, TPR, 2, FMT, false, false, 0, true, false, true>();
+        }
+        return xf ? inst<1, CPT, TPR, RP, FMT, false, false, 0, true, false, true>()
+                  : inst<1, CPT, TPR, RP, FMT, false, false, 0, false, false, true>();
+    } else {
+        (void)tall;
+        if (xf == 8) return inst<2, CPT, TPR, 8, FMT, false, false, 0, true, false, true>();
+        return xf ? inst<2, CPT, TPR, 4, FMT, false, false, 0, true, false, true>()
+                  : inst<2, CPT, TPR, 4, FMT, false, false, 0, false, false, true>();
+    }
+}
+
+template <int M, int CPT, int TPR, int FMT>
+Decode pick_fmt(bool swi, bool norm, bool tall, int sa, int xf, bool rope, bool lora) {
+    // the plain product's rows with an adapter per row
+    if constexpr (M <= 2 && (CPT == 1 || TPR == 256)) {
+        if (lora) return pick_lora<M, CPT, TPR, FMT>(tall, xf);
+    }
     if constexpr (M == 1) {
         constexpr int RN = TPR <= 128 ? 6 : 2;   // fused norm
         constexpr int RSN = TPR <= 128 ? 4 : 2;  // SwiGLU pairs with the fused norm
@@ -682,33 +773,34 @@ Decode pick_fmt(bool swi, bool norm, bool tall, int sa, int xf, bool rope) {
         (void)sa;
         (void)xf;
         (void)rope;
+        (void)lora;
         if (swi) return inst<M, CPT, TPR, 2, FMT, true, false>();
         return inst<M, CPT, TPR, 4, FMT, false, false>();
     }
 }
 
 template <int M, int CPT, int TPR>
-Decode pick_swi(int fmt, bool swi, bool norm, bool tall, int sa, int xf, bool rope) {
-    return fmt == 0 ? pick_fmt<M, CPT, TPR, 0>(swi, norm, tall, sa, xf, rope)
-                    : pick_fmt<M, CPT, TPR, 1>(swi, norm, tall, sa, xf, rope);
+Decode pick_swi(int fmt, bool swi, bool norm, bool tall, int sa, int xf, bool rope, bool lora) {
+    return fmt == 0 ? pick_fmt<M, CPT, TPR, 0>(swi, norm, tall, sa, xf, rope, lora)
+                    : pick_fmt<M, CPT, TPR, 1>(swi, norm, tall, sa, xf, rope, lora);
 }
 
 template <int M, int CPT>
-Decode pick_tpr(int tpr, int fmt, bool swi, bool norm, bool tall, int sa, int xf, bool rope) {
+Decode pick_tpr(int tpr, int fmt, bool swi, bool norm, bool tall, int sa, int xf, bool rope, bool lora) {
     switch (tpr) {
-    case 64: return pick_swi<M, CPT, 64>(fmt, swi, norm, tall, sa, xf, rope);
-    case 128: return pick_swi<M, CPT, 128>(fmt, swi, norm, tall, sa, xf, rope);
-    default: return pick_swi<M, CPT, 256>(fmt, swi, norm, tall, sa, xf, rope);
+    case 64: return pick_swi<M, CPT, 64>(fmt, swi, norm, tall, sa, xf, rope, lora);
+    case 128: return pick_swi<M, CPT, 128>(fmt, swi, norm, tall, sa, xf, rope, lora);
+    default: return pick_swi<M, CPT, 256>(fmt, swi, norm, tall, sa, xf, rope, lora);
     }
 }
 
 template <int M>
-Decode pick_cpt(int cpt, int tpr, int fmt, bool swi, bool norm, bool tall, int sa, int xf, bool rope) {
+Decode pick_cpt(int cpt, int tpr, int fmt, bool swi, bool norm, bool tall, int sa, int xf, bool rope, bool lora) {
     switch (cpt) {
-    case 1: return pick_tpr<M, 1>(tpr, fmt, swi, norm, tall, sa, xf, rope);
-    case 2: return pick_tpr<M, 2>(tpr, fmt, swi, norm, tall, sa, xf, rope);
-    case 3: return pick_tpr<M, 3>(tpr, fmt, swi, norm, tall, sa, xf, rope);
-    default: return pick_tpr<M, 4>(tpr, fmt, swi, norm, tall, sa, xf, rope);
+    case 1: return pick_tpr<M, 1>(tpr, fmt, swi, norm, tall, sa, xf, rope, lora);
+    case 2: return pick_tpr<M, 2>(tpr, fmt, swi, norm, tall, sa, xf, rope, lora);
+    case 3: return pick_tpr<M, 3>(tpr, fmt, swi, norm, tall, sa, xf, rope, lora);
+    default: return pick_tpr<M, 4>(tpr, fmt, swi, norm, tall, sa, xf, rope, lora);
     }
 }
 
@@ -716,7 +808,7 @@ Decode pick_cpt(int cpt, int tpr, int fmt, bool swi, bool norm, bool tall, int s
 
 // The kernel instance for a supported call and the weight rows each of its
 // blocks covers (block j: rows j * rows ..).
-static Decode plan(const rq_qweight &w, bool swi, bool norm, int m, int sa, bool xf, bool rope, int *rows) {
+static Decode plan(const rq_qweight &w, bool swi, bool norm, int m, int sa, bool xf, bool rope, bool lora, int *rows) {
     const int64_t N = w.n_out, K = w.k_in;
     const int C = (int)(K / 16);
     const int tpr = C <= 64 ? 64 : (C <= 128 ? 128 : 256);
@@ -727,9 +819,9 @@ static Decode plan(const rq_qweight &w, bool swi, bool norm, int m, int sa, bool
     const int xr = !xf ? 0
                    : mt == 2 ? (N / 8 >= 512 ? 8 : 4)
                              : (N / 8 >= 1024 || (K > 4096 && N / 8 >= 512)) ? 8 : (N / 4 >= 1024 ? 4 : 2);
-    const Decode d = mt == 1 ? pick_cpt<1>(cpt, tpr, fmt, swi, norm, tall && !rope, sa, xr, rope)
-                             : mt == 2 ? pick_cpt<2>(cpt, tpr, fmt, swi, false, false, 0, xr, false)
-                                       : pick_cpt<4>(cpt, tpr, fmt, swi, false, false, 0, false, false);
+    const Decode d = mt == 1 ? pick_cpt<1>(cpt, tpr, fmt, swi, norm, tall && !rope, sa, xr, rope, lora)
+                             : mt == 2 ? pick_cpt<2>(cpt, tpr, fmt, swi, false, false, 0, xr, false, lora)
+                                       : pick_cpt<4>(cpt, tpr, fmt, swi, false, false, 0, false, false, false);
     *rows = d.r * (DT / tpr);
     return d;
 }
@@ -739,7 +831,7 @@ static Decode plan(const rq_qweight &w, bool swi, bool norm, int m, int sa, bool
 // partials to combine (sa per head of attn_hd elements).
 static int launch_decode(const rq_qweight &w, const rq_qweight *w2, const void *x, const _Float16 *nw, float eps,
                          void *y, int ymode, int m, hipStream_t s, int sa = 0, int attn_hd = 0, bool xf = false,
-                         const RopeDecode *rd = nullptr) {
+                         const RopeDecode *rd = nullptr, const LoraDecode *ld = nullptr) {
     const int64_t N = w.n_out, K = w.k_in;
     // f32 activations: m <= 2 and the plain row only; 32-bit offsets into X
     if (xf && (m > 2 || nw || sa || (int64_t)m * K * 4 > 0x7fffffffll)) return RQ_ERR_UNSUPPORTED;
@@ -759,20 +851,27 @@ static int launch_decode(const rq_qweight &w, const rq_qweight *w2, const void *
                N != (int64_t)(rd->n_heads + 2 * rd->n_kv) * rd->hd || N * K > 0xffffffffll || !rd->pos ||
                !rd->rope || !rd->q || !rd->kc || !rd->vc))
         return RQ_ERR_UNSUPPORTED;
+    // (B's offsets are 32 bits)
+    if (ld && (m > 2 || ld->rank * N * 4 > 0x7fffffffll)) return RQ_ERR_UNSUPPORTED;
     int rows;
-    const Decode d = plan(w, w2 != nullptr, nw != nullptr, m, sa, xf, rd != nullptr, &rows);
+    const Decode d = plan(w, w2 != nullptr, nw != nullptr, m, sa, xf, rd != nullptr, ld != nullptr, &rows);
     const bool fx = nw || sa || xf;  // x is an f32 source
     const int64_t blocks = cdiv(N, rows);
     hipLaunchKernelGGL(d.fn, dim3((unsigned)blocks), dim3(DT), 0, s, (const uint8_t *)w.codes, w.scales, w.biases,
                        w2 ? (const uint8_t *)w2->codes : nullptr, w2 ? w2->scales : nullptr, w2 ? w2->biases : nullptr,
                        fx ? nullptr : (const _Float16 *)x, fx ? (const float *)x : nullptr, nw, eps, y, ymode, m,
-                       (int)N, (int)K, w.group, attn_hd, rd ? *rd : RopeDecode{});
+                       (int)N, (int)K, w.group, attn_hd, rd ? *rd : RopeDecode{}, ld ? *ld : LoraDecode{});
     RQ_LAUNCH_CHECK();
     return RQ_OK;
 }
 
 int launch_gemv_decode(const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dtype yt, int m, hipStream_t s) {
     return launch_decode(w, nullptr, x, nullptr, 0.0f, y, yt == RQ_F16 ? kYF16 : kYF32, m, s, 0, 0, xt == RQ_F32);
+}
+
+int launch_gemv_decode_loras(const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dtype yt, int m,
+                             const LoraDecode &ld, hipStream_t s) {
+    return launch_decode(w, nullptr, x, nullptr, 0.0f, y, yt == RQ_F16 ? kYF16 : kYF32, m, s, 0, 0, xt == RQ_F32, nullptr, &ld);
 }
 
 int launch_gemv_decode_add(const rq_qweight &w, const void *x, float *y, int m, hipStream_t s) {

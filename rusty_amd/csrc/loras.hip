@@ -7,6 +7,8 @@
 // once.  Small batches are bound by the launches and by the weight's bytes, which
 // each used adapter adds (k_in + n_out) rank elements to; prompts by the shared product.
 //
+// One or two rows of 8-bit codes take two launches: the decode GEMV adds its rows' adapters itself.
+//
 // k_loras_in: rows of X are the rows of a matrix instruction, 16 rows of A_i its
 // columns, k runs along both (16-byte loads, no LDS).  Rows of a tile may have
 // different adapters: each one's product is formed for all its rows and
@@ -19,7 +21,7 @@
 // t as two fp16 terms).
 //
 // Measured (us, 4096 x 4096; X . A / shared product / t . B; the bytes at 6.9 TB/s, the products at 1157
-// TFLOP/s): one row, 8-bit rows, rank 16: 3.3 / 4.7 / 2.7 (2.5); 61 rows of 11 adapters, 4-bit groups,
+// TFLOP/s): one row, 8-bit rows, rank 16: 3.3 / 5.1 with t . B, 8.6 a call (2.5; in three launches 3.3 / 4.7 / 2.7, 12.3); 61 rows of 11 adapters, 4-bit groups,
 // f32 rows, rank 32: 5.0 / 16.8 / 3.9 (4.9); 2048 rows, 8-bit, rank 32: 9.4 / 66 / 18.9 (60).  One launch for X . A and
 // the shared product of a few rows took 8 us where the two take 6.1.
 #include <algorithm>
@@ -532,6 +534,12 @@ int rq_qmatmul_loras(rq_ctx *ctx, const rq_qweight *w, const rq_lora_set *set, c
     const bool adapters = set->n_adapters > 0;
     if (adapters && (st = run_in(p, x_dtype, set->dtype, ctx->num_cus, s)) != RQ_OK) return st;
     if (!adapters) return qmatmul_dispatch(ctx, *w, x, x_dtype, y, y_dtype, m, gemm_workspace(ctx, s), s);
+    // One or two rows: the decode GEMV adds its rows' adapters itself.
+    if (m <= 2 && w->format != RQ_Q_AFFINE_U4 && w->k_in > 0) {
+        const LoraDecode ld{p.b, p.factors, p.part, p.ids, p.ranks, p.n_adapters, p.rank, p.slices, set->dtype == RQ_F16};
+        st = launch_gemv_decode_loras(*w, x, x_dtype, y, y_dtype, (int)m, ld, s);
+        if (st != RQ_ERR_UNSUPPORTED) return st;
+    }
     if ((st = qmatmul_dispatch(ctx, *w, x, x_dtype, const_cast<float *>(p.main), RQ_F32, m, gemm_workspace(ctx, s), s)) != RQ_OK)
         return st;
     return run_out(p, set->dtype, y_dtype, s);

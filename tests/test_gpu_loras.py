@@ -294,3 +294,14 @@ def test_infinite_beside_large(ctx, engine, m):
     x = np.full((m, k), 1e34, np.float32)  # 1e34 6e4 > 3.4e38 > 64 1e34 1e-3 > 65504
     got = run(ctx, engine, x, w, a, b, None, np.zeros(m, int), None, "f32", "f32", "f16")
     assert np.all(got == np.inf)
+
+
+@pytest.mark.parametrize("x_t,y_t,a_t", TYPES)
+@pytest.mark.parametrize("form", ["rowwise8", "affine8"])
+@pytest.mark.parametrize("m", [1, 2])
+@pytest.mark.parametrize("n,k,rank", [(40, 16384, 100), (16400, 64, 256), (131, 2048, 65), (2056, 4160, 16), (7, 1024, 3)])
+def test_one_and_two_rows(ctx, engine, x_t, y_t, a_t, form, m, n, k, rank):
+    """The decode form: many slices of k, ranks of more than a wave, tall weights, adapters of fewer ranks (0 among them)."""
+    g = np.random.default_rng(n)
+    for ids in ([0, 2], [1, 1], [-1, 1], [2, 5]):
+        case(ctx, engine, n + k + ids[0] + 7, m, n, k, 3, rank, form, x_t, y_t, a_t, ids=ids[:m], some_ranks=bool(g.integers(2)))
