@@ -344,7 +344,8 @@ __global__ __launch_bounds__(DT) void k_gemv_decode(const uint8_t *__restrict__ 
         }
     // LORA: the first 8 slices of t's and B's ranks lane, lane + 64, ... (one each), t 0 past the rank
     constexpr int TS = 8;
-    float tq[LORA ? TS : 1], bq[LORA ? NTW : 1], lora[LORA ? NTW : 1];
+    float tq[LORA ? TS : 1], lora[LORA ? NTW : 1];
+    uint32_t bq[LORA ? NTW : 1];
     int lrank[LORA ? M : 1];
     float lfactor[LORA ? M : 1];
     int64_t lbase[LORA ? M : 1];
@@ -356,17 +357,20 @@ __global__ __launch_bounds__(DT) void k_gemv_decode(const uint8_t *__restrict__ 
         return lm ? b : a;
     };
     const int ranks4 = LORA ? (ld.rank + 3) / 4 * 4 : 0, bsize = LORA && ld.f16 ? 2 : 4;
-    auto b_of = [&](int r, int row) {
+    // (B's bits: a conversion here would wait for all loads)
+    auto b_of = [&](int r, int row) -> uint32_t {
         const int rank = of_lm(lrank);
         const auto rb = make_rsrc(static_cast<const char *>(ld.b) + of_lm(lbase), (uint32_t)rank * (uint32_t)N * (uint32_t)bsize);
         const uint32_t off = r < rank ? ((uint32_t)r * (uint32_t)N + (uint32_t)row) * (uint32_t)bsize : kOOB;
-        if (ld.f16) return (float)__builtin_bit_cast(_Float16, __builtin_amdgcn_raw_buffer_load_b16(rb, off, 0, 0));
-        return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rb, off, 0, 0));
+        return ld.f16 ? (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rb, off, 0, 0) : __builtin_amdgcn_raw_buffer_load_b32(rb, off, 0, 0);
     };
-    auto t_of = [&](int r, int j) {
+    auto b_value = [&](uint32_t v) {
+        return ld.f16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)v) : __builtin_bit_cast(float, v);
+    };
+    auto t_of = [&](int r, int j) {  // (past the last slice: past the resource)
         const auto rt = make_rsrc(ld.part + (size_t)lm * ld.slices * ranks4, (uint32_t)(ld.slices * ranks4) * 4u);
-        const bool live = r < of_lm(lrank) && j < ld.slices;
-        return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rt, live ? (uint32_t)(j * ranks4 + r) * 4u : kOOB, 0, 0));
+        const uint32_t off = (r < of_lm(lrank) ? (uint32_t)r * 4u : kOOB) + (uint32_t)(j * ranks4) * 4u;
+        return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rt, off, 0, 0));
     };
     if constexpr (LORA) {
 #pragma unroll
@@ -578,12 +582,12 @@ __global__ __launch_bounds__(DT) void k_gemv_decode(const uint8_t *__restrict__ 
         for (int j = 0; j < TS; ++j) tl += tq[j];
         for (int j = TS; j < ld.slices; ++j) tl += t_of(lane, j);
 #pragma unroll
-        for (int i = 0; i < NTW; ++i) lora[i] = lane < rank ? f * tl * bq[i] : 0.0f;
+        for (int i = 0; i < NTW; ++i) lora[i] = lane < rank ? f * tl * b_value(bq[i]) : 0.0f;
         for (int r = lane + 64; r - lane < rank; r += 64) {
             float v = 0.0f;
             for (int j = 0; j < ld.slices; ++j) v += t_of(r, j);
 #pragma unroll
-            for (int i = 0; i < NTW; ++i) lora[i] = r < rank ? __builtin_fmaf(f * v, b_of(r, lrow(i)), lora[i]) : lora[i];
+            for (int i = 0; i < NTW; ++i) lora[i] = r < rank ? __builtin_fmaf(f * v, b_value(b_of(r, lrow(i))), lora[i]) : lora[i];
         }
     }
     __syncthreads();
