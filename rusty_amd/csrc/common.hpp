@@ -139,8 +139,10 @@ struct RopeOut {
 };
 int launch_gemm_qkv_rope(const rq_qweight &w, const _Float16 *x, int64_t m, const RopeOut &ro, _Float16 *q,
                          int num_cus, const GemmWorkspace &ws, hipStream_t s);
+// ld: an adapter per row added before y is rounded (as launch_gemv_decode_loras; RQ_ERR_UNSUPPORTED, nothing
+// written to y, where the product's tiles do not).
 int launch_gemm(const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dtype yt, int64_t m, int num_cus,
-                const GemmWorkspace &ws, hipStream_t s);
+                const GemmWorkspace &ws, hipStream_t s, const LoraDecode *ld = nullptr);
 // Y = (xscale[row] * X[row]) . (scales * W)^T for per-row int8 W and fp16 X
 // (xscale: a power of two per activation row); RQ_ERR_UNSUPPORTED outside the
 // prefill GEMM's tiles (k_in % 64, alignment).

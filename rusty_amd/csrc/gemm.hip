@@ -164,15 +164,22 @@ __device__ __forceinline__ void tile_of(int b, int tiles_m, int tiles_n, int gm,
 // rotary embedding to q and k heads -- o[d] = a c - b s, o[d + 32] = a s + b c
 // for a, b the f32 results at d and d + 32 -- and writes q (Yv) and the K and
 // V caches (RopeOut) in fp16 instead of the f32 product.
+// LORA (128 tokens, 8 waves): an adapter per token (ld, fp16 B).  The scaled tile waits in LDS as f32 rows, a
+// wave takes 16 of them, and for each adapter of the tile's tokens, 32 ranks at a time (their B to
+// LDS by all waves), adds B^T . t^T on the matrix instructions: t, scaled by a power of two per
+// row, as two fp16 terms (off by at most 2^-22), B's fragments by transposing LDS reads.
+// Then the rows are rounded and written.  Products of rows that have another adapter are dropped, not
+// added as zeros, so nothing a foreign adapter holds reaches a row.
 template <int BM, int BN, bool PINGPONG, int S, int NW, int WGN, int KG = 1, bool W2 = false, int FMT = 0,
-          bool PAIR = false, bool ROPE = false>
+          bool PAIR = false, bool ROPE = false, bool LORA = false>
 __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restrict__ W, const float *__restrict__ scales,
                                                      const _Float16 *__restrict__ X, void *__restrict__ Yv,
                                                      int y_f16, int M, int N, int K, int tiles_m, int tiles_n,
                                                      int gm, int splits, float *__restrict__ skw,
                                                      int *__restrict__ skc, int group, const uint8_t *__restrict__ Wb,
                                                      const float *__restrict__ scalesb, int n_split, RopeOut ro,
-                                                     const float *__restrict__ xscale) {
+                                                     const float *__restrict__ xscale, LoraDecode ld) {
+    static_assert(!LORA || (!PAIR && !ROPE && BM == 128 && NW == 8 && BN % 128 == 0), "adapters: 16 rows per wave");
     static_assert(!ROPE || (BN == 64 && !PAIR), "rotary epilogue: one 64-wide head per tile");
     // KG k-groups of NW/KG waves: group g takes k16 slices [g*K16, (g+1)*K16)
     // of every 64-k stage, so a wave tile covers KG times the outputs for the
@@ -198,7 +205,9 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restr
     constexpr int RING_X = W2 ? S * BM * 128 + 2 * BN * 128 : S * (BM * 128 + BN * 64);  // X and W stages
     constexpr int RING_K = RING_X + S * SCB;  // k-loop stages
     // the epilogue reuses the ring to stage a tile of f32 (or fp16) rows
-    constexpr int RING = RING_K > BM * (BN * 4 + 16) ? RING_K : BM * (BN * 4 + 16);
+    // (LORA: and 32 ranks of an adapter's B behind it)
+    constexpr int STAGED = BM * (BN * 4 + 16) + (LORA ? 32 * BN * 2 : 0);
+    constexpr int RING = RING_K > STAGED ? RING_K : STAGED;
     static_assert(S >= 3 && RING <= 160 * 1024, "ring does not fit in LDS");
     constexpr int XOPS = XUW + (FMT == 1 ? 1 : 0);  // DMA ops per wave issued with each X stage
     constexpr int NOUT = XOPS + WUW;  // DMA ops per wave per k-step (W2: W on odd steps only)
@@ -698,6 +707,16 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restr
         constexpr int RS = BN * EB + 16;           // padded LDS row stride
         static_assert(BM * RS <= RING, "output staging does not fit in the ring");
         uint8_t *ot = reinterpret_cast<uint8_t *>(&ring[0]);
+        // LORA: the adapters of the tile's tokens, lane l's of tokens l and l + 64; -1: none
+        auto adapter_of = [&](int row) {
+            const int i = row < M ? ld.ids[row] : -1;
+            return (uint32_t)i < (uint32_t)ld.n_adapters ? i : -1;
+        };
+        int ida = -1, idb = -1;
+        if constexpr (LORA) {
+            ida = adapter_of(m0 + lane);
+            idb = adapter_of(m0 + 64 + lane);
+        }
         __syncthreads();  // every wave is done with the ring (and the k-group exchange)
 #pragma unroll
         for (int i = 0; i < FN; ++i) {
@@ -759,6 +778,123 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restr
             }
             return;
         }
+        if constexpr (LORA) {
+            constexpr int CB = BN / 64, CH = BN / 8, RPU = 64 / CH, BU = 32 * BN * 2 / 1024 / NW;
+            typedef short short4v __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) short4v lds_short4;
+            // chunk s of B's row r holds global chunk s ^ swz(r): a transposing read's 4 rows x 4 pieces cover the banks
+            auto swz = [](int r) { return (r & 1) | (r & 2) << 2; };
+            uint8_t *bt = ot + BM * RS;
+            const int col = lane & 15, qt = lane >> 4, row = wave * 16 + col, ranks4 = (ld.rank + 3) / 4 * 4;
+            floatx4 out[CB][4];
+#pragma unroll
+            for (int c = 0; c < CB; ++c)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) out[c][v] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+            uint64_t la = __builtin_amdgcn_ballot_w64(ida >= 0), lb = __builtin_amdgcn_ballot_w64(idb >= 0);
+#pragma unroll 1
+            while (la | lb) {
+                const int i = la ? __builtin_amdgcn_readlane(ida, __builtin_ctzll(la | 1ull << 63))
+                                 : __builtin_amdgcn_readlane(idb, __builtin_ctzll(lb | 1ull << 63));
+                const uint64_t sa = __builtin_amdgcn_ballot_w64(ida == i), sb = __builtin_amdgcn_ballot_w64(idb == i);
+                la &= ~sa;
+                lb &= ~sb;
+                const uint32_t own = (uint32_t)((wave < 4 ? sa : sb) >> (16 * (wave & 3))) & 0xffffu;
+                const int rank = ld.ranks ? min(max(ld.ranks[i], 0), ld.rank) : ld.rank;
+                const float f = ld.factors ? ld.factors[i] : 1.0f;
+                const _Float16 *b = static_cast<const _Float16 *>(ld.b) + (int64_t)i * ld.rank * N;
+#pragma unroll 1
+                for (int r0 = 0; r0 < rank; r0 += 32) {
+                    // t of this lane's row, ranks r0 + 8 qt ..: the slices summed in order
+                    floatx4 tv[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+                    const int r1 = r0 + 8 * qt;
+                    if (own) {
+                        const float *q = ld.part + (int64_t)min(m0 + row, M - 1) * ld.slices * ranks4 + r1;
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            if (r1 + 4 * u < ranks4) {
+#pragma unroll 8
+                                for (int j = 0; j < ld.slices; ++j)
+                                    tv[u] += *reinterpret_cast<const floatx4 *>(q + (int64_t)j * ranks4 + 4 * u);
+                            }
+                    }
+                    __syncthreads();  // the last ranks' B have been read
+#pragma unroll
+                    for (int q = 0; q < BU; ++q) {
+                        const int r = (wave * BU + q) * RPU + lane / CH, n = min(n0 + (lane % CH ^ swz(r)) * 8, N - 8);
+                        dma16_kept(reinterpret_cast<const char *>(b + (int64_t)min(r0 + r, rank - 1) * N + n),
+                                   lds_addr(bt) + (uint32_t)((wave * BU + q) * 1024));
+                    }
+                    wait_vmcnt<0>();
+                    // (what lies past the rank is another rank's, and may be infinite)
+#pragma unroll
+                    for (int q = 0; q < BU; ++q)
+                        if (r0 + (wave * BU + q) * RPU + lane / CH >= rank)
+                            *reinterpret_cast<uint4 *>(bt + (wave * BU + q) * 1024 + lane * 16) = make_uint4(0, 0, 0, 0);
+                    __syncthreads();
+                    if (!own) continue;
+                    float most = 0.0f;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            tv[u][e] = r1 + 4 * u + e < rank ? f * tv[u][e] : 0.0f;
+                            most = fmaxf(most, __builtin_isfinite(tv[u][e]) ? fabsf(tv[u][e]) : 0.0f);
+                        }
+                    most = fmaxf(most, __shfl_xor(most, 16));
+                    most = fmaxf(most, __shfl_xor(most, 32));
+                    // the row's largest that is finite in [2^14, 2^15)
+                    const int ex = most > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+                    half8 hi, lo;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float x = __builtin_ldexpf(tv[e / 4][e % 4], ex);
+                        hi[e] = (_Float16)x;
+                        lo[e] = __builtin_isfinite((float)hi[e]) ? (_Float16)(x - (float)hi[e]) : (_Float16)0.0f;
+                    }
+                    const float scale = __builtin_ldexpf(1.0f, -ex);
+                    const bool has = own >> col & 1;
+                    // 16 lanes take 4 ranks x 4 x 4 columns; each gets one column's 4 ranks
+                    const uint32_t at = lds_addr(bt) + (uint32_t)((8 * qt + col / 4) * (BN * 2));
+#pragma unroll
+                    for (int c = 0; c < CB; ++c)
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) {
+                            const int ch = (c * 8 + (col & 3) * 2 + v / 2) ^ swz(col / 4);
+                            lds_short4 *p = (lds_short4 *)(uintptr_t)(at + (uint32_t)(ch * 16 + (v & 1) * 8));
+                            const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
+                            const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p + 4 * BN * 2 / 8));
+                            const half8 bf = __builtin_bit_cast(half8, make_uint4(x.x, x.y, y.x, y.y));
+                            floatx4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+                            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf, hi, a, 0, 0, 0);
+                            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf, lo, a, 0, 0, 0);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) out[c][v][e] = has ? __builtin_fmaf(a[e], scale, out[c][v][e]) : out[c][v][e];
+                        }
+                }
+            }
+            // lane: row `row`, columns 64 c + 16 qt + 4 v + e
+            const int oe = y_f16 ? 2 : 4;
+            const auto ry = make_rsrc(static_cast<uint8_t *>(Yv) + ((size_t)m0 * N + n0) * oe, (uint32_t)min(BM, M - m0) * (uint32_t)N * oe);
+#pragma unroll
+            for (int c = 0; c < CB; ++c)
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {  // 8 columns
+                    const int n = 64 * c + 16 * qt + 8 * hh;
+                    const floatx4 *mp = reinterpret_cast<const floatx4 *>(ot + row * RS + n * 4);
+                    const floatx4 a0 = mp[0] + out[c][2 * hh], a1 = mp[1] + out[c][2 * hh + 1];
+                    const uint32_t off = n0 + n < N ? (uint32_t)row * (uint32_t)N * oe + (uint32_t)(n * oe) : kOOB;
+                    if (y_f16) {
+                        const half8 o = {(_Float16)a0[0], (_Float16)a0[1], (_Float16)a0[2], (_Float16)a0[3],
+                                         (_Float16)a1[0], (_Float16)a1[1], (_Float16)a1[2], (_Float16)a1[3]};
+                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), ry, off, 0, 2);
+                    } else {
+                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, a0), ry, off, 0, 2);
+                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, a1), ry, off + 16, 0, 2);
+                    }
+                }
+            return;
+        }
         constexpr int OB = PAIR ? HB * 2 : BN * EB;  // output bytes per tile row
         constexpr int CPR = OB / 16;                 // 16-byte pieces per tile row
         constexpr int RPP = 64 * NW / CPR;           // rows per pass
@@ -796,7 +932,10 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restr
                 __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), ry, off, 0, 2);
         }
     };
-    if constexpr (ROPE) {
+    if constexpr (LORA) {
+        staged(std::integral_constant<int, 4>{});  // the host guarantees N % 8 == 0 and 32-bit offsets
+        return;
+    } else if constexpr (ROPE) {
         staged(std::integral_constant<int, 4>{});  // f32 rows, rotated and written as fp16 q / k / v
         return;
     } else if constexpr (PAIR) {
@@ -870,7 +1009,7 @@ struct GemmPair {
 template <int BM, int BN, bool PINGPONG, int S, int NW, int WGN, int KG = 1, bool W2 = false, bool PAIR = false>
 int launch_tiled(const rq_qweight &w, const float *scales, int fmt, const void *x, void *y, rq_dtype yt, int64_t m,
                  int gm, int64_t cus, const GemmWorkspace &ws, hipStream_t s, const GemmPair &pair = GemmPair{},
-                 const RopeOut *rope = nullptr, const float *xscale = nullptr) {
+                 const RopeOut *rope = nullptr, const float *xscale = nullptr, const LoraDecode *ld = nullptr) {
     const int64_t N = w.n_out, K = w.k_in;
     const int tiles_m = (int)cdiv(m, BM), tiles_n = (int)cdiv(N, BN);
     const int64_t tiles = (int64_t)tiles_m * tiles_n;
@@ -887,8 +1026,17 @@ int launch_tiled(const rq_qweight &w, const float *scales, int fmt, const void *
                            scales, (const _Float16 *)x, y, yt == RQ_F16 ? 1 : 0, (int)m, (int)N, (int)K, tiles_m,
                            tiles_n, gm < 1 ? 1 : gm, (int)splits, ws.partials, ws.counters, fmt == 1 ? w.group : 64,
                            pair.w, pair.scales, (int)(pair.n_split ? pair.n_split : N), rope ? *rope : RopeOut{},
-                           xscale);
+                           xscale, ld ? *ld : LoraDecode{});
     };
+    if constexpr (BM == 128 && NW == 8 && !PAIR) {
+        if (ld) {
+            if (fmt == 1) go(k_gemm_rowwise<BM, BN, PINGPONG, S, NW, WGN, KG, W2, 1, false, false, true>);
+            else go(k_gemm_rowwise<BM, BN, PINGPONG, S, NW, WGN, KG, W2, 0, false, false, true>);
+            RQ_LAUNCH_CHECK();
+            return RQ_OK;
+        }
+    }
+    if (ld) return RQ_ERR_UNSUPPORTED;
     if constexpr (BN == 64 && !PAIR) {
         if (rope) {
             if (fmt == 1) go(k_gemm_rowwise<BM, BN, PINGPONG, S, NW, WGN, KG, W2, 1, false, true>);
@@ -1160,7 +1308,7 @@ int choose_pair_tile(int fmt, int64_t m, int64_t N, int64_t nk, int64_t cus) {
 // The fp16-activation GEMM over m rows, tile chosen by shape.
 int gemm_tiles(const rq_qweight &w, const float *scales, int fmt, const void *x, void *y, rq_dtype yt, int64_t m,
                int64_t cus, const GemmWorkspace &ws, hipStream_t s, const GemmPair &pair = GemmPair{},
-               const float *xscale = nullptr) {
+               const float *xscale = nullptr, const LoraDecode *ld = nullptr) {
     // Groups of 4 token panels per XCD and the ping-pong fragments beat
     // token-major order and single buffering by 5-15 % at m = 2048.  The tiles
     // of 128 columns and more run two k-groups of 4 waves with the weight staged
@@ -1179,7 +1327,7 @@ int gemm_tiles(const rq_qweight &w, const float *scales, int fmt, const void *x,
         }
     }
     const GemmPair np{};
-    auto go = [&](auto launch) { return launch(w, scales, fmt, x, y, yt, m, 4, cus, ws, s, np, nullptr, xscale); };
+    auto go = [&](auto launch) { return launch(w, scales, fmt, x, y, yt, m, 4, cus, ws, s, np, nullptr, xscale, ld); };
     switch (choose_tile(fmt, m, N, nk, cus)) {
     case T128x256: return go(launch_tiled<128, 256, true, 4, 8, 4, 2, true>);
     case T192x128: return go(launch_tiled<192, 128, true, 4, 8, 2, 2, true>);
@@ -1281,7 +1429,7 @@ int launch_gemm_f16_scaled(const rq_qweight &w, const float *scales, const _Floa
 }
 
 int launch_gemm(const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dtype yt, int64_t m, int num_cus,
-                const GemmWorkspace &ws, hipStream_t s) {
+                const GemmWorkspace &ws, hipStream_t s, const LoraDecode *ld) {
     const int64_t N = w.n_out, K = w.k_in;
     const int fmt = w.format == RQ_Q_AFFINE_U8 ? 1 : 0;
     // 32-bit buffer offsets: a 256-row panel of X (256 * K * 2 bytes) must stay below 2^31.
@@ -1291,10 +1439,18 @@ int launch_gemm(const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dty
     if (yt == RQ_F16 ? !aligned(y, 8) : !aligned(y, 16)) return RQ_ERR_UNSUPPORTED;
     if (!aligned(x, 16)) return RQ_ERR_UNSUPPORTED;
     const int64_t cus = num_cus > 0 ? num_cus : 256;
-    if (fmt == 0 && xt == RQ_F16) return gemm_tiles(w, w.scales, 0, x, y, yt, m, cus, ws, s);
+    // adapters: tiles of 128 tokens and 8 waves, whole 16-byte pieces of B and Y
+    if (ld) {
+        const int id = choose_tile(fmt, m, N, K / 64, cus);
+        if ((id != T128x256 && id != T128x128) || !ld->f16 || N % 8 != 0 || !aligned(ld->b, 16) || !aligned(y, 16) ||
+            128 * N * 4 > 0x7fffffff)
+            return RQ_ERR_UNSUPPORTED;
+    }
+    const GemmPair none{};
+    if (fmt == 0 && xt == RQ_F16) return gemm_tiles(w, w.scales, 0, x, y, yt, m, cus, ws, s, none, nullptr, ld);
     // affine scales: the table prepared at load, else built here per call
     const bool table = fmt == 1 && w.prep && affine_prep_bytes(w) > 0;
-    if (fmt == 1 && table && xt == RQ_F16) return gemm_tiles(w, w.prep, 1, x, y, yt, m, cus, ws, s);
+    if (fmt == 1 && table && xt == RQ_F16) return gemm_tiles(w, w.prep, 1, x, y, yt, m, cus, ws, s, none, nullptr, ld);
     if (!ws.prep) return RQ_ERR_UNSUPPORTED;
     uint8_t *prep = static_cast<uint8_t *>(ws.prep);
     size_t used = 0;
@@ -1308,12 +1464,12 @@ int launch_gemm(const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dty
         scales = sct;
         used = sc_bytes;
     }
-    if (xt == RQ_F16) return gemm_tiles(w, scales, fmt, x, y, yt, m, cus, ws, s);
+    if (xt == RQ_F16) return gemm_tiles(w, scales, fmt, x, y, yt, m, cus, ws, s, none, nullptr, ld);
     // f32 activations: cast a chunk of rows (a multiple of 128) to fp16, each
     // row scaled by a power of two (the factors after the rows), multiply it
     const size_t row_bytes = (size_t)K * 2 + 4;
     const int64_t chunk = std::min<int64_t>(m, (int64_t)((ws.prep_bytes - used - 256) / row_bytes) / 128 * 128);
-    if (chunk < std::min<int64_t>(m, 128)) return RQ_ERR_UNSUPPORTED;
+    if (chunk < std::min<int64_t>(m, 128) || (ld && chunk < m)) return RQ_ERR_UNSUPPORTED;
     _Float16 *x16 = reinterpret_cast<_Float16 *>(prep + used);
     float *xs = reinterpret_cast<float *>(prep + used + (((size_t)chunk * K * 2 + 255) & ~size_t(255)));
     const size_t eb = yt == RQ_F16 ? 2 : 4;
@@ -1328,7 +1484,7 @@ int launch_gemm(const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dty
         else hipLaunchKernelGGL(k_cast_f16_rows<0>, dim3((unsigned)mc), dim3(256), 0, s, xc, x16, xs, (int)K);
         RQ_LAUNCH_CHECK();
         const int st = gemm_tiles(w, scales, fmt, x16, static_cast<uint8_t *>(y) + (size_t)r0 * (size_t)N * eb, yt, mc,
-                                  cus, ws, s, GemmPair{}, xs);
+                                  cus, ws, s, none, xs, ld);
         if (st != RQ_OK) return st;
     }
     return RQ_OK;

@@ -534,10 +534,11 @@ int rq_qmatmul_loras(rq_ctx *ctx, const rq_qweight *w, const rq_lora_set *set, c
     const bool adapters = set->n_adapters > 0;
     if (adapters && (st = run_in(p, x_dtype, set->dtype, ctx->num_cus, s)) != RQ_OK) return st;
     if (!adapters) return qmatmul_dispatch(ctx, *w, x, x_dtype, y, y_dtype, m, gemm_workspace(ctx, s), s);
-    // One or two rows: the decode GEMV adds its rows' adapters itself.
-    if (m <= 2 && w->format != RQ_Q_AFFINE_U4 && w->k_in > 0) {
+    // One or two rows, and many: the product's kernel adds its rows' adapters itself, where it does.
+    if (w->format != RQ_Q_AFFINE_U4 && w->k_in > 0 && (m <= 2 || m > kFewRows)) {
         const LoraDecode ld{p.b, p.factors, p.part, p.ids, p.ranks, p.n_adapters, p.rank, p.slices, set->dtype == RQ_F16};
-        st = launch_gemv_decode_loras(*w, x, x_dtype, y, y_dtype, (int)m, ld, s);
+        st = m <= 2 ? launch_gemv_decode_loras(*w, x, x_dtype, y, y_dtype, (int)m, ld, s)
+                    : launch_gemm(*w, x, x_dtype, y, y_dtype, m, ctx->num_cus, gemm_workspace(ctx, s), s, &ld);
         if (st != RQ_ERR_UNSUPPORTED) return st;
     }
     if ((st = qmatmul_dispatch(ctx, *w, x, x_dtype, const_cast<float *>(p.main), RQ_F32, m, gemm_workspace(ctx, s), s)) != RQ_OK)

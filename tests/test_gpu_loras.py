@@ -6,10 +6,12 @@ Tolerance, per output, u = 2^-24, W the shared weight, P = sum |x| |W|, T_r = su
   * t_r = x . A_r, f32 sums of exact or rounded products: (k + 8) u T_r;
   * factor t . B, f32: (rank + 8) u of sum |f t_r b_r|, and t's error in it;
   * their sum (u) and the rounding to the output's type: 2^-11 (fp16, at least 2^-25) or u."""
+import ctypes
+
 import numpy as np
 import pytest
 
-from rusty_amd import DType, LoraSet, QuantizedTensor, UnifiedTensor, synth
+from rusty_amd import DType, LoraSet, QuantizedTensor, UnifiedTensor, _lib, synth
 from rusty_amd._lib import call
 from rusty_amd.hiprt import Graph, Stream
 
@@ -305,3 +307,40 @@ def test_one_and_two_rows(ctx, engine, x_t, y_t, a_t, form, m, n, k, rank):
     g = np.random.default_rng(n)
     for ids in ([0, 2], [1, 1], [-1, 1], [2, 5]):
         case(ctx, engine, n + k + ids[0] + 7, m, n, k, 3, rank, form, x_t, y_t, a_t, ids=ids[:m], some_ranks=bool(g.integers(2)))
+
+
+def tile(form, m, n, k):
+    f = _lib.lib().rusty_gemm_tile
+    f.argtypes, f.restype = [ctypes.c_int] + [ctypes.c_int64] * 3 + [ctypes.c_int] * 2, ctypes.c_int
+    return f(int(form != "rowwise8"), m, n, k, 256, 0)
+
+
+@pytest.mark.parametrize("x_t,y_t", [("f16", "f16"), ("f32", "f32"), ("f16", "f32"), ("f32", "f16")])
+@pytest.mark.parametrize("form,m,n,k,rank,want", [("rowwise8", 1100, 5640, 192, 32, 128256), ("rowwise8", 515, 10264, 64, 70, 128256),
+                                                  ("affine8", 900, 6152, 192, 21, 128256), ("affine8", 700, 3712, 128, 40, 128128),
+                                                  ("rowwise8", 1024, 4096, 1024, 16, 128128)])
+def test_in_the_products_tiles(ctx, engine, form, m, n, k, rank, want, x_t, y_t):
+    """Where the shared product takes tiles of 128 rows and 8 waves, its kernel adds the adapters: prompts of one adapter
+    behind another, and every row another one, with ranks that differ."""
+    assert tile(form, m, n, k) == want
+    g = np.random.default_rng(m)
+    prompts = np.repeat(g.integers(-1, 5, m // 90 + 1), 90)[:m]
+    case(ctx, engine, m, m, n, k, 5, rank, form, x_t, y_t, "f16", ids=prompts)
+    case(ctx, engine, m + 1, m, n, k, 5, rank, form, x_t, y_t, "f16", ids=g.integers(-1, 6, m), some_ranks=True)
+
+
+def test_in_the_products_tiles_not_finite(ctx, engine):
+    """Adapters that hold infinities and NaN, in the same tiles as rows of others: those rows are as without them."""
+    g = np.random.default_rng(16)
+    m, n, k = 1100, 5640, 192
+    w, w64 = weight(ctx, g, n, k, "rowwise8")
+    a, b = adapters(g, 4, 40, k, n, "f16")
+    a[1], b[1], b[2, :, ::3], b[3, 33] = np.nan, np.inf, np.inf, np.nan
+    x = g.standard_normal((m, k)).astype(np.float16)
+    ids = g.integers(-1, 4, m)
+    want, tol = truth(x, w64, a[:1], b[:1], np.ones(4), np.where(ids == 0, 0, -1), [40], "f16", False)
+    got = run(ctx, engine, x, w, a, b, None, ids, [40, 40, 40, 33], "f16", "f16", "f16")
+    own = (ids == 0) | (ids == -1)
+    check(got[own], want[own], tol[own], "rows beside")
+    assert not np.isfinite(got[ids == 1]).any() and not np.isfinite(got[ids == 2][:, ::3]).any()
+    assert np.isfinite(got[ids == 3]).all()
