@@ -205,9 +205,10 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restr
     constexpr int RING_X = W2 ? S * BM * 128 + 2 * BN * 128 : S * (BM * 128 + BN * 64);  // X and W stages
     constexpr int RING_K = RING_X + S * SCB;  // k-loop stages
     // the epilogue reuses the ring to stage a tile of f32 (or fp16) rows
-    // (LORA: and 32 ranks of an adapter's B behind it)
-    constexpr int STAGED = BM * (BN * 4 + 16) + (LORA ? 32 * BN * 2 : 0);
-    constexpr int RING = RING_K > STAGED ? RING_K : STAGED;
+    constexpr int STAGED = BM * (BN * 4 + 16);
+    constexpr int LORA_B = RING_K > STAGED ? RING_K : STAGED;  // LORA: 32 ranks of an adapter's B, then the tokens' adapters
+    constexpr int LORA_I = LORA_B + 32 * BN * 2;
+    constexpr int RING = LORA ? LORA_I + BM * 4 : LORA_B;
     static_assert(S >= 3 && RING <= 160 * 1024, "ring does not fit in LDS");
     constexpr int XOPS = XUW + (FMT == 1 ? 1 : 0);  // DMA ops per wave issued with each X stage
     constexpr int NOUT = XOPS + WUW;  // DMA ops per wave per k-step (W2: W on odd steps only)
@@ -300,6 +301,9 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restr
             for (int q = 0; q < WUW; ++q) dma16(rw, sw + (uint32_t)(wave * WUW + q) * 1024u, live ? woff[q] + kt * 64 : kOOB);
         }
     };
+    if constexpr (LORA)
+        if (wave < BM / 64)
+            dma4(make_rsrc(ld.ids + m0, (uint32_t)min(BM, M - m0) * 4u), ring_lds + (uint32_t)(LORA_I + wave * 256), (uint32_t)t * 4u);
     // W2: the weight of steps kt, kt + 1 (kt even) into pair slot `pair`.  The
     // second step past this block's k range reads the next bytes of the row
     // (or zeros past the weight): finite codes that only meet zero activations.
@@ -538,7 +542,52 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restr
             }
         }
     }
-    wait_vmcnt<0>();  // no DMA in flight past this point
+    wait_vmcnt<0>();  // no DMA in flight past this point (LORA: but the first B)
+
+    // LORA: the adapters of the tile's tokens, lane l's of tokens l and l + 64 (-1: none); the one whose turn it is (li, -1: none
+    // left) and its ranks; and which of this wave's 16 rows have it
+    int ida = -1, idb = -1, li = -1, lrank = 0;
+    uint32_t own = 0;
+    uint64_t la = 0, lb = 0;
+    auto next_adapter = [&] {
+        li = -1;
+        while (li < 0 && (la | lb)) {
+            const int i = la ? __builtin_amdgcn_readlane(ida, __builtin_ctzll(la | 1ull << 63))
+                             : __builtin_amdgcn_readlane(idb, __builtin_ctzll(lb | 1ull << 63));
+            const uint64_t sa = __builtin_amdgcn_ballot_w64(ida == i), sb = __builtin_amdgcn_ballot_w64(idb == i);
+            la &= ~sa;
+            lb &= ~sb;
+            own = (uint32_t)((wave < 4 ? sa : sb) >> (16 * (wave & 3))) & 0xffffu;
+            lrank = ld.ranks ? min(max(ld.ranks[i], 0), ld.rank) : ld.rank;
+            if (lrank > 0) li = i;
+        }
+    };
+    // 32 ranks of its B from r0 on to LDS, chunk s of row r holding global chunk s ^ swz(r): a transposing read's 4 rows
+    // x 4 pieces cover the banks
+    constexpr int CH = BN / 8, RPU = 64 / CH, BU = LORA ? 32 * BN * 2 / 1024 / NW : 1;
+    auto swz = [](int r) { return (r & 1) | (r & 2) << 2; };
+    auto fetch_b = [&](int r0) {
+        const _Float16 *b = static_cast<const _Float16 *>(ld.b) + (int64_t)li * ld.rank * N;
+#pragma unroll
+        for (int q = 0; q < BU; ++q) {
+            const int r = (wave * BU + q) * RPU + lane / CH, n = min(n0 + (lane % CH ^ swz(r)) * 8, N - 8);
+            dma16_kept(reinterpret_cast<const char *>(b + (int64_t)min(r0 + r, lrank - 1) * N + n),
+                       ring_lds + (uint32_t)(LORA_B + (wave * BU + q) * 1024));
+        }
+    };
+    if constexpr (LORA) {
+        __syncthreads();  // the adapters have landed
+        auto of = [&](int row) {
+            const int i = reinterpret_cast<const int *>(&ring[LORA_I])[row];
+            return m0 + row < M && (uint32_t)i < (uint32_t)ld.n_adapters ? i : -1;
+        };
+        ida = of(lane);
+        idb = of(64 + lane);
+        la = __builtin_amdgcn_ballot_w64(ida >= 0);
+        lb = __builtin_amdgcn_ballot_w64(idb >= 0);
+        next_adapter();
+        if (li >= 0) fetch_b(0);
+    }
 
     if constexpr (KG == 2) {
         // Group g finishes its half of the wave tile (see mine): it hands its
@@ -707,16 +756,6 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restr
         constexpr int RS = BN * EB + 16;           // padded LDS row stride
         static_assert(BM * RS <= RING, "output staging does not fit in the ring");
         uint8_t *ot = reinterpret_cast<uint8_t *>(&ring[0]);
-        // LORA: the adapters of the tile's tokens, lane l's of tokens l and l + 64; -1: none
-        auto adapter_of = [&](int row) {
-            const int i = row < M ? ld.ids[row] : -1;
-            return (uint32_t)i < (uint32_t)ld.n_adapters ? i : -1;
-        };
-        int ida = -1, idb = -1;
-        if constexpr (LORA) {
-            ida = adapter_of(m0 + lane);
-            idb = adapter_of(m0 + 64 + lane);
-        }
         __syncthreads();  // every wave is done with the ring (and the k-group exchange)
 #pragma unroll
         for (int i = 0; i < FN; ++i) {
@@ -746,7 +785,7 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restr
                 }
             }
         }
-        __syncthreads();
+        if constexpr (!LORA) __syncthreads();
         if constexpr (ROPE) {
             // 8 threads per tile row: thread c rotates the pairs (4c + e, 4c + e + 32)
             const int c = t % 8, hh = n0 / 64, kvh = hh - ro.n_heads;
@@ -779,32 +818,22 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restr
             return;
         }
         if constexpr (LORA) {
-            constexpr int CB = BN / 64, CH = BN / 8, RPU = 64 / CH, BU = 32 * BN * 2 / 1024 / NW;
+            constexpr int CB = BN / 64;
             typedef short short4v __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) short4v lds_short4;
-            // chunk s of B's row r holds global chunk s ^ swz(r): a transposing read's 4 rows x 4 pieces cover the banks
-            auto swz = [](int r) { return (r & 1) | (r & 2) << 2; };
-            uint8_t *bt = ot + BM * RS;
             const int col = lane & 15, qt = lane >> 4, row = wave * 16 + col, ranks4 = (ld.rank + 3) / 4 * 4;
             floatx4 out[CB][4];
 #pragma unroll
             for (int c = 0; c < CB; ++c)
 #pragma unroll
                 for (int v = 0; v < 4; ++v) out[c][v] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-            uint64_t la = __builtin_amdgcn_ballot_w64(ida >= 0), lb = __builtin_amdgcn_ballot_w64(idb >= 0);
+            if (li < 0) __syncthreads();
+            bool first = true;
 #pragma unroll 1
-            while (la | lb) {
-                const int i = la ? __builtin_amdgcn_readlane(ida, __builtin_ctzll(la | 1ull << 63))
-                                 : __builtin_amdgcn_readlane(idb, __builtin_ctzll(lb | 1ull << 63));
-                const uint64_t sa = __builtin_amdgcn_ballot_w64(ida == i), sb = __builtin_amdgcn_ballot_w64(idb == i);
-                la &= ~sa;
-                lb &= ~sb;
-                const uint32_t own = (uint32_t)((wave < 4 ? sa : sb) >> (16 * (wave & 3))) & 0xffffu;
-                const int rank = ld.ranks ? min(max(ld.ranks[i], 0), ld.rank) : ld.rank;
-                const float f = ld.factors ? ld.factors[i] : 1.0f;
-                const _Float16 *b = static_cast<const _Float16 *>(ld.b) + (int64_t)i * ld.rank * N;
+            while (li >= 0) {
+                const float f = ld.factors ? ld.factors[li] : 1.0f;
 #pragma unroll 1
-                for (int r0 = 0; r0 < rank; r0 += 32) {
+                for (int r0 = 0; r0 < lrank; r0 += 32) {
                     // t of this lane's row, ranks r0 + 8 qt ..: the slices summed in order
                     floatx4 tv[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
                     const int r1 = r0 + 8 * qt;
@@ -818,27 +847,24 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restr
                                     tv[u] += *reinterpret_cast<const floatx4 *>(q + (int64_t)j * ranks4 + 4 * u);
                             }
                     }
-                    __syncthreads();  // the last ranks' B have been read
-#pragma unroll
-                    for (int q = 0; q < BU; ++q) {
-                        const int r = (wave * BU + q) * RPU + lane / CH, n = min(n0 + (lane % CH ^ swz(r)) * 8, N - 8);
-                        dma16_kept(reinterpret_cast<const char *>(b + (int64_t)min(r0 + r, rank - 1) * N + n),
-                                   lds_addr(bt) + (uint32_t)((wave * BU + q) * 1024));
+                    if (!first || r0 > 0) {
+                        __syncthreads();  // the last ranks' B have been read
+                        fetch_b(r0);
                     }
                     wait_vmcnt<0>();
                     // (what lies past the rank is another rank's, and may be infinite)
 #pragma unroll
                     for (int q = 0; q < BU; ++q)
-                        if (r0 + (wave * BU + q) * RPU + lane / CH >= rank)
-                            *reinterpret_cast<uint4 *>(bt + (wave * BU + q) * 1024 + lane * 16) = make_uint4(0, 0, 0, 0);
-                    __syncthreads();
+                        if (r0 + (wave * BU + q) * RPU + lane / CH >= lrank)
+                            *reinterpret_cast<uint4 *>(&ring[LORA_B] + (wave * BU + q) * 1024 + lane * 16) = make_uint4(0, 0, 0, 0);
+                    __syncthreads();  // (the first: and the tile's rows are staged)
                     if (!own) continue;
                     float most = 0.0f;
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            tv[u][e] = r1 + 4 * u + e < rank ? f * tv[u][e] : 0.0f;
+                            tv[u][e] = r1 + 4 * u + e < lrank ? f * tv[u][e] : 0.0f;
                             most = fmaxf(most, __builtin_isfinite(tv[u][e]) ? fabsf(tv[u][e]) : 0.0f);
                         }
                     most = fmaxf(most, __shfl_xor(most, 16));
@@ -855,7 +881,7 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restr
                     const float scale = __builtin_ldexpf(1.0f, -ex);
                     const bool has = own >> col & 1;
                     // 16 lanes take 4 ranks x 4 x 4 columns; each gets one column's 4 ranks
-                    const uint32_t at = lds_addr(bt) + (uint32_t)((8 * qt + col / 4) * (BN * 2));
+                    const uint32_t at = ring_lds + (uint32_t)(LORA_B + (8 * qt + col / 4) * (BN * 2));
 #pragma unroll
                     for (int c = 0; c < CB; ++c)
 #pragma unroll
@@ -872,6 +898,8 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restr
                             for (int e = 0; e < 4; ++e) out[c][v][e] = has ? __builtin_fmaf(a[e], scale, out[c][v][e]) : out[c][v][e];
                         }
                 }
+                next_adapter();
+                first = false;
             }
             // lane: row `row`, columns 64 c + 16 qt + 4 v + e
             const int oe = y_f16 ? 2 : 4;
