@@ -289,8 +289,8 @@ int rq_qmatmul_lora_ex(rq_ctx *ctx, const rq_qweight *w, const void *x, rq_dtype
  * products), the weight's as rq_qmatmul's in f32; Y is rounded once.  m, k_in and n_out
  * go up to 2^24 - 256 (RQ_ERR_SHAPE past that); 16-byte loads are taken where k_in (for X and A)
  * and n_out (for B and Y) are multiples of 8 elements and the pointers 16-byte
- * aligned.  A row's result does not depend on the other rows' adapters, whatever they
- * hold.  workspace: rq_qmatmul_loras_workspace(...) bytes, 256-byte aligned, one
+ * aligned.  Nothing that another row's adapter holds reaches a row (which rows are beside
+ * it may change the rounding of its sums).  workspace: rq_qmatmul_loras_workspace(...) bytes, 256-byte aligned, one
  * per call in flight (a captured call keeps its own); Y overlaps no input.
  * Uses the context's GEMM workspace as rq_qmatmul does. */
 typedef struct rq_lora_set {

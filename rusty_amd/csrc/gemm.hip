@@ -144,6 +144,11 @@ __device__ __forceinline__ void tile_of(int b, int tiles_m, int tiles_n, int gm,
     tn = r / gsize;
 }
 
+// Adapters of a tile's rows that LORA (below) takes one after another (about 4 us each, 32 ranks); of more, its rows
+// are taken one by one (16 a wave, about 4 us each).  2048x4096x4096, rows' adapters at random among 12 / 64: 141 / 182 us,
+// one by one 143 / 182, in a pass of their own 130 / 179 (side by side, as prompts have them, 6: 81, 92).
+constexpr int kTileAdapters = 16;
+
 // FMT 0: per-row int8 codes, scales[n] applied in the epilogue.  FMT 1: the
 // reference's affine u8 codes with a scale and bias per group of G (a multiple
 // of 64) along k; `scales` then holds them transposed, per group g a row of N
@@ -549,6 +554,7 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restr
     int ida = -1, idb = -1, li = -1, lrank = 0;
     uint32_t own = 0;
     uint64_t la = 0, lb = 0;
+    bool many = false;  // the tile has more adapters than are taken one after another: row by row
     auto next_adapter = [&] {
         li = -1;
         while (li < 0 && (la | lb)) {
@@ -585,6 +591,9 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restr
         idb = of(64 + lane);
         la = __builtin_amdgcn_ballot_w64(ida >= 0);
         lb = __builtin_amdgcn_ballot_w64(idb >= 0);
+        for (int n = 0; (la | lb) && n <= kTileAdapters; many = ++n > kTileAdapters) next_adapter();
+        la = many ? 0 : __builtin_amdgcn_ballot_w64(ida >= 0);
+        lb = many ? 0 : __builtin_amdgcn_ballot_w64(idb >= 0);
         next_adapter();
         if (li >= 0) fetch_b(0);
     }
@@ -828,6 +837,42 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restr
 #pragma unroll
                 for (int v = 0; v < 4; ++v) out[c][v] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
             if (li < 0) __syncthreads();
+            if (many) {
+                // a row at a time: lanes CL columns each, the adapter's ranks one fma at a time, into the staged row
+                constexpr int CL = BN / 64, RC = 32;  // ranks at once
+                typedef _Float16 vecb __attribute__((ext_vector_type(CL)));
+                typedef float vecf __attribute__((ext_vector_type(CL)));
+                const int n = min(n0 + lane * CL, N - CL);
+#pragma unroll 1
+                for (int rr = 0; rr < 16; ++rr) {
+                    const int i = __builtin_amdgcn_readlane(wave < 4 ? ida : idb, (wave & 3) * 16 + rr);
+                    if (i < 0) continue;
+                    const int rank = ld.ranks ? min(max(ld.ranks[i], 0), ld.rank) : ld.rank;
+                    const float f = ld.factors ? ld.factors[i] : 1.0f;
+                    const _Float16 *b = static_cast<const _Float16 *>(ld.b) + (int64_t)i * ld.rank * N + n;
+                    const float *q = ld.part + (int64_t)(m0 + wave * 16 + rr) * ld.slices * ranks4;
+                    vecf sum = {};
+#pragma unroll 1
+                    for (int r0 = 0; r0 < rank; r0 += RC) {
+                        vecb bv[RC];
+#pragma unroll
+                        for (int u = 0; u < RC; ++u) bv[u] = *reinterpret_cast<const vecb *>(b + (int64_t)min(r0 + u, rank - 1) * N);
+                        // t of rank r0 + lane % 32, the wave's halves take every other slice
+                        float tr = 0.0f;
+                        if (r0 + (lane & 31) < rank)
+                            for (int j = lane >> 5; j < ld.slices; j += 2) tr += q[(int64_t)j * ranks4 + r0 + (lane & 31)];
+                        tr = f * (tr + __shfl_xor(tr, 32));
+#pragma unroll
+                        for (int u = 0; u < RC; ++u) {
+                            const bool live = r0 + u < rank;
+                            const float tu = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, tr), u));
+#pragma unroll
+                            for (int e = 0; e < CL; ++e) sum[e] = __builtin_fmaf(tu, live ? (float)bv[u][e] : 0.0f, sum[e]);
+                        }
+                    }
+                    *reinterpret_cast<vecf *>(ot + (wave * 16 + rr) * RS + lane * CL * 4) += sum;
+                }
+            }
             bool first = true;
 #pragma unroll 1
             while (li >= 0) {
@@ -1333,6 +1378,21 @@ int choose_pair_tile(int fmt, int64_t m, int64_t N, int64_t nk, int64_t cus) {
     return best;
 }
 
+// The tile of a product that adds its rows' adapters (LORA: those of 128 rows and 8 waves), -1 where the best
+// tile and the adapters in a pass of their own are faster.  Adding takes about 8 us a round of tiles, the pass and
+// the f32 product between 4 and 2.6 per million outputs, two of them kept as a margin (us, one adapter in
+// rank 16, apart / in the tiles: 2048x4096x4096 92 / 82, 1024x4096x4096 51.6 / 46.7, 2048x2560x2048 43.3 / 37.7,
+// 1293x4096x4096 65 / 61.5, 3000x4096x4096 131 / 131, 777x11008x4096 112 / 120, 512x4096x4096 34.4 / 37.5).
+int choose_lora_tile(int fmt, int64_t m, int64_t N, int64_t nk, int64_t cus) {
+    const int best = choose_tile(fmt, m, N, nk, cus);
+    const int id = best == T128x256 || best == T128x128                                                       ? best
+                   : tile_cost(T128x256, fmt, m, N, nk, cus) < tile_cost(T128x128, fmt, m, N, nk, cus) ? T128x256
+                                                                                                              : T128x128;
+    const int64_t rounds = cdiv(cdiv(m, kTile[id].bm) * cdiv(N, kTile[id].bn), cus);
+    const double apart = tile_cost(best, fmt, m, N, nk, cus) + 2.0 + 2.6e-6 * (double)m * (double)N;
+    return tile_launches(id, m, N) && tile_cost(id, fmt, m, N, nk, cus) + 8.0 * (double)rounds < apart ? id : -1;
+}
+
 // The fp16-activation GEMM over m rows, tile chosen by shape.
 int gemm_tiles(const rq_qweight &w, const float *scales, int fmt, const void *x, void *y, rq_dtype yt, int64_t m,
                int64_t cus, const GemmWorkspace &ws, hipStream_t s, const GemmPair &pair = GemmPair{},
@@ -1356,7 +1416,7 @@ int gemm_tiles(const rq_qweight &w, const float *scales, int fmt, const void *x,
     }
     const GemmPair np{};
     auto go = [&](auto launch) { return launch(w, scales, fmt, x, y, yt, m, 4, cus, ws, s, np, nullptr, xscale, ld); };
-    switch (choose_tile(fmt, m, N, nk, cus)) {
+    switch (ld ? choose_lora_tile(fmt, m, N, nk, cus) : choose_tile(fmt, m, N, nk, cus)) {
     case T128x256: return go(launch_tiled<128, 256, true, 4, 8, 4, 2, true>);
     case T192x128: return go(launch_tiled<192, 128, true, 4, 8, 2, 2, true>);
     case T128x128: return go(launch_tiled<128, 128, true, 4, 8, 2, 2, true>);
@@ -1469,8 +1529,7 @@ int launch_gemm(const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dty
     const int64_t cus = num_cus > 0 ? num_cus : 256;
     // adapters: tiles of 128 tokens and 8 waves, whole 16-byte pieces of B and Y
     if (ld) {
-        const int id = choose_tile(fmt, m, N, K / 64, cus);
-        if ((id != T128x256 && id != T128x128) || !ld->f16 || N % 8 != 0 || !aligned(ld->b, 16) || !aligned(y, 16) ||
+        if (choose_lora_tile(fmt, m, N, K / 64, cus) < 0 || !ld->f16 || N % 8 != 0 || !aligned(ld->b, 16) || !aligned(y, 16) ||
             128 * N * 4 > 0x7fffffff)
             return RQ_ERR_UNSUPPORTED;
     }
@@ -1523,10 +1582,11 @@ int launch_gemm(const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dty
 // For the tests, no part of the C ABI: the tile (bm * 1000 + bn) that the
 // fp16-activation GEMM takes for an m x n_out x k_in product (fmt 0: per-row
 // codes, 1: affine), or with `pair` for SwiGLU's gate and up of n_out rows
-// each; -1 where the two are multiplied one after the other.  Host arithmetic.
+// each (1), or with an adapter per row (2); -1 where the parts run one after the other.  Host arithmetic.
 extern "C" int rusty_gemm_tile(int fmt, int64_t m, int64_t n_out, int64_t k_in, int num_cus, int pair) {
     using namespace rq;
-    const int id = pair ? choose_pair_tile(fmt, m, 2 * n_out, k_in / 64, num_cus)
-                        : choose_tile(fmt, m, n_out, k_in / 64, num_cus);
+    const int id = pair == 2 ? choose_lora_tile(fmt, m, n_out, k_in / 64, num_cus)
+                   : pair    ? choose_pair_tile(fmt, m, 2 * n_out, k_in / 64, num_cus)
+                             : choose_tile(fmt, m, n_out, k_in / 64, num_cus);
     return id < 0 ? -1 : kTile[id].bm * 1000 + kTile[id].bn;
 }

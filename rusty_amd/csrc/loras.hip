@@ -7,7 +7,8 @@
 // once.  Small batches are bound by the launches and by the weight's bytes, which
 // each used adapter adds (k_in + n_out) rank elements to; prompts by the shared product.
 //
-// One or two rows of 8-bit codes take two launches: the decode GEMV adds its rows' adapters itself.
+// One or two rows of 8-bit codes, and prompts for which the product takes tiles of 128 rows, take
+// two launches: the decode GEMV or the GEMM adds its rows' adapters itself.
 //
 // k_loras_in: rows of X are the rows of a matrix instruction, 16 rows of A_i its
 // columns, k runs along both (16-byte loads, no LDS).  Rows of a tile may have
@@ -20,10 +21,11 @@
 // instructions, an adapter of theirs after another (f32 B: f32 instructions; fp16 B:
 // t as two fp16 terms).
 //
-// Measured (us, 4096 x 4096; X . A / shared product / t . B; the bytes at 6.9 TB/s, the products at 1157
-// TFLOP/s): one row, 8-bit rows, rank 16: 3.3 / 5.1 with t . B, 8.6 a call (2.5; in three launches 3.3 / 4.7 / 2.7, 12.3); 61 rows of 11 adapters, 4-bit groups,
-// f32 rows, rank 32: 5.0 / 16.8 / 3.9 (4.9); 2048 rows, 8-bit, rank 32: 9.4 / 66 / 18.9 (60).  One launch for X . A and
-// the shared product of a few rows took 8 us where the two take 6.1.
+// Measured (us, 4096 x 4096; X . A / shared product / t . B; in brackets the bytes at 6.9 TB/s or the products at
+// 1157 TFLOP/s): one row, 8-bit rows, rank 16: 3.2 / 5.7 with t . B, 8.7 a call (2.5; apart 3.3 / 4.7 / 2.7, 12.3);
+// 61 rows of 11 adapters, 4-bit groups, f32 rows, rank 32: 5.0 / 16.8 / 3.9 (4.9); 2048 rows, 8-bit, rank 32: 9.4 / 70
+// with t . B, 80 a call (60; apart 9.4 / 66 / 18.9, 91).  X . A and the shared product of a few rows in one launch took
+// 8 us, 6.1 in two.
 #include <algorithm>
 #include <type_traits>
 

@@ -312,7 +312,7 @@ def test_one_and_two_rows(ctx, engine, x_t, y_t, a_t, form, m, n, k, rank):
 def tile(form, m, n, k):
     f = _lib.lib().rusty_gemm_tile
     f.argtypes, f.restype = [ctypes.c_int] + [ctypes.c_int64] * 3 + [ctypes.c_int] * 2, ctypes.c_int
-    return f(int(form != "rowwise8"), m, n, k, 256, 0)
+    return f(int(form != "rowwise8"), m, n, k, 256, 2)
 
 
 @pytest.mark.parametrize("x_t,y_t", [("f16", "f16"), ("f32", "f32"), ("f16", "f32"), ("f32", "f16")])
@@ -344,3 +344,19 @@ def test_in_the_products_tiles_not_finite(ctx, engine):
     check(got[own], want[own], tol[own], "rows beside")
     assert not np.isfinite(got[ids == 1]).any() and not np.isfinite(got[ids == 2][:, ::3]).any()
     assert np.isfinite(got[ids == 3]).all()
+
+
+@pytest.mark.parametrize("x_t,y_t", [("f16", "f16"), ("f32", "f32")])
+@pytest.mark.parametrize("form,m,n,k,rank,want", [("rowwise8", 1100, 5640, 192, 32, 128256), ("affine8", 700, 3712, 128, 90, 128128)])
+@pytest.mark.parametrize("count", [8, 16, 17, 60])
+def test_in_the_products_tiles_many_adapters(ctx, engine, form, m, n, k, rank, want, count, x_t, y_t):
+    """More adapters in a tile's rows than are taken one after another."""
+    assert tile(form, m, n, k) == want
+    g = np.random.default_rng(count)
+    case(ctx, engine, m, m, n, k, count, rank, form, x_t, y_t, "f16", ids=g.integers(-1, count, m), some_ranks=count == 60)
+
+
+def test_tiles_that_add_adapters():
+    """Where the product's tiles add the adapters, and where they are added in a pass of their own."""
+    assert [tile("rowwise8", m, n, 4096) for m, n in ((2048, 4096), (1024, 4096), (1293, 4096))] == [128256, 128128, 128256]
+    assert [tile("rowwise8", m, n, 4096) for m, n in ((300, 4096), (512, 4096), (777, 11008))] == [-1, -1, -1]
