@@ -360,3 +360,76 @@ def test_tiles_that_add_adapters():
     """Where the product's tiles add the adapters, and where they are added in a pass of their own."""
     assert [tile("rowwise8", m, n, 4096) for m, n in ((2048, 4096), (1024, 4096), (1293, 4096))] == [128256, 128128, 128256]
     assert [tile("rowwise8", m, n, 4096) for m, n in ((300, 4096), (512, 4096), (777, 11008))] == [-1, -1, -1]
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 256, 512), (2, 256, 512), (1100, 5640, 192)])
+@pytest.mark.parametrize("own", [True, False])
+def test_graph_of_two_launches(ctx, engine, m, n, k, own):
+    """The forms in which the product's kernel adds the adapters, captured on the context's stream or another, replayed with
+    other ids between eager calls."""
+    g = np.random.default_rng(m)
+    other = Stream()
+    stream = ctx.stream if own else other.h
+    w, w64 = weight(ctx, g, n, k, "rowwise8")
+    a, b = adapters(g, 4, 16, k, n, "f16")
+    s = LoraSet(dev(ctx, a), dev(ctx, b))
+    x = g.standard_normal((m, k)).astype(np.float16)
+    X, I = dev(ctx, x), dev(ctx, np.zeros(m, np.int32), DType.I32)
+    outs = [dev(ctx, np.zeros((m, n), np.float16)) for _ in range(2)]
+    works = [engine.qmatmul_loras_workspace(ctx, X, w, s, outs[0]) for _ in range(2)]
+    ctx.sync()
+    graph = Graph(stream, lambda: engine.qmatmul_loras(ctx, X, w, s, I, outs[0], workspace=works[0],
+                                                       stream=None if own else stream))
+    for i in range(3):
+        ids = g.integers(-1, 4, m).astype(np.int32)
+        call("rq_memcpy_h2d", ctx.handle, I.ptr, ids.ctypes.data, ids.nbytes, None)
+        ctx.sync()
+        graph.launch()
+        if not own:
+            other.synchronize()
+        want, tol = truth(x, w64, a, b, np.ones(4), ids, [16] * 4, "f16", False)
+        check(outs[0].to_vec(), want, tol, f"replay {i}")
+        engine.qmatmul_loras(ctx, X, w, s, I, outs[1], workspace=works[1])
+        assert np.array_equal(outs[1].to_vec(), outs[0].to_vec())
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 128, 256), (2, 128, 256), (1100, 5640, 192)])
+@pytest.mark.parametrize("exp", [-60, -20, 14, 40])
+def test_large_and_small_products_of_two_launches(ctx, engine, m, n, k, exp):
+    """t far outside fp16's range, and far below it, in rows side by side."""
+    g = np.random.default_rng(18)
+    rank, count = 40, 4
+    w = QuantizedTensor.rowwise(ctx, np.zeros((n, k), np.int8), np.ones(n, np.float32))
+    a, b = adapters(g, count, rank, k, n, "f16")
+    f = np.array([2.0 ** exp, 1.0, 2.0 ** (exp // 2), -1.0], np.float32)
+    x = g.standard_normal((m, k)).astype(np.float16)
+    ids = np.arange(m) % count
+    want, tol = truth(x, np.zeros((n, k)), a, b, f, ids, [rank] * count, "f32", False)
+    check(run(ctx, engine, x, w, a, b, f, ids, None, "f16", "f32", "f16"), want, tol, f"factors 2^{exp}")
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 64, 64), (2, 64, 64), (1100, 5640, 64)])
+def test_infinite_beside_large_of_two_launches(ctx, engine, m, n, k):
+    w = QuantizedTensor.rowwise(ctx, np.zeros((n, k), np.int8), np.ones(n, np.float32))
+    a, b = np.full((2, 2, k), 6e4, np.float16), np.ones((2, 2, n), np.float16)
+    a[0, 1], b[0, 1, ::2] = 1e-3, -1.0
+    a[1] = 1e-30  # (zero in fp16)
+    x = np.full((m, k), 1e34, np.float32)
+    ids = np.arange(m) % 2
+    got = run(ctx, engine, x, w, a, b, None, ids, None, "f32", "f32", "f16")
+    assert np.all(got[0::2] == np.inf) and np.all(got[1::2] == 0.0)
+
+
+def test_one_row_off_its_alignment(ctx, engine):
+    """Activations and results in whatever place their elements allow: the decode form is left for others."""
+    g = np.random.default_rng(19)
+    w, w64 = weight(ctx, g, 72, 128, "rowwise8")
+    a, b = adapters(g, 2, 8, 128, 72, "f16")
+    s = LoraSet(dev(ctx, a), dev(ctx, b))
+    x = g.standard_normal((2, 128)).astype(np.float16)
+    held, out = dev(ctx, np.concatenate([np.zeros(1, np.float16), x.ravel()])), dev(ctx, np.zeros(145, np.float16))
+    X, Y = UnifiedTensor(ctx, held.ptr + 2, (2, 128), DType.FP16, owner=False), UnifiedTensor(ctx, out.ptr + 2, (2, 72), DType.FP16, owner=False)
+    engine.qmatmul_loras(ctx, X, w, s, dev(ctx, np.array([1, 0], np.int32), DType.I32), Y)
+    got = out.to_vec()
+    check(got[1:].reshape(2, 72), *truth(x, w64, a, b, np.ones(2), [1, 0], [8, 8], "f16", False), "off alignment")
+    assert got[0] == 0.0
