@@ -173,7 +173,8 @@ constexpr int kTileAdapters = 16;
 // wave takes 16 of them, and for each adapter of the tile's tokens, 32 ranks at a time (their B to
 // LDS by all waves), adds B^T . t^T on the matrix instructions: t, scaled by a power of two per
 // row, as two fp16 terms (off by at most 2^-22), B's fragments by transposing LDS reads.
-// Then the rows are rounded and written.  Products of rows that have another adapter are dropped, not
+// Then the rows are rounded and leave in whole pieces (straight from the fragments, 32 bytes a lane, they were
+// written twice: 2048x4096x4096 80.6 us, so 78.6; 2048x11008x4096 203, 190).  Products of rows that have another adapter are dropped, not
 // added as zeros, so nothing a foreign adapter holds reaches a row.
 template <int BM, int BN, bool PINGPONG, int S, int NW, int WGN, int KG = 1, bool W2 = false, int FMT = 0,
           bool PAIR = false, bool ROPE = false, bool LORA = false>
@@ -946,26 +947,31 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restr
                 next_adapter();
                 first = false;
             }
-            // lane: row `row`, columns 64 c + 16 qt + 4 v + e
-            const int oe = y_f16 ? 2 : 4;
-            const auto ry = make_rsrc(static_cast<uint8_t *>(Yv) + ((size_t)m0 * N + n0) * oe, (uint32_t)min(BM, M - m0) * (uint32_t)N * oe);
+            // lane: row `row`, columns 64 c + 16 qt + 4 v + e; into the staged rows, which leave in whole pieces as below
 #pragma unroll
             for (int c = 0; c < CB; ++c)
 #pragma unroll
-                for (int hh = 0; hh < 2; ++hh) {  // 8 columns
-                    const int n = 64 * c + 16 * qt + 8 * hh;
-                    const floatx4 *mp = reinterpret_cast<const floatx4 *>(ot + row * RS + n * 4);
-                    const floatx4 a0 = mp[0] + out[c][2 * hh], a1 = mp[1] + out[c][2 * hh + 1];
-                    const uint32_t off = n0 + n < N ? (uint32_t)row * (uint32_t)N * oe + (uint32_t)(n * oe) : kOOB;
-                    if (y_f16) {
-                        const half8 o = {(_Float16)a0[0], (_Float16)a0[1], (_Float16)a0[2], (_Float16)a0[3],
-                                         (_Float16)a1[0], (_Float16)a1[1], (_Float16)a1[2], (_Float16)a1[3]};
-                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), ry, off, 0, 2);
-                    } else {
-                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, a0), ry, off, 0, 2);
-                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, a1), ry, off + 16, 0, 2);
-                    }
+                for (int v = 0; v < 4; ++v)
+                    *reinterpret_cast<floatx4 *>(ot + row * RS + (64 * c + 16 * qt + 4 * v) * 4) += out[c][v];
+            const int oe = y_f16 ? 2 : 4;
+            const auto ry = make_rsrc(static_cast<uint8_t *>(Yv) + ((size_t)m0 * N + n0) * oe, (uint32_t)min(BM, M - m0) * (uint32_t)N * oe);
+            constexpr int P8 = BN / 8, RP8 = 64 / P8;  // 8 columns a lane: pieces of a row, rows at once
+            const int n = lane % P8 * 8;
+#pragma unroll
+            for (int rr = 0; rr < 16; rr += RP8) {
+                const int r = wave * 16 + rr + lane / P8;
+                const floatx4 *mp = reinterpret_cast<const floatx4 *>(ot + r * RS + n * 4);
+                const floatx4 a0 = mp[0], a1 = mp[1];
+                const uint32_t off = n0 + n < N ? (uint32_t)r * (uint32_t)N * oe + (uint32_t)(n * oe) : kOOB;
+                if (y_f16) {
+                    const half8 o = {(_Float16)a0[0], (_Float16)a0[1], (_Float16)a0[2], (_Float16)a0[3],
+                                     (_Float16)a1[0], (_Float16)a1[1], (_Float16)a1[2], (_Float16)a1[3]};
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), ry, off, 0, 2);
+                } else {
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, a0), ry, off, 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, a1), ry, off + 16, 0, 0);
                 }
+            }
             return;
         }
         constexpr int OB = PAIR ? HB * 2 : BN * EB;  // output bytes per tile row
@@ -1380,8 +1386,8 @@ int choose_pair_tile(int fmt, int64_t m, int64_t N, int64_t nk, int64_t cus) {
 
 // The tile of a product that adds its rows' adapters (LORA: those of 128 rows and 8 waves), -1 where the best
 // tile and the adapters in a pass of their own are faster.  Adding takes about 8 us a round of tiles, the pass and
-// the f32 product between 4 and 2.6 per million outputs, two of them kept as a margin (us, one adapter in
-// rank 16, apart / in the tiles: 2048x4096x4096 92 / 82, 1024x4096x4096 51.6 / 46.7, 2048x2560x2048 43.3 / 37.7,
+// the f32 product between 4 and 2.6 per million outputs, two of them kept as a margin (us, two adapters of rank 16,
+// apart / in the tiles: 2048x4096x4096 92 / 82, 1024x4096x4096 51.6 / 46.7, 2048x2560x2048 43.3 / 37.7,
 // 1293x4096x4096 65 / 61.5, 3000x4096x4096 131 / 131, 777x11008x4096 112 / 120, 512x4096x4096 34.4 / 37.5).
 int choose_lora_tile(int fmt, int64_t m, int64_t N, int64_t nk, int64_t cus) {
     const int best = choose_tile(fmt, m, N, nk, cus);
