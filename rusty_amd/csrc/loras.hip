@@ -69,24 +69,38 @@ __device__ __forceinline__ int rank_of(const LoraArgs &p, int i) {
     return p.ranks ? min(max(p.ranks[i], 0), p.rank) : p.rank;
 }
 
-// N consecutive values at p + e as floats or halves, those at and past `end` zero.  VEC: whole or not at all, aligned.
+// N consecutive values at p + e as floats or halves, those at and past `end` zero.  VEC: whole or not at all, aligned;
+// otherwise of any alignment (16-byte loads allow it; element by element 1037 rows of 5001 x 2048, rank 100, took 566 us).
 template <typename S, int N, bool VEC, typename D>
 __device__ __forceinline__ D load_n(const S *p, int64_t e, int64_t end) {
-    typedef S vec __attribute__((ext_vector_type(N)));
+    typedef S vec __attribute__((ext_vector_type(N), aligned(VEC ? sizeof(S) * N : sizeof(S))));
     D r;
-    if constexpr (VEC) {
-        vec v = {};
-        if (e < end) v = *reinterpret_cast<const vec *>(p + e);
-#pragma unroll
-        for (int i = 0; i < N; ++i) r[i] = (std::remove_reference_t<decltype(r[0] + r[0])>)v[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) r[i] = 0;
+    vec v = {};
+    if (VEC ? e < end : e + N <= end) {
+        v = *reinterpret_cast<const vec *>(p + e);
+    } else if constexpr (!VEC) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (e + i < end) r[i] = p[e + i];
+            if (e + i < end) v[i] = p[e + i];
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = (std::remove_reference_t<decltype(r[0] + r[0])>)v[i];
     return r;
+}
+// The same for stores.
+template <typename S, int N, bool VEC, typename D>
+__device__ __forceinline__ void store_n(S *p, int64_t e, int64_t end, D d) {
+    typedef S vec __attribute__((ext_vector_type(N), aligned(VEC ? sizeof(S) * N : sizeof(S))));
+    vec v;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = (S)d[i];
+    if (VEC ? e < end : e + N <= end) {
+        *reinterpret_cast<vec *>(p + e) = v;
+    } else if constexpr (!VEC) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (e + i < end) p[e + i] = v[i];
+    }
 }
 
 // Block (TM tiles of 16 rows, slice of k, z): of the rows' distinct adapters every gridDim.z-th, 16 RT of their
@@ -190,18 +204,7 @@ __global__ __launch_bounds__(256) void k_loras_out_row(LoraArgs p) {
         }
     }
     if (c >= p.n) return;
-    Y *y = static_cast<Y *>(p.y) + t * p.n;
-    typedef Y vec __attribute__((ext_vector_type(8)));
-    if constexpr (VEC) {
-        vec o;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = (Y)(main[e] + acc[e]);
-        *reinterpret_cast<vec *>(y + c) = o;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (c + e < p.n) y[c + e] = (Y)(main[e] + acc[e]);
-    }
+    store_n<Y, 8, VEC>(static_cast<Y *>(p.y) + t * p.n, c, p.n, main + acc);
 }
 
 // Many rows: block (16 rows, stretch of 256 columns), a wave 64 of them: B^T . t^T on the matrix instructions, so
@@ -213,7 +216,7 @@ __global__ __launch_bounds__(256) void k_loras_out_row(LoraArgs p) {
 // fp16 B: t, scaled by a power of two per row, is two fp16 terms (off by at most 2^-22), two instructions of 32 ranks
 // a 16 columns, B's fragments by transposing LDS reads; f32 instructions of 4 ranks took 3 us longer at 2048 x 4096, rank 32.
 __host__ __device__ constexpr int out_ranks(int rank) { return (rank + 31) / 32 * 32; }
-template <typename B, typename Y>
+template <typename B, typename Y, bool VEC>
 __global__ __launch_bounds__(256) void k_loras_out(LoraArgs p) {
     constexpr bool F16 = sizeof(B) == 2;
     constexpr int R = F16 ? 32 : 16;  // ranks of a step
@@ -249,6 +252,21 @@ __global__ __launch_bounds__(256) void k_loras_out(LoraArgs p) {
         return s.r0 < s.rank ? s : adapter(s.left);
     };
     auto fetch = [&](const Step &s, int buffer) {
+        if constexpr (!VEC) {
+            // (DMA takes whole, aligned pieces)
+            constexpr int E = 16 / (int)sizeof(B);
+            typedef B piece __attribute__((ext_vector_type(E)));
+            const B *b = static_cast<const B *>(p.b) + (int64_t)s.i * p.rank * p.n;
+            piece v[UN];
+#pragma unroll
+            for (int u = 0; u < UN; ++u)
+                v[u] = load_n<B, E, false, piece>(b + (int64_t)min(s.r0 + u * RPU + lane / CH, max(s.rank - 1, 0)) * p.n,
+                                                  c0 + lane % CH * E, p.n);
+#pragma unroll
+            for (int u = 0; u < UN; ++u) *reinterpret_cast<piece *>(bs + (buffer * R + u * RPU) * 64 + lane * E) = v[u];
+            wait_lgkm0();
+            return;
+        }
         const int64_t c = min(c0 + lane % CH * (16 / (int)sizeof(B)), p.n - 16 / (int)sizeof(B));
         const B *b = static_cast<const B *>(p.b) + (int64_t)s.i * p.rank * p.n + c;
 #pragma unroll
@@ -261,7 +279,8 @@ __global__ __launch_bounds__(256) void k_loras_out(LoraArgs p) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const int r = 4 * e + qt;
-        dma16_at(reinterpret_cast<const char *>(p.main + min(t0 + r, p.m - 1) * p.n + min(c0 + 4 * (col ^ r), p.n - 4)),
+        if constexpr (!VEC) main[wv][r][col] = load_n<float, 4, false, floatx4>(p.main + min(t0 + r, p.m - 1) * p.n, c0 + 4 * (col ^ r), p.n);
+        else dma16_at(reinterpret_cast<const char *>(p.main + min(t0 + r, p.m - 1) * p.n + min(c0 + 4 * (col ^ r), p.n - 4)),
                  lds_addr(&main[wv][4 * e][0]));
     }
     {
@@ -382,19 +401,12 @@ __global__ __launch_bounds__(256) void k_loras_out(LoraArgs p) {
     }
     const int64_t t = t0 + col, c = c0 + 16 * qt;
     if (t >= p.m) return;
-    Y *y = static_cast<Y *>(p.y) + t * p.n + c;
+    typedef float floatx8 __attribute__((ext_vector_type(8)));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {  // 8 columns
-        if (c + 8 * h >= p.n) break;
         const floatx4 a0 = main[wv][col][(4 * qt + 2 * h) ^ col] + out[2 * h], a1 = main[wv][col][(4 * qt + 2 * h + 1) ^ col] + out[2 * h + 1];
-        typedef Y vec8 __attribute__((ext_vector_type(8)));
-        vec8 o;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            o[e] = (Y)a0[e];
-            o[4 + e] = (Y)a1[e];
-        }
-        *reinterpret_cast<vec8 *>(y + 8 * h) = o;
+        store_n<Y, 8, VEC>(static_cast<Y *>(p.y) + t * p.n, c + 8 * h, p.n,
+                           floatx8{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]});
     }
 }
 
@@ -489,9 +501,9 @@ int run_in(const LoraArgs &p, rq_dtype xt, int at, int num_cus, hipStream_t s) {
     });
 }
 
-// Few rows, or columns that 16-byte pieces do not divide: a row per block; else 16.
+// Few rows: a row per block; else 16.
 int run_out(const LoraArgs &p, int bt, rq_dtype yt, hipStream_t s) {
-    const bool vec = p.n % 8 == 0 && aligned(p.b, 16) && aligned(p.y, 16), rows = p.m <= kFewRows || !vec;
+    const bool vec = p.n % 8 == 0 && aligned(p.b, 16) && aligned(p.y, 16), rows = p.m <= kFewRows;
     const int64_t bx = rows ? p.m : cdiv(p.m, 16), by = cdiv(p.n, rows ? 2048 : 256);
     const dim3 grid((unsigned)bx, (unsigned)by);
     return by_type(bt, [&](auto *b) {
@@ -500,7 +512,8 @@ int run_out(const LoraArgs &p, int bt, rq_dtype yt, hipStream_t s) {
             using Y = std::remove_pointer_t<decltype(y)>;
             const int r = sizeof(B) == 2 ? 32 : 16;
             const size_t lds = 16 * (out_ranks(p.rank) + 4) * sizeof(float) + (p.rank > r ? 2 : 1) * (size_t)(4 * r * 64) * sizeof(B);
-            if (!rows) hipLaunchKernelGGL((k_loras_out<B, Y>), grid, dim3(256), lds, s, p);
+            if (!rows && vec) hipLaunchKernelGGL((k_loras_out<B, Y, true>), grid, dim3(256), lds, s, p);
+            else if (!rows) hipLaunchKernelGGL((k_loras_out<B, Y, false>), grid, dim3(256), lds, s, p);
             else if (vec) hipLaunchKernelGGL((k_loras_out_row<B, Y, true>), grid, dim3(256), 0, s, p);
             else hipLaunchKernelGGL((k_loras_out_row<B, Y, false>), grid, dim3(256), 0, s, p);
             RQ_LAUNCH_CHECK();
