@@ -286,12 +286,13 @@ int rq_qmatmul_lora_ex(rq_ctx *ctx, const rq_qweight *w, const void *x, rq_dtype
  * nothing added where i is no adapter (outside 0..n_adapters-1).  ids: device
  * int32[m], in any order; rows of one adapter side by side are fastest.  The
  * adapter's products are summed in f32 (with fp16 X and adapters, exact
- * products), the weight's as rq_qmatmul's in f32; Y is rounded once.  m, k_in and n_out
- * go up to 2^24 - 256 (RQ_ERR_SHAPE past that); 16-byte loads are taken where k_in (for X and A)
- * and n_out (for B and Y) are multiples of 8 elements and the pointers 16-byte
- * aligned.  Nothing that another row's adapter holds reaches a row (which rows are beside
- * it may change the rounding of its sums).  workspace: rq_qmatmul_loras_workspace(...) bytes, 256-byte aligned, one
- * per call in flight (a captured call keeps its own); Y overlaps no input.
+ * products), the weight's as rq_qmatmul's in f32; Y is rounded once.  m, k_in and
+ * n_out go up to 2^24 - 256 (RQ_ERR_SHAPE past that); pointers are aligned to their
+ * elements, and calls are fastest where k_in and n_out are multiples of 8 and the
+ * pointers 16-byte aligned.  Nothing that another row's adapter holds reaches a row
+ * (which rows are beside it may change the rounding of its sums).  workspace:
+ * rq_qmatmul_loras_workspace(...) bytes, 256-byte aligned, one per call in flight (a
+ * captured call keeps its own); Y overlaps no input.
  * Uses the context's GEMM workspace as rq_qmatmul does. */
 typedef struct rq_lora_set {
     const void *a;         /* device [n_adapters][rank][k_in]: the reference's A transposed */
@@ -529,10 +530,10 @@ int rq_rope_append(rq_ctx *ctx, const rq_rope *rope, const rq_attn *attn, const 
  * sequences): row s of q sees the positions 0 .. lengths[s]-1 of sequence s
  * (device int32[n_seqs], clamped to 0..capacity; the token's own position is the
  * last of them, already cached) that lie in a page, and gets zeros if there are none.
- * n_seqs is at most 65536; out overlaps no input.  Arithmetic as in rq_attn_tree;
- * of attn, k_row and v_row are not used.  workspace: rq_attn_paged_workspace(...)
- * bytes, 16-byte aligned, one per call in flight (a captured call keeps its own).  On
- * the context's own stream the call uses the counters of the context's GEMM workspace, as
+ * n_seqs is at most 65536; out overlaps no input.  Arithmetic as in rq_attn_tree; of
+ * attn, k_row and v_row are not used.  workspace: rq_attn_paged_workspace(...) bytes,
+ * 16-byte aligned, one per call in flight (a captured call keeps its own).  On the
+ * context's own stream the call uses the counters of the context's GEMM workspace, as
  * rq_qmatmul does: a graph captured there is replayed there. */
 size_t rq_attn_paged_workspace(const rq_attn *attn, const rq_kv_pages *cache);
 int rq_attn_paged(rq_ctx *ctx, const rq_attn *attn, const rq_kv_pages *cache, const void *q, const int32_t *lengths,

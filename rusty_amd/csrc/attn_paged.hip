@@ -3,7 +3,9 @@
 //   out[s, h] = sum_j p_j v[j] / sum_j p_j,  p_j = 2^(c q.k_j - m),  c = scale log2 e
 //
 // in one pass over the keys with a running maximum m.  K and V are read once, so
-// the bound is their way from memory; the matrix instructions only have to keep up.
+// the bound is their way from memory; the matrix instructions only have to keep up.  fp16 weights p are
+// rounded to fp16 for the products with V (2^-11 of each, 2.7e-4 rms of the output with its own rounding); m,
+// sums and accumulators are f32.
 //
 // The query heads of a key/value head are the 16 columns of a matrix
 // instruction (more heads: more blocks), so one pass serves them all:
