@@ -174,8 +174,8 @@ constexpr int kTileAdapters = 16;
 // LDS by all waves), adds B^T . t^T on the matrix instructions: t, scaled by a power of two per
 // row, as two fp16 terms (off by at most 2^-22), B's fragments by transposing LDS reads.
 // Then the rows are rounded and leave in whole pieces (straight from the fragments, 32 bytes a lane, they were
-// written twice: 2048x4096x4096 80.6 us, so 78.6; 2048x11008x4096 203, 190).  Products of rows that have another adapter are dropped, not
-// added as zeros, so nothing a foreign adapter holds reaches a row.
+// written twice: 2048x4096x4096 80.6 us, so 78.6; 2048x11008x4096 203, 190).  Products of rows that have
+// another adapter are dropped, not added as zeros, so nothing a foreign adapter holds reaches a row.
 template <int BM, int BN, bool PINGPONG, int S, int NW, int WGN, int KG = 1, bool W2 = false, int FMT = 0,
           bool PAIR = false, bool ROPE = false, bool LORA = false>
 __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restrict__ W, const float *__restrict__ scales,
@@ -1391,9 +1391,8 @@ int choose_pair_tile(int fmt, int64_t m, int64_t N, int64_t nk, int64_t cus) {
 // 1293x4096x4096 65 / 61.5, 3000x4096x4096 131 / 131, 777x11008x4096 112 / 120, 512x4096x4096 34.4 / 37.5).
 int choose_lora_tile(int fmt, int64_t m, int64_t N, int64_t nk, int64_t cus) {
     const int best = choose_tile(fmt, m, N, nk, cus);
-    const int id = best == T128x256 || best == T128x128                                                       ? best
-                   : tile_cost(T128x256, fmt, m, N, nk, cus) < tile_cost(T128x128, fmt, m, N, nk, cus) ? T128x256
-                                                                                                              : T128x128;
+    const int other = tile_cost(T128x256, fmt, m, N, nk, cus) < tile_cost(T128x128, fmt, m, N, nk, cus) ? T128x256 : T128x128;
+    const int id = best == T128x256 || best == T128x128 ? best : other;
     const int64_t rounds = cdiv(cdiv(m, kTile[id].bm) * cdiv(N, kTile[id].bn), cus);
     const double apart = tile_cost(best, fmt, m, N, nk, cus) + 2.0 + 2.6e-6 * (double)m * (double)N;
     return tile_launches(id, m, N) && tile_cost(id, fmt, m, N, nk, cus) + 8.0 * (double)rounds < apart ? id : -1;

@@ -279,9 +279,11 @@ __global__ __launch_bounds__(256) void k_loras_out(LoraArgs p) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const int r = 4 * e + qt;
-        if constexpr (!VEC) main[wv][r][col] = load_n<float, 4, false, floatx4>(p.main + min(t0 + r, p.m - 1) * p.n, c0 + 4 * (col ^ r), p.n);
-        else dma16_at(reinterpret_cast<const char *>(p.main + min(t0 + r, p.m - 1) * p.n + min(c0 + 4 * (col ^ r), p.n - 4)),
-                 lds_addr(&main[wv][4 * e][0]));
+        const float *from = p.main + min(t0 + r, p.m - 1) * p.n;
+        if constexpr (VEC)
+            dma16_at(reinterpret_cast<const char *>(from + min(c0 + 4 * (col ^ r), p.n - 4)), lds_addr(&main[wv][4 * e][0]));
+        else
+            main[wv][r][col] = load_n<float, 4, false, floatx4>(from, c0 + 4 * (col ^ r), p.n);
     }
     {
         // t, 16 threads a row, 4 ranks each: the slices summed in order, times the factor; of rows without an

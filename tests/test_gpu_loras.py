@@ -433,3 +433,11 @@ def test_one_row_off_its_alignment(ctx, engine):
     got = out.to_vec()
     check(got[1:].reshape(2, 72), *truth(x, w64, a, b, np.ones(2), [1, 0], [8, 8], "f16", False), "off alignment")
     assert got[0] == 0.0
+
+
+@pytest.mark.parametrize("x_t,y_t,a_t", TYPES)
+@pytest.mark.parametrize("m", [200, 270])
+@pytest.mark.parametrize("n,k,rank", [(7, 130, 33), (5001, 130, 100), (130, 131, 256), (518, 260, 17)])
+def test_widths_that_pieces_do_not_divide(ctx, engine, x_t, y_t, a_t, m, n, k, rank):
+    """Rows of B and Y that begin anywhere, several steps of ranks, adapters of fewer ranks."""
+    case(ctx, engine, n, m, n, k, 3, rank, "rowwise8", x_t, y_t, a_t, some_ranks=True)
