@@ -3,9 +3,9 @@
 //   out[s, h] = sum_j p_j v[j] / sum_j p_j,  p_j = 2^(c q.k_j - m),  c = scale log2 e
 //
 // in one pass over the keys with a running maximum m.  K and V are read once, so
-// the bound is their way from memory; the matrix instructions only have to keep up.  fp16 weights p are
-// rounded to fp16 for the products with V (2^-11 of each, 2.7e-4 rms of the output with its own rounding); m,
-// sums and accumulators are f32.
+// the bound is their way from memory; the matrix instructions only have to keep up.  For the products with fp16 V
+// the weights p are two fp16 terms (off by 2^-22 of each: 2.0e-4 rms of the output, its own rounding); m, sums and
+// accumulators are f32.
 //
 // The query heads of a key/value head are the 16 columns of a matrix
 // instruction (more heads: more blocks), so one pass serves them all:
@@ -244,6 +244,10 @@ __device__ __forceinline__ void write_out(const PagedArgs &a, int s, int64_t at,
     *reinterpret_cast<vec4 *>(a.out + s * a.out_row + at * (int)sizeof(T)) = y;
 }
 
+// fp16: weights enter the products with V at 2^8 of their place below the maximum (2^14 at most, as it may lag by 2^6) and
+// as two terms, hi = fp16(p) and fp16(p - hi): off by 2^-22 of p or, near fp16's smallest, 2^-33 of the largest
+// weight, so a light key beside a heavy one keeps its share.
+//
 // Block (key/value head, 16 of its query heads, run).  WIDE: the rows of a DMA instruction lie in one page.
 template <typename T, int HD, bool WIDE>
 __global__ __launch_bounds__(TH, NW * blocks_per_cu(HD) / 4) void k_attn_paged(PagedArgs a) {
@@ -251,6 +255,7 @@ __global__ __launch_bounds__(TH, NW * blocks_per_cu(HD) / 4) void k_attn_paged(P
     constexpr bool F16 = SH::F16;
     constexpr int KT = SH::KT, ROW = SH::ROW, CH = SH::CH, TILE = SH::TILE, RPU = SH::RPU, UN = SH::UN, L = SH::L;
     constexpr int DT = HD / 16, KS = F16 ? HD / 32 : HD / 16;  // 16-dim tiles; 16-byte pieces of a row per lane
+    constexpr float UP = F16 ? 256.0f : 1.0f;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[NW * SH::RING];
     __shared__ float joined[2][NW][16];
     __shared__ int last[2];
@@ -475,17 +480,22 @@ __global__ __launch_bounds__(TH, NW * blocks_per_cu(HD) / 4) void k_attn_paged(P
                 wait_lgkm0();
             }
             if constexpr (F16) {
-                half8 pf;
+                half8 pf, pl, vf[DT];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) pf[e] = (_Float16)sc[e / 4][e % 4];
+                for (int e = 0; e < 8; ++e) pf[e] = (_Float16)(sc[e / 4][e % 4] * UP);
+                asm("" : "+v"(pf));  // (formed once: otherwise each is formed for the second term again)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) pl[e] = (_Float16)__builtin_fmaf(sc[e / 4][e % 4], UP, -(float)pf[e]);
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
                     lds_short4 *p = (lds_short4 *)(uintptr_t)(vt + va[d]);
                     const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
                     const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p + 16 * ROW / 8));
-                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, make_uint4(x.x, x.y, y.x, y.y)), pf,
-                                                                  o[d], 0, 0, 0);
+                    vf[d] = __builtin_bit_cast(half8, make_uint4(x.x, x.y, y.x, y.y));
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], pf, o[d], 0, 0, 0);
                 }
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], pl, o[d], 0, 0, 0);
             } else {
                 // instruction (e, h, i): key 4 qt + e, dims 64 h + 4 col + i
 #pragma unroll
@@ -503,6 +513,10 @@ __global__ __launch_bounds__(TH, NW * blocks_per_cu(HD) / 4) void k_attn_paged(P
             if (i + 1 < n) dma(vb, voff, vt);
         }
         l = join4(l, [](float x, float y) { return x + y; });
+        if constexpr (F16) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d] *= 1.0f / UP;
+        }
         // -inf as the maximum means no key at all: keys whose scores are all -inf give NaN, as 0 / 0
         if (any && mc == -__builtin_inff()) mc = -3.0e38f;
 
