@@ -9,7 +9,8 @@
 // A pass reads and writes every element once and is bound by that; all heads of
 // a token share its rot / 2 angles.  A block takes a few whole tokens: it asks
 // for its first elements, forms the tokens' (cos, sin) once into LDS -- the angle
-// in 64 bits, reduced to a fraction of a turn there, then f32 functions -- and turns
+// in 64 bits, reduced to a fraction of a turn there, then f32 functions of its f32 value, and the
+// remainder to first order (without it rows of (1, 0) were off by up to 1.85 2^-24, so by 1.31) -- and turns
 // the elements, 16 bytes a load at any alignment: where a head's parts are no
 // whole number of such pieces, the last one overlaps the one before it, unless the call
 // works in place (4096 tokens of 32 heads of 128, 86 of them turned, fp16: element by element 34 us, so 13.6).
@@ -134,9 +135,13 @@ __global__ __launch_bounds__(TH) void k_rope(RopeArgs a) {
     for (int i = threadIdx.x; i < nt * half; i += TH) {
         const int t = i / half;
         const double turns = (double)a.positions[t0 + t] * (a.freqs[i - t * half] * 0.15915494309189535);  // 1 / 2 pi
+        const double turn = turns - rint(turns);
+        const float near = (float)turn;
         float s, c;
-        sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-        cs[i] = make_float2(c * a.magnitude, s * (a.magnitude * a.sign));
+        sincospif(2.0f * near, &s, &c);
+        // what f32 leaves of the angle, up to 2^-26 of a turn (its square does not tell)
+        const float off = (float)(turn - (double)near) * 6.2831855f;
+        cs[i] = make_float2(__builtin_fmaf(-s, off, c) * a.magnitude, __builtin_fmaf(c, off, s) * (a.magnitude * a.sign));
     }
     if constexpr (APPEND) {
         for (int t = threadIdx.x >> 6; t < nt; t += TH / 64) {
