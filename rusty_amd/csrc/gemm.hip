@@ -862,7 +862,8 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restr
                         float tr = 0.0f;
                         if (r0 + (lane & 31) < rank)
                             for (int j = lane >> 5; j < ld.slices; j += 2) tr += q[(int64_t)j * ranks4 + r0 + (lane & 31)];
-                        tr = f * (tr + __shfl_xor(tr, 32));
+                        tr += __shfl_xor(tr, 32);
+                        tr = r0 + (lane & 31) < rank ? f * tr : 0.0f;  // (0 past the rank, also with an infinite factor)
 #pragma unroll
                         for (int u = 0; u < RC; ++u) {
                             const bool live = r0 + u < rank;

@@ -195,7 +195,7 @@ __global__ __launch_bounds__(256) void k_loras_out_row(LoraArgs p) {
             for (int j = lane >> 4; j < p.slices; j += 4) s += p.part[(t * p.slices + j) * p.ranks4 + r0 + u0];
         s += __shfl_xor(s, 16);
         s += __shfl_xor(s, 32);
-        s *= f;
+        s = r0 + u0 < rank ? f * s : 0.0f;  // (0 past the rank, also with an infinite factor)
 #pragma unroll
         for (int u = 0; u < RC; ++u) {
             const float su = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s), u));
