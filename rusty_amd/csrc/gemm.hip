@@ -72,6 +72,7 @@
 
 #include "common.hpp"
 #include "lds_dma.hpp"
+#include "loras.hpp"
 
 namespace rq {
 namespace {
@@ -171,8 +172,7 @@ constexpr int kTileAdapters = 16;
 // V caches (RopeOut) in fp16 instead of the f32 product.
 // LORA (128 tokens, 8 waves): an adapter per token (ld, fp16 B).  The scaled tile waits in LDS as f32 rows, a
 // wave takes 16 of them, and for each adapter of the tile's tokens, 32 ranks at a time (their B to
-// LDS by all waves), adds B^T . t^T on the matrix instructions: t, scaled by a power of two per
-// row, as two fp16 terms (off by at most 2^-22), B's fragments by transposing LDS reads.
+// LDS by all waves), adds B^T . t^T on the matrix instructions (t as loras.hpp says, a scale per 32 ranks), B's fragments by transposing LDS reads.
 // Then the rows are rounded and leave in whole pieces (straight from the fragments, 32 bytes a lane, they were
 // written twice: 2048x4096x4096 80.6 us, so 78.6; 2048x11008x4096 203, 190).  Products of rows that have
 // another adapter are dropped, not added as zeros, so nothing a foreign adapter holds reaches a row.
@@ -906,44 +906,60 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restr
                             *reinterpret_cast<uint4 *>(&ring[LORA_B] + (wave * BU + q) * 1024 + lane * 16) = make_uint4(0, 0, 0, 0);
                     __syncthreads();  // (the first: and the tile's rows are staged)
                     if (!own) continue;
-                    float most = 0.0f;
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            tv[u][e] = r1 + 4 * u + e < lrank ? f * tv[u][e] : 0.0f;
-                            most = fmaxf(most, __builtin_isfinite(tv[u][e]) ? fabsf(tv[u][e]) : 0.0f);
-                        }
+                        for (int e = 0; e < 4; ++e) tv[u][e] = r1 + 4 * u + e < lrank ? f * tv[u][e] : 0.0f;
+                    const bool has = own >> col & 1;
+                    float most = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float x = tv[e / 4][e % 4];
+                        most = fmaxf(most, __builtin_isfinite(x) ? fabsf(x) : 0.0f);
+                    }
                     most = fmaxf(most, __shfl_xor(most, 16));
                     most = fmaxf(most, __shfl_xor(most, 32));
-                    // the row's largest that is finite in [2^14, 2^15)
-                    const int ex = most > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+                    const int ex = lora_exponent(most);
                     half8 hi, lo;
+                    bool low = false;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const float x = __builtin_ldexpf(tv[e / 4][e % 4], ex);
-                        hi[e] = (_Float16)x;
-                        lo[e] = __builtin_isfinite((float)hi[e]) ? (_Float16)(x - (float)hi[e]) : (_Float16)0.0f;
+                        _Float16 h, l;
+                        lora_split(x, h, l);
+                        hi[e] = h;
+                        lo[e] = l;
+                        low = low || lora_low(x);
                     }
                     const float scale = __builtin_ldexpf(1.0f, -ex);
-                    const bool has = own >> col & 1;
                     // 16 lanes take 4 ranks x 4 x 4 columns; each gets one column's 4 ranks
                     const uint32_t at = ring_lds + (uint32_t)(LORA_B + (8 * qt + col / 4) * (BN * 2));
+                    auto add = [&](auto product) {
 #pragma unroll
-                    for (int c = 0; c < CB; ++c)
+                        for (int c = 0; c < CB; ++c)
 #pragma unroll
-                        for (int v = 0; v < 4; ++v) {
-                            const int ch = (c * 8 + (col & 3) * 2 + v / 2) ^ swz(col / 4);
-                            lds_short4 *p = (lds_short4 *)(uintptr_t)(at + (uint32_t)(ch * 16 + (v & 1) * 8));
-                            const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
-                            const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p + 4 * BN * 2 / 8));
-                            const half8 bf = __builtin_bit_cast(half8, make_uint4(x.x, x.y, y.x, y.y));
-                            floatx4 a = {0.0f, 0.0f, 0.0f, 0.0f};
-                            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf, hi, a, 0, 0, 0);
-                            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf, lo, a, 0, 0, 0);
+                            for (int v = 0; v < 4; ++v) {
+                                const int ch = (c * 8 + (col & 3) * 2 + v / 2) ^ swz(col / 4);
+                                lds_short4 *p = (lds_short4 *)(uintptr_t)(at + (uint32_t)(ch * 16 + (v & 1) * 8));
+                                const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
+                                const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p + 4 * BN * 2 / 8));
+                                const floatx4 sum = product(__builtin_bit_cast(half8, make_uint4(x.x, x.y, y.x, y.y)), out[c][v]);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) out[c][v][e] = has ? __builtin_fmaf(a[e], scale, out[c][v][e]) : out[c][v][e];
-                        }
+                                for (int e = 0; e < 4; ++e) out[c][v][e] = has ? sum[e] : out[c][v][e];
+                            }
+                    };
+                    if (__builtin_amdgcn_ballot_w64(has && low)) {
+                        add([&](half8 bf, floatx4 sum) { return lora_add_f32(bf, tv, sum); });
+                    } else {
+                        add([&](half8 bf, floatx4 sum) {
+                            const floatx4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+                            const floatx4 a = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf, hi, zero, 0, 0, 0);
+                            const floatx4 b = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf, lo, zero, 0, 0, 0);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(__builtin_fmaf(b[e], kLoraLo, a[e]), scale, sum[e]);
+                            return sum;
+                        });
+                    }
                 }
                 next_adapter();
                 first = false;

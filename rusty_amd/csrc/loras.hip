@@ -31,6 +31,7 @@
 
 #include "common.hpp"
 #include "lds_dma.hpp"
+#include "loras.hpp"
 
 namespace rq {
 namespace {
@@ -213,18 +214,19 @@ __global__ __launch_bounds__(256) void k_loras_out_row(LoraArgs p) {
 // that a tile with one adapter of up to 32 ranks reads is asked for together, and what B and the shared product take
 // waits in LDS (DMA): few registers, many waves.  B's buffers hold 32 ranks (f32 B: 16); with more ranks there are two,
 // else further adapters wait for their turn with one (2048 x 11008, rank 16: two buffers 45 us, one 40).
-// fp16 B: t, scaled by a power of two per row, is two fp16 terms (off by at most 2^-22), two instructions of 32 ranks
-// a 16 columns, B's fragments by transposing LDS reads; f32 instructions of 4 ranks took 3 us longer at 2048 x 4096, rank 32.
+// fp16 B: t as two fp16 terms (loras.hpp, a scale per row), two instructions of 32 ranks a 16 columns, B's fragments by
+// transposing LDS reads; f32 instructions of 4 ranks took 3 us longer at 2048 x 4096, rank 32.
 __host__ __device__ constexpr int out_ranks(int rank) { return (rank + 31) / 32 * 32; }
 template <typename B, typename Y, bool VEC>
-__global__ __launch_bounds__(256) void k_loras_out(LoraArgs p) {
+__global__ __launch_bounds__(256, sizeof(B) == 2 ? 4 : 1) void k_loras_out(LoraArgs p) {
     constexpr bool F16 = sizeof(B) == 2;
     constexpr int R = F16 ? 32 : 16;  // ranks of a step
     constexpr int CH = 64 * (int)sizeof(B) / 16, RPU = 64 / CH, UN = R / RPU;  // B: 16-byte pieces of a row, rows of a DMA
     typedef short short4v __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) short4v lds_short4;
     __shared__ __attribute__((aligned(16))) floatx4 main[4][16][16];       // [wave][row][16-byte piece ^ row]
-    // [16][out_ranks + 4]: t, fp16 B: its two terms side by side; then B [wave][buffer][rank][column]
+    // [16][out_ranks + 4]: t, fp16 B: its two terms side by side (a row that is low: t as it is), the row's scale and
+    // whether it is low; then B [wave][buffer][rank][column]
     extern __shared__ __attribute__((aligned(16))) float ts[];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, col = lane & 15, qt = lane >> 4;
     const int64_t t0 = (int64_t)blockIdx.x * 16, c0 = ((int64_t)blockIdx.y * 4 + wv) * 64;
@@ -290,9 +292,10 @@ __global__ __launch_bounds__(256) void k_loras_out(LoraArgs p) {
         // adapter not written, and not used
         const int tr = threadIdx.x >> 4, u = threadIdx.x & 15, i = __shfl(mine, tr);
         float *to = ts + tr * row4;
-        float most = 0.0f;
+        float most = 0.0f, least = __builtin_inff();
         if (i >= 0) {
             const float f = p.factors ? p.factors[i] : 1.0f;
+            const int rank = rank_of(p, i);
             for (int r = 4 * u; r < ranks; r += 64) {
                 const float *q = p.part + (t0 + tr) * p.slices * p.ranks4 + r;
                 floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -300,31 +303,38 @@ __global__ __launch_bounds__(256) void k_loras_out(LoraArgs p) {
 #pragma unroll 8
                     for (int j = 0; j < p.slices; ++j) v += *reinterpret_cast<const floatx4 *>(q + (int64_t)j * p.ranks4);
                 }
-                const int rank = rank_of(p, i);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     v[e] = r + e < rank ? f * v[e] : 0.0f;
                     most = fmaxf(most, __builtin_isfinite(v[e]) ? fabsf(v[e]) : 0.0f);
+                    least = fminf(least, v[e] != 0.0f ? fabsf(v[e]) : __builtin_inff());
                 }
                 *reinterpret_cast<floatx4 *>(to + r) = v;
             }
         }
         if constexpr (F16) {
 #pragma unroll
-            for (int w = 1; w < 16; w <<= 1) most = fmaxf(most, __shfl_xor(most, w));
-            // the largest that is finite in [2^14, 2^15)
-            const int e = most > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
-            if (u == 0) to[ranks] = __builtin_ldexpf(1.0f, -e);
-            if (i >= 0)
+            for (int w = 1; w < 16; w <<= 1) {
+                most = fmaxf(most, __shfl_xor(most, w));
+                least = fminf(least, __shfl_xor(least, w));
+            }
+            const int ex = lora_exponent(most);
+            const bool low = lora_low(__builtin_ldexpf(least, ex));
+            if (u == 0) {
+                to[ranks] = __builtin_ldexpf(1.0f, -ex);
+                to[ranks + 1] = low ? 1.0f : 0.0f;
+            }
+            if (i >= 0 && !low)
                 for (int r = 4 * u; r < ranks; r += 64) {
                     const floatx4 v = *reinterpret_cast<const floatx4 *>(to + r);
                     typedef _Float16 half4 __attribute__((ext_vector_type(4)));
                     half4 hi, lo;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float x = __builtin_ldexpf(v[k], e);
-                        hi[k] = (_Float16)x;
-                        lo[k] = __builtin_isfinite((float)hi[k]) ? (_Float16)(x - (float)hi[k]) : (_Float16)0.0f;
+                    for (int e = 0; e < 4; ++e) {
+                        _Float16 h, l;
+                        lora_split(__builtin_ldexpf(v[e], ex), h, l);
+                        hi[e] = h;
+                        lo[e] = l;
                     }
                     // (8 ranks: 16 bytes of first terms, 16 of second)
                     half4 *h = reinterpret_cast<half4 *>(to + r / 8 * 8) + r / 4 % 2;
@@ -335,9 +345,12 @@ __global__ __launch_bounds__(256) void k_loras_out(LoraArgs p) {
         }
     }
     __syncthreads();
-    floatx4 out[4], acc[4];
+    floatx4 out[4], acc[4], acc_lo[4];
 #pragma unroll
-    for (int v = 0; v < 4; ++v) out[v] = acc[v] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int v = 0; v < 4; ++v) out[v] = acc[v] = acc_lo[v] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    // (of a row without an adapter: whatever was there, and not used)
+    const float row_scale = F16 ? ts[col * row4 + ranks] : 1.0f, row_low = F16 ? ts[col * row4 + ranks + 1] : 0.0f;
+    auto f32 = [&](const Step &s) { return __builtin_amdgcn_ballot_w64((s.same >> col & 1) && row_low != 0.0f) != 0; };
     wait_vmcnt<0>();
     for (int k = 0; s.same; ++k) {
         const Step next = after(s);
@@ -359,17 +372,34 @@ __global__ __launch_bounds__(256) void k_loras_out(LoraArgs p) {
                         *reinterpret_cast<half8 *>(b + (u * RPU + lane / CH) * 64 + lane % CH * 8) = half8{};
                 wait_lgkm0();
             }
-            const half8 *t = reinterpret_cast<const half8 *>(ts + col * row4 + s.r0 + 8 * qt);
-            const half8 hi = t[0], lo = t[1];
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
+            const half8 *tp = reinterpret_cast<const half8 *>(ts + col * row4 + s.r0 + 8 * qt);
+            const half8 hi = tp[0], lo = tp[1];
+            auto fragment = [&](int v) {
                 // 16 lanes take 4 ranks x 4 x 4 columns; each gets one column's 4 ranks
                 lds_short4 *a = (lds_short4 *)(uintptr_t)(lds_addr(b) + (uint32_t)((8 * qt + col / 4) * 128 + (col & 3) * 32 + v * 8));
                 const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(a));
                 const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(a + 4 * 128 / 8));
-                const half8 bt = __builtin_bit_cast(half8, make_uint4(x.x, x.y, y.x, y.y));
-                acc[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bt, hi, acc[v], 0, 0, 0);
-                acc[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bt, lo, acc[v], 0, 0, 0);
+                return __builtin_bit_cast(half8, make_uint4(x.x, x.y, y.x, y.y));
+            };
+            if (f32(s)) {
+                floatx4 t[2] = {__builtin_bit_cast(floatx4, hi), __builtin_bit_cast(floatx4, lo)};
+                if (row_low == 0.0f) {  // (beside a row that is low)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) t[e / 4][e % 4] = __builtin_fmaf((float)lo[e], kLoraLo, (float)hi[e]) * row_scale;
+                }
+#pragma unroll 1
+                for (int v = 0; v < 4; ++v) {
+                    const floatx4 sum = lora_add_f32(fragment(v), t, v == 0 ? acc[0] : v == 1 ? acc[1] : v == 2 ? acc[2] : acc[3]);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) acc[w] = v == w ? sum : acc[w];
+                }
+            } else {
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const half8 bt = fragment(v);
+                    acc[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bt, hi, acc[v], 0, 0, 0);
+                    acc_lo[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bt, lo, acc_lo[v], 0, 0, 0);
+                }
             }
         } else {
             float bv[R / 4][4], tv[R / 4];  // (all read before the first is used)
@@ -387,12 +417,15 @@ __global__ __launch_bounds__(256) void k_loras_out(LoraArgs p) {
         }
         if (next.i != s.i || !next.same) {
             const bool has = s.same >> col & 1;
-            const float scale = F16 ? ts[col * row4 + ranks] : 1.0f;
+            const bool plain = !F16 || f32(s);
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) out[v][e] = has ? acc[v][e] * scale : out[v][e];
-                acc[v] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int e = 0; e < 4; ++e) {
+                    const float sum = plain ? acc[v][e] : __builtin_fmaf(acc_lo[v][e], kLoraLo, acc[v][e]) * row_scale;
+                    out[v][e] = has ? sum : out[v][e];
+                }
+                acc[v] = acc_lo[v] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
             }
         }
         if (next.same && buffers == 1) {
