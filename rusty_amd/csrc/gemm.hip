@@ -956,7 +956,7 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_rowwise(const uint8_t *__restr
                             const floatx4 a = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf, hi, zero, 0, 0, 0);
                             const floatx4 b = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf, lo, zero, 0, 0, 0);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(__builtin_fmaf(b[e], kLoraLo, a[e]), scale, sum[e]);
+                            for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(lora_join(a[e], b[e]), scale, sum[e]);
                             return sum;
                         });
                     }

@@ -422,7 +422,7 @@ __global__ __launch_bounds__(256, sizeof(B) == 2 ? 4 : 1) void k_loras_out(LoraA
             for (int v = 0; v < 4; ++v) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float sum = plain ? acc[v][e] : __builtin_fmaf(acc_lo[v][e], kLoraLo, acc[v][e]) * row_scale;
+                    const float sum = plain ? acc[v][e] : lora_join(acc[v][e], acc_lo[v][e]) * row_scale;
                     out[v][e] = has ? sum : out[v][e];
                 }
                 acc[v] = acc_lo[v] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};

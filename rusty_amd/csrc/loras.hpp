@@ -27,6 +27,11 @@ __device__ __forceinline__ void lora_split(float x, _Float16 &hi, _Float16 &lo) 
     hi = (_Float16)x;
     lo = __builtin_isfinite((float)hi) ? (_Float16)((x - (float)hi) * 2048.0f) : (_Float16)0.0f;
 }
+// The two products joined.  An infinite B makes the second one infinite of either sign, or NaN as 0 times infinity; the
+// first has what the sum is then, so the second is kept finite.
+__device__ __forceinline__ float lora_join(float hi, float lo) {
+    return __builtin_fmaf(__builtin_amdgcn_fmed3f(lo, -3e38f, 3e38f), kLoraLo, hi);
+}
 // acc + B^T . t^T in f32 instructions: b and t of 32 ranks as operands of v_mfma_f32_16x16x32_f16 (a lane: column or row
 // lane % 16, ranks 8 (lane / 16) ..); instruction e takes rank e of each quarter wave.
 __device__ __forceinline__ lora_float4 lora_add_f32(lora_half8 b, const lora_float4 (&t)[2], lora_float4 acc) {

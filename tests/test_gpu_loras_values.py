@@ -64,3 +64,16 @@ def test_infinite_factor(ctx, engine, x_t, y_t, a_t, m, n, k, count, rank, own):
     ids = (np.arange(m) + 1) % count
     got = run(ctx, engine, x, zeros(ctx, n, k), a, b, f, ids, [own] * count, x_t, y_t, a_t)
     assert np.all(got[ids % 2 == 1] == np.inf) and np.all(got[ids % 2 == 0] == own * 128.0)
+
+
+@pytest.mark.parametrize("m,n,k", [(2, 64, 64), (100, 64, 64), (300, 64, 64), (300, 65, 64), (1100, 5640, 64)])
+def test_infinite_adapter(ctx, engine, m, n, k):
+    """An infinity in B reaches its column as itself, with its sign, in rows of any number."""
+    a, b = np.ones((2, 40, k), np.float16), np.ones((2, 40, n), np.float16)
+    b[1, 3, ::3], b[1, 35, 1::3] = np.inf, -np.inf
+    a[:, 35] = 1.0 / 3.0
+    x = np.full((m, k), 2.0, np.float16)
+    ids = (np.arange(m) + 1) % 2
+    got = run(ctx, engine, x, zeros(ctx, n, k), a, b, None, ids, None, "f16", "f32", "f16")
+    assert np.isfinite(got[ids == 0]).all() and np.isfinite(got[ids == 1][:, 2::3]).all()
+    assert np.all(got[ids == 1][:, ::3] == np.inf) and np.all(got[ids == 1][:, 1::3] == -np.inf)
