@@ -246,7 +246,8 @@ __device__ __forceinline__ void write_out(const PagedArgs &a, int s, int64_t at,
 
 // fp16: weights enter the products with V at 2^8 of their place below the maximum (2^14 at most, as it may lag by 2^6) and
 // as two terms, hi = fp16(p) and fp16(p - hi): off by 2^-22 of p or, near fp16's smallest, 2^-33 of the largest
-// weight, so a light key beside a heavy one keeps its share.
+// weight, so a light key beside a heavy one keeps its share.  The terms' sums stay apart: the second terms, 0 or
+// below, make NaN of an infinite V, or the other infinity; the first ones have the infinity, and the others' sum is kept finite.
 //
 // Block (key/value head, 16 of its query heads, run).  WIDE: the rows of a DMA instruction lie in one page.
 template <typename T, int HD, bool WIDE>
@@ -404,9 +405,9 @@ __global__ __launch_bounds__(TH, NW * blocks_per_cu(HD) / 4) void k_attn_paged(P
         }
 
         float mc = -__builtin_inff(), l = 0.0f;  // running maximum (scaled), this lane's share of the sum
-        floatx4 o[DT];
+        floatx4 o[DT], ol[F16 ? DT : 1];
 #pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int d = 0; d < DT; ++d) o[d] = ol[F16 ? d : 0] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
         bool any = false;
 
         for (int i = 0; i < per; ++i) {
@@ -459,7 +460,10 @@ __global__ __launch_bounds__(TH, NW * blocks_per_cu(HD) / 4) void k_attn_paged(P
                 mc = rose ? mt : mc;
                 l *= alpha;
 #pragma unroll
-                for (int d = 0; d < DT; ++d) o[d] *= alpha;
+                for (int d = 0; d < DT; ++d) {
+                    o[d] *= alpha;
+                    if constexpr (F16) ol[d] *= alpha;
+                }
             }
             const float off = mc == -__builtin_inff() ? 0.0f : -mc;  // no key yet: every weight is 2^-inf
 #pragma unroll
@@ -480,7 +484,7 @@ __global__ __launch_bounds__(TH, NW * blocks_per_cu(HD) / 4) void k_attn_paged(P
                 wait_lgkm0();
             }
             if constexpr (F16) {
-                half8 pf, pl, vf[DT];
+                half8 pf, pl;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) pf[e] = (_Float16)(sc[e / 4][e % 4] * UP);
                 asm("" : "+v"(pf));  // (formed once: otherwise each is formed for the second term again)
@@ -491,11 +495,10 @@ __global__ __launch_bounds__(TH, NW * blocks_per_cu(HD) / 4) void k_attn_paged(P
                     lds_short4 *p = (lds_short4 *)(uintptr_t)(vt + va[d]);
                     const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
                     const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p + 16 * ROW / 8));
-                    vf[d] = __builtin_bit_cast(half8, make_uint4(x.x, x.y, y.x, y.y));
-                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], pf, o[d], 0, 0, 0);
+                    const half8 vf = __builtin_bit_cast(half8, make_uint4(x.x, x.y, y.x, y.y));
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf, o[d], 0, 0, 0);
+                    ol[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, ol[d], 0, 0, 0);
                 }
-#pragma unroll
-                for (int d = 0; d < DT; ++d) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], pl, o[d], 0, 0, 0);
             } else {
                 // instruction (e, h, i): key 4 qt + e, dims 64 h + 4 col + i
 #pragma unroll
@@ -515,7 +518,9 @@ __global__ __launch_bounds__(TH, NW * blocks_per_cu(HD) / 4) void k_attn_paged(P
         l = join4(l, [](float x, float y) { return x + y; });
         if constexpr (F16) {
 #pragma unroll
-            for (int d = 0; d < DT; ++d) o[d] *= 1.0f / UP;
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[d][e] = (o[d][e] + __builtin_amdgcn_fmed3f(ol[d][e], -3e38f, 3e38f)) * (1.0f / UP);
         }
         // -inf as the maximum means no key at all: keys whose scores are all -inf give NaN, as 0 / 0
         if (any && mc == -__builtin_inff()) mc = -3.0e38f;

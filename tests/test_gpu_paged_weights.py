@@ -66,3 +66,18 @@ def test_many_light_keys_beside_a_heavy_one(ctx, engine, n, low):
     put(pools, table[0], "heads", page, k, v)
     want, tol = truth(q, [[k, v]], 1 / 8)
     check(run(ctx, engine, q, pools, table, [n], "heads", "f16"), want, tol, f"{n} keys of 2^-{low}")
+
+
+@pytest.mark.parametrize("heads,kv,dim,n", [(4, 2, 64, 64), (3, 1, 128, 128), (8, 1, 64, 3000)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_infinite_values(ctx, engine, heads, kv, dim, n, sign):
+    """An infinity in V, at every place of a unit of keys, reaches its dimension as itself, and no other."""
+    q, pools, table, rows = make(25, [n], heads, kv, dim, 16, "heads", "f16")
+    k, v = rows[0]
+    g = np.random.default_rng(26)
+    hit = g.random(dim) < 0.8
+    for d in np.nonzero(hit)[0]:
+        v[:, (d * 37 + n // 2) % n, d] = sign * np.inf
+    put(pools, table[0], "heads", 16, k, v)
+    got = run(ctx, engine, q, pools, table, [n], "heads", "f16")[0]
+    assert np.all(got[:, hit] == sign * np.inf) and np.isfinite(got[:, ~hit]).all()
