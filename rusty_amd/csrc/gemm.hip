@@ -1402,17 +1402,23 @@ int choose_pair_tile(int fmt, int64_t m, int64_t N, int64_t nk, int64_t cus) {
 }
 
 // The tile of a product that adds its rows' adapters (LORA: those of 128 rows and 8 waves), -1 where the best
-// tile and the adapters in a pass of their own are faster.  Adding takes about 8 us a round of tiles, the pass and
-// the f32 product between 4 and 2.6 per million outputs, two of them kept as a margin (us, two adapters of rank 16,
-// apart / in the tiles: 2048x4096x4096 92 / 82, 1024x4096x4096 51.6 / 46.7, 2048x2560x2048 43.3 / 37.7,
-// 1293x4096x4096 65 / 61.5, 3000x4096x4096 131 / 131, 777x11008x4096 112 / 120, 512x4096x4096 34.4 / 37.5).
-int choose_lora_tile(int fmt, int64_t m, int64_t N, int64_t nk, int64_t cus) {
+// tile and the adapters in a pass of their own are faster.  Adding takes about 5 us a round of tiles and 2.5 for each
+// of a tile's turns, 32 ranks of an adapter; the pass and the f32 product between 4 and 2.6 per million outputs, two
+// of them kept as a margin.  The ids are on the device: a tile is taken to have as many adapters as if each one's
+// rows lay side by side.  us, apart / in the tiles, over 4 adapters of 4 prompts and 64 of prompts of 8 rows:
+//   2048x4096x4096, rank 16  95 / 80,  96 / 111   64  96 / 85, 120 / 167   128  111 / 99, 159 / 273   256  137 / 132, 258 / 503
+//   1024x4096x4096, rank 16  54 / 48,  57 / 77    64  59 / 56,  75 / 121   128   67 / 69, 100 / 204   256   83 / 98,  161 / 385
+//   2048x2560x2048, rank 16  46 / 40,  50 / 77    64  50 / 45,  65 / 143   128   61 / 59,  93 / 259   256   83 / 84,  152 / 517
+// Over those and as many of prompts of 32 rows and of rows at random among 4, 16 and 64, the choice takes 1.024 of the
+// better form's time (a choice by m, N and K alone 1.28), at worst 1.33 (64 ranks, rows at random among 16; 3.4).
+int choose_lora_tile(int fmt, int64_t m, int64_t N, int64_t nk, int64_t cus, int64_t rank, int64_t n_adapters) {
     const int best = choose_tile(fmt, m, N, nk, cus);
     const int other = tile_cost(T128x256, fmt, m, N, nk, cus) < tile_cost(T128x128, fmt, m, N, nk, cus) ? T128x256 : T128x128;
     const int id = best == T128x256 || best == T128x128 ? best : other;
     const int64_t rounds = cdiv(cdiv(m, kTile[id].bm) * cdiv(N, kTile[id].bn), cus);
+    const double turns = std::min((double)n_adapters, 1.0 + 127.0 * (double)n_adapters / (double)m) * (double)cdiv(rank, 32);
     const double apart = tile_cost(best, fmt, m, N, nk, cus) + 2.0 + 2.6e-6 * (double)m * (double)N;
-    return tile_launches(id, m, N) && tile_cost(id, fmt, m, N, nk, cus) + 8.0 * (double)rounds < apart ? id : -1;
+    return tile_launches(id, m, N) && tile_cost(id, fmt, m, N, nk, cus) + (5.0 + 2.5 * turns) * (double)rounds < apart ? id : -1;
 }
 
 // The fp16-activation GEMM over m rows, tile chosen by shape.
@@ -1438,7 +1444,7 @@ int gemm_tiles(const rq_qweight &w, const float *scales, int fmt, const void *x,
     }
     const GemmPair np{};
     auto go = [&](auto launch) { return launch(w, scales, fmt, x, y, yt, m, 4, cus, ws, s, np, nullptr, xscale, ld); };
-    switch (ld ? choose_lora_tile(fmt, m, N, nk, cus) : choose_tile(fmt, m, N, nk, cus)) {
+    switch (ld ? choose_lora_tile(fmt, m, N, nk, cus, ld->rank, ld->n_adapters) : choose_tile(fmt, m, N, nk, cus)) {
     case T128x256: return go(launch_tiled<128, 256, true, 4, 8, 4, 2, true>);
     case T192x128: return go(launch_tiled<192, 128, true, 4, 8, 2, 2, true>);
     case T128x128: return go(launch_tiled<128, 128, true, 4, 8, 2, 2, true>);
@@ -1551,7 +1557,7 @@ int launch_gemm(const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dty
     const int64_t cus = num_cus > 0 ? num_cus : 256;
     // adapters: tiles of 128 tokens and 8 waves, whole 16-byte pieces of B and Y
     if (ld) {
-        if (choose_lora_tile(fmt, m, N, K / 64, cus) < 0 || !ld->f16 || N % 8 != 0 || !aligned(ld->b, 16) || !aligned(y, 16) ||
+        if (choose_lora_tile(fmt, m, N, K / 64, cus, ld->rank, ld->n_adapters) < 0 || !ld->f16 || N % 8 != 0 || !aligned(ld->b, 16) || !aligned(y, 16) ||
             128 * N * 4 > 0x7fffffff)
             return RQ_ERR_UNSUPPORTED;
     }
@@ -1604,11 +1610,17 @@ int launch_gemm(const rq_qweight &w, const void *x, rq_dtype xt, void *y, rq_dty
 // For the tests, no part of the C ABI: the tile (bm * 1000 + bn) that the
 // fp16-activation GEMM takes for an m x n_out x k_in product (fmt 0: per-row
 // codes, 1: affine), or with `pair` for SwiGLU's gate and up of n_out rows
-// each (1), or with an adapter per row (2); -1 where the parts run one after the other.  Host arithmetic.
+// each (1), or with an adapter per row (2, two of rank 16 in all); -1 where the parts run one after the other.  Host arithmetic.
 extern "C" int rusty_gemm_tile(int fmt, int64_t m, int64_t n_out, int64_t k_in, int num_cus, int pair) {
     using namespace rq;
-    const int id = pair == 2 ? choose_lora_tile(fmt, m, n_out, k_in / 64, num_cus)
+    const int id = pair == 2 ? choose_lora_tile(fmt, m, n_out, k_in / 64, num_cus, 16, 2)
                    : pair    ? choose_pair_tile(fmt, m, 2 * n_out, k_in / 64, num_cus)
                              : choose_tile(fmt, m, n_out, k_in / 64, num_cus);
+    return id < 0 ? -1 : kTile[id].bm * 1000 + kTile[id].bn;
+}
+// The same with an adapter per row of a set of n_adapters of `rank`.
+extern "C" int rusty_gemm_lora_tile(int fmt, int64_t m, int64_t n_out, int64_t k_in, int num_cus, int64_t rank, int64_t n_adapters) {
+    using namespace rq;
+    const int id = choose_lora_tile(fmt, m, n_out, k_in / 64, num_cus, rank, n_adapters);
     return id < 0 ? -1 : kTile[id].bm * 1000 + kTile[id].bn;
 }
