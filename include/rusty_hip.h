@@ -227,7 +227,7 @@ int rq_matmul_at(rq_ctx *ctx, const float *a, const float *b, float *out, int64_
  * fp16-MFMA prefill path), each row scaled first by the power of two that
  * puts its largest magnitude in [2^14, 2^15) and its outputs scaled back, so
  * there too any finite row is served, at fp16 accuracy; it rounds affine
- * weights to fp16 likewise.
+ * weights to fp16 likewise, as 3..16 fp16 rows of affine codes do.
  * RQ_Q_AFFINE_U4 weights go 16 rows at a time with exact codes up to m = 48,
  * f32 rows at f32 accuracy whatever their magnitude (two fp16 terms again, scaled
  * per 32 values of a row for one or two rows of up to 16384, else per row and 256 k where
@@ -530,8 +530,8 @@ int rq_rope_append(rq_ctx *ctx, const rq_rope *rope, const rq_attn *attn, const 
  * sequences): row s of q sees the positions 0 .. lengths[s]-1 of sequence s
  * (device int32[n_seqs], clamped to 0..capacity; the token's own position is the
  * last of them, already cached) that lie in a page, and gets zeros if there are none.
- * n_seqs is at most 65536; out overlaps no input.  Arithmetic as in rq_attn_tree; of
- * attn, k_row and v_row are not used.  workspace: rq_attn_paged_workspace(...) bytes,
+ * n_seqs is at most 65536; out overlaps no input.  Arithmetic as in rq_attn_tree, but that
+ * fp16 calls carry the weights of the keys in two fp16 terms (off by 2^-22 of each); of attn, k_row and v_row are not used.  workspace: rq_attn_paged_workspace(...) bytes,
  * 16-byte aligned, one per call in flight (a captured call keeps its own).  On the
  * context's own stream the call uses the counters of the context's GEMM workspace, as
  * rq_qmatmul does: a graph captured there is replayed there. */

@@ -57,7 +57,8 @@ def sources() -> list[Path]:
 #  * k_cast_f16_rows: the row maximum and the x * 2^-e scaling.  An f32
 #    denormal element reads as 0; where the row maximum is normal such an
 #    element is below the fp16 result's resolution (2^-24 of the maximum) in
-#    any case, so only rows made entirely of denormals change (to zero).
+#    any case, so only rows made entirely of denormals change (to zero);
+#  * an adapter's t = factor X . A^T (rq_qmatmul_loras): below 2^-126 it reads as 0.
 FILE_FLAGS = {"gemm.hip": ["-fgpu-flush-denormals-to-zero"]}
 
 

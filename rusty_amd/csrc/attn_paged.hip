@@ -29,11 +29,12 @@
 // smaller than that.
 //
 // Times (us; the bytes at the rate of a plain read of as much, 6.9 TB/s): six sequences
-// of up to 32701 keys, 32/8 heads of 128, 67 (55); f32, seven of up to 3001, 16/16 heads of 128, 25.8
-// (16); 48 chats of 37 to 2047 keys, 32/4 heads of 64, 12.5 (3.6); one of 513 7.2.  What is left is
+// of up to 32701 keys, 32/8 heads of 128, 68 (55); f32, seven of up to 3001, 16/16 heads of 128, 26
+// (16); 48 chats of 37 to 2047 keys, 32/4 heads of 64, 12.5 (3.6); one of 513 7.4.  What is left is
 // latency: about 1 us each for the launch, the lengths, a page's entry, the first keys, and 3 for a join (the
-// stores' acknowledgement, the counter, the pieces); and that blocks of one size are not done at one time (the
-// first of six long sequences' at 50 us, the last at 61).  Loads that leave the caches alone (nt) took 10 % off the
+// stores' acknowledgement, the counter, the pieces); that blocks of one size are not done at one time (the
+// first of six long sequences' at 50 us, the last at 61); and that short batches are not dealt evenly (the 48 chats' 765
+// units to 61 of 128 runs, 3 to 30 each).  Loads that leave the caches alone (nt) took 10 % off the
 // long calls, one block of eight waves per CU over two of four 2 %, waves in step (s_barrier) 3 %.
 #include <math.h>
 
@@ -116,8 +117,8 @@ __device__ __forceinline__ int scan_add(int v) {  // inclusive, over the wave
 }
 
 // A run's units: an equal share, at least 12; and a sequence of up to so many units is not cut, the run
-// that it begins in has all of it.  Shorter runs and more cuts cost joining, longer ones the waves' turns (us, 48
-// chats of 37 to 2047 keys, 32/4 heads of 64 / one sequence of 513: at least 8, all cut 12.9 / 7.9, up to 16
+// that it begins in has all of it.  Shorter runs and more cuts cost joining, longer ones the waves' turns (us, weights in one
+// term, 48 chats of 37 to 2047 keys, 32/4 heads of 64 / one sequence of 513: at least 8, all cut 12.9 / 7.9, up to 16
 // whole 12.6 / 7.9; 12, up to 24 whole 12.5 / 7.3; 24, up to 24 whole 14.2 / 7.1).
 __device__ __forceinline__ int run_length(const PagedArgs &a, int total) { return max(12, a.by_runs(total + a.runs - 1)); }
 __device__ __forceinline__ int whole_units(int len) { return min(2 * len, 24); }

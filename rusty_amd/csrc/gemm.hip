@@ -146,8 +146,9 @@ __device__ __forceinline__ void tile_of(int b, int tiles_m, int tiles_n, int gm,
 }
 
 // Adapters of a tile's rows that LORA (below) takes one after another (about 4 us each, 32 ranks); of more, its rows
-// are taken one by one (16 a wave, about 4 us each).  2048x4096x4096, rows' adapters at random among 12 / 64: 141 / 182 us,
-// one by one 143 / 182, in a pass of their own 130 / 179 (side by side, as prompts have them, 6: 81, 92).
+// are taken one by one (16 a wave, about 4 us each); both grow with the ranks alike.  2048x4096x4096, rank 32, rows' adapters
+// at random among 12 / 64: 143 / 182 us, one by one 143 / 182, in a pass of their own 130 / 179 (side by side, as prompts
+// have them, 6: 81, 92).
 constexpr int kTileAdapters = 16;
 
 // FMT 0: per-row int8 codes, scales[n] applied in the epilogue.  FMT 1: the

@@ -23,8 +23,8 @@
 //
 // Measured (us; X . A / shared product / t . B; in brackets the bytes at 6.9 TB/s or the products at 1157 TFLOP/s):
 // one row of 4096 x 4096, 8-bit rows, rank 16: 3.2 / 5.8 with t . B, 8.9 a call (2.5; apart 3.3 / 4.7 / 2.7, 12.3);
-// 16 rows of 11 adapters of rank 16, 11008 x 4096, 4-bit groups: 4.9 / 16.8 / 4.0, 23.5 a call (4.9); 2048 rows of 4096 x
-// 4096, 8-bit rows, rank 32: 9.9 / 69 with t . B, 78.6 a call (60; apart 9.4 / 66 / 18.9, 91).  X . A and the shared product
+// 16 rows of 8 to 10 adapters of rank 16, 11008 x 4096, 4-bit groups: 4.8 / 16.7 / 4.0, 23.4 a call (4.7 to 4.9); 2048 rows
+// of 4096 x 4096, 8-bit rows, rank 32: 9.8 / 69 with t . B, 79 a call (60; apart 9.4 / 66 / 18.9, 91).  X . A and the shared product
 // of a few rows in one launch took 8 us, 6.1 in two.
 #include <algorithm>
 #include <type_traits>
