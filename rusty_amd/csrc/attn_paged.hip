@@ -30,7 +30,7 @@
 //
 // Times (us; the bytes at the rate of a plain read of as much, 6.9 TB/s): six sequences
 // of up to 32701 keys, 32/8 heads of 128, 68 (55); f32, seven of up to 3001, 16/16 heads of 128, 26
-// (16); 48 chats of 37 to 2047 keys, 32/4 heads of 64, 12.5 (3.6); one of 513 7.4.  What is left is
+// (16); 48 chats of 37 to 2047 keys, 32/4 heads of 64, 12.5 (3.6); one of 513 7.5.  What is left is
 // latency: about 1 us each for the launch, the lengths, a page's entry, the first keys, and 3 for a join (the
 // stores' acknowledgement, the counter, the pieces); that blocks of one size are not done at one time (the
 // first of six long sequences' at 50 us, the last at 61); and that short batches are not dealt evenly (the 48 chats' 765
@@ -409,7 +409,7 @@ __global__ __launch_bounds__(TH, NW * blocks_per_cu(HD) / 4) void k_attn_paged(P
         floatx4 o[DT], ol[F16 ? DT : 1];
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] = ol[F16 ? d : 0] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-        bool any = false;
+        bool any = false, far = false;
 
         for (int i = 0; i < per; ++i) {
             if (i > 0) __builtin_amdgcn_s_barrier();  // (for an even pace: older waves' loads go first)
@@ -459,6 +459,8 @@ __global__ __launch_bounds__(TH, NW * blocks_per_cu(HD) / 4) void k_attn_paged(P
             if (__builtin_amdgcn_ballot_w64(rose)) {
                 const float alpha = rose ? __builtin_amdgcn_exp2f(mc - mt) : 1.0f;
                 mc = rose ? mt : mc;
+                // An fma takes the product unrounded where mc was rounded: past 2^22, where that tells, it is rounded first.
+                far = __builtin_amdgcn_ballot_w64(fabsf(mc) > 4194304.0f && mc != -__builtin_inff()) != 0;
                 l *= alpha;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
@@ -467,11 +469,22 @@ __global__ __launch_bounds__(TH, NW * blocks_per_cu(HD) / 4) void k_attn_paged(P
                 }
             }
             const float off = mc == -__builtin_inff() ? 0.0f : -mc;  // no key yet: every weight is 2^-inf
+            if (__builtin_expect(far, false)) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float x = sc[t][e] * a.c;
+                        asm volatile("" : "+v"(x));  // (kept here: moved across, it takes 12 registers)
+                        sc[t][e] = x;
+                    }
+            }
+            const float c = far ? 1.0f : a.c;
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    sc[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][e], a.c, off));
+                    sc[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][e], c, off));
                     l += sc[t][e];
                 }
             if (i + 1 < n) wait_vmcnt<UN>();

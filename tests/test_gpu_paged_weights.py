@@ -81,3 +81,26 @@ def test_infinite_values(ctx, engine, heads, kv, dim, n, sign):
     put(pools, table[0], "heads", 16, k, v)
     got = run(ctx, engine, q, pools, table, [n], "heads", "f16")[0]
     assert np.all(got[:, hit] == sign * np.inf) and np.isfinite(got[:, ~hit]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("scale", [1e-3, 1.0, 30.0, 1e3, -1e3])
+@pytest.mark.parametrize("n", [5, 70, 3000])
+def test_scores_past_the_exponentials_reach(ctx, engine, dtype, scale, n):
+    """Scores so large that a step of f32 between them is many times the exponential's range: the largest has all
+    the weight, two alike share it."""
+    q, pools, table, rows = make(27, [n], 4, 2, 64, 16, "heads", dtype)
+    g = np.random.default_rng(28)
+    k, v = rows[0]
+    q[...], k[...] = 0.0, 0.0
+    q[..., 0] = np.sign(scale) * (5e4 + 1e4 * g.random(q.shape[:2]))
+    k[:, :, 0] = np.linspace(1e4, 4e4, n)  # (fp16: steps of 8 to 32, alike in places; the largest two are not)
+    top = [n // 3, n - 2]
+    k[:, top, 0] = 6e4
+    put(pools, table[0], "heads", 16, k, v)
+    want = np.repeat(v[:, top].astype(np.float64).mean(1), 2, 0)
+    got = run(ctx, engine, q, pools, table, [n], "heads", dtype, scale=scale)[0]
+    half, u = (2.0 ** -11 if dtype == "f16" else 2.0 ** -24), 2.0 ** -24
+    # the two weights are equal; a sum, a quotient and the output's rounding
+    tol = (half + 4 * u) * np.abs(want) + 4 * u * np.abs(v[:, top].astype(np.float64)).max(1).repeat(2, 0) + 2.0 ** -25
+    check(got, want, tol, f"{n} keys, scale {scale}")
