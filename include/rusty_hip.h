@@ -530,11 +530,12 @@ int rq_rope_append(rq_ctx *ctx, const rq_rope *rope, const rq_attn *attn, const 
  * sequences): row s of q sees the positions 0 .. lengths[s]-1 of sequence s
  * (device int32[n_seqs], clamped to 0..capacity; the token's own position is the
  * last of them, already cached) that lie in a page, and gets zeros if there are none.
- * n_seqs is at most 65536; out overlaps no input.  Arithmetic as in rq_attn_tree, but that
- * fp16 calls carry the weights of the keys in two fp16 terms (off by 2^-22 of each); of attn, k_row and v_row are not used.  workspace: rq_attn_paged_workspace(...) bytes,
- * 16-byte aligned, one per call in flight (a captured call keeps its own).  On the
- * context's own stream the call uses the counters of the context's GEMM workspace, as
- * rq_qmatmul does: a graph captured there is replayed there. */
+ * n_seqs is at most 65536; out overlaps no input.  Arithmetic as in rq_attn_tree, but
+ * that fp16 calls carry the weights of the keys in two fp16 terms (off by 2^-22 of
+ * each); of attn, k_row and v_row are not used.  workspace: rq_attn_paged_workspace(...)
+ * bytes, 16-byte aligned, one per call in flight (a captured call keeps its own).  On
+ * the context's own stream the call uses the counters of the context's GEMM workspace,
+ * as rq_qmatmul does: a graph captured there is replayed there. */
 size_t rq_attn_paged_workspace(const rq_attn *attn, const rq_kv_pages *cache);
 int rq_attn_paged(rq_ctx *ctx, const rq_attn *attn, const rq_kv_pages *cache, const void *q, const int32_t *lengths,
                   void *out, void *workspace, size_t workspace_bytes, rq_stream stream);

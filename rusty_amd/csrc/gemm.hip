@@ -173,7 +173,8 @@ constexpr int kTileAdapters = 16;
 // V caches (RopeOut) in fp16 instead of the f32 product.
 // LORA (128 tokens, 8 waves): an adapter per token (ld, fp16 B).  The scaled tile waits in LDS as f32 rows, a
 // wave takes 16 of them, and for each adapter of the tile's tokens, 32 ranks at a time (their B to
-// LDS by all waves), adds B^T . t^T on the matrix instructions (t as loras.hpp says, a scale per 32 ranks), B's fragments by transposing LDS reads.
+// LDS by all waves), adds B^T . t^T on the matrix instructions: t as two fp16 terms (loras.hpp, a scale per row and
+// 32 ranks), B's fragments by transposing LDS reads.
 // Then the rows are rounded and leave in whole pieces (straight from the fragments, 32 bytes a lane, they were
 // written twice: 2048x4096x4096 80.6 us, so 78.6; 2048x11008x4096 203, 190).  Products of rows that have
 // another adapter are dropped, not added as zeros, so nothing a foreign adapter holds reaches a row.
